@@ -154,6 +154,17 @@ EXPORTS = (
     "ane_decode_token_ggml",
     "ane_ggml_backend_get_stream",
     "ane_ggml_backend_set_stream",
+    "ane_hip_paged_rope_append",
+    "ane_hip_attention_prompt_workspace_size",
+    "ane_hip_attention_prompt",
+    "ane_hip_attention_shared_workspace_size",
+    "ane_hip_attention_shared",
+    "ane_hip_pages_workspace_size",
+    "ane_hip_pages_reserve",
+    "ane_hip_pages_fork",
+    "ane_hip_pages_free",
+    "ane_hip_pages_copy",
+    "ane_hip_pages_compact",
 )
 
 _lib: ctypes.CDLL | None = None
@@ -244,6 +255,24 @@ _SIGS: dict[str, tuple[Any, list[Any]]] = {
     "ane_decode_token_ggml": (_c.c_int, [_P, _P, _P, _c.c_float, _c.c_uint32, _P, _P, _c.c_size_t, _P, _c.c_int]),
     "ane_ggml_backend_get_stream": (_P, [_P]),
     "ane_ggml_backend_set_stream": (None, [_P, _P]),
+    "ane_hip_paged_rope_append": (
+        _c.c_int, [_P, _c.c_uint32, _P, _c.c_uint32, _P, _c.c_uint32, _c.c_int, _P, _c.c_uint64, _P, _P, _c.c_uint64,
+                   _P, _c.c_uint32, _c.c_int, _P, _c.c_uint64, _P]),
+    "ane_hip_attention_prompt_workspace_size": (_c.c_size_t, [_P, _c.c_uint32, _c.c_uint32, _c.c_uint32]),
+    "ane_hip_attention_prompt": (
+        _c.c_int, [_P, _c.c_uint32, _P, _c.c_uint32, _P, _c.c_uint32, _c.c_uint32, _c.c_int, _P, _c.c_uint64,
+                   _c.c_float, _P, _c.c_uint64, _P, _c.c_size_t, _P]),
+    "ane_hip_attention_shared_workspace_size": (
+        _c.c_size_t, [_P, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32]),
+    "ane_hip_attention_shared": (
+        _c.c_int, [_P, _c.c_uint32, _P, _c.c_uint32, _c.c_uint32, _P, _P, _c.c_uint32, _c.c_uint32, _c.c_int, _P,
+                   _c.c_uint64, _c.c_float, _P, _c.c_uint64, _P, _c.c_size_t, _P]),
+    "ane_hip_pages_workspace_size": (_c.c_size_t, [_P]),
+    "ane_hip_pages_reserve": (_c.c_int, [_P, _c.c_uint32, _P, _P, _P, _P, _c.c_size_t, _P]),
+    "ane_hip_pages_fork": (_c.c_int, [_P, _c.c_uint32, _P, _P, _P, _P, _c.c_size_t, _P]),
+    "ane_hip_pages_free": (_c.c_int, [_P, _c.c_uint32, _P, _P]),
+    "ane_hip_pages_copy": (_c.c_int, [_P, _c.c_uint32, _P, _P, _P]),
+    "ane_hip_pages_compact": (_c.c_int, [_P, _P, _P, _P, _P, _c.c_size_t, _P]),
 }
 
 
@@ -965,3 +994,250 @@ def decode_token(cfg, layers, table, pos, x, workspace, stream=None):
     L = lib()
     check(L.ane_decode_token(ctypes.byref(cfg), layers, _p(table), pos, _p(x), _p(workspace),
                              workspace.numel(), _stream_handle(stream)), "decode_token")
+
+
+# ---------------------------------------------------------------- paged cache, batches
+NO_PAGE = -1  # ANE_NO_PAGE in the int32 tensors of page numbers
+
+
+class PagedCache(ctypes.Structure):
+    """Mirror of struct ane_paged_cache (include/ane_decode.h), over device
+    tensors that it keeps alive: k_pages, v_pages fp16 [layers][pages][kv heads]
+    [page size][head dim], page_table int32 [sequences][max pages] (NO_PAGE in
+    unused entries), kv_len int32 [sequences], page_refs int32 [pages]."""
+
+    _fields_ = [(n, ctypes.c_uint32) for n in ("n_layers", "n_heads", "n_kv_heads", "head_dim", "page_size", "n_pages",
+                                                "n_seqs", "max_pages")] + [
+        (n, ctypes.c_void_p) for n in ("k_ptr", "v_ptr", "table_ptr", "len_ptr", "refs_ptr")]
+
+    def __init__(self, n_heads, k_pages, v_pages, page_table, kv_len, page_refs=None):
+        import torch
+
+        if k_pages.dim() != 5 or k_pages.shape != v_pages.shape or page_table.dim() != 2:
+            raise ValueError("k_pages and v_pages are [layers][pages][kv heads][page size][head dim], page_table "
+                             "[sequences][max pages]")
+        ints = [page_table, kv_len] + ([] if page_refs is None else [page_refs])
+        if any(t.dtype != torch.float16 for t in (k_pages, v_pages)) or any(t.dtype != torch.int32 for t in ints):
+            raise ValueError("pages are float16; page_table, kv_len and page_refs int32")
+        if not all(t.is_contiguous() and t.device == k_pages.device for t in (k_pages, v_pages, *ints)):
+            raise ValueError("the cache's tensors are contiguous and on one device")
+        n_layers, n_pages, n_kv, page_size, head_dim = k_pages.shape
+        if kv_len.numel() != page_table.shape[0] or (page_refs is not None and page_refs.numel() != n_pages):
+            raise ValueError("kv_len has an entry for each sequence, page_refs one for each page")
+        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
+        self.kv_len, self.page_refs = kv_len, page_refs
+        super().__init__(n_layers, n_heads, n_kv, head_dim, page_size, n_pages, page_table.shape[0],
+                         page_table.shape[1], _p(k_pages), _p(v_pages), _p(page_table), _p(kv_len), _p(page_refs))
+
+    @classmethod
+    def empty(cls, n_layers, n_heads, n_kv_heads, head_dim, page_size, n_pages, n_seqs, max_pages, device="cuda"):
+        """A cache whose pages are all free."""
+        import torch
+
+        shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.float16, device=device) for _ in range(2))
+        table = torch.full((n_seqs, max_pages), NO_PAGE, dtype=torch.int32, device=device)
+        kv_len, refs = (torch.zeros(m, dtype=torch.int32, device=device) for m in (n_seqs, n_pages))
+        return cls(n_heads, k, v, table, kv_len, refs)
+
+
+def _type_of(t, what):
+    import torch
+
+    if t.dtype == torch.float32:
+        return 0
+    if t.dtype == torch.float16:
+        return 1
+    raise ValueError(f"{what} is float32 or float16")
+
+
+def _rows(t, heads, cache, what):
+    """Row stride of activations [tokens][heads][head_dim] whose heads are contiguous."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != cache.head_dim:
+        raise ValueError(f"{what} is [tokens][{heads}][{cache.head_dim}]")
+    if t.shape[0] and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != cache.head_dim)):
+        raise ValueError(f"the heads of a token of {what} are contiguous")
+    return t.stride(0) if t.shape[0] > 1 else heads * cache.head_dim
+
+
+def _ints(t, n, what):
+    """A device array of at least n int32, or None."""
+    import torch
+
+    if t is None:
+        return 0
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{what} is a contiguous int32 tensor of {n} entries")
+    return _p(t)
+
+
+class _On:
+    """The cache's device as the current one during a call, and the call's stream there."""
+
+    def __init__(self, cache, stream):
+        import torch
+
+        dev = cache.k_pages.device
+        self.guard = None if dev.type != "cuda" or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        self.stream = stream
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return _stream_handle(self.stream)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _batch(q_start, seqs, rows):
+    """(n, q_start pointer, seqs pointer) of a packed batch of `rows` tokens."""
+    n = rows if q_start is None else q_start.numel() - 1
+    if n < 0:
+        raise ValueError("q_start has an entry more than the batch has rows")
+    return n, _ints(q_start, n + 1, "q_start"), _ints(seqs, n, "seqs")
+
+
+def paged_rope_append(cache, layer, q_start, q, k, v, table, q_out, seqs=None, stream=None):
+    """RoPE of q and k and the append of k and v to the pages of one layer:
+    q, k, v [tokens][heads][head_dim] (views of one qkv tensor will do), the new
+    tokens of batch row i in rows q_start[i] .. q_start[i+1]-1 (None: one each);
+    q_out takes the rotated q; q and q_out None: k and v only; table None: no
+    rotation."""
+    n, qs, sq = _batch(q_start, seqs, k.shape[0])
+    ks = _rows(k, cache.n_kv_heads, cache, "k")
+    if _rows(v, cache.n_kv_heads, cache, "v") != ks or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("k and v have the same shape, strides and type")
+    if (q is None) != (q_out is None) or (q is not None and (q.dtype != k.dtype or q.shape[0] != k.shape[0]
+                                                              or q_out.shape[0] < q.shape[0])):
+        raise ValueError("q and q_out go together, q with the tokens and type of k")
+    if table is not None and (str(table.dtype) != "torch.float32" or not table.is_contiguous()
+                              or table.numel() != table.shape[0] * cache.head_dim):
+        raise ValueError("table is a contiguous float32 [positions][head_dim/2][2]")
+    with _On(cache, stream) as st:
+        check(lib().ane_hip_paged_rope_append(
+            ctypes.byref(cache), layer, sq, n, qs, k.shape[0], _type_of(k, "k"), _p(q),
+            0 if q is None else _rows(q, cache.n_heads, cache, "q"), _p(k), _p(v), ks, _p(table),
+            0 if table is None else table.shape[0], 0 if q is None else _type_of(q_out, "q_out"), _p(q_out),
+            0 if q is None else _rows(q_out, cache.n_heads, cache, "q_out"), st), "paged_rope_append")
+
+
+def _attention_rows(cache, q, out):
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out has the shape and type of q")
+    return _type_of(q, "q"), _rows(q, cache.n_heads, cache, "q"), _rows(out, cache.n_heads, cache, "out")
+
+
+def attention_prompt_workspace_size(cache, n, n_tokens, max_len=None) -> int:
+    return int(lib().ane_hip_attention_prompt_workspace_size(ctypes.byref(cache), n, n_tokens, max_len or 0))
+
+
+def attention_prompt_workspace(cache, n, n_tokens, max_len=None):
+    """A workspace for attention_prompt calls of these sizes, for callers that keep one."""
+    return _scratch(attention_prompt_workspace_size(cache, n, n_tokens, max_len), cache.k_pages.device)
+
+
+def attention_prompt(cache, layer, q_start, q, out, max_len=None, scale=None, seqs=None, workspace=None, stream=None):
+    """Causal attention of packed prompts over the pages of one layer: q and out
+    [tokens][heads][head_dim] float32 or float16, the new tokens of batch row i
+    (its sequence's last positions, already appended) in rows q_start[i] ..
+    q_start[i+1]-1.  max_len bounds the sequences' lengths; scale None:
+    1/sqrt(head_dim)."""
+    n, qs, sq = _batch(q_start, seqs, q.shape[0])
+    ty, s0, s1 = _attention_rows(cache, q, out)
+    with _On(cache, stream) as st:
+        need = attention_prompt_workspace_size(cache, n, q.shape[0], max_len)
+        ws = workspace if workspace is not None else _scratch(need, q.device, stream) if need else None
+        check(lib().ane_hip_attention_prompt(
+            ctypes.byref(cache), layer, sq, n, qs, q.shape[0], max_len or 0, ty, _p(q), s0,
+            cache.head_dim ** -0.5 if scale is None else scale, _p(out), s1, _p(ws),
+            0 if ws is None else ws.numel() * ws.element_size(), st), "attention_prompt")
+
+
+def attention_shared_workspace_size(cache, n, n_groups=0, max_prefix=None, max_len=None) -> int:
+    return int(lib().ane_hip_attention_shared_workspace_size(ctypes.byref(cache), n, n_groups, max_prefix or 0,
+                                                             max_len or 0))
+
+
+def attention_shared_workspace(cache, n, n_groups=0, max_prefix=None, max_len=None):
+    """A workspace for attention_shared calls of these sizes, for callers that keep one."""
+    return _scratch(attention_shared_workspace_size(cache, n, n_groups, max_prefix, max_len), cache.k_pages.device)
+
+
+def attention_shared(cache, layer, q, out, max_len=None, group_start=None, prefix_len=None, max_prefix=None, scale=None,
+                     seqs=None, workspace=None, stream=None):
+    """One token of each batch row over the pages of one layer: q and out [rows]
+    [heads][head_dim].  Rows group_start[g] .. group_start[g+1]-1 share their
+    first prefix_len[g] positions, which are read once for the group;
+    group_start None: no row shares anything."""
+    n = q.shape[0]
+    sq = _ints(seqs, n, "seqs")
+    if (group_start is None) != (prefix_len is None):
+        raise ValueError("group_start and prefix_len go together")
+    groups = 0 if group_start is None else group_start.numel() - 1
+    gs, pl = _ints(group_start, groups + 1, "group_start"), _ints(prefix_len, groups, "prefix_len")
+    ty, s0, s1 = _attention_rows(cache, q, out)
+    with _On(cache, stream) as st:
+        need = attention_shared_workspace_size(cache, n, groups, max_prefix, max_len)
+        ws = workspace if workspace is not None else _scratch(need, q.device, stream) if need else None
+        check(lib().ane_hip_attention_shared(
+            ctypes.byref(cache), layer, sq, n, groups, gs, pl, max_prefix or 0, max_len or 0, ty, _p(q), s0,
+            cache.head_dim ** -0.5 if scale is None else scale, _p(out), s1, _p(ws),
+            0 if ws is None else ws.numel() * ws.element_size(), st), "attention_shared")
+
+
+def pages_workspace(cache):
+    """A workspace for the page calls on this cache."""
+    return _scratch(lib().ane_hip_pages_workspace_size(ctypes.byref(cache)), cache.k_pages.device)
+
+
+def _pages_ws(cache, workspace, stream):
+    need = int(lib().ane_hip_pages_workspace_size(ctypes.byref(cache)))
+    ws = workspace if workspace is not None else _scratch(need, cache.k_pages.device, stream)
+    return ws, ws.numel() * ws.element_size()
+
+
+def pages_reserve(cache, seqs, new_len, served=None, workspace=None, stream=None):
+    """Sequences seqs[i] grow to new_len[i] positions (int32 device tensors);
+    served[i]: 1 where the pool had the pages."""
+    n = seqs.numel()
+    a, b, c = _ints(seqs, n, "seqs"), _ints(new_len, n, "new_len"), _ints(served, n, "served")
+    with _On(cache, stream) as st:
+        ws, size = _pages_ws(cache, workspace, stream)
+        check(lib().ane_hip_pages_reserve(ctypes.byref(cache), n, a, b, c, _p(ws), size, st), "pages_reserve")
+
+
+def pages_fork(cache, src, dst, served=None, workspace=None, stream=None):
+    """Empty sequences dst[i] become copies of src[i] that share their whole pages."""
+    n = src.numel()
+    a, b, c = _ints(src, n, "src"), _ints(dst, n, "dst"), _ints(served, n, "served")
+    with _On(cache, stream) as st:
+        ws, size = _pages_ws(cache, workspace, stream)
+        check(lib().ane_hip_pages_fork(ctypes.byref(cache), n, a, b, c, _p(ws), size, st), "pages_fork")
+
+
+def pages_free(cache, seqs, stream=None):
+    """The sequences become empty and give their pages up."""
+    with _On(cache, stream) as st:
+        check(lib().ane_hip_pages_free(ctypes.byref(cache), seqs.numel(), _ints(seqs, seqs.numel(), "seqs"), st),
+              "pages_free")
+
+
+def pages_copy(cache, src, dst, stream=None):
+    """Pages dst[i] become copies of pages src[i] in every layer."""
+    n = src.numel()
+    with _On(cache, stream) as st:
+        check(lib().ane_hip_pages_copy(ctypes.byref(cache), n, _ints(src, n, "src"), _ints(dst, n, "dst"), st),
+              "pages_copy")
+
+
+def pages_compact(cache, table_out=None, refs_out=None, n_live=None, workspace=None, stream=None):
+    """The live pages move to the front of the pool; the new table and counts go
+    to table_out and refs_out (None: the cache's own), the number of live pages
+    to n_live."""
+    t = _ints(table_out, cache.n_seqs * cache.max_pages, "table_out")
+    r, l = _ints(refs_out, cache.n_pages, "refs_out"), _ints(n_live, 1, "n_live")
+    with _On(cache, stream) as st:
+        ws, size = _pages_ws(cache, workspace, stream)
+        check(lib().ane_hip_pages_compact(ctypes.byref(cache), t, r, l, _p(ws), size, st), "pages_compact")

@@ -1,0 +1,593 @@
+// paged.hip -- the paged K/V cache: RoPE and append of packed tokens, and the
+// page calls (reserve, fork, free, copy, compact).
+//
+// The page calls keep their whole state on the device: one workgroup looks
+// through the reference counts and assigns pages (the lowest free ones first,
+// by prefix sums and not by atomics, so that a result never depends on
+// timing), then a wide launch moves the data.
+#include "paged.hpp"
+
+namespace ane {
+namespace {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+// ------------------------------------------------------------ RoPE + append
+struct AppendArgs {
+    const void *q, *k, *v;
+    void* q_out;
+    const float* rope;
+    uint16_t *kp, *vp;  // this layer's pages
+    const uint32_t *table, *kv_len, *seqs, *q_start;
+    uint64_t q_stride, kv_stride, q_out_stride;
+    uint32_t n, n_tokens, rope_len, n_heads, n_kv, hd, ps, n_pages, max_pages, n_seqs;
+};
+
+template <class T>
+__device__ __forceinline__ void load8(const void* p, uint64_t i, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const h8 a = *reinterpret_cast<const h8*>(static_cast<const _Float16*>(p) + i);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = (float)a[e];
+    }
+}
+template <class T>
+__device__ __forceinline__ void store8(void* p, uint64_t i, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        float* o = static_cast<float*>(p) + i;
+        *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(o + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        h8 a;
+#pragma unroll
+        for (int e = 0; e < 8; e++) a[e] = (_Float16)x[e];
+        *reinterpret_cast<h8*>(static_cast<_Float16*>(p) + i) = a;
+    }
+}
+
+// One workgroup per token; a thread takes 8 values (4 pairs) of one head at a
+// time: [q heads | k heads | v heads] x hd/8 units.  The values of the first
+// kAhead units are loaded before the token's sequence is looked up, so that
+// the chain start -> length -> page runs while they arrive.
+constexpr uint32_t kAhead = 3;
+template <class TI, class TQ>
+__global__ void __launch_bounds__(256) k_paged_append(AppendArgs a) {
+    const uint32_t t = blockIdx.x, tid = threadIdx.x;
+    const uint32_t per = a.hd / 8, qu = a.q ? a.n_heads * per : 0, ku = a.n_kv * per, units = qu + 2 * ku;
+    auto load = [&](uint32_t u, float(&x)[8]) {
+        if (u < qu) load8<TI>(a.q, t * a.q_stride + u * 8, x);
+        else if (u < qu + ku) load8<TI>(a.k, t * a.kv_stride + (u - qu) * 8, x);
+        else if (u < units) load8<TI>(a.v, t * a.kv_stride + (u - qu - ku) * 8, x);
+    };
+    float x[kAhead][8];
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; i++) load(tid + i * 256, x[i]);
+
+    // the token's sequence, position and page
+    uint32_t s = t, first = t, last = t + 1;
+    if (a.q_start) {
+        s = wave_search(a.n, t, [&](uint32_t i) { return (uint64_t)a.q_start[i]; });
+        first = a.q_start[s];
+        last = a.q_start[s + 1];
+        if (t < first || t >= last) return;  // before the first sequence or behind the last
+    }
+    const uint32_t id = a.seqs ? a.seqs[s] : s;
+    int64_t pos = -1;
+    uint32_t page = ANE_NO_PAGE, row = 0;
+    if (id < a.n_seqs) {
+        pos = (int64_t)a.kv_len[id] - (int64_t)(last - t);
+        const uint64_t pi = pos < 0 ? a.max_pages : (uint64_t)pos / a.ps;
+        if (pi < a.max_pages && (!a.rope || pos < a.rope_len)) {
+            page = a.table[(uint64_t)id * a.max_pages + pi];
+            row = (uint32_t)pos % a.ps;
+        } else {
+            pos = -1;
+        }
+    }
+    auto put = [&](uint32_t u, float(&v)[8]) {
+        if (u >= units) return;
+        const bool isv = u >= qu + ku;
+        const uint32_t d = u % per * 8;
+        if (pos < 0) {
+            if (u < qu) {
+                const float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                store8<TQ>(a.q_out, t * a.q_out_stride + u * 8, z);
+            }
+            return;
+        }
+        if (a.rope && !isv) {
+            const float* cs = a.rope + (uint64_t)pos * a.hd + d;
+            float c[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) c[e] = cs[e];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float p = v[e], r = v[e + 1];
+                v[e] = __fsub_rn(__fmul_rn(p, c[e]), __fmul_rn(r, c[e + 1]));
+                v[e + 1] = __fadd_rn(__fmul_rn(p, c[e + 1]), __fmul_rn(r, c[e]));
+            }
+        }
+        if (u < qu) {
+            store8<TQ>(a.q_out, t * a.q_out_stride + u * 8, v);
+        } else if (page < a.n_pages) {
+            const uint32_t g = (u - qu - (isv ? ku : 0)) / per;
+            store8<_Float16>(isv ? a.vp : a.kp, (((uint64_t)page * a.n_kv + g) * a.ps + row) * a.hd + d, v);
+        }
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; i++) put(tid + i * 256, x[i]);
+    for (uint32_t u = tid + kAhead * 256; u < units; u += 256) {
+        load(u, x[0]);
+        put(u, x[0]);
+    }
+}
+
+// -------------------------------------------------------- assigning pages
+constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kScan = 16;
+
+// Exclusive prefix sums over the workgroup's 1024 threads; *total: the sum.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* sh, uint64_t* total) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t s = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint64_t o = __shfl_up((unsigned long long)s, off, 64);
+        if (lane >= (uint32_t)off) s += o;
+    }
+    if (lane == 63) sh[wave] = s;
+    __syncthreads();
+    uint64_t before = 0, all = 0;
+    for (uint32_t w = 0; w < kPlanWaves; w++) {
+        if (w < wave) before += sh[w];
+        all += sh[w];
+    }
+    __syncthreads();
+    *total = all;
+    return before + s - v;
+}
+
+// The pages i in [from, to) with pick(refs[i]), in ascending order: found(rank,
+// i) for each of the first `want`.  Returns how many there are (counting
+// stops once `want` are found).  kScan x 1024 counts a step, all loads of a
+// step in flight at once.  The whole workgroup calls it.
+template <class Pick, class Found>
+__device__ __forceinline__ uint64_t pick_pages(const uint32_t* refs, uint32_t from, uint32_t to, uint64_t want,
+                                               uint64_t* sh, Pick pick, Found found) {
+    __shared__ uint32_t cnt[kScan * kPlanWaves];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t have = 0;
+    for (uint64_t base = from; base < to && have < want; base += kScan * kPlanThreads) {
+        uint32_t r[kScan];
+#pragma unroll
+        for (uint32_t j = 0; j < kScan; j++) {
+            const uint64_t i = base + j * kPlanThreads + threadIdx.x;
+            r[j] = i < to ? refs[i] : 0;
+        }
+        uint64_t mask[kScan];
+#pragma unroll
+        for (uint32_t j = 0; j < kScan; j++) {
+            const uint64_t i = base + j * kPlanThreads + threadIdx.x;
+            mask[j] = __ballot(i < to && pick(r[j]));
+            if (lane == 0) cnt[j * kPlanWaves + wave] = __popcll(mask[j]);
+        }
+        __syncthreads();
+        // counts in page order: step j, then wave
+        const uint32_t mine = threadIdx.x < kScan * kPlanWaves ? cnt[threadIdx.x] : 0;
+        uint64_t all;
+        const uint64_t before = block_scan(mine, sh, &all);
+        if (threadIdx.x < kScan * kPlanWaves) cnt[threadIdx.x] = (uint32_t)before;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < kScan; j++) {
+            const uint64_t rank = have + cnt[j * kPlanWaves + wave] + __popcll(mask[j] & ((1ull << lane) - 1));
+            if ((mask[j] >> lane & 1) && rank < want)
+                found(rank, (uint32_t)(base + j * kPlanThreads + threadIdx.x));
+        }
+        have += all;
+        __syncthreads();
+    }
+    return have;
+}
+
+struct PagesWs {
+    uint32_t *list, *movers, *map;  // [n_pages] each
+    uint32_t* claim;                // [n_seqs]
+    uint32_t *req_len, *req_page;   // [kMaxRequests]
+    uint32_t* count;                // [1]
+};
+
+size_t pages_layout(const ane_paged_cache* c, void* base, PagesWs* w) {
+    size_t off = 0;
+    auto take = [&](uint64_t words) {
+        const size_t o = off;
+        off += ceil_to(words * 4, 256);
+        return base ? reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(base) + o) : nullptr;
+    };
+    PagesWs p;
+    p.list = take(c->n_pages);
+    p.movers = take(c->n_pages);
+    p.map = take(c->n_pages);
+    p.claim = take(c->n_seqs);
+    p.req_len = take(kMaxRequests);
+    p.req_page = take(kMaxRequests);
+    p.count = take(1);
+    if (w) *w = p;
+    return off;
+}
+
+// claim[seq] = the first request i with ok(i) that names it.
+template <class Seq>
+__device__ __forceinline__ void claim_first(uint32_t n, uint32_t* claim, Seq seq) {
+    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
+        const uint32_t s = seq(i);
+        if (s != ANE_NO_PAGE) claim[s] = ANE_NO_PAGE;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
+        const uint32_t s = seq(i);
+        if (s != ANE_NO_PAGE) atomicMin(&claim[s], i);
+    }
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(kPlanThreads)
+k_pages_reserve(ane_paged_cache c, uint32_t n, const uint32_t* seqs, const uint32_t* new_len, uint32_t* served,
+                PagesWs w) {
+    __shared__ uint64_t sh[kPlanWaves];
+    const uint64_t cap = (uint64_t)c.max_pages * c.page_size;
+    auto seq = [&](uint32_t i) {
+        const uint32_t s = seqs[i];
+        return s < c.n_seqs && new_len[i] <= cap ? s : ANE_NO_PAGE;
+    };
+    claim_first(n, w.claim, seq);
+    // pages request i asks for (0 where it is refused) and the first new entry of its row
+    auto need = [&](uint32_t i, bool& ok, uint32_t& s, uint32_t& at) {
+        s = seq(i);
+        ok = s != ANE_NO_PAGE && __atomic_load_n(&w.claim[s], __ATOMIC_RELAXED) == i;
+        if (!ok) return 0u;
+        at = (uint32_t)((min((uint64_t)c.kv_len[s], cap) + c.page_size - 1) / c.page_size);
+        const uint32_t to = (uint32_t)(((uint64_t)new_len[i] + c.page_size - 1) / c.page_size);
+        return to > at ? to - at : 0u;
+    };
+    uint64_t total = 0;
+    for (uint32_t base = 0; base < n; base += kPlanThreads) {
+        const uint32_t i = base + threadIdx.x;
+        bool ok = false;
+        uint32_t s, at;
+        uint64_t all;
+        block_scan(i < n ? need(i, ok, s, at) : 0, sh, &all);
+        total += all;
+    }
+    const uint64_t want = min(total, (uint64_t)c.n_pages);
+    const uint64_t have = pick_pages(c.page_refs, 0, c.n_pages, want, sh, [](uint32_t r) { return r == 0; },
+                                     [&](uint64_t rank, uint32_t i) { w.list[rank] = i; });
+    __syncthreads();
+    uint64_t before = 0;
+    for (uint32_t base = 0; base < n; base += kPlanThreads) {
+        const uint32_t i = base + threadIdx.x;
+        bool ok = false;
+        uint32_t s = 0, at = 0;
+        uint64_t all;
+        const uint32_t k = i < n ? need(i, ok, s, at) : 0;
+        const uint64_t r0 = before + block_scan(k, sh, &all);
+        before += all;
+        const bool fits = ok && r0 + k <= have;
+        if (i < n && served) served[i] = fits;
+        if (fits) {
+            for (uint32_t j = 0; j < k; j++) {
+                const uint32_t p = w.list[r0 + j];
+                c.page_table[(uint64_t)s * c.max_pages + at + j] = p;
+                c.page_refs[p] = 1;
+            }
+            if (new_len[i] > c.kv_len[s]) c.kv_len[s] = new_len[i];
+        }
+    }
+}
+
+// Which forks are served: the length each dst takes (0: none) and its fresh page.
+__global__ void __launch_bounds__(kPlanThreads)
+k_pages_fork_plan(ane_paged_cache c, uint32_t n, const uint32_t* src, const uint32_t* dst, uint32_t* served, PagesWs w) {
+    __shared__ uint64_t sh[kPlanWaves];
+    const uint64_t cap = (uint64_t)c.max_pages * c.page_size;
+    auto to = [&](uint32_t i) {
+        const uint32_t a = src[i], b = dst[i];
+        return a < c.n_seqs && b < c.n_seqs && a != b && c.kv_len[b] == 0 ? b : ANE_NO_PAGE;
+    };
+    claim_first(n, w.claim, to);
+    uint64_t total = 0;
+    for (uint32_t base = 0; base < n; base += kPlanThreads) {
+        const uint32_t i = base + threadIdx.x;
+        uint32_t part = 0;
+        if (i < n) {
+            const uint32_t b = to(i);
+            const bool ok = b != ANE_NO_PAGE && __atomic_load_n(&w.claim[b], __ATOMIC_RELAXED) == i;
+            const uint32_t len = ok ? (uint32_t)min((uint64_t)c.kv_len[src[i]], cap) : 0;
+            part = ok && len % c.page_size != 0;
+            w.req_len[i] = len;
+            w.req_page[i] = ok;  // for the second pass: whether it is valid
+        }
+        uint64_t all;
+        block_scan(part, sh, &all);
+        total += all;
+    }
+    const uint64_t have = pick_pages(c.page_refs, 0, c.n_pages, total, sh, [](uint32_t r) { return r == 0; },
+                                     [&](uint64_t rank, uint32_t i) { w.list[rank] = i; });
+    __syncthreads();
+    uint64_t before = 0;
+    for (uint32_t base = 0; base < n; base += kPlanThreads) {
+        const uint32_t i = base + threadIdx.x;
+        const bool ok = i < n && w.req_page[i];
+        const uint32_t len = ok ? w.req_len[i] : 0, part = len % c.page_size != 0;
+        uint64_t all;
+        const uint64_t r0 = before + block_scan(part, sh, &all);
+        before += all;
+        if (i < n) {
+            const bool fits = ok && r0 + part <= have;
+            if (served) served[i] = fits;
+            w.req_len[i] = fits ? len : 0;
+            w.req_page[i] = fits && part ? w.list[r0] : ANE_NO_PAGE;
+        }
+    }
+}
+
+// One workgroup per fork and slice of its work: slice 0 writes the row, the
+// counts and the length; the used rows of the part page are copied by all
+// slices, one wave per (layer, K or V, kv head).  src rows are never written
+// here: a src with positions is no dst.
+__global__ void __launch_bounds__(256)
+k_pages_fork(ane_paged_cache c, const uint32_t* src, const uint32_t* dst, PagesWs w) {
+    const uint32_t i = blockIdx.x, len = w.req_len[i];
+    if (len == 0) return;
+    const uint32_t whole = len / c.page_size, part = len % c.page_size, fresh = w.req_page[i];
+    const uint32_t* from = c.page_table + (uint64_t)src[i] * c.max_pages;
+    if (blockIdx.y == 0) {
+        uint32_t* row = c.page_table + (uint64_t)dst[i] * c.max_pages;
+        for (uint32_t j = threadIdx.x; j < whole + (part ? 1 : 0); j += 256) {
+            const uint32_t p = j < whole ? from[j] : fresh;
+            row[j] = p;
+            if (p < c.n_pages) atomicAdd(&c.page_refs[p], 1u);
+        }
+        if (threadIdx.x == 0) c.kv_len[dst[i]] = len;
+    }
+    if (!part) return;
+    const uint32_t old = from[whole];
+    if (old >= c.n_pages || fresh >= c.n_pages) return;
+    const uint32_t lane = threadIdx.x & 63, hv = c.head_dim / 8;  // 16-byte vectors a row
+    const uint32_t jobs = c.n_layers * 2 * c.n_kv_heads, vecs = part * hv;
+    for (uint32_t j = blockIdx.y * 4 + (threadIdx.x >> 6); j < jobs; j += gridDim.y * 4) {
+        const uint32_t g = j % c.n_kv_heads, kv = j / c.n_kv_heads % 2, l = j / c.n_kv_heads / 2;
+        uint4* pool = reinterpret_cast<uint4*>(kv ? c.v_pages : c.k_pages);
+        const uint64_t head = (uint64_t)c.page_size * hv, base = (uint64_t)l * c.n_pages * c.n_kv_heads;
+        const uint4* a = pool + (base + (uint64_t)old * c.n_kv_heads + g) * head;
+        uint4* b = pool + (base + (uint64_t)fresh * c.n_kv_heads + g) * head;
+        for (uint32_t e = lane; e < vecs; e += 256) {
+            uint4 t[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++)
+                if (e + k * 64 < vecs) t[k] = a[e + k * 64];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++)
+                if (e + k * 64 < vecs) b[e + k * 64] = t[k];
+        }
+    }
+}
+
+// One workgroup per request; of two that name a sequence the first to take its
+// length gives its pages up.
+__global__ void __launch_bounds__(256) k_pages_free(ane_paged_cache c, const uint32_t* seqs) {
+    __shared__ uint32_t len_sh;
+    const uint32_t s = seqs[blockIdx.x];
+    if (s >= c.n_seqs) return;
+    if (threadIdx.x == 0) len_sh = atomicExch(&c.kv_len[s], 0u);
+    __syncthreads();
+    const uint64_t len = min((uint64_t)len_sh, (uint64_t)c.max_pages * c.page_size);
+    const uint32_t pages = (uint32_t)((len + c.page_size - 1) / c.page_size);
+    uint32_t* row = c.page_table + (uint64_t)s * c.max_pages;
+    for (uint32_t j = threadIdx.x; j < pages; j += 256) {
+        const uint32_t p = row[j];
+        row[j] = ANE_NO_PAGE;
+        if (p < c.n_pages && atomicSub(&c.page_refs[p], 1u) == 0) atomicAdd(&c.page_refs[p], 1u);  // never below 0
+    }
+}
+
+// The moves of a compaction: the r-th live page at or past the live count into
+// the r-th free one before it; the counts and the numbers that follow.
+__global__ void __launch_bounds__(kPlanThreads)
+k_pages_compact_plan(ane_paged_cache c, uint32_t* refs_out, uint32_t* n_live, PagesWs w) {
+    __shared__ uint64_t sh[kPlanWaves];
+    const uint32_t* refs = c.page_refs;
+    auto live = [](uint32_t r) { return r != 0; };
+    const uint32_t n = (uint32_t)pick_pages(refs, 0, c.n_pages, ~0ull, sh, live, [](uint64_t, uint32_t) {});
+    const uint32_t holes = (uint32_t)pick_pages(refs, 0, n, ~0ull, sh, [](uint32_t r) { return r == 0; },
+                                                [&](uint64_t rank, uint32_t i) { w.list[rank] = i; });
+    // numbers at or past the live count: a live page's new one, another's own
+    for (uint64_t i = n + threadIdx.x; i < c.n_pages; i += kPlanThreads) w.map[i] = (uint32_t)i;
+    if (refs_out != refs)
+        for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) refs_out[i] = refs[i];
+    __syncthreads();
+    pick_pages(refs, n, c.n_pages, ~0ull, sh, live, [&](uint64_t rank, uint32_t i) {
+        const uint32_t to = w.list[rank];
+        w.movers[rank] = i;
+        w.map[i] = to;
+        refs_out[to] = refs[i];
+    });
+    for (uint64_t i = n + threadIdx.x; i < c.n_pages; i += kPlanThreads) refs_out[i] = 0;
+    if (threadIdx.x == 0) {
+        *w.count = holes;
+        if (n_live) *n_live = n;
+        w.count[1] = n;
+    }
+}
+
+// Page copies, 16 KB of a page a workgroup at a time; source and destination
+// pages are disjoint.  n: on the device for a compaction.
+constexpr uint32_t kCopyVecs = 1024;  // 16-byte vectors a step
+__device__ __forceinline__ void copy_pages(const ane_paged_cache& c, uint32_t n, const uint32_t* src, const uint32_t* dst) {
+    const uint64_t vecs = (uint64_t)c.n_kv_heads * c.page_size * (c.head_dim / 8);
+    const uint64_t steps = (vecs + kCopyVecs - 1) / kCopyVecs, jobs = (uint64_t)n * c.n_layers * 2 * steps;
+    for (uint64_t j = blockIdx.x; j < jobs; j += gridDim.x) {
+        const uint64_t st = j % steps, r = j / steps;
+        const uint32_t kv = r & 1, l = (uint32_t)(r / 2 % c.n_layers), i = (uint32_t)(r / 2 / c.n_layers);
+        const uint32_t a = src[i], b = dst[i];
+        if (a >= c.n_pages || b >= c.n_pages || a == b) continue;
+        uint4* pool = reinterpret_cast<uint4*>(kv ? c.v_pages : c.k_pages) + (uint64_t)l * c.n_pages * vecs;
+        const uint4* from = pool + a * vecs;
+        uint4* to = pool + b * vecs;
+        uint4 t[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint64_t e = st * kCopyVecs + k * 256 + threadIdx.x;
+            if (e < vecs) t[k] = from[e];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint64_t e = st * kCopyVecs + k * 256 + threadIdx.x;
+            if (e < vecs) to[e] = t[k];
+        }
+    }
+}
+__global__ void __launch_bounds__(256)
+k_pages_copy(ane_paged_cache c, uint32_t n, const uint32_t* src, const uint32_t* dst) {
+    copy_pages(c, n, src, dst);
+}
+__global__ void __launch_bounds__(256) k_pages_compact(ane_paged_cache c, uint32_t* table_out, PagesWs w) {
+    const uint32_t live = w.count[1];
+    const uint64_t entries = (uint64_t)c.n_seqs * c.max_pages;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < entries; i += gridDim.x * 256ull) {
+        const uint32_t p = c.page_table[i];
+        const uint32_t to = p >= live && p < c.n_pages ? w.map[p] : p;
+        if (to != p || table_out != c.page_table) table_out[i] = to;
+    }
+    copy_pages(c, *w.count, w.movers, w.list);
+}
+
+int pages_status(const ane_paged_cache* c, uint32_t n) {
+    const int st = cache_status(c);
+    if (st) return st;
+    if (!c->page_refs) return ANE_ERR_BAD_POINTER;
+    return n > kMaxRequests ? ANE_ERR_INVALID_ARG : ANE_OK;
+}
+bool bad_workspace(const void* ws, size_t bytes, size_t need) {
+    return need && (!ws || (((uintptr_t)ws) & 255) || bytes < need);
+}
+uint32_t copy_grid(uint64_t jobs) { return (uint32_t)(jobs < 4096 ? (jobs ? jobs : 1) : 4096); }
+
+}  // namespace
+}  // namespace ane
+
+using namespace ane;
+
+extern "C" int ane_hip_paged_rope_append(const ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
+                                         const uint32_t* q_start, uint32_t n_tokens, int in_type, const void* q,
+                                         uint64_t q_stride, const void* k, const void* v, uint64_t kv_stride,
+                                         const float* rope_table, uint32_t rope_len, int q_out_type, void* q_out,
+                                         uint64_t q_out_stride, void* stream) {
+    const int st = cache_status(cache);
+    if (st) return st;
+    if (layer >= cache->n_layers || n_tokens > kMaxTokens || (in_type != ANE_TYPE_F32 && in_type != ANE_TYPE_F16) ||
+        (q_out_type != ANE_TYPE_F32 && q_out_type != ANE_TYPE_F16) || (!q_start && n_tokens != n) ||
+        (rope_table && rope_len == 0))
+        return ANE_ERR_INVALID_ARG;
+    if (n == 0 || n_tokens == 0) return ANE_OK;
+    if (!k || !v || (!q != !q_out)) return ANE_ERR_BAD_POINTER;
+    const uint32_t isz = in_type == ANE_TYPE_F32 ? 4 : 2, osz = q_out_type == ANE_TYPE_F32 ? 4 : 2;
+    if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)q_out) | ((uintptr_t)rope_table)) & 15 ||
+        (kv_stride * isz) & 15 || kv_stride < (uint64_t)cache->n_kv_heads * cache->head_dim ||
+        (q && ((q_stride * isz) & 15 || (q_out_stride * osz) & 15 ||
+               q_stride < (uint64_t)cache->n_heads * cache->head_dim ||
+               q_out_stride < (uint64_t)cache->n_heads * cache->head_dim)))
+        return ANE_ERR_INVALID_ARG;
+    AppendArgs a;
+    const uint64_t lo = page_elems(cache) * cache->n_pages * layer;
+    a.q = q, a.k = k, a.v = v, a.q_out = q_out, a.rope = rope_table;
+    a.kp = cache->k_pages + lo, a.vp = cache->v_pages + lo;
+    a.table = cache->page_table, a.kv_len = cache->kv_len, a.seqs = seqs, a.q_start = q_start;
+    a.q_stride = q_stride, a.kv_stride = kv_stride, a.q_out_stride = q_out_stride;
+    a.n = n, a.n_tokens = n_tokens, a.rope_len = rope_len, a.n_heads = cache->n_heads, a.n_kv = cache->n_kv_heads;
+    a.hd = cache->head_dim, a.ps = cache->page_size, a.n_pages = cache->n_pages, a.max_pages = cache->max_pages;
+    a.n_seqs = cache->n_seqs;
+    auto* f = in_type == ANE_TYPE_F32
+                  ? (q_out_type == ANE_TYPE_F32 ? k_paged_append<float, float> : k_paged_append<float, _Float16>)
+                  : (q_out_type == ANE_TYPE_F32 ? k_paged_append<_Float16, float> : k_paged_append<_Float16, _Float16>);
+    hipLaunchKernelGGL(f, dim3(n_tokens), dim3(256), 0, (hipStream_t)stream, a);
+    ANE_HIP_CHECK_LAUNCH();
+    return ANE_OK;
+}
+
+extern "C" size_t ane_hip_pages_workspace_size(const ane_paged_cache* cache) {
+    return cache_status(cache) ? 0 : pages_layout(cache, nullptr, nullptr);
+}
+
+extern "C" int ane_hip_pages_reserve(const ane_paged_cache* cache, uint32_t n, const uint32_t* seqs,
+                                     const uint32_t* new_len, uint32_t* served, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+    const int st = pages_status(cache, n);
+    if (st || n == 0) return st;
+    if (!seqs || !new_len) return ANE_ERR_BAD_POINTER;
+    if (bad_workspace(workspace, workspace_bytes, pages_layout(cache, nullptr, nullptr))) return ANE_ERR_WORKSPACE;
+    PagesWs w;
+    pages_layout(cache, workspace, &w);
+    hipLaunchKernelGGL(k_pages_reserve, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, *cache, n, seqs, new_len,
+                       served, w);
+    ANE_HIP_CHECK_LAUNCH();
+    return ANE_OK;
+}
+
+extern "C" int ane_hip_pages_fork(const ane_paged_cache* cache, uint32_t n, const uint32_t* src, const uint32_t* dst,
+                                  uint32_t* served, void* workspace, size_t workspace_bytes, void* stream) {
+    const int st = pages_status(cache, n);
+    if (st || n == 0) return st;
+    if (!src || !dst) return ANE_ERR_BAD_POINTER;
+    if (bad_workspace(workspace, workspace_bytes, pages_layout(cache, nullptr, nullptr))) return ANE_ERR_WORKSPACE;
+    PagesWs w;
+    pages_layout(cache, workspace, &w);
+    hipStream_t s = (hipStream_t)stream;
+    hipLaunchKernelGGL(k_pages_fork_plan, dim3(1), dim3(kPlanThreads), 0, s, *cache, n, src, dst, served, w);
+    // four waves a workgroup, one (layer, K or V, kv head) a wave; at most 4096 workgroups more than the forks
+    const uint64_t jobs = ((uint64_t)cache->n_layers * 2 * cache->n_kv_heads + 3) / 4, room = 4096 / n + 1;
+    hipLaunchKernelGGL(k_pages_fork, dim3(n, (uint32_t)(jobs < room ? jobs : room)), dim3(256), 0, s, *cache, src, dst, w);
+    ANE_HIP_CHECK_LAUNCH();
+    return ANE_OK;
+}
+
+extern "C" int ane_hip_pages_free(const ane_paged_cache* cache, uint32_t n, const uint32_t* seqs, void* stream) {
+    const int st = pages_status(cache, n);
+    if (st || n == 0) return st;
+    if (!seqs) return ANE_ERR_BAD_POINTER;
+    hipLaunchKernelGGL(k_pages_free, dim3(n), dim3(256), 0, (hipStream_t)stream, *cache, seqs);
+    ANE_HIP_CHECK_LAUNCH();
+    return ANE_OK;
+}
+
+extern "C" int ane_hip_pages_copy(const ane_paged_cache* cache, uint32_t n, const uint32_t* src, const uint32_t* dst,
+                                  void* stream) {
+    const int st = pages_status(cache, n);
+    if (st || n == 0) return st;
+    if (!src || !dst) return ANE_ERR_BAD_POINTER;
+    const uint64_t steps = (page_elems(cache) / 8 + kCopyVecs - 1) / kCopyVecs;
+    hipLaunchKernelGGL(k_pages_copy, dim3(copy_grid(steps * 2 * cache->n_layers * n)), dim3(256), 0, (hipStream_t)stream,
+                       *cache, n, src, dst);
+    ANE_HIP_CHECK_LAUNCH();
+    return ANE_OK;
+}
+
+extern "C" int ane_hip_pages_compact(const ane_paged_cache* cache, uint32_t* page_table_out, uint32_t* page_refs_out,
+                                     uint32_t* n_live, void* workspace, size_t workspace_bytes, void* stream) {
+    const int st = pages_status(cache, 0);
+    if (st) return st;
+    if (bad_workspace(workspace, workspace_bytes, pages_layout(cache, nullptr, nullptr))) return ANE_ERR_WORKSPACE;
+    PagesWs w;
+    pages_layout(cache, workspace, &w);
+    hipStream_t s = (hipStream_t)stream;
+    hipLaunchKernelGGL(k_pages_compact_plan, dim3(1), dim3(kPlanThreads), 0, s, *cache,
+                       page_refs_out ? page_refs_out : cache->page_refs, n_live, w);
+    const uint64_t steps = (page_elems(cache) / 8 + kCopyVecs - 1) / kCopyVecs;
+    hipLaunchKernelGGL(k_pages_compact, dim3(copy_grid(steps * 2 * cache->n_layers * (uint64_t)cache->n_pages)), dim3(256),
+                       0, s, *cache, page_table_out ? page_table_out : cache->page_table, w);
+    ANE_HIP_CHECK_LAUNCH();
+    return ANE_OK;
+}

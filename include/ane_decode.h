@@ -193,6 +193,146 @@ int ane_decode_token_ggml(const struct ane_decode_config* cfg, const struct ane_
                           const float* rope_table, float rope_theta, uint32_t pos, float* x, void* workspace,
                           size_t workspace_bytes, struct ane_ggml_backend* backend, int arith);
 
+/* ------------------------------------------------ paged cache, batches
+ *
+ * Several sequences on one K/V cache whose positions live in pages, so that
+ * sequences grow without reserving ctx positions each and can share the pages
+ * of a common prefix.  No counterpart in the reference.
+ *
+ * Sequence s holds positions 0 .. kv_len[s]-1; position p is row p % page_size
+ * of page page_table[s][p / page_size].  Entries of the table past the
+ * sequence's pages hold ANE_NO_PAGE.  page_refs[i] counts the table entries
+ * that name page i; 0 means the page is free.  Every array is device memory
+ * and is read when the kernels run, so a captured call follows the lengths and
+ * tables of its replay.
+ *
+ * A page number outside the pool reads as zeros and is never written, and a
+ * length past max_pages * page_size counts as that many positions: a broken
+ * table gives wrong results, never an access outside the pool.  All calls are
+ * asynchronous on stream; pointers must belong to the current device. */
+#define ANE_NO_PAGE 0xffffffffu
+
+/* Element types of activations (ggml's numbers). */
+#define ANE_TYPE_F32 0
+#define ANE_TYPE_F16 1
+
+struct ane_paged_cache {
+    uint32_t n_layers;
+    uint32_t n_heads;     /* query heads: a multiple of n_kv_heads, at most 128 each */
+    uint32_t n_kv_heads;
+    uint32_t head_dim;    /* 64 or 128 */
+    uint32_t page_size;   /* positions a page: a multiple of 16, at most 2^20 */
+    uint32_t n_pages;     /* pages in the pool, below 2^31 */
+    uint32_t n_seqs;      /* rows of page_table */
+    uint32_t max_pages;   /* entries a row; max_pages * page_size below 2^31 */
+    uint16_t* k_pages;    /* fp16 [n_layers][n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned */
+    uint16_t* v_pages;    /* the same shape */
+    uint32_t* page_table; /* [n_seqs][max_pages] */
+    uint32_t* kv_len;     /* [n_seqs] */
+    uint32_t* page_refs;  /* [n_pages]; NULL where only attention or append is called */
+};
+
+/* The batched calls below take n sequences: row i of the batch is sequence
+ * seqs[i] of the cache (seqs NULL: sequence i; a number outside the cache is a
+ * sequence without positions).  Packed rows: the new tokens of batch row i are
+ * rows q_start[i] .. q_start[i+1]-1 of the activations (ascending, q_start[n]
+ * <= n_tokens), its last positions: token t of m sits at kv_len - m + t.
+ * q_start NULL: one new token a row.  Rows from q_start[n] on are left as they
+ * were.  At most 2^23 tokens a call.  Strides are in elements from one token
+ * to the next; a token's heads are contiguous.  q, k, v, q_out and out are
+ * 16-byte aligned and their strides multiples of 16 bytes. */
+
+/* RoPE of q and k (adjacent pairs, the fp32 operations of
+ * ane_hip_rope_kv_append) and the append of k and v, rounded to fp16, to the
+ * pages of one layer.  in_type: of q, k and v; q_out: the rotated q in
+ * q_out_type (may be q itself when the types and strides agree).  q and q_out
+ * NULL: k and v only.  rope_table NULL: no rotation; else fp32 [rope_len]
+ * [head_dim/2][2].  A token whose position is negative, past its sequence's
+ * pages or not below rope_len is not appended and its q_out row is zeros.
+ * kv_len counts the new tokens already (ane_hip_pages_reserve); appending to a
+ * page that two sequences hold changes both. */
+int ane_hip_paged_rope_append(const struct ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
+                              const uint32_t* q_start, uint32_t n_tokens, int in_type, const void* q,
+                              uint64_t q_stride, const void* k, const void* v, uint64_t kv_stride,
+                              const float* rope_table, uint32_t rope_len, int q_out_type, void* q_out,
+                              uint64_t q_out_stride, void* stream);
+
+/* Causal attention of packed prompts with grouped heads: for each new token at
+ * position p, out[h] = softmax(scale * q[h] . K[g][0..p]^T) V[g][0..p],
+ * g = h / (n_heads / n_kv_heads); zeros for a token at a negative position.
+ * Keys a token does not see never touch its result, whatever they hold.
+ * type: of q and out.  F32: products of fp32 accuracy (q and the softmax
+ * weights enter the matrix cores as two fp16 parts each); F16: q and the
+ * weights are fp16.  Scores, softmax and sums are fp32 in both.  scale: finite
+ * and positive.  max_len: a bound on the lengths, which sizes the workspace and
+ * the split of long rows (longer sequences are still computed whole); 0 stands
+ * for max_pages * page_size.  out may be q when the strides agree.  The
+ * workspace (256-byte aligned; NULL when its size is 0) belongs to the call
+ * until it has run. */
+size_t ane_hip_attention_prompt_workspace_size(const struct ane_paged_cache* cache, uint32_t n, uint32_t n_tokens,
+                                               uint32_t max_len);
+int ane_hip_attention_prompt(const struct ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
+                             const uint32_t* q_start, uint32_t n_tokens, uint32_t max_len, int type, const void* q,
+                             uint64_t q_stride, float scale, void* out, uint64_t out_stride, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* One new token of each of n sequences (row i of q and out), attending to
+ * positions 0 .. kv_len-1 of its sequence; zeros where there are none.
+ * With n_groups > 0, batch rows group_start[g] .. group_start[g+1]-1 (device,
+ * [n_groups+1], ascending) share their first prefix_len[g] positions (device,
+ * [n_groups]): those are read once for the whole group, out of the pages of
+ * its first row; rows outside every group share nothing.  A prefix longer than
+ * a row's or the first row's length counts as that length.  max_prefix and
+ * max_len bound the prefix lengths and the lengths as max_len does above. */
+size_t ane_hip_attention_shared_workspace_size(const struct ane_paged_cache* cache, uint32_t n, uint32_t n_groups,
+                                               uint32_t max_prefix, uint32_t max_len);
+int ane_hip_attention_shared(const struct ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
+                             uint32_t n_groups, const uint32_t* group_start, const uint32_t* prefix_len,
+                             uint32_t max_prefix, uint32_t max_len, int type, const void* q, uint64_t q_stride,
+                             float scale, void* out, uint64_t out_stride, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* Pages.  Requests are device arrays of n entries, at most 65536 a call;
+ * free pages are always taken lowest number first, so results do not depend
+ * on timing.  served (optional, [n]): 1 for a request carried out, else 0.
+ * Calls that change one cache must be ordered (one stream, or events).
+ * The workspace (ane_hip_pages_workspace_size bytes, 256-byte aligned) belongs
+ * to the call until it has run.
+ *
+ * reserve: sequence seqs[i] grows to new_len[i] positions (one that is that
+ * long already stays as it is).  One for an unknown sequence, past max_pages *
+ * page_size or for a sequence an earlier valid one names is refused; the others
+ * are served in order, up to the first whose pages the pool does not have: it
+ * and all later ones are refused.
+ * fork: sequence dst[i], which must be empty, becomes a copy of src[i]: it
+ * shares the whole pages and gets its own copy, in every layer, of the rows
+ * used in a last, part-filled one, so that appending to either sequence
+ * changes no other.  Served in order while the free pages last, as in
+ * reserve; refused where dst is unknown, not empty, src itself or named by an
+ * earlier valid request, or src is unknown.  A src that is another request's
+ * dst counts as empty, as it was.
+ * free: the sequences become empty and give their pages up (naming one twice
+ * is naming it once).
+ * copy: page dst[i] becomes a copy of page src[i] in every layer; a page
+ * number outside the pool is skipped.  No dst may occur twice or be a src.
+ * compact: the live pages move to the front of the pool (those at or past the
+ * live count go, in order, into the free ones before it); page_table_out,
+ * page_refs_out (NULL: the cache's own) get the table and counts that go with
+ * it, n_live (optional) the number of live pages.  With arrays of their own
+ * the cache's table and the moved pages stay readable as before until free
+ * pages are written. */
+size_t ane_hip_pages_workspace_size(const struct ane_paged_cache* cache);
+int ane_hip_pages_reserve(const struct ane_paged_cache* cache, uint32_t n, const uint32_t* seqs,
+                          const uint32_t* new_len, uint32_t* served, void* workspace, size_t workspace_bytes,
+                          void* stream);
+int ane_hip_pages_fork(const struct ane_paged_cache* cache, uint32_t n, const uint32_t* src, const uint32_t* dst,
+                       uint32_t* served, void* workspace, size_t workspace_bytes, void* stream);
+int ane_hip_pages_free(const struct ane_paged_cache* cache, uint32_t n, const uint32_t* seqs, void* stream);
+int ane_hip_pages_copy(const struct ane_paged_cache* cache, uint32_t n, const uint32_t* src, const uint32_t* dst,
+                       void* stream);
+int ane_hip_pages_compact(const struct ane_paged_cache* cache, uint32_t* page_table_out, uint32_t* page_refs_out,
+                          uint32_t* n_live, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
