@@ -81,6 +81,13 @@ struct Work {
     uint32_t id, tok0, toks, row0, rows;  // first token, tokens, first row of the tile, rows in all
     int32_t kbeg, kend, lo;               // lo: keys before it are masked (kbeg rounds it down to 16)
     int32_t len;
+
+    // Every lane holds the same values; the compiler has to be told, or each
+    // copy to LDS loops over its lanes' descriptors.
+    __device__ __forceinline__ void uniform() {
+        for (uint32_t* x : {&id, &tok0, &toks, &row0, &rows}) *x = __builtin_amdgcn_readfirstlane(*x);
+        for (int32_t* x : {&kbeg, &kend, &lo, &len}) *x = __builtin_amdgcn_readfirstlane(*x);
+    }
 };
 
 template <int MODE, int BM>
@@ -168,6 +175,7 @@ struct Loader {
         const uint32_t p = page(a, u);
         ids = (int32_t)u * 16 < w.kend && u < (1u << 27) && p < a.max_pages
                   ? a.table[(uint64_t)w.id * a.max_pages + p] : ANE_NO_PAGE;
+        asm volatile("" : "+v"(ids));  // the wait for it here, not before each copy that follows
     }
     // group u (wave-uniform), whose page number is in lane `from`, of kv head g
     __device__ __forceinline__ void copy(const AttnArgs& a, const Work& w, uint32_t g, uint32_t u, uint32_t from,
@@ -175,7 +183,8 @@ struct Loader {
         const uint32_t id = __builtin_amdgcn_readlane(ids, from);
         const uint32_t row = u * 16 - page(a, u) * a.ps;
         const int32_t left = w.kend - (int32_t)(u * 16);
-        const uint32_t bytes = id < a.n_pages ? (uint32_t)min(max(left, 0), 16) * RB : 0;
+        // (a clamp goes through the vector ALU: back to a scalar, as above)
+        const uint32_t bytes = __builtin_amdgcn_readfirstlane(id < a.n_pages ? (uint32_t)min(max(left, 0), 16) * RB : 0);
         const uint64_t at = (((uint64_t)(id < a.n_pages ? id : 0) * a.n_kv + g) * a.ps + row) * HD;
         const __amdgpu_buffer_rsrc_t rk = make_rsrc(a.kp + at, bytes), rv = make_rsrc(a.vp + at, bytes);
 #pragma unroll
@@ -199,6 +208,13 @@ __device__ __forceinline__ h8 as_h8(v4i x) {
     return r;
 }
 
+// The transposing read.  Its pointer is restrict for the alias information that
+// leaves on the read once inlined: without any, the compiler waits for every
+// copy to LDS in flight first.
+__device__ __forceinline__ s4 read_tr(const uint8_t* __restrict__ p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
+}
+
 // The running maximum may lag by kLag (in log2) before O and l are rescaled;
 // weights are e^s 2^kLift relative to it, at most 2^(kLag + kLift) = 2^14, so that
 // fp16 keeps weights 2^-20 of the largest with full precision.
@@ -210,7 +226,7 @@ template <int HD, bool F32>
 struct Rows {
     static constexpr int NS = HD / 16, ND = HD / 32;
     static constexpr uint32_t RB = HD * 2;
-    h8 qh[NS], ql[F32 ? NS : 1];
+    h8 qh[NS], ql[F32 ? NS : 1];  // q, its low part
     f16v o[ND];
     float m, l, c;  // maximum (log2, lagging), this half's sum, score factor
     int32_t lim;    // keys below it are seen
@@ -229,10 +245,6 @@ struct Rows {
                 const uint32_t hi = HD == 128 ? d ^ (i >> 2) : d ^ (i >> 3);
                 va[j * ND + d] = (4 * half + 8 * j + (i >> 2)) * RB + (((hi << 2) | (low ^ (half + 2 * j))) << 4) + (i & 1) * 8;
             }
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
         m = -INFINITY, l = 0.0f, c = scale_log2e;
         lim = live ? limit : 0;
         wmin = live ? limit : 0x7fffffff, wmax = lim;
@@ -247,11 +259,15 @@ struct Rows {
     __device__ __forceinline__ void load_q(const void* q, uint64_t at, bool live) {
         if constexpr (!F32) {
 #pragma unroll
+            for (int e = 0; e < 8; e++) ql[0][e] = (_Float16)0.0f;
+#pragma unroll
             for (int s = 0; s < NS; s++) {
                 v4i x = {0, 0, 0, 0};
                 if (live) x = *reinterpret_cast<const v4i*>(static_cast<const _Float16*>(q) + at + 16 * s + 8 * half);
                 qh[s] = as_h8(x);
             }
+#pragma unroll
+            for (int s = 0; s < NS; s++) asm volatile("" : "+v"(qh[s]));  // the wait for q here, not in the loop
         } else {
             float4 x[NS][2];
             uint32_t top = 0;
@@ -281,28 +297,47 @@ struct Rows {
                 }
         }
     }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    }
     __device__ __forceinline__ v4i vfrag(const uint8_t* v, int s, int d) const {
-        const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(v + va[d] + s * 16 * RB));
-        const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(v + va[ND + d] + s * 16 * RB));
+        const s4 a = read_tr(v + va[d] + s * 16 * RB);
+        const s4 b = read_tr(v + va[ND + d] + s * 16 * RB);
         v4i r;
         __builtin_memcpy(&r, &a, 8);
         __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &b, 8);
         return r;
     }
-    // KT blocks of 32 keys from position t0 on; keys before lo are masked
+    // KT blocks of 32 keys from position t0 on; keys before lo are masked.
     template <int KT>
     __device__ __forceinline__ void step(const uint8_t* k, const uint8_t* v, int32_t t0, int32_t lo) {
+        // Fragments are read kAhead products before their use and the order is
+        // pinned: left alone, the scheduler reads all of them first and spills.
+        constexpr int kAhead = 4;
         f16v s[KT];
         const uint32_t kx = swz<HD>(ka & 15);
+        auto kfrag = [&](int i) {  // products in the order (e, t)
+            const int e = i / KT, t = i % KT;
+            return as_h8(*reinterpret_cast<const v4i*>(k + (t * 32 + ka) * RB + (((2 * e + half) ^ kx) << 4)));
+        };
+        {
+            h8 kf[kAhead];
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
+            for (int i = 0; i < kAhead; i++) kf[i] = kfrag(i);
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[t][r] = 0.0f;
+            for (int t = 0; t < KT; t++)
 #pragma unroll
-            for (int e = 0; e < NS; e++) {
-                const h8 kf = as_h8(*reinterpret_cast<const v4i*>(k + (t * 32 + ka) * RB + (((2 * e + half) ^ kx) << 4)));
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[e], s[t], 0, 0, 0);
-                if constexpr (F32) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[e], s[t], 0, 0, 0);
+                for (int r = 0; r < 16; r++) s[t][r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NS * KT; i++) {
+                const int e = i / KT, t = i % KT;
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], qh[e], s[t], 0, 0, 0);
+                if constexpr (F32) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], ql[e], s[t], 0, 0, 0);
+                if (i + kAhead < NS * KT) kf[i % kAhead] = kfrag(i + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         const bool masked = t0 + 32 * KT > wmin || t0 < lo;  // uniform
@@ -350,70 +385,69 @@ struct Rows {
                     pl[2 * t + r / 8][r % 8 + 1] = lw.y;
                 }
             }
-        if (masked) {
-            // A value a row does not see has weight 0, and 0 times an infinity
-            // or NaN would be NaN: such tiles take a second form.
-            uint32_t bad = 0;
+        h8 vf[kAhead];
 #pragma unroll
-            for (int e = 0; e < 2 * KT; e++)
+        for (int i = 0; i < kAhead; i++) vf[i] = as_h8(vfrag(v, i / ND, i % ND));
 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const v4i x = vfrag(v, e, d);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) bad |= (((uint32_t)x[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                }
-            if (__any(bad != 0)) {
-                nonfinite<KT>(v, ph, pl, t0, lo);
-                return;
-            }
+        for (int i = 0; i < 2 * KT * ND; i++) {
+            const int e = i / ND, d = i % ND;
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % kAhead], ph[e], o[d], 0, 0, 0);
+            if constexpr (F32) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % kAhead], pl[e], o[d], 0, 0, 0);
+            if (i + kAhead < 2 * KT * ND) vf[i % kAhead] = as_h8(vfrag(v, (i + kAhead) / ND, (i + kAhead) % ND));
+            __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int e = 0; e < 2 * KT; e++)
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                const h8 vf = as_h8(vfrag(v, e, d));
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[e], o[d], 0, 0, 0);
-                if constexpr (F32) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[e], o[d], 0, 0, 0);
-            }
     }
-    // The values' product where some value is not finite: the finite ones as
-    // above, and what the seen others make of each sum from a second product of
-    // marks (1 for +inf, 128 for -inf, 16384 for NaN: at most 64 keys, so the three
-    // counts stay apart) with 1 for each key the row sees.
-    template <int KT, class PL>
-    __device__ __forceinline__ void nonfinite(const uint8_t* v, const h8 (&ph)[2 * KT], const PL& pl, int32_t t0, int32_t lo) {
+    // Values that are not finite and that a row sees, added to its sums (whatever
+    // their weight): keys [from, to).  tidy() took them out of the products.
+    __device__ __forceinline__ void add_nonfinite(const AttnArgs& a, const Work& w, uint32_t g, int32_t from, int32_t to) {
+#pragma unroll 1
+        for (int32_t key = max(from, w.lo); key < min(to, w.kend); key++) {
+            const uint32_t p = (uint32_t)((uint64_t)((uint32_t)key / 16) * a.div_magic >> a.div_shift);
+            const uint32_t id = p < a.max_pages ? a.table[(uint64_t)w.id * a.max_pages + p] : ANE_NO_PAGE;
+            if (id >= a.n_pages) continue;
+            const uint16_t* v = a.vp + (((uint64_t)id * a.n_kv + g) * a.ps + (uint32_t)key - p * a.ps) * HD + 4 * half;
+            const bool sees = key < lim;
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            f16v marks;
+            for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) marks[r] = 0.0f;
+                for (int e = 0; e < 4; e++) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(v + d * 32 + 8 * e);
+                    const uint32_t y[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
 #pragma unroll
-            for (int e = 0; e < 2 * KT; e++) {
-                const h8 x = as_h8(vfrag(v, e, d));
-                h8 fin, mark, sees;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float f = (float)x[j];
-                    const bool nan = f != f, inf = fabsf(f) == INFINITY;
-                    fin[j] = nan || inf ? (_Float16)0.0f : x[j];
-                    mark[j] = (_Float16)(nan ? 16384.0f : inf ? (f > 0.0f ? 1.0f : 128.0f) : 0.0f);
-                    const int32_t key = t0 + 16 * e + 8 * (j / 4) + 4 * (int32_t)half + j % 4;
-                    sees[j] = (_Float16)(key < lim && key >= lo ? 1.0f : 0.0f);
+                    for (int i = 0; i < 4; i++)
+                        o[d][4 * e + i] += sees && (y[i] & 0x7c00u) == 0x7c00u ? half_bits_to_float(y[i]) : 0.0f;
                 }
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fin, ph[e], o[d], 0, 0, 0);
-                if constexpr (F32) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fin, pl[e], o[d], 0, 0, 0);
-                marks = __builtin_amdgcn_mfma_f32_32x32x16_f16(mark, sees, marks, 0, 0, 0);
-            }
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int32_t k = (int32_t)marks[r];
-                if (k & 127) o[d][r] += INFINITY;
-                if ((k >> 7) & 127) o[d][r] -= INFINITY;
-                if (k >> 14) o[d][r] = NAN;
-            }
         }
     }
 };
+
+// A masked tile's values that are not finite are taken out of LDS (a value that a
+// row does not see has weight 0 there, and 0 times an infinity or NaN would be
+// NaN) and added to the rows that see them at the end.  One wave does 16 rows of
+// V; true: there were some.
+template <int HD>
+__device__ __forceinline__ bool tidy(uint8_t* v) {
+    v4i* p = reinterpret_cast<v4i*>(v) + (threadIdx.x & 63);
+    uint32_t bad = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < HD / 32; i++) {
+        const v4i x = p[i * 64];
+#pragma unroll
+        for (int k = 0; k < 4; k++) bad |= ((uint32_t)x[k] & 0x7c007c00u) + 0x04000400u;  // bit 15 of a half: exponent all ones
+    }
+    if (!__any((bad & 0x80008000u) != 0)) return false;
+#pragma unroll 1
+    for (uint32_t i = 0; i < HD / 32; i++) {
+        v4i x = p[i * 64];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t e = (((uint32_t)x[k] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+            x[k] &= ~(int)((e >> 15) * 0xffffu);
+        }
+        p[i * 64] = x;
+    }
+    return true;
+}
 
 template <bool F32>
 __device__ __forceinline__ void put4(void* out, uint64_t at, float4 x) {
@@ -435,12 +469,19 @@ __device__ __forceinline__ uint32_t block_wave() { return __builtin_amdgcn_readf
 template <int HD, bool F32, int MODE>
 __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slots) {
     constexpr uint32_t kT = 64 * HD * 2;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kT];  // K, V of each stage
+    // K, V of each stage, then one word a wave: its rows' least limit, and whether
+    // its group of a tile of each parity holds a value that is not finite.  One
+    // array on purpose: with several, the compiler tells LDS accesses apart, and
+    // then waits for all copies in flight before it reads what they may alias.
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kT + 48];
+    int32_t* least = reinterpret_cast<int32_t*>(smem + 4 * kT);
+    int32_t *odd = least + 4, odd_from = 0x7fffffff, odd_to = 0;
     const uint32_t wave = block_wave(), lane = threadIdx.x & 63, g = blockIdx.x % a.n_kv;
     // a causal prompt's last tiles have the most keys: they start first
     const uint32_t slot = slots - 1 - blockIdx.x / a.n_kv, part = blockIdx.y;
     Work w;
     if (!find_work<MODE, 128>(a, slot, part, w)) return;
+    w.uniform();
 
     Loader<HD> ld;
     ld.init();
@@ -457,17 +498,37 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
     const bool live = row < w.rows;
     r.init(a.scale_log2e, live ? row_limit<MODE>(a, w, tok) : 0, live);
     r.load_q(a.q, live ? (w.tok0 + tok) * a.q_stride + head * HD : 0, live);
+    __builtin_amdgcn_sched_barrier(0);
+    r.clear();
 
+    if (lane == 0) least[wave] = r.wmin;
+    wait_lgkmcnt0();
+    lds_barrier();
+    const int32_t wg_min = min(min(least[0], least[1]), min(least[2], least[3]));
     if (w.kend > w.kbeg)
         for (uint32_t t = 0; t < tiles; t++) {
-            wait_vmcnt<0>();   // this wave's copies of tile t
-            wait_lgkmcnt0();   // and its reads of tile t - 1
-            lds_barrier();     // everybody's
-            if (t + 1 < tiles) issue(t + 1);
             const int32_t t0 = w.kbeg + (int32_t)t * 64;
             const uint8_t* st = smem + (t & 1) * 2 * kT;
-            if (t0 < r.wmax) r.template step<2>(st, st + kT, t0, w.lo);
+            const bool masked = t0 + 64 > wg_min || t0 < w.lo;
+            wait_vmcnt<0>();  // this wave's copies of tile t
+            int32_t* flag = odd + (t & 1) * 4;
+            if (masked) {
+                const bool bad = tidy<HD>(smem + (t & 1) * 2 * kT + kT + wave * (kT / 4));
+                if (lane == 0) flag[wave] = bad;
+            }
+            wait_lgkmcnt0();  // and its reads of tile t - 1
+            lds_barrier();    // everybody's
+            if (t + 1 < tiles) issue(t + 1);
+            if (masked && __builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3]))
+                odd_from = min(odd_from, t0), odd_to = t0 + 64;
+            if constexpr (F32) {  // 32 keys at a time: the two parts of q and of 64 weights do not fit 256 registers
+                if (t0 < r.wmax) r.template step<1>(st, st + kT, t0, w.lo);
+                if (t0 + 32 < r.wmax) r.template step<1>(st + kT / 2, st + kT + kT / 2, t0 + 32, w.lo);
+            } else {
+                if (t0 < r.wmax) r.template step<2>(st, st + kT, t0, w.lo);
+            }
         }
+    if (odd_from < odd_to) r.add_nonfinite(a, w, g, odd_from, odd_to);
 
     if (!live) return;
     const float l = other_sum(r.l);
@@ -496,20 +557,24 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
 // fourth block of 32 keys each, on rings of their own (no barrier until the
 // end), and are merged through LDS.
 template <int HD, bool F32, int MODE>
-__global__ void __launch_bounds__(256, 1) k_attn_few(AttnArgs a) {
+__global__ void __launch_bounds__(256, 2) k_attn_few(AttnArgs a) {
     constexpr uint32_t kT = 32 * HD * 2, kPad = HD + 4;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[16 * kT];  // per wave: K, V of two stages
-    __shared__ float sm[4][32], sl[4][32];
-    static_assert(4 * 32 * kPad * 4 <= sizeof(smem), "the merge reuses the rings");
+    // per wave: K, V of two stages; one array, as above, which the merge reuses
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[16 * kT];
+    float* oo = reinterpret_cast<float*>(smem);
+    float *sm = oo + 4 * 32 * kPad, *sl = sm + 128;
+    static_assert((4 * 32 * kPad + 256) * 4 <= sizeof(smem), "the merge fits the rings");
     const uint32_t wave = block_wave(), lane = threadIdx.x & 63, g = blockIdx.x % a.n_kv, part = blockIdx.y;
     Work w;
     if (!find_work<MODE, 32>(a, blockIdx.x / a.n_kv, part, w)) return;
+    w.uniform();
 
     Loader<HD> ld;
     ld.init();
     const int32_t first = w.kbeg + (int32_t)wave * 32;
     const uint32_t u0 = (uint32_t)first / 16, tiles = w.kend > first ? (uint32_t)(w.kend - first + 127) / 128 : 0;
     uint8_t* ring = smem + wave * 4 * kT;
+    int32_t odd_from = 0x7fffffff, odd_to = 0;
     auto issue = [&](uint32_t t) {
         if ((t & 31) == 0) ld.lookup(a, w, u0 + (t + lane / 2) * 8 + (lane & 1));
         uint8_t* st = ring + (t & 1) * 2 * kT;
@@ -524,6 +589,8 @@ __global__ void __launch_bounds__(256, 1) k_attn_few(AttnArgs a) {
     const bool live = row < w.rows;
     r.init(a.scale_log2e, live ? row_limit<MODE>(a, w, tok) : 0, live);
     r.load_q(a.q, live ? (w.tok0 + tok) * a.q_stride + head * HD : 0, live);
+    __builtin_amdgcn_sched_barrier(0);
+    r.clear();
 
     for (uint32_t t = 0; t < tiles; t++) {
         if (t + 1 < tiles) {
@@ -534,16 +601,21 @@ __global__ void __launch_bounds__(256, 1) k_attn_few(AttnArgs a) {
             wait_vmcnt<0>();
         }
         const int32_t t0 = first + (int32_t)t * 128;
-        const uint8_t* st = ring + (t & 1) * 2 * kT;
+        uint8_t* st = ring + (t & 1) * 2 * kT;
+        if (t0 + 32 > r.wmin || t0 < w.lo) {
+            const bool b0 = tidy<HD>(st + kT), b1 = tidy<HD>(st + kT + kT / 2);
+            if (b0 || b1) odd_from = min(odd_from, t0), odd_to = t0 + 32;
+        }
         if (t0 < r.wmax) r.template step<1>(st, st + kT, t0, w.lo);
     }
+    // (this wave's keys of that range only: the other waves add their own)
+    for (int32_t t0 = odd_from; t0 < odd_to; t0 += 128) r.add_nonfinite(a, w, g, t0, t0 + 32);
 
     // merge the four waves: rows of HD + 4 floats keep 16-byte stores of
     // neighbouring rows on different banks
     const float l = other_sum(r.l);
     __syncthreads();
-    float* oo = reinterpret_cast<float*>(smem);
-    if (r.half == 0) sm[wave][lane] = r.m, sl[wave][lane] = l;
+    if (r.half == 0) sm[wave * 32 + lane] = r.m, sl[wave * 32 + lane] = l;
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
 #pragma unroll
@@ -554,15 +626,16 @@ __global__ void __launch_bounds__(256, 1) k_attn_few(AttnArgs a) {
     const uint32_t rows = min(w.rows - w.row0, 32u);
     for (uint32_t e = threadIdx.x; e < rows * (HD / 4); e += 256) {
         const uint32_t i = e / (HD / 4), d = e % (HD / 4) * 4;
-        const float M = fmaxf(fmaxf(sm[0][i], sm[1][i]), fmaxf(sm[2][i], sm[3][i]));
+        const float M = fmaxf(fmaxf(sm[i], sm[32 + i]), fmaxf(sm[64 + i], sm[96 + i]));
         float L = 0.0f;
         float4 x = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (sm[k][i] == -INFINITY && sl[k][i] == 0.0f) continue;  // no key of this row
-            const float f = __builtin_amdgcn_exp2f(sm[k][i] - M);
+            const float m = sm[k * 32 + i], l1 = sl[k * 32 + i];
+            if (m == -INFINITY && l1 == 0.0f) continue;  // no key of this row
+            const float f = __builtin_amdgcn_exp2f(m - M);
             const float4 y = *reinterpret_cast<const float4*>(oo + (k * 32 + i) * kPad + d);
-            L = __builtin_fmaf(sl[k][i], f, L);
+            L = __builtin_fmaf(l1, f, L);
             x.x = __builtin_fmaf(y.x, f, x.x), x.y = __builtin_fmaf(y.y, f, x.y);
             x.z = __builtin_fmaf(y.z, f, x.z), x.w = __builtin_fmaf(y.w, f, x.w);
         }
