@@ -1028,6 +1028,16 @@ class PagedCache(ctypes.Structure):
         self.kv_len, self.page_refs = kv_len, page_refs
         super().__init__(n_layers, n_heads, n_kv, head_dim, page_size, n_pages, page_table.shape[0],
                          page_table.shape[1], _p(k_pages), _p(v_pages), _p(page_table), _p(kv_len), _p(page_refs))
+        # what every call asks for, as plain attributes (a field or a tensor's
+        # property costs several times as much to read)
+        self._at = ctypes.addressof(self)
+        self._q, self._kv = (n_heads, head_dim), (n_kv, head_dim)
+        self._scale = head_dim ** -0.5
+        self._device = k_pages.device.index if k_pages.device.type == "cuda" else None
+        self._types = {torch.float32: 0, torch.float16: 1}
+        self._int32 = torch.int32
+        self._cuda = torch.cuda
+        self._pages_need = None
 
     @classmethod
     def empty(cls, n_layers, n_heads, n_kv_heads, head_dim, page_size, n_pages, n_seqs, max_pages, device="cuda"):
@@ -1041,62 +1051,62 @@ class PagedCache(ctypes.Structure):
         return cls(n_heads, k, v, table, kv_len, refs)
 
 
-def _type_of(t, what):
-    import torch
-
-    if t.dtype == torch.float32:
-        return 0
-    if t.dtype == torch.float16:
-        return 1
-    raise ValueError(f"{what} is float32 or float16")
-
-
-def _rows(t, heads, cache, what):
-    """Row stride of activations [tokens][heads][head_dim] whose heads are contiguous."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != cache.head_dim:
-        raise ValueError(f"{what} is [tokens][{heads}][{cache.head_dim}]")
-    if t.shape[0] and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != cache.head_dim)):
+def _rows(t, width, cache, what):
+    """(pointer, type, tokens, row stride) of activations [tokens][heads][head_dim] whose heads are contiguous."""
+    tokens, *rest = t.shape
+    if tuple(rest) != width:
+        raise ValueError(f"{what} is [tokens][{width[0]}][{width[1]}]")
+    ty = cache._types.get(t.dtype)
+    if ty is None:
+        raise ValueError(f"{what} is float32 or float16")
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 or (s1 != width[1] and width[0] > 1)) and tokens:
         raise ValueError(f"the heads of a token of {what} are contiguous")
-    return t.stride(0) if t.shape[0] > 1 else heads * cache.head_dim
+    return t.data_ptr(), ty, tokens, s0 if tokens > 1 else width[0] * width[1]
 
 
-def _ints(t, n, what):
-    """A device array of at least n int32, or None."""
-    import torch
-
+def _ints(t, n, cache, what):
+    """The pointer of a device array of at least n int32, or None."""
     if t is None:
-        return 0
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n:
+        return None
+    if t.dtype != cache._int32 or not t.is_contiguous() or t.numel() < n:
         raise ValueError(f"{what} is a contiguous int32 tensor of {n} entries")
-    return _p(t)
+    return t.data_ptr()
 
 
-class _On:
-    """The cache's device as the current one during a call, and the call's stream there."""
+def _launch(fn, cache, what, stream, args):
+    """fn(*args, stream) on the cache's device and, unless given, its current stream."""
+    if cache._device is None or cache._device == cache._cuda.current_device():
+        st = fn(*args, _stream_on(cache, stream))
+    else:
+        with cache._cuda.device(cache._device):
+            st = fn(*args, _stream_on(cache, stream))
+    if st:
+        check(st, what)
 
-    def __init__(self, cache, stream):
+
+def _stream_on(cache, stream):
+    if stream is None and cache._device is not None:
         import torch
 
-        dev = cache.k_pages.device
-        self.guard = None if dev.type != "cuda" or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-        self.stream = stream
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return _stream_handle(self.stream)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+        return torch._C._cuda_getCurrentRawStream(cache._device)
+    return _stream_handle(stream)
 
 
-def _batch(q_start, seqs, rows):
+def _batch(q_start, seqs, rows, cache):
     """(n, q_start pointer, seqs pointer) of a packed batch of `rows` tokens."""
     n = rows if q_start is None else q_start.numel() - 1
     if n < 0:
         raise ValueError("q_start has an entry more than the batch has rows")
-    return n, _ints(q_start, n + 1, "q_start"), _ints(seqs, n, "seqs")
+    return n, _ints(q_start, n + 1, cache, "q_start"), _ints(seqs, n, cache, "seqs")
+
+
+def _work(cache, workspace, need, stream):
+    """(workspace, pointer, bytes): the caller's, or a temporary one of need() bytes (the tensor has to
+    live until the call is queued)."""
+    if workspace is None:
+        workspace = _scratch(need(), cache.k_pages.device, stream)
+    return workspace, workspace.data_ptr(), workspace.nbytes
 
 
 def paged_rope_append(cache, layer, q_start, q, k, v, table, q_out, seqs=None, stream=None):
@@ -1105,32 +1115,40 @@ def paged_rope_append(cache, layer, q_start, q, k, v, table, q_out, seqs=None, s
     tokens of batch row i in rows q_start[i] .. q_start[i+1]-1 (None: one each);
     q_out takes the rotated q; q and q_out None: k and v only; table None: no
     rotation."""
-    n, qs, sq = _batch(q_start, seqs, k.shape[0])
-    ks = _rows(k, cache.n_kv_heads, cache, "k")
-    if _rows(v, cache.n_kv_heads, cache, "v") != ks or v.shape != k.shape or v.dtype != k.dtype:
+    kp, ty, tokens, ks = _rows(k, cache._kv, cache, "k")
+    vp, tv, nv, vs = _rows(v, cache._kv, cache, "v")
+    if (ty, tokens, ks) != (tv, nv, vs):
         raise ValueError("k and v have the same shape, strides and type")
-    if (q is None) != (q_out is None) or (q is not None and (q.dtype != k.dtype or q.shape[0] != k.shape[0]
-                                                              or q_out.shape[0] < q.shape[0])):
-        raise ValueError("q and q_out go together, q with the tokens and type of k")
-    if table is not None and (str(table.dtype) != "torch.float32" or not table.is_contiguous()
-                              or table.numel() != table.shape[0] * cache.head_dim):
-        raise ValueError("table is a contiguous float32 [positions][head_dim/2][2]")
-    with _On(cache, stream) as st:
-        check(lib().ane_hip_paged_rope_append(
-            ctypes.byref(cache), layer, sq, n, qs, k.shape[0], _type_of(k, "k"), _p(q),
-            0 if q is None else _rows(q, cache.n_heads, cache, "q"), _p(k), _p(v), ks, _p(table),
-            0 if table is None else table.shape[0], 0 if q is None else _type_of(q_out, "q_out"), _p(q_out),
-            0 if q is None else _rows(q_out, cache.n_heads, cache, "q_out"), st), "paged_rope_append")
+    n, qs, sq = _batch(q_start, seqs, tokens, cache)
+    qp = op = None
+    q0 = o0 = to = 0
+    if q is not None and q_out is not None:
+        qp, tq, nq, q0 = _rows(q, cache._q, cache, "q")
+        op, to, no, o0 = _rows(q_out, cache._q, cache, "q_out")
+        if tq != ty or nq != tokens or no < tokens:
+            raise ValueError("q has the tokens and type of k, q_out room for them")
+    elif q is not None or q_out is not None:
+        raise ValueError("q and q_out go together")
+    tp, positions = None, 0
+    if table is not None:
+        positions = table.shape[0]
+        if cache._types.get(table.dtype) != 0 or not table.is_contiguous() or table.numel() != positions * cache._q[1]:
+            raise ValueError("table is a contiguous float32 [positions][head_dim/2][2]")
+        tp = table.data_ptr()
+    _launch(lib().ane_hip_paged_rope_append, cache, "paged_rope_append", stream,
+            (cache._at, layer, sq, n, qs, tokens, ty, qp, q0, kp, vp, ks, tp, positions, to, op, o0))
 
 
 def _attention_rows(cache, q, out):
-    if out.shape != q.shape or out.dtype != q.dtype:
+    qp, ty, tokens, q0 = _rows(q, cache._q, cache, "q")
+    op, to, no, o0 = _rows(out, cache._q, cache, "out")
+    if (ty, tokens) != (to, no):
         raise ValueError("out has the shape and type of q")
-    return _type_of(q, "q"), _rows(q, cache.n_heads, cache, "q"), _rows(out, cache.n_heads, cache, "out")
+    return ty, tokens, qp, q0, op, o0
 
 
 def attention_prompt_workspace_size(cache, n, n_tokens, max_len=None) -> int:
-    return int(lib().ane_hip_attention_prompt_workspace_size(ctypes.byref(cache), n, n_tokens, max_len or 0))
+    return int(lib().ane_hip_attention_prompt_workspace_size(cache._at, n, n_tokens, max_len or 0))
 
 
 def attention_prompt_workspace(cache, n, n_tokens, max_len=None):
@@ -1144,20 +1162,17 @@ def attention_prompt(cache, layer, q_start, q, out, max_len=None, scale=None, se
     (its sequence's last positions, already appended) in rows q_start[i] ..
     q_start[i+1]-1.  max_len bounds the sequences' lengths; scale None:
     1/sqrt(head_dim)."""
-    n, qs, sq = _batch(q_start, seqs, q.shape[0])
-    ty, s0, s1 = _attention_rows(cache, q, out)
-    with _On(cache, stream) as st:
-        need = attention_prompt_workspace_size(cache, n, q.shape[0], max_len)
-        ws = workspace if workspace is not None else _scratch(need, q.device, stream) if need else None
-        check(lib().ane_hip_attention_prompt(
-            ctypes.byref(cache), layer, sq, n, qs, q.shape[0], max_len or 0, ty, _p(q), s0,
-            cache.head_dim ** -0.5 if scale is None else scale, _p(out), s1, _p(ws),
-            0 if ws is None else ws.numel() * ws.element_size(), st), "attention_prompt")
+    ty, tokens, qp, q0, op, o0 = _attention_rows(cache, q, out)
+    n, qs, sq = _batch(q_start, seqs, tokens, cache)
+    workspace, wp, size = _work(cache, workspace,
+                                lambda: attention_prompt_workspace_size(cache, n, tokens, max_len), stream)
+    _launch(lib().ane_hip_attention_prompt, cache, "attention_prompt", stream,
+            (cache._at, layer, sq, n, qs, tokens, max_len or 0, ty, qp, q0, cache._scale if scale is None else scale, op,
+             o0, wp, size))
 
 
 def attention_shared_workspace_size(cache, n, n_groups=0, max_prefix=None, max_len=None) -> int:
-    return int(lib().ane_hip_attention_shared_workspace_size(ctypes.byref(cache), n, n_groups, max_prefix or 0,
-                                                             max_len or 0))
+    return int(lib().ane_hip_attention_shared_workspace_size(cache._at, n, n_groups, max_prefix or 0, max_len or 0))
 
 
 def attention_shared_workspace(cache, n, n_groups=0, max_prefix=None, max_len=None):
@@ -1171,73 +1186,65 @@ def attention_shared(cache, layer, q, out, max_len=None, group_start=None, prefi
     [heads][head_dim].  Rows group_start[g] .. group_start[g+1]-1 share their
     first prefix_len[g] positions, which are read once for the group;
     group_start None: no row shares anything."""
-    n = q.shape[0]
-    sq = _ints(seqs, n, "seqs")
+    ty, n, qp, q0, op, o0 = _attention_rows(cache, q, out)
+    sq = _ints(seqs, n, cache, "seqs")
     if (group_start is None) != (prefix_len is None):
         raise ValueError("group_start and prefix_len go together")
     groups = 0 if group_start is None else group_start.numel() - 1
-    gs, pl = _ints(group_start, groups + 1, "group_start"), _ints(prefix_len, groups, "prefix_len")
-    ty, s0, s1 = _attention_rows(cache, q, out)
-    with _On(cache, stream) as st:
-        need = attention_shared_workspace_size(cache, n, groups, max_prefix, max_len)
-        ws = workspace if workspace is not None else _scratch(need, q.device, stream) if need else None
-        check(lib().ane_hip_attention_shared(
-            ctypes.byref(cache), layer, sq, n, groups, gs, pl, max_prefix or 0, max_len or 0, ty, _p(q), s0,
-            cache.head_dim ** -0.5 if scale is None else scale, _p(out), s1, _p(ws),
-            0 if ws is None else ws.numel() * ws.element_size(), st), "attention_shared")
+    gs, pl = _ints(group_start, groups + 1, cache, "group_start"), _ints(prefix_len, groups, cache, "prefix_len")
+    workspace, wp, size = _work(
+        cache, workspace, lambda: attention_shared_workspace_size(cache, n, groups, max_prefix, max_len), stream)
+    _launch(lib().ane_hip_attention_shared, cache, "attention_shared", stream,
+            (cache._at, layer, sq, n, groups, gs, pl, max_prefix or 0, max_len or 0, ty, qp, q0,
+             cache._scale if scale is None else scale, op, o0, wp, size))
+
+
+def _pages_need(cache) -> int:
+    if cache._pages_need is None:
+        cache._pages_need = int(lib().ane_hip_pages_workspace_size(cache._at))
+    return cache._pages_need
 
 
 def pages_workspace(cache):
     """A workspace for the page calls on this cache."""
-    return _scratch(lib().ane_hip_pages_workspace_size(ctypes.byref(cache)), cache.k_pages.device)
-
-
-def _pages_ws(cache, workspace, stream):
-    need = int(lib().ane_hip_pages_workspace_size(ctypes.byref(cache)))
-    ws = workspace if workspace is not None else _scratch(need, cache.k_pages.device, stream)
-    return ws, ws.numel() * ws.element_size()
+    return _scratch(_pages_need(cache), cache.k_pages.device)
 
 
 def pages_reserve(cache, seqs, new_len, served=None, workspace=None, stream=None):
     """Sequences seqs[i] grow to new_len[i] positions (int32 device tensors);
     served[i]: 1 where the pool had the pages."""
     n = seqs.numel()
-    a, b, c = _ints(seqs, n, "seqs"), _ints(new_len, n, "new_len"), _ints(served, n, "served")
-    with _On(cache, stream) as st:
-        ws, size = _pages_ws(cache, workspace, stream)
-        check(lib().ane_hip_pages_reserve(ctypes.byref(cache), n, a, b, c, _p(ws), size, st), "pages_reserve")
+    a, b, c = (_ints(t, n, cache, w) for t, w in ((seqs, "seqs"), (new_len, "new_len"), (served, "served")))
+    workspace, wp, size = _work(cache, workspace, lambda: _pages_need(cache), stream)
+    _launch(lib().ane_hip_pages_reserve, cache, "pages_reserve", stream, (cache._at, n, a, b, c, wp, size))
 
 
 def pages_fork(cache, src, dst, served=None, workspace=None, stream=None):
     """Empty sequences dst[i] become copies of src[i] that share their whole pages."""
     n = src.numel()
-    a, b, c = _ints(src, n, "src"), _ints(dst, n, "dst"), _ints(served, n, "served")
-    with _On(cache, stream) as st:
-        ws, size = _pages_ws(cache, workspace, stream)
-        check(lib().ane_hip_pages_fork(ctypes.byref(cache), n, a, b, c, _p(ws), size, st), "pages_fork")
+    a, b, c = (_ints(t, n, cache, w) for t, w in ((src, "src"), (dst, "dst"), (served, "served")))
+    workspace, wp, size = _work(cache, workspace, lambda: _pages_need(cache), stream)
+    _launch(lib().ane_hip_pages_fork, cache, "pages_fork", stream, (cache._at, n, a, b, c, wp, size))
 
 
 def pages_free(cache, seqs, stream=None):
     """The sequences become empty and give their pages up."""
-    with _On(cache, stream) as st:
-        check(lib().ane_hip_pages_free(ctypes.byref(cache), seqs.numel(), _ints(seqs, seqs.numel(), "seqs"), st),
-              "pages_free")
+    n = seqs.numel()
+    _launch(lib().ane_hip_pages_free, cache, "pages_free", stream, (cache._at, n, _ints(seqs, n, cache, "seqs")))
 
 
 def pages_copy(cache, src, dst, stream=None):
     """Pages dst[i] become copies of pages src[i] in every layer."""
     n = src.numel()
-    with _On(cache, stream) as st:
-        check(lib().ane_hip_pages_copy(ctypes.byref(cache), n, _ints(src, n, "src"), _ints(dst, n, "dst"), st),
-              "pages_copy")
+    _launch(lib().ane_hip_pages_copy, cache, "pages_copy", stream,
+            (cache._at, n, _ints(src, n, cache, "src"), _ints(dst, n, cache, "dst")))
 
 
 def pages_compact(cache, table_out=None, refs_out=None, n_live=None, workspace=None, stream=None):
     """The live pages move to the front of the pool; the new table and counts go
     to table_out and refs_out (None: the cache's own), the number of live pages
     to n_live."""
-    t = _ints(table_out, cache.n_seqs * cache.max_pages, "table_out")
-    r, l = _ints(refs_out, cache.n_pages, "refs_out"), _ints(n_live, 1, "n_live")
-    with _On(cache, stream) as st:
-        ws, size = _pages_ws(cache, workspace, stream)
-        check(lib().ane_hip_pages_compact(ctypes.byref(cache), t, r, l, _p(ws), size, st), "pages_compact")
+    t = _ints(table_out, cache.page_table.numel(), cache, "table_out")
+    r, l = _ints(refs_out, cache.k_pages.shape[1], cache, "refs_out"), _ints(n_live, 1, cache, "n_live")
+    workspace, wp, size = _work(cache, workspace, lambda: _pages_need(cache), stream)
+    _launch(lib().ane_hip_pages_compact, cache, "pages_compact", stream, (cache._at, t, r, l, wp, size))

@@ -46,9 +46,14 @@ struct AttnArgs {
     uint64_t q_stride, out_stride;
     uint32_t n, n_tokens, n_groups, n_heads, n_kv, G, ps, n_pages, max_pages, n_seqs;
     uint32_t div_magic, div_shift;                // 16-position group -> page, see page_div
-    uint32_t chunk, part0, n_parts, parts_total;  // keys a part, this launch's parts
-    uint32_t chunk_prefix, n_parts_prefix;        // of the prefix launch, for the merge
+    struct Parts {
+        uint32_t chunk, n, first;  // keys a part, parts, number of the first
+    } own, pre;                    // of a row's own keys (all of a prompt's), of the shared prefix
+    uint32_t parts_total;
     float scale_log2e;
+
+    template <int MODE>
+    __device__ __forceinline__ const Parts& parts() const { return MODE == kPrefix ? pre : own; }
 };
 
 // u / (ps / 16) for u < 2^27 as (u * magic) >> shift: with shift = 27 +
@@ -62,76 +67,109 @@ void page_div(uint32_t ps, uint32_t* magic, uint32_t* shift) {
     *magic = (uint32_t)(((1ull << *shift) + d - 1) / d);
 }
 
+// No branches: a load in flight next to the others costs less than its test.
 __device__ __forceinline__ uint32_t seq_id(const AttnArgs& a, uint32_t s) { return a.seqs ? a.seqs[s] : s; }
 __device__ __forceinline__ uint32_t seq_len(const AttnArgs& a, uint32_t id) {
-    return id < a.n_seqs ? (uint32_t)min((uint64_t)a.kv_len[id], (uint64_t)a.max_pages * a.ps) : 0;
+    const uint32_t len = a.kv_len[min(id, a.n_seqs - 1)];
+    return id < a.n_seqs ? (uint32_t)min((uint64_t)len, (uint64_t)a.max_pages * a.ps) : 0;
 }
-// The positions batch row s shares with its group (0: none).
-__device__ __forceinline__ uint32_t shared_len(const AttnArgs& a, uint32_t s, uint32_t len) {
-    if (a.n_groups == 0) return 0;
-    const uint32_t g = wave_search(a.n_groups, s, [&](uint32_t i) { return (uint64_t)a.group_start[i]; });
-    const uint32_t first = a.group_start[g];
-    if (first > s || s >= a.group_start[g + 1]) return 0;
-    return min(min(a.prefix[g], len), seq_len(a, seq_id(a, first)));
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, uint32_t lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ uint32_t last_lane(bool yes) {  // the last lane that says yes, 0 if none
+    const uint64_t m = __ballot(yes);
+    return m ? 63 - (uint32_t)__builtin_clzll(m) : 0;
 }
 
 // What a workgroup computes: BM rows of one kv head of one batch row (of one
-// group in kPrefix), keys [kbeg, kend) from the pages of sequence id.
+// group in kPrefix), keys [kbeg, kend) from the pages of sequence id.  All of it
+// is wave-uniform and goes through v_readfirstlane: the compiler has to be told,
+// or each copy to LDS loops over its lanes' (equal) descriptors.
 struct Work {
-    uint32_t id, tok0, toks, row0, rows;  // first token, tokens, first row of the tile, rows in all
-    int32_t kbeg, kend, lo;               // lo: keys before it are masked (kbeg rounds it down to 16)
-    int32_t len;
-
-    // Every lane holds the same values; the compiler has to be told, or each
-    // copy to LDS loops over its lanes' descriptors.
-    __device__ __forceinline__ void uniform() {
-        for (uint32_t* x : {&id, &tok0, &toks, &row0, &rows}) *x = __builtin_amdgcn_readfirstlane(*x);
-        for (int32_t* x : {&kbeg, &kend, &lo, &len}) *x = __builtin_amdgcn_readfirstlane(*x);
-    }
+    uint32_t s, id, tok0, toks, row0, rows;  // batch row or group, sequence, first token, tokens, first row, rows in all
+    int32_t kbeg, kend, lo, len;             // lo: keys before it are masked (kbeg rounds it down to 16)
+    bool alone;                              // kOwn: no group has the row
 };
 
+__device__ __forceinline__ void uniform(uint32_t& x) { x = __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ void uniform(int32_t& x) { x = __builtin_amdgcn_readfirstlane(x); }
+
+// The rows of slot `slot`.  Row tiles of batch row s are slots start[s] * G / BM
+// + s onwards (floor), which never overlap; what is left between is empty.
 template <int MODE, int BM>
-__device__ __forceinline__ bool find_work(const AttnArgs& a, uint32_t slot, uint32_t part, Work& w) {
+__device__ __forceinline__ bool find_rows(const AttnArgs& a, uint32_t slot, Work& w) {
     const uint32_t* start = MODE == kPrefix ? a.group_start : MODE == kPrompt ? a.q_start : nullptr;
-    const uint32_t n = MODE == kPrefix ? a.n_groups : a.n;
-    uint32_t s, tile;
-    if (start) {  // tiles of row s: slots start[s] * G / BM + s onwards, which never overlap
-        auto key = [&](uint32_t i) { return (uint64_t)start[i] * a.G / BM + i; };
-        s = wave_search(n, slot, key);
-        if (key(s) > slot) return false;
-        tile = slot - (uint32_t)key(s);
-        w.tok0 = start[s];
-        const uint32_t end = min(start[s + 1], a.n_tokens);
-        w.toks = end > w.tok0 ? end - w.tok0 : 0;
+    const uint32_t n = MODE == kPrefix ? a.n_groups : a.n, lane = threadIdx.x & 63;
+    uint32_t tile, first, end;
+    if (start) {
+        auto key = [&](uint32_t from, uint32_t i) { return (uint64_t)from * a.G / BM + i; };
+        uint32_t base = 0;  // the 64 entries from `base` hold the row
+        if (n > 63) {
+            base = wave_search(n, slot, [&](uint32_t i) { return key(start[i], i); });
+            base = base > 31 ? base - 31 : 0;
+        }
+        const uint32_t v = start[min(base + lane, n)];
+        const uint32_t l = last_lane(base + lane < n && key(v, base + lane) <= slot);
+        w.s = base + l, first = lane_of(v, l), end = min(lane_of(v, l + 1), a.n_tokens);
+        const uint64_t k = key(first, w.s);
+        if (k > slot) return false;
+        tile = slot - (uint32_t)k;
     } else {
         const uint32_t tiles = (a.G + BM - 1) / BM;
-        s = slot / tiles, tile = slot % tiles;
-        if (s >= n) return false;
-        w.tok0 = s, w.toks = 1;
+        w.s = slot / tiles, tile = slot % tiles;
+        if (w.s >= n) return false;
+        first = w.s, end = w.s + 1;
     }
+    w.tok0 = first, w.toks = end > first ? end - first : 0;
     w.rows = w.toks * a.G;  // below 2^30
     w.row0 = tile * BM;
     if (tile >= (1u << 24) || w.row0 >= w.rows) return false;
-    w.id = seq_id(a, MODE == kPrefix ? w.tok0 : s);
+    w.id = seq_id(a, MODE == kPrefix ? w.tok0 : w.s);
+    uniform(w.s), uniform(w.id), uniform(w.tok0), uniform(w.toks), uniform(w.row0), uniform(w.rows);
+    return true;
+}
+
+// The positions batch row s shares with its group; alone: it is in none.
+__device__ __forceinline__ uint32_t shared_len(const AttnArgs& a, uint32_t s, uint32_t len, bool& alone) {
+    alone = true;
+    if (a.n_groups == 0) return 0;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t base = 0;
+    if (a.n_groups > 63) {
+        base = wave_search(a.n_groups, s, [&](uint32_t i) { return (uint64_t)a.group_start[i]; });
+        base = base > 31 ? base - 31 : 0;
+    }
+    const uint32_t v = a.group_start[min(base + lane, a.n_groups)], p = a.prefix[min(base + lane, a.n_groups - 1)];
+    const uint32_t l = last_lane(base + lane < a.n_groups && v <= s), first = lane_of(v, l);
+    if (first > s || s >= lane_of(v, l + 1)) return 0;
+    alone = false;
+    return min(min(lane_of(p, l), len), seq_len(a, seq_id(a, first)));
+}
+
+// The keys of part `part`; at: its first position, where the work has any.
+template <int MODE>
+__device__ __forceinline__ void find_keys(const AttnArgs& a, uint32_t bm, uint32_t part, Work& w) {
     w.len = (int32_t)seq_len(a, w.id);
     w.kbeg = w.lo = 0;
     w.kend = w.len;
+    w.alone = true;
     if (MODE == kPrompt) {
-        const int32_t last = (int32_t)((min(w.row0 + BM, w.rows) - 1) / a.G);
+        const int32_t last = (int32_t)((min(w.row0 + bm, w.rows) - 1) / a.G);
         w.kend = min(w.len, w.len - (int32_t)w.toks + last + 1);
     } else if (MODE == kPrefix) {
-        w.kend = (int32_t)min(a.prefix[s], (uint32_t)w.len);
+        w.kend = (int32_t)min(a.prefix[w.s], (uint32_t)w.len);
     } else {
-        w.lo = (int32_t)shared_len(a, s, (uint32_t)w.len);
+        w.lo = (int32_t)shared_len(a, w.s, (uint32_t)w.len, w.alone);
         w.kbeg = w.lo & ~15;
         if (w.lo >= w.kend) w.kend = w.kbeg;
     }
-    const int64_t b = w.kbeg + (int64_t)part * a.chunk;
-    if (b >= w.kend && a.parts_total > 1) return false;  // the merge does not read it
-    if (part + 1 < a.n_parts) w.kend = (int32_t)min((int64_t)w.kend, b + a.chunk);
+    const int64_t b = w.kbeg + (int64_t)part * a.parts<MODE>().chunk;
+    if (part + 1 < a.parts<MODE>().n) w.kend = (int32_t)min((int64_t)w.kend, b + a.parts<MODE>().chunk);
     w.kbeg = (int32_t)min(b, (int64_t)max(w.kend, 0));
-    return true;
+    uniform(w.kbeg), uniform(w.kend), uniform(w.lo), uniform(w.len);
 }
+// Whether the first key's position is known before any length is.
+template <int MODE>
+__device__ __forceinline__ bool early_keys(const AttnArgs& a) { return MODE != kOwn || a.n_groups == 0; }
+
 // Keys of the work a row (token t of the work's) sees: those below.
 template <int MODE>
 __device__ __forceinline__ int32_t row_limit(const AttnArgs& a, const Work& w, uint32_t t) {
@@ -171,26 +209,29 @@ struct Loader {
         return (uint32_t)((uint64_t)u * a.div_magic >> a.div_shift);
     }
     // u: this lane's 16-position group
-    __device__ __forceinline__ void lookup(const AttnArgs& a, const Work& w, uint32_t u) {
-        const uint32_t p = page(a, u);
-        ids = (int32_t)u * 16 < w.kend && u < (1u << 27) && p < a.max_pages
-                  ? a.table[(uint64_t)w.id * a.max_pages + p] : ANE_NO_PAGE;
-        asm volatile("" : "+v"(ids));  // the wait for it here, not before each copy that follows
+    __device__ __forceinline__ void lookup(const AttnArgs& a, uint32_t id, uint32_t u) {
+        const uint32_t p = min(page(a, min(u, (1u << 27) - 1)), a.max_pages - 1);
+        ids = a.table[(uint64_t)min(id, a.n_seqs - 1) * a.max_pages + p];
     }
-    // group u (wave-uniform), whose page number is in lane `from`, of kv head g
-    __device__ __forceinline__ void copy(const AttnArgs& a, const Work& w, uint32_t g, uint32_t u, uint32_t from,
-                                         uint8_t* k, uint8_t* v) const {
+    // the wait for the numbers here, not before each copy that follows
+    __device__ __forceinline__ void settle() { asm volatile("" : "+v"(ids)); }
+    // 16 rows of x from group u (wave-uniform) on, whose page number is in lane `from`, of kv head g
+    // (nt: of keys no other workgroup reads)
+    template <bool NT = false>
+    __device__ __forceinline__ void copy(const AttnArgs& a, const uint16_t* x, const Work& w, uint32_t g, uint32_t u,
+                                         uint32_t from, uint8_t* dst) const {
         const uint32_t id = __builtin_amdgcn_readlane(ids, from);
         const uint32_t row = u * 16 - page(a, u) * a.ps;
         const int32_t left = w.kend - (int32_t)(u * 16);
         // (a clamp goes through the vector ALU: back to a scalar, as above)
         const uint32_t bytes = __builtin_amdgcn_readfirstlane(id < a.n_pages ? (uint32_t)min(max(left, 0), 16) * RB : 0);
         const uint64_t at = (((uint64_t)(id < a.n_pages ? id : 0) * a.n_kv + g) * a.ps + row) * HD;
-        const __amdgpu_buffer_rsrc_t rk = make_rsrc(a.kp + at, bytes), rv = make_rsrc(a.vp + at, bytes);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(x + at, bytes);
 #pragma unroll
-        for (uint32_t i = 0; i < kCopies; i++) copy16_to_lds(rk, k + i * 1024, off[i]);
-#pragma unroll
-        for (uint32_t i = 0; i < kCopies; i++) copy16_to_lds(rv, v + i * 1024, off[i]);
+        for (uint32_t i = 0; i < kCopies; i++) {
+            if constexpr (NT) copy16_to_lds_nt(r, dst + i * 1024, off[i]);
+            else copy16_to_lds(r, dst + i * 1024, off[i]);
+        }
     }
 };
 
@@ -256,29 +297,40 @@ struct Rows {
         wmin = __builtin_amdgcn_readfirstlane(wmin);
         wmax = __builtin_amdgcn_readfirstlane(wmax);
     }
-    __device__ __forceinline__ void load_q(const void* q, uint64_t at, bool live) {
+    struct Raw {  // a row of q on its way
+        v4i x[NS * (F32 ? 2 : 1)];
+    };
+    __device__ __forceinline__ void fetch_q(const void* q, uint64_t at, bool live, Raw& w) const {
+        const uint32_t h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            if constexpr (F32) {
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    w.x[2 * s + e] = *reinterpret_cast<const v4i*>(static_cast<const float*>(q) + at + 16 * s + 8 * h + 4 * e);
+            } else {
+                w.x[s] = *reinterpret_cast<const v4i*>(static_cast<const _Float16*>(q) + at + 16 * s + 8 * h);
+            }
+        }
+        if (!live)
+#pragma unroll
+            for (auto& x : w.x) x = v4i{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ void take_q(const Raw& w) {
         if constexpr (!F32) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) ql[0][e] = (_Float16)0.0f;
-#pragma unroll
             for (int s = 0; s < NS; s++) {
-                v4i x = {0, 0, 0, 0};
-                if (live) x = *reinterpret_cast<const v4i*>(static_cast<const _Float16*>(q) + at + 16 * s + 8 * half);
-                qh[s] = as_h8(x);
+                qh[s] = as_h8(w.x[s]);
+                asm volatile("" : "+v"(qh[s]));  // the wait for q here, not in the loop
             }
 #pragma unroll
-            for (int s = 0; s < NS; s++) asm volatile("" : "+v"(qh[s]));  // the wait for q here, not in the loop
+            for (int e = 0; e < 8; e++) ql[0][e] = (_Float16)0.0f;
         } else {
-            float4 x[NS][2];
             uint32_t top = 0;
 #pragma unroll
-            for (int s = 0; s < NS; s++)
+            for (int s = 0; s < 2 * NS; s++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    x[s][e] = live ? *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + 16 * s + 8 * half + 4 * e)
-                                   : make_float4(0, 0, 0, 0);
-                    top = max(max(top, abs_key(x[s][e].x)), max(abs_key(x[s][e].y), max(abs_key(x[s][e].z), abs_key(x[s][e].w))));
-                }
+                for (int k = 0; k < 4; k++) top = max(top, (uint32_t)w.x[s][k] & 0x7fffffffu);
             top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
             // 2^(140 - ex) brings the largest |q| (exponent field ex) to [2^13, 2^14)
             const uint32_t ex = max(top >> 23, 20u);
@@ -287,13 +339,10 @@ struct Rows {
 #pragma unroll
             for (int s = 0; s < NS; s++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const float v[4] = {x[s][e].x * up, x[s][e].y * up, x[s][e].z * up, x[s][e].w * up};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        qh[s][4 * e + k] = (_Float16)v[k];
-                        ql[s][4 * e + k] = (_Float16)(v[k] - (float)qh[s][4 * e + k]);
-                    }
+                for (int k = 0; k < 8; k++) {
+                    const float v = __int_as_float(w.x[2 * s + k / 4][k % 4]) * up;
+                    qh[s][k] = (_Float16)v;
+                    ql[s][k] = (_Float16)(v - (float)qh[s][k]);
                 }
         }
     }
@@ -311,37 +360,41 @@ struct Rows {
         __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &b, 8);
         return r;
     }
-    // KT blocks of 32 keys from position t0 on; keys before lo are masked.
+    // Fragments are read kAhead products before their use and the order is
+    // pinned: left alone, the scheduler reads all of them first and spills.
+    static constexpr int kAhead = 4;
     template <int KT>
-    __device__ __forceinline__ void step(const uint8_t* k, const uint8_t* v, int32_t t0, int32_t lo) {
-        // Fragments are read kAhead products before their use and the order is
-        // pinned: left alone, the scheduler reads all of them first and spills.
-        constexpr int kAhead = 4;
-        f16v s[KT];
+    struct Weights {  // of 32 KT keys: the B operands of 16-key products
+        h8 h[2 * KT], l[F32 ? 2 * KT : 1];
+    };
+    template <int KT>
+    __device__ __forceinline__ void scores(const uint8_t* k, f16v (&s)[KT]) const {
         const uint32_t kx = swz<HD>(ka & 15);
-        auto kfrag = [&](int i) {  // products in the order (e, t)
+        auto frag = [&](int i) {  // products in the order (chunk e, block t)
             const int e = i / KT, t = i % KT;
             return as_h8(*reinterpret_cast<const v4i*>(k + (t * 32 + ka) * RB + (((2 * e + half) ^ kx) << 4)));
         };
-        {
-            h8 kf[kAhead];
+        h8 kf[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; i++) kf[i] = kfrag(i);
+        for (int i = 0; i < kAhead; i++) kf[i] = frag(i);
 #pragma unroll
-            for (int t = 0; t < KT; t++)
+        for (int t = 0; t < KT; t++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[t][r] = 0.0f;
+            for (int r = 0; r < 16; r++) s[t][r] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NS * KT; i++) {
-                const int e = i / KT, t = i % KT;
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], qh[e], s[t], 0, 0, 0);
-                if constexpr (F32) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], ql[e], s[t], 0, 0, 0);
-                if (i + kAhead < NS * KT) kf[i % kAhead] = kfrag(i + kAhead);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int i = 0; i < NS * KT; i++) {
+            const int e = i / KT, t = i % KT;
+            s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], qh[e], s[t], 0, 0, 0);
+            if constexpr (F32) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], ql[e], s[t], 0, 0, 0);
+            if (i + kAhead < NS * KT) kf[i % kAhead] = frag(i + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        const bool masked = t0 + 32 * KT > wmin || t0 < lo;  // uniform
-        if (masked) {
+    }
+    // Scores of keys from position t0 on to weights; keys before lo are masked.
+    template <int KT>
+    __device__ __forceinline__ void weights(f16v (&s)[KT], int32_t t0, int32_t lo, Weights<KT>& p) {
+        if (t0 + 32 * KT > wmin || t0 < lo) {  // uniform
+            asm volatile("");  // a branch, not two selects a score in every tile
 #pragma unroll
             for (int t = 0; t < KT; t++)
 #pragma unroll
@@ -367,35 +420,51 @@ struct Rows {
                 for (int r = 0; r < 16; r++) o[d][r] *= w;
         }
         const float b = kLift - (m == -INFINITY ? 0.0f : m);
-        h8 ph[2 * KT], pl[F32 ? 2 * KT : 1];
 #pragma unroll
         for (int t = 0; t < KT; t++)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                const f2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], c, b)),
+                const f2 x = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], c, b)),
                               __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + 1], c, b))};
-                l += p.x + p.y;
-                const h2 hi = __builtin_convertvector(p, h2);
-                ph[2 * t + r / 8][r % 8] = hi.x;
-                ph[2 * t + r / 8][r % 8 + 1] = hi.y;
+                l += x.x + x.y;
+                asm volatile("" : "+v"(l));  // here: put off, the sums would keep all weights alive
+                const h2 hi = __builtin_convertvector(x, h2);
+                p.h[2 * t + r / 8][r % 8] = hi.x;
+                p.h[2 * t + r / 8][r % 8 + 1] = hi.y;
                 if constexpr (F32) {
-                    const f2 rest = {__builtin_fmaf((float)hi.x, -1.0f, p.x), __builtin_fmaf((float)hi.y, -1.0f, p.y)};
+                    f2 rest;  // x - hi, with hi read as fp16: one instruction a weight
+                    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest.x) : "v"(hi), "v"(x.x));
+                    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rest.y) : "v"(hi), "v"(x.y));
                     const h2 lw = __builtin_convertvector(rest, h2);
-                    pl[2 * t + r / 8][r % 8] = lw.x;
-                    pl[2 * t + r / 8][r % 8 + 1] = lw.y;
+                    p.l[2 * t + r / 8][r % 8] = lw.x;
+                    p.l[2 * t + r / 8][r % 8 + 1] = lw.y;
                 }
             }
-        h8 vf[kAhead];
+    }
+    __device__ __forceinline__ void first_values(const uint8_t* v, h8 (&vf)[kAhead]) const {
 #pragma unroll
         for (int i = 0; i < kAhead; i++) vf[i] = as_h8(vfrag(v, i / ND, i % ND));
+    }
+    template <int KT>
+    __device__ __forceinline__ void values(const uint8_t* v, h8 (&vf)[kAhead], const Weights<KT>& p) {
 #pragma unroll
         for (int i = 0; i < 2 * KT * ND; i++) {
             const int e = i / ND, d = i % ND;
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % kAhead], ph[e], o[d], 0, 0, 0);
-            if constexpr (F32) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % kAhead], pl[e], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % kAhead], p.h[e], o[d], 0, 0, 0);
+            if constexpr (F32) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % kAhead], p.l[e], o[d], 0, 0, 0);
             if (i + kAhead < 2 * KT * ND) vf[i % kAhead] = as_h8(vfrag(v, (i + kAhead) / ND, (i + kAhead) % ND));
             __builtin_amdgcn_sched_barrier(0);
         }
+    }
+    template <int KT>
+    __device__ __forceinline__ void step(const uint8_t* k, const uint8_t* v, int32_t t0, int32_t lo) {
+        f16v s[KT];
+        Weights<KT> p;
+        h8 vf[kAhead];
+        scores<KT>(k, s);
+        weights<KT>(s, t0, lo, p);
+        first_values(v, vf);
+        values<KT>(v, vf, p);
     }
     // Values that are not finite and that a row sees, added to its sums (whatever
     // their weight): keys [from, to).  tidy() took them out of the products.
@@ -462,6 +531,17 @@ __device__ __forceinline__ void put4(void* out, uint64_t at, float4 x) {
     }
 }
 
+// A row that no group has: nobody else writes its parts of the prefix launch.
+__device__ __forceinline__ void no_prefix(const AttnArgs& a, const Work& w, uint32_t g, uint32_t part, uint32_t rows) {
+    if (part != 0 || !w.alone) return;
+    const uint64_t all = (uint64_t)a.n_tokens * a.n_heads;
+    for (uint32_t i = threadIdx.x; i < a.pre.n * rows; i += 256) {
+        const uint32_t r = w.row0 + i % rows;
+        const uint64_t pr = i / rows * all + (uint64_t)(w.tok0 + r / a.G) * a.n_heads + g * a.G + r % a.G;
+        *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(-INFINITY, 0.0f);
+    }
+}
+
 __device__ __forceinline__ uint32_t block_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // 128 rows a workgroup, 32 a wave; the four waves share tiles of 64 keys on a
@@ -480,24 +560,35 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
     // a causal prompt's last tiles have the most keys: they start first
     const uint32_t slot = slots - 1 - blockIdx.x / a.n_kv, part = blockIdx.y;
     Work w;
-    if (!find_work<MODE, 128>(a, slot, part, w)) return;
-    w.uniform();
+    if (!find_rows<MODE, 128>(a, slot, w)) return;
 
+    // page numbers, length and q are under way together; then the first copies
     Loader<HD> ld;
-    ld.init();
-    const uint32_t u0 = (uint32_t)w.kbeg / 16 + wave, tiles = (uint32_t)(w.kend - w.kbeg + 63) / 64;
-    auto issue = [&](uint32_t t) {
-        if ((t & 63) == 0) ld.lookup(a, w, u0 + (t + lane) * 4);
-        uint8_t* st = smem + (t & 1) * 2 * kT + wave * (kT / 4);
-        ld.copy(a, w, g, u0 + t * 4, t & 63, st, st + kT);
-    };
-    if (w.kend > w.kbeg) issue(0);
-
+    uint32_t u0 = part * (a.parts<MODE>().chunk / 16) + wave;
+    if (early_keys<MODE>(a)) ld.lookup(a, w.id, u0 + lane * 4);
     Rows<HD, F32> r;
-    const uint32_t row = w.row0 + wave * 32 + (lane & 31), tok = row / a.G, head = g * a.G + row % a.G;
+    typename Rows<HD, F32>::Raw raw;
+    const uint32_t row = w.row0 + wave * 32 + (lane & 31), tok = min(row, w.rows - 1) / a.G;
+    const uint32_t head = g * a.G + min(row, w.rows - 1) % a.G;
     const bool live = row < w.rows;
-    r.init(a.scale_log2e, live ? row_limit<MODE>(a, w, tok) : 0, live);
-    r.load_q(a.q, live ? (w.tok0 + tok) * a.q_stride + head * HD : 0, live);
+    r.fetch_q(a.q, (w.tok0 + tok) * a.q_stride + head * HD, live, raw);
+    find_keys<MODE>(a, 128, part, w);
+    if (!early_keys<MODE>(a)) {
+        u0 = (uint32_t)w.kbeg / 16 + wave;
+        ld.lookup(a, w.id, u0 + lane * 4);
+    }
+    ld.settle();
+    ld.init();
+    const uint32_t tiles = w.kend > w.kbeg ? (uint32_t)(w.kend - w.kbeg + 63) / 64 : 0;
+    auto issue = [&](uint32_t t) {
+        if (t && (t & 63) == 0) ld.lookup(a, w.id, u0 + (t + lane) * 4), ld.settle();
+        uint8_t* st = smem + (t & 1) * 2 * kT + wave * (kT / 4);
+        ld.copy(a, a.kp, w, g, u0 + t * 4, t & 63, st);
+        ld.copy(a, a.vp, w, g, u0 + t * 4, t & 63, st + kT);
+    };
+    if (tiles) issue(0);
+    r.init(a.scale_log2e, row_limit<MODE>(a, w, tok), live);
+    r.take_q(raw);
     __builtin_amdgcn_sched_barrier(0);
     r.clear();
 
@@ -505,7 +596,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
     wait_lgkmcnt0();
     lds_barrier();
     const int32_t wg_min = min(min(least[0], least[1]), min(least[2], least[3]));
-    if (w.kend > w.kbeg)
+    {
         for (uint32_t t = 0; t < tiles; t++) {
             const int32_t t0 = w.kbeg + (int32_t)t * 64;
             const uint8_t* st = smem + (t & 1) * 2 * kT;
@@ -522,14 +613,17 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
             if (masked && __builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3]))
                 odd_from = min(odd_from, t0), odd_to = t0 + 64;
             if constexpr (F32) {  // 32 keys at a time: the two parts of q and of 64 weights do not fit 256 registers
-                if (t0 < r.wmax) r.template step<1>(st, st + kT, t0, w.lo);
-                if (t0 + 32 < r.wmax) r.template step<1>(st + kT / 2, st + kT + kT / 2, t0 + 32, w.lo);
+#pragma unroll 1
+                for (int h = 0; h < 2; h++)
+                    if (t0 + 32 * h < r.wmax) r.template step<1>(st + h * (kT / 2), st + kT + h * (kT / 2), t0 + 32 * h, w.lo);
             } else {
                 if (t0 < r.wmax) r.template step<2>(st, st + kT, t0, w.lo);
             }
         }
+    }
     if (odd_from < odd_to) r.add_nonfinite(a, w, g, odd_from, odd_to);
 
+    if (MODE == kOwn) no_prefix(a, w, g, part, min(w.rows - w.row0, 128u));
     if (!live) return;
     const float l = other_sum(r.l);
     if (a.parts_total == 1) {
@@ -542,8 +636,9 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
                 put4<F32>(a.out, at + d * 32 + 8 * e, make_float4(r.o[d][4 * e] * inv, r.o[d][4 * e + 1] * inv,
                                                                  r.o[d][4 * e + 2] * inv, r.o[d][4 * e + 3] * inv));
     } else {
-        const uint64_t pr = (uint64_t)(a.part0 + part) * a.n_tokens * a.n_heads + (uint64_t)(w.tok0 + tok) * a.n_heads + head;
+        const uint64_t pr = (uint64_t)(a.parts<MODE>().first + part) * a.n_tokens * a.n_heads + (uint64_t)(w.tok0 + tok) * a.n_heads + head;
         if (r.half == 0) *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(r.m, l);
+        if (l == 0.0f) return;
 #pragma unroll
         for (int d = 0; d < HD / 32; d++)
 #pragma unroll
@@ -554,59 +649,82 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
 }
 
 // Few rows: 32 a workgroup, all of them in every wave; the waves take every
-// fourth block of 32 keys each, on rings of their own (no barrier until the
-// end), and are merged through LDS.
+// fourth block of 32 keys each, through tiles of their own (no barrier until the
+// end), and are merged through LDS.  A tile has one stage: K of the next block is
+// copied once the scores have read this one's, V once the sums have, so that two
+// workgroups fit a CU and one's start hides behind the other.
+template <int HD>
+constexpr uint32_t few_lds() {  // K and V of four waves, or their merge
+    return std::max<uint32_t>(8 * 32 * HD * 2, (4 * 32 * (HD + 4) + 256) * 4);
+}
 template <int HD, bool F32, int MODE>
-__global__ void __launch_bounds__(256, 2) k_attn_few(AttnArgs a) {
-    constexpr uint32_t kT = 32 * HD * 2, kPad = HD + 4;
-    // per wave: K, V of two stages; one array, as above, which the merge reuses
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[16 * kT];
+__device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint32_t part, uint32_t g, uint8_t* smem) {
+    constexpr uint32_t kT = 32 * HD * 2, kPad = HD + 4, kC = 2 * Loader<HD>::kCopies;
     float* oo = reinterpret_cast<float*>(smem);
     float *sm = oo + 4 * 32 * kPad, *sl = sm + 128;
-    static_assert((4 * 32 * kPad + 256) * 4 <= sizeof(smem), "the merge fits the rings");
-    const uint32_t wave = block_wave(), lane = threadIdx.x & 63, g = blockIdx.x % a.n_kv, part = blockIdx.y;
+    const uint32_t wave = block_wave(), lane = threadIdx.x & 63;
     Work w;
-    if (!find_work<MODE, 32>(a, blockIdx.x / a.n_kv, part, w)) return;
-    w.uniform();
+    if (!find_rows<MODE, 32>(a, slot, w)) return;
 
     Loader<HD> ld;
+    uint32_t u0 = part * (a.parts<MODE>().chunk / 16) + wave * 2;
+    if (early_keys<MODE>(a)) ld.lookup(a, w.id, u0 + lane / 2 * 8 + (lane & 1));
+    Rows<HD, F32> r;
+    typename Rows<HD, F32>::Raw raw;
+    const uint32_t row = w.row0 + (lane & 31), tok = min(row, w.rows - 1) / a.G;
+    const uint32_t head = g * a.G + min(row, w.rows - 1) % a.G;
+    const bool live = row < w.rows;
+    r.fetch_q(a.q, (w.tok0 + tok) * a.q_stride + head * HD, live, raw);
+    find_keys<MODE>(a, 32, part, w);
+    if (!early_keys<MODE>(a)) {
+        u0 = (uint32_t)w.kbeg / 16 + wave * 2;
+        ld.lookup(a, w.id, u0 + lane / 2 * 8 + (lane & 1));
+    }
+    ld.settle();
     ld.init();
     const int32_t first = w.kbeg + (int32_t)wave * 32;
-    const uint32_t u0 = (uint32_t)first / 16, tiles = w.kend > first ? (uint32_t)(w.kend - first + 127) / 128 : 0;
-    uint8_t* ring = smem + wave * 4 * kT;
-    int32_t odd_from = 0x7fffffff, odd_to = 0;
-    auto issue = [&](uint32_t t) {
-        if ((t & 31) == 0) ld.lookup(a, w, u0 + (t + lane / 2) * 8 + (lane & 1));
-        uint8_t* st = ring + (t & 1) * 2 * kT;
+    const uint32_t tiles = w.kend > first ? (uint32_t)(w.kend - first + 127) / 128 : 0;
+    uint8_t *kt = smem + wave * 2 * kT, *vt = kt + kT;
+    auto issue = [&](const uint16_t* x, uint32_t t, uint8_t* dst) {
 #pragma unroll
-        for (uint32_t i = 0; i < 2; i++)
-            ld.copy(a, w, g, u0 + t * 8 + i, (t & 31) * 2 + i, st + i * (kT / 2), st + kT + i * (kT / 2));
+        for (uint32_t i = 0; i < 2; i++) ld.template copy<MODE == kOwn>(a, x, w, g, u0 + t * 8 + i, (t & 31) * 2 + i, dst + i * (kT / 2));
     };
-    if (tiles) issue(0);
-
-    Rows<HD, F32> r;
-    const uint32_t row = w.row0 + (lane & 31), tok = row / a.G, head = g * a.G + row % a.G;
-    const bool live = row < w.rows;
-    r.init(a.scale_log2e, live ? row_limit<MODE>(a, w, tok) : 0, live);
-    r.load_q(a.q, live ? (w.tok0 + tok) * a.q_stride + head * HD : 0, live);
+    if (tiles) issue(a.kp, 0, kt), issue(a.vp, 0, vt);
+    r.init(a.scale_log2e, row_limit<MODE>(a, w, tok), live);
+    r.take_q(raw);
     __builtin_amdgcn_sched_barrier(0);
     r.clear();
 
+    int32_t odd_from = 0x7fffffff, odd_to = 0;
     for (uint32_t t = 0; t < tiles; t++) {
-        if (t + 1 < tiles) {
-            wait_lgkmcnt0();  // the reads of tile t - 1, whose stage is refilled
-            issue(t + 1);
-            wait_vmcnt<4 * Loader<HD>::kCopies>();  // tile t has landed, tile t + 1 is on its way
-        } else {
-            wait_vmcnt<0>();
-        }
         const int32_t t0 = first + (int32_t)t * 128;
-        uint8_t* st = ring + (t & 1) * 2 * kT;
-        if (t0 + 32 > r.wmin || t0 < w.lo) {
-            const bool b0 = tidy<HD>(st + kT), b1 = tidy<HD>(st + kT + kT / 2);
-            if (b0 || b1) odd_from = min(odd_from, t0), odd_to = t0 + 32;
+        const bool more = t + 1 < tiles;
+        f16v s[1];
+        h8 vf[Rows<HD, F32>::kAhead];
+        typename Rows<HD, F32>::template Weights<1> p;
+        wait_vmcnt<kC>();  // K of this block has landed, V may be on its way
+        r.template scores<1>(kt, s);
+        wait_lgkmcnt0();
+        if (more) {
+            if (((t + 1) & 31) == 0) {
+                wait_vmcnt<0>();
+                ld.lookup(a, w.id, u0 + (t + 1 + lane / 2) * 8 + (lane & 1));
+                ld.settle();
+            }
+            issue(a.kp, t + 1, kt);
         }
-        if (t0 < r.wmax) r.template step<1>(st, st + kT, t0, w.lo);
+        r.template weights<1>(s, t0, w.lo, p);
+        if (more) wait_vmcnt<kC>();
+        else wait_vmcnt<0>();
+        if (t0 + 32 > r.wmin || t0 < w.lo) {
+            const bool b0 = tidy<HD>(vt), b1 = tidy<HD>(vt + kT / 2);
+            if (b0 || b1) odd_from = min(odd_from, t0), odd_to = t0 + 32;
+            wait_lgkmcnt0();
+        }
+        r.first_values(vt, vf);
+        r.template values<1>(vt, vf, p);
+        wait_lgkmcnt0();
+        if (more) issue(a.vp, t + 1, vt);
     }
     // (this wave's keys of that range only: the other waves add their own)
     for (int32_t t0 = odd_from; t0 < odd_to; t0 += 128) r.add_nonfinite(a, w, g, t0, t0 + 32);
@@ -624,6 +742,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_few(AttnArgs a) {
                 make_float4(r.o[d][4 * e], r.o[d][4 * e + 1], r.o[d][4 * e + 2], r.o[d][4 * e + 3]);
     __syncthreads();
     const uint32_t rows = min(w.rows - w.row0, 32u);
+    if (MODE == kOwn) no_prefix(a, w, g, part, rows);
     for (uint32_t e = threadIdx.x; e < rows * (HD / 4); e += 256) {
         const uint32_t i = e / (HD / 4), d = e % (HD / 4) * 4;
         const float M = fmaxf(fmaxf(sm[i], sm[32 + i]), fmaxf(sm[64 + i], sm[96 + i]));
@@ -644,9 +763,9 @@ __global__ void __launch_bounds__(256, 2) k_attn_few(AttnArgs a) {
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             put4<F32>(a.out, (w.tok0 + t) * a.out_stride + h * HD + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
         } else {
-            const uint64_t pr = (uint64_t)(a.part0 + part) * a.n_tokens * a.n_heads + (uint64_t)(w.tok0 + t) * a.n_heads + h;
+            const uint64_t pr = (uint64_t)(a.parts<MODE>().first + part) * a.n_tokens * a.n_heads + (uint64_t)(w.tok0 + t) * a.n_heads + h;
             if (d == 0) *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(M, L);
-            put4<true>(a.po, pr * HD + d, x);
+            if (L != 0.0f) put4<true>(a.po, pr * HD + d, x);
         }
     }
 }
@@ -657,50 +776,79 @@ __device__ __forceinline__ float wave_max_all(float x) {
     return x;
 }
 
-// One wave per (token, head): the parts of its keys joined, o = sum o_c 2^(m_c - M).
+// (one LDS array in both kernels, as above)
 template <int HD, bool F32, int MODE>
-__global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
+__global__ void __launch_bounds__(256, 2) k_attn_few(AttnArgs a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
+    attn_few<HD, F32, MODE>(a, blockIdx.x / a.n_kv, blockIdx.y, blockIdx.x % a.n_kv, smem);
+}
+// A batch with few rows a group: prefix and own keys in one launch, the prefix's
+// workgroups, which have more keys, first (64 rows behind 8192 shared positions:
+// TIMES).
+template <int HD, bool F32>
+__global__ void __launch_bounds__(256, 2) k_attn_shared(AttnArgs a, uint32_t prefix_slots, uint32_t prefix_blocks) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
+    const uint32_t b = blockIdx.x / a.n_kv, g = blockIdx.x % a.n_kv;
+    if (b < prefix_blocks) attn_few<HD, F32, kPrefix>(a, b % prefix_slots, b / prefix_slots, g, smem);
+    else attn_few<HD, F32, kOwn>(a, (b - prefix_blocks) / a.own.n, (b - prefix_blocks) % a.own.n, g, smem);
+}
+
+// One wave per (token, head): the parts of its keys joined, o = sum o_c 2^(m_c - M).
+// Every part of every covered row has its (maximum, sum) written, (-inf, 0) where
+// it has no key, so nothing is looked up here: the pairs (one a lane) and the
+// first parts' sums are in flight at once.
+template <int HD, bool F32, uint32_t kBatch>
+__global__ void __launch_bounds__(64) k_attn_join(AttnArgs a) {
     constexpr int E = HD / 64;
-    const uint64_t row = blockIdx.x * 4ull + block_wave();
-    const uint32_t lane = threadIdx.x & 63;
-    if (row >= (uint64_t)a.n_tokens * a.n_heads) return;
-    const uint32_t tok = (uint32_t)(row / a.n_heads), head = (uint32_t)(row % a.n_heads);
-    uint32_t s = tok, back = 0, na = 0, nb = 0;
-    if (MODE == kPrompt && a.q_start) {
-        s = wave_search(a.n, tok, [&](uint32_t i) { return (uint64_t)a.q_start[i]; });
-        const uint32_t end = min(a.q_start[s + 1], a.n_tokens);
-        if (tok < a.q_start[s] || tok >= end) return;
-        back = end - 1 - tok;
-    }
-    const uint32_t len = seq_len(a, seq_id(a, s));
-    if (MODE == kPrompt) {
-        if (len > back) nb = min(a.n_parts, (len - back + a.chunk - 1) / a.chunk);
-    } else {
-        const uint32_t pre = shared_len(a, s, len);
-        na = min(a.n_parts_prefix, pre ? (pre + a.chunk_prefix - 1) / a.chunk_prefix : 0);
-        if (len > pre) nb = min(a.n_parts, (len - (pre & ~15u) + a.chunk - 1) / a.chunk);
-    }
+    typedef float fe __attribute__((ext_vector_type(E)));
+    const uint32_t row = blockIdx.x, lane = threadIdx.x, parts = a.parts_total;
+    const uint32_t tok = row / a.n_heads, head = row % a.n_heads;
     const uint64_t rows = (uint64_t)a.n_tokens * a.n_heads;
-    auto at = [&](uint32_t i) { return (uint64_t)(i < na ? i : a.n_parts_prefix + i - na) * rows + row; };
-    float M = -INFINITY;
-    for (uint32_t i = lane; i < na + nb; i += 64) M = fmaxf(M, a.pml[at(i) * 2]);
-    M = wave_max_all(M);
-    float L = 0.0f, o[E] = {};
-    for (uint32_t i = 0; i < na + nb; i++) {
-        const uint64_t p = at(i);
-        const float2 ml = *reinterpret_cast<const float2*>(a.pml + p * 2);
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // no key of this row
-        const float f = __builtin_amdgcn_exp2f(ml.x - M);
-        L = __builtin_fmaf(ml.y, f, L);
+    const float* po = a.po + (uint64_t)row * HD + lane * E;
+    auto pair = [&](uint32_t i) {
+        return i < parts ? *reinterpret_cast<const float2*>(a.pml + (i * rows + row) * 2) : make_float2(-INFINITY, 0.0f);
+    };
+    fe v[kBatch];
+    const float2 p0 = pair(lane);
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(a.po[p * HD + lane * E + e], f, o[e]);
+    for (uint32_t k = 0; k < kBatch; k++) v[k] = *reinterpret_cast<const fe*>(po + min(k, parts - 1) * rows * HD);
+    if (a.q_start && (tok < a.q_start[0] || tok >= a.q_start[a.n])) return;  // a row of no sequence
+    float M = p0.x;
+    for (uint32_t i = lane + 64; i < parts; i += 64) M = fmaxf(M, pair(i).x);
+    M = wave_max_all(M);
+    float L = 0.0f;
+    fe o;
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = 0.0f;
+    for (uint32_t c = 0; c < parts; c += 64) {
+        const float2 p = c ? pair(c + lane) : p0;
+        const float w = p.x == -INFINITY && p.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p.x - M);
+        L += p.y == 0.0f ? 0.0f : p.y * w;
+        for (uint32_t k0 = 0; k0 < min(parts - c, 64u); k0 += kBatch) {
+            if (c + k0) {
+#pragma unroll
+                for (uint32_t k = 0; k < kBatch; k++)
+                    v[k] = *reinterpret_cast<const fe*>(po + min(c + k0 + k, parts - 1) * rows * HD);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kBatch; k++) {
+                const float wk = __shfl(w, k0 + k, 64);
+                const float lk = __shfl(p.y, k0 + k, 64);
+                if (lk == 0.0f) continue;  // no key: its sums are not written
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(v[k][e], wk, o[e]);
+            }
+        }
     }
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) L += __shfl_xor(L, x, 64);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const uint64_t to = tok * a.out_stride + head * HD + lane * E;
+    if constexpr (F32) {
+        *reinterpret_cast<fe*>(static_cast<float*>(a.out) + to) = o * inv;
+    } else {
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        if constexpr (F32) static_cast<float*>(a.out)[to + e] = o[e] * inv;
-        else static_cast<_Float16*>(a.out)[to + e] = (_Float16)(o[e] * inv);
+        for (int e = 0; e < E; e++) static_cast<_Float16*>(a.out)[to + e] = (_Float16)(o[e] * inv);
     }
 }
 
@@ -732,12 +880,13 @@ struct Launch {
 // group are counted; single: one token each.
 Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len) {
     Launch l;
-    const uint64_t G = c->n_heads / c->n_kv_heads;
-    l.few = tokens * G <= 32ull * units;
+    const uint64_t G = c->n_heads / c->n_kv_heads, rows = tokens * G;
+    l.few = rows <= 1024 * units || rows * c->n_kv_heads <= 256 * 128;
     const uint64_t bm = l.few ? 32 : 128;
-    l.slots = single ? units * ((G + bm - 1) / bm) : tokens * G / bm + units;
-    const uint64_t wgs = l.slots * c->n_kv_heads, step = l.few ? 128 : 64, least = l.few ? 256 : 512;
-    uint64_t parts = (512 + wgs - 1) / wgs;
+    l.slots = single ? units * ((G + bm - 1) / bm) : rows / bm + units;
+    const uint64_t wgs = (rows + units * bm - 1) / (units * bm) * units * c->n_kv_heads;  // of equally long sequences
+    const uint64_t step = l.few ? 128 : 64, least = l.few ? 256 : 512;
+    uint64_t parts = (l.few ? 512 : 256) / wgs;
     parts = std::max<uint64_t>(1, std::min(parts, (max_len + least - 1) / least));
     l.chunk = (uint32_t)(((max_len + parts - 1) / parts + step - 1) / step * step);
     l.parts = (uint32_t)((max_len + l.chunk - 1) / l.chunk);
@@ -767,17 +916,24 @@ void launch_as(const AttnArgs& a, const Launch& l, uint32_t hd, int type, hipStr
     if (hd == 128) type == ANE_TYPE_F32 ? launch<128, true, MODE>(a, l, s) : launch<128, false, MODE>(a, l, s);
     else type == ANE_TYPE_F32 ? launch<64, true, MODE>(a, l, s) : launch<64, false, MODE>(a, l, s);
 }
-template <int MODE>
+void both_as(const AttnArgs& a, const Launch& pre, const Launch& own, uint32_t hd, int type, hipStream_t s) {
+    auto* f = hd == 128 ? (type == ANE_TYPE_F32 ? k_attn_shared<128, true> : k_attn_shared<128, false>)
+                        : (type == ANE_TYPE_F32 ? k_attn_shared<64, true> : k_attn_shared<64, false>);
+    const uint32_t pb = (uint32_t)(pre.slots * pre.parts), ob = (uint32_t)(own.slots * own.parts);
+    hipLaunchKernelGGL(f, dim3((pb + ob) * a.n_kv), dim3(256), 0, s, a, (uint32_t)pre.slots, pb);
+}
 void join_as(const AttnArgs& a, uint32_t hd, int type, hipStream_t s) {
-    auto* f = hd == 128 ? (type == ANE_TYPE_F32 ? k_attn_join<128, true, MODE> : k_attn_join<128, false, MODE>)
-                        : (type == ANE_TYPE_F32 ? k_attn_join<64, true, MODE> : k_attn_join<64, false, MODE>);
-    const uint64_t rows = (uint64_t)a.n_tokens * a.n_heads;
-    hipLaunchKernelGGL(f, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a);
+    auto pick = [&](auto few, auto many) { return a.parts_total <= 4 ? few : many; };
+    auto* f = hd == 128 ? (type == ANE_TYPE_F32 ? pick(k_attn_join<128, true, 4>, k_attn_join<128, true, 16>)
+                                                : pick(k_attn_join<128, false, 4>, k_attn_join<128, false, 16>))
+                        : (type == ANE_TYPE_F32 ? pick(k_attn_join<64, true, 4>, k_attn_join<64, true, 16>)
+                                                : pick(k_attn_join<64, false, 4>, k_attn_join<64, false, 16>));
+    hipLaunchKernelGGL(f, dim3(a.n_tokens * a.n_heads), dim3(64), 0, s, a);
 }
 
 bool plan_fits(const ane_paged_cache* c, const Launch& l, uint64_t n_tokens, uint32_t parts_total) {
-    return launch_fits(l.slots * c->n_kv_heads, 256) && l.parts <= 65535 &&
-           (parts_total == 1 || launch_fits((n_tokens * c->n_heads + 3) / 4, 256));
+    return launch_fits(l.slots * l.parts * c->n_kv_heads, 512) && l.parts <= 65535 &&
+           (parts_total == 1 || launch_fits(n_tokens * c->n_heads, 64));
 }
 
 AttnArgs attn_args(const ane_paged_cache* c, uint32_t layer, const uint32_t* seqs, uint32_t n, uint32_t n_tokens,
@@ -828,10 +984,10 @@ extern "C" int ane_hip_attention_prompt(const ane_paged_cache* cache, uint32_t l
     a.q_start = q_start;
     a.po = static_cast<float*>(workspace);
     a.pml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ml);
-    a.chunk = l.chunk, a.n_parts = a.parts_total = l.parts;
+    a.own = {l.chunk, l.parts, 0}, a.parts_total = l.parts;
     hipStream_t s = (hipStream_t)stream;
     launch_as<kPrompt>(a, l, cache->head_dim, type, s);
-    if (l.parts > 1) join_as<kPrompt>(a, cache->head_dim, type, s);
+    if (l.parts > 1) join_as(a, cache->head_dim, type, s);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;
 }
@@ -874,15 +1030,15 @@ extern "C" int ane_hip_attention_shared(const ane_paged_cache* cache, uint32_t l
     a.po = static_cast<float*>(workspace);
     a.pml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ml);
     a.parts_total = p.parts;
-    a.chunk_prefix = p.prefix.chunk, a.n_parts_prefix = p.prefix.parts;
+    a.pre = {p.prefix.chunk, p.prefix.parts, 0}, a.own = {p.own.chunk, p.own.parts, p.prefix.parts};
     hipStream_t s = (hipStream_t)stream;
-    if (n_groups) {
-        a.chunk = p.prefix.chunk, a.n_parts = p.prefix.parts, a.part0 = 0;
-        launch_as<kPrefix>(a, p.prefix, cache->head_dim, type, s);
+    if (n_groups && p.prefix.few && p.own.few) {
+        both_as(a, p.prefix, p.own, cache->head_dim, type, s);
+    } else {
+        if (n_groups) launch_as<kPrefix>(a, p.prefix, cache->head_dim, type, s);
+        launch_as<kOwn>(a, p.own, cache->head_dim, type, s);
     }
-    a.chunk = p.own.chunk, a.n_parts = p.own.parts, a.part0 = p.prefix.parts;
-    launch_as<kOwn>(a, p.own, cache->head_dim, type, s);
-    if (p.parts > 1) join_as<kOwn>(a, cache->head_dim, type, s);
+    if (p.parts > 1) join_as(a, cache->head_dim, type, s);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;
 }
