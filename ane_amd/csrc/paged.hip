@@ -127,71 +127,91 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a) {
 }
 
 // -------------------------------------------------------- assigning pages
-constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kScan = 16;
+constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kLook = 1 << 16;
 
 // Exclusive prefix sums over the workgroup's 1024 threads; *total: the sum.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* sh, uint64_t* total) {
+template <class T>
+__device__ __forceinline__ T block_scan(T v, T* total) {
+    __shared__ T sums[kPlanWaves];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t s = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint64_t o = __shfl_up((unsigned long long)s, off, 64);
-        if (lane >= (uint32_t)off) s += o;
-    }
-    if (lane == 63) sh[wave] = s;
+    auto scan = [&](T x, int n) {
+        for (int off = 1; off < n; off <<= 1) {
+            const T o = __shfl_up(x, off, 64);
+            if (lane >= (uint32_t)off) x += o;
+        }
+        return x;
+    };
+    const T s = scan(v, 64);
+    if (lane == 63) sums[wave] = s;
     __syncthreads();
-    uint64_t before = 0, all = 0;
-    for (uint32_t w = 0; w < kPlanWaves; w++) {
-        if (w < wave) before += sh[w];
-        all += sh[w];
-    }
+    const T t = scan(lane < kPlanWaves ? sums[lane] : 0, kPlanWaves);  // the waves' sums, scanned by every wave
+    const T before = wave ? __shfl(t, wave - 1, 64) : 0;
+    *total = __shfl(t, kPlanWaves - 1, 64);
     __syncthreads();
-    *total = all;
     return before + s - v;
 }
 
-// The pages i in [from, to) with pick(refs[i]), in ascending order: found(rank,
-// i) for each of the first `want`.  Returns how many there are (counting
-// stops once `want` are found).  kScan x 1024 counts a step, all loads of a
-// step in flight at once.  The whole workgroup calls it.
-template <class Pick, class Found>
-__device__ __forceinline__ uint64_t pick_pages(const uint32_t* refs, uint32_t from, uint32_t to, uint64_t want,
-                                               uint64_t* sh, Pick pick, Found found) {
-    __shared__ uint32_t cnt[kScan * kPlanWaves];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t have = 0;
-    for (uint64_t base = from; base < to && have < want; base += kScan * kPlanThreads) {
-        uint32_t r[kScan];
+// The free pages as bits in LDS, 65536 pages a look: a smaller pool is looked at
+// once, however many passes a call makes over it.  Short loops on purpose: one
+// workgroup runs them once, and what it waits for is mostly code and the few
+// loads (unrolled over registers, the plan of a compaction took 13 us, not 6).
+struct Pool {
+    const uint32_t* refs;
+    uint32_t pages;
+    uint64_t* bits;    // [kLook / 64], 1: free
+    uint32_t* before;  // [kLook / 64]
+
+    __device__ __forceinline__ void look(uint64_t base) const {
+        const uint32_t lane = threadIdx.x & 63, masks = (uint32_t)min((uint64_t)kLook, pages - base + 63) / 64;
+        for (uint32_t j = threadIdx.x >> 6; j < masks; j += 4 * kPlanWaves) {
+            uint32_t r[4];
 #pragma unroll
-        for (uint32_t j = 0; j < kScan; j++) {
-            const uint64_t i = base + j * kPlanThreads + threadIdx.x;
-            r[j] = i < to ? refs[i] : 0;
-        }
-        uint64_t mask[kScan];
+            for (uint32_t k = 0; k < 4; k++) {
+                const uint64_t i = base + (j + k * kPlanWaves) * 64 + lane;
+                r[k] = i < pages ? refs[i] : 1;
+            }
 #pragma unroll
-        for (uint32_t j = 0; j < kScan; j++) {
-            const uint64_t i = base + j * kPlanThreads + threadIdx.x;
-            mask[j] = __ballot(i < to && pick(r[j]));
-            if (lane == 0) cnt[j * kPlanWaves + wave] = __popcll(mask[j]);
+            for (uint32_t k = 0; k < 4; k++) {
+                const uint64_t m = __ballot(r[k] == 0);
+                if (lane == 0 && j + k * kPlanWaves < masks) bits[j + k * kPlanWaves] = m;
+            }
         }
-        __syncthreads();
-        // counts in page order: step j, then wave
-        const uint32_t mine = threadIdx.x < kScan * kPlanWaves ? cnt[threadIdx.x] : 0;
-        uint64_t all;
-        const uint64_t before = block_scan(mine, sh, &all);
-        if (threadIdx.x < kScan * kPlanWaves) cnt[threadIdx.x] = (uint32_t)before;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t j = 0; j < kScan; j++) {
-            const uint64_t rank = have + cnt[j * kPlanWaves + wave] + __popcll(mask[j] & ((1ull << lane) - 1));
-            if ((mask[j] >> lane & 1) && rank < want)
-                found(rank, (uint32_t)(base + j * kPlanThreads + threadIdx.x));
-        }
-        have += all;
         __syncthreads();
     }
-    return have;
-}
+    // The free (or live) pages i in [from, to) in ascending order: found(rank, i)
+    // for each of the first `want`; returns how many there are (counting stops
+    // once `want` are found).  After a look at the pool's first pages; the whole
+    // workgroup calls it.
+    template <class Found>
+    __device__ __forceinline__ uint32_t pick(bool free, uint32_t from, uint32_t to, uint32_t want, Found found) const {
+        const uint32_t lane = threadIdx.x & 63;
+        uint32_t have = 0;
+        for (uint64_t base = from / kLook * kLook; base < to && have < want; base += kLook) {
+            if (pages > kLook) look(base);
+            const uint32_t masks = (uint32_t)min((uint64_t)kLook, pages - base + 63) / 64;
+            auto mask = [&](uint32_t j) {  // those of [from, to)
+                uint64_t m = free ? bits[j] : ~bits[j];
+                const uint64_t i = base + j * 64ull;
+                if (i < from) m &= from - i < 64 ? ~0ull << (from - i) : 0;
+                if (i + 64 > to) m &= to > i ? ~0ull >> (64 - (to - i)) : 0;
+                return m;
+            };
+            uint32_t all;
+            const uint32_t mine = threadIdx.x < masks ? __popcll(mask(threadIdx.x)) : 0;
+            before[threadIdx.x] = block_scan(mine, &all);
+            __syncthreads();
+            for (uint32_t j = threadIdx.x >> 6; j < masks; j += kPlanWaves) {
+                const uint64_t m = mask(j);
+                const uint32_t rank = have + before[j] + __popcll(m & ((1ull << lane) - 1));
+                if ((m >> lane & 1) && rank < want) found(rank, (uint32_t)(base + j * 64 + lane));
+            }
+            have += all;
+            __syncthreads();
+        }
+        return have;
+    }
+};
+static_assert(kLook / 64 == kPlanThreads, "a thread a mask");
 
 struct PagesWs {
     uint32_t *list, *movers, *map;  // [n_pages] each
@@ -219,7 +239,9 @@ size_t pages_layout(const ane_paged_cache* c, void* base, PagesWs* w) {
     return off;
 }
 
-// claim[seq] = the first request i with ok(i) that names it.
+// claim[seq] = the first valid request that names it (seq(i): ANE_NO_PAGE for one
+// that is not valid).  In LDS where the cache has few sequences.
+constexpr uint32_t kLdsSeqs = 4096, kLdsList = 4096;
 template <class Seq>
 __device__ __forceinline__ void claim_first(uint32_t n, uint32_t* claim, Seq seq) {
     for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
@@ -234,144 +256,151 @@ __device__ __forceinline__ void claim_first(uint32_t n, uint32_t* claim, Seq seq
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(kPlanThreads)
-k_pages_reserve(ane_paged_cache c, uint32_t n, const uint32_t* seqs, const uint32_t* new_len, uint32_t* served,
-                PagesWs w) {
-    __shared__ uint64_t sh[kPlanWaves];
-    const uint64_t cap = (uint64_t)c.max_pages * c.page_size;
-    auto seq = [&](uint32_t i) {
-        const uint32_t s = seqs[i];
-        return s < c.n_seqs && new_len[i] <= cap ? s : ANE_NO_PAGE;
-    };
-    claim_first(n, w.claim, seq);
-    // pages request i asks for (0 where it is refused) and the first new entry of its row
-    auto need = [&](uint32_t i, bool& ok, uint32_t& s, uint32_t& at) {
-        s = seq(i);
-        ok = s != ANE_NO_PAGE && __atomic_load_n(&w.claim[s], __ATOMIC_RELAXED) == i;
-        if (!ok) return 0u;
-        at = (uint32_t)((min((uint64_t)c.kv_len[s], cap) + c.page_size - 1) / c.page_size);
-        const uint32_t to = (uint32_t)(((uint64_t)new_len[i] + c.page_size - 1) / c.page_size);
-        return to > at ? to - at : 0u;
+// A request of a planning pass: its sequence (ANE_NO_PAGE: not valid), the pages
+// it asks for, and what its call needs besides.  A thread keeps those of the first
+// 1024 requests; the others are looked up again in each pass.
+struct Request {
+    uint32_t seq, need, x, y;
+};
+
+// Passes over the requests: who names a sequence first, how many pages are asked
+// for, which are free, and then done(i, request, served, its pages).
+template <class Look, class Done>
+__device__ __forceinline__ void serve(const ane_paged_cache& c, uint32_t n, PagesWs& w, Look look, Done done) {
+    __shared__ uint32_t claim_lds[kLdsSeqs], list_lds[kLdsList], before_lds[kPlanThreads];
+    __shared__ uint64_t bits[kPlanThreads];
+    const uint32_t tid = threadIdx.x;
+    const Pool pool = {c.page_refs, c.n_pages, bits, before_lds};
+    pool.look(0);
+    const Request mine = tid < n ? look(tid) : Request{ANE_NO_PAGE, 0, 0, 0};
+    auto request = [&](uint32_t i) { return i == tid ? mine : look(i); };
+    uint32_t* claim = c.n_seqs <= kLdsSeqs ? claim_lds : w.claim;
+    claim_first(n, claim, [&](uint32_t i) { return request(i).seq; });
+    auto valid = [&](uint32_t i, const Request& r) {
+        return r.seq != ANE_NO_PAGE && __atomic_load_n(&claim[r.seq], __ATOMIC_RELAXED) == i;
     };
     uint64_t total = 0;
     for (uint32_t base = 0; base < n; base += kPlanThreads) {
-        const uint32_t i = base + threadIdx.x;
-        bool ok = false;
-        uint32_t s, at;
-        uint64_t all;
-        block_scan(i < n ? need(i, ok, s, at) : 0, sh, &all);
+        const uint32_t i = base + tid;
+        uint64_t k = 0, all;
+        if (i < n) {
+            const Request r = request(i);
+            if (valid(i, r)) k = r.need;
+        }
+        block_scan(k, &all);
         total += all;
     }
-    const uint64_t want = min(total, (uint64_t)c.n_pages);
-    const uint64_t have = pick_pages(c.page_refs, 0, c.n_pages, want, sh, [](uint32_t r) { return r == 0; },
-                                     [&](uint64_t rank, uint32_t i) { w.list[rank] = i; });
-    __syncthreads();
+    const uint32_t want = (uint32_t)min(total, (uint64_t)c.n_pages);
+    uint32_t* list = want <= kLdsList ? list_lds : w.list;
+    const uint32_t have = pool.pick(true, 0, c.n_pages, want, [&](uint32_t rank, uint32_t i) { list[rank] = i; });
     uint64_t before = 0;
     for (uint32_t base = 0; base < n; base += kPlanThreads) {
-        const uint32_t i = base + threadIdx.x;
+        const uint32_t i = base + tid;
+        Request r = {ANE_NO_PAGE, 0, 0, 0};
         bool ok = false;
-        uint32_t s = 0, at = 0;
-        uint64_t all;
-        const uint32_t k = i < n ? need(i, ok, s, at) : 0;
-        const uint64_t r0 = before + block_scan(k, sh, &all);
-        before += all;
-        const bool fits = ok && r0 + k <= have;
-        if (i < n && served) served[i] = fits;
-        if (fits) {
-            for (uint32_t j = 0; j < k; j++) {
-                const uint32_t p = w.list[r0 + j];
-                c.page_table[(uint64_t)s * c.max_pages + at + j] = p;
-                c.page_refs[p] = 1;
-            }
-            if (new_len[i] > c.kv_len[s]) c.kv_len[s] = new_len[i];
+        if (i < n) {
+            r = request(i);
+            ok = valid(i, r);
         }
+        uint64_t all;
+        const uint64_t r0 = before + block_scan<uint64_t>(ok ? r.need : 0, &all);
+        before += all;
+        if (i < n) done(i, r, ok && r0 + r.need <= have, list + r0);
     }
+}
+
+__global__ void __launch_bounds__(kPlanThreads)
+k_pages_reserve(ane_paged_cache c, uint32_t n, const uint32_t* seqs, const uint32_t* new_len, uint32_t* served,
+                PagesWs w) {
+    const uint64_t cap = (uint64_t)c.max_pages * c.page_size;
+    serve(c, n, w,
+          [&](uint32_t i) {  // x: the new length, y: the row's first new entry
+              Request r = {seqs[i], 0, new_len[i], 0};
+              if (r.seq >= c.n_seqs || r.x > cap) return Request{ANE_NO_PAGE, 0, 0, 0};
+              r.y = (uint32_t)((min((uint64_t)c.kv_len[r.seq], cap) + c.page_size - 1) / c.page_size);
+              const uint32_t to = (uint32_t)(((uint64_t)r.x + c.page_size - 1) / c.page_size);
+              r.need = to > r.y ? to - r.y : 0;
+              return r;
+          },
+          [&](uint32_t i, const Request& r, bool yes, const uint32_t* pages) {
+              if (served) served[i] = yes;
+              if (!yes) return;
+              for (uint32_t j = 0; j < r.need; j++) {
+                  const uint32_t p = pages[j];
+                  c.page_table[(uint64_t)r.seq * c.max_pages + r.y + j] = p;
+                  c.page_refs[p] = 1;
+              }
+              if (r.x > c.kv_len[r.seq]) c.kv_len[r.seq] = r.x;
+          });
 }
 
 // Which forks are served: the length each dst takes (0: none) and its fresh page.
 __global__ void __launch_bounds__(kPlanThreads)
 k_pages_fork_plan(ane_paged_cache c, uint32_t n, const uint32_t* src, const uint32_t* dst, uint32_t* served, PagesWs w) {
-    __shared__ uint64_t sh[kPlanWaves];
     const uint64_t cap = (uint64_t)c.max_pages * c.page_size;
-    auto to = [&](uint32_t i) {
-        const uint32_t a = src[i], b = dst[i];
-        return a < c.n_seqs && b < c.n_seqs && a != b && c.kv_len[b] == 0 ? b : ANE_NO_PAGE;
-    };
-    claim_first(n, w.claim, to);
-    uint64_t total = 0;
-    for (uint32_t base = 0; base < n; base += kPlanThreads) {
-        const uint32_t i = base + threadIdx.x;
-        uint32_t part = 0;
-        if (i < n) {
-            const uint32_t b = to(i);
-            const bool ok = b != ANE_NO_PAGE && __atomic_load_n(&w.claim[b], __ATOMIC_RELAXED) == i;
-            const uint32_t len = ok ? (uint32_t)min((uint64_t)c.kv_len[src[i]], cap) : 0;
-            part = ok && len % c.page_size != 0;
-            w.req_len[i] = len;
-            w.req_page[i] = ok;  // for the second pass: whether it is valid
-        }
-        uint64_t all;
-        block_scan(part, sh, &all);
-        total += all;
-    }
-    const uint64_t have = pick_pages(c.page_refs, 0, c.n_pages, total, sh, [](uint32_t r) { return r == 0; },
-                                     [&](uint64_t rank, uint32_t i) { w.list[rank] = i; });
-    __syncthreads();
-    uint64_t before = 0;
-    for (uint32_t base = 0; base < n; base += kPlanThreads) {
-        const uint32_t i = base + threadIdx.x;
-        const bool ok = i < n && w.req_page[i];
-        const uint32_t len = ok ? w.req_len[i] : 0, part = len % c.page_size != 0;
-        uint64_t all;
-        const uint64_t r0 = before + block_scan(part, sh, &all);
-        before += all;
-        if (i < n) {
-            const bool fits = ok && r0 + part <= have;
-            if (served) served[i] = fits;
-            w.req_len[i] = fits ? len : 0;
-            w.req_page[i] = fits && part ? w.list[r0] : ANE_NO_PAGE;
-        }
-    }
+    serve(c, n, w,
+          [&](uint32_t i) {  // x: the length
+              const uint32_t a = src[i], b = dst[i];
+              if (a >= c.n_seqs || b >= c.n_seqs || a == b) return Request{ANE_NO_PAGE, 0, 0, 0};
+              const uint32_t la = c.kv_len[a], lb = c.kv_len[b];
+              if (lb != 0) return Request{ANE_NO_PAGE, 0, 0, 0};
+              const uint32_t len = (uint32_t)min((uint64_t)la, cap);
+              return Request{b, len % c.page_size != 0, len, 0};
+          },
+          [&](uint32_t i, const Request& r, bool yes, const uint32_t* pages) {
+              if (served) served[i] = yes;
+              w.req_len[i] = yes ? r.x : 0;
+              w.req_page[i] = yes && r.need ? pages[0] : ANE_NO_PAGE;
+          });
 }
 
 // One workgroup per fork and slice of its work: slice 0 writes the row, the
 // counts and the length; the used rows of the part page are copied by all
-// slices, one wave per (layer, K or V, kv head).  src rows are never written
-// here: a src with positions is no dst.
+// slices, one wave per (layer, K or V, four kv heads), eight 16-byte vectors a
+// lane in flight.  src rows are never written here: a src with positions is no
+// dst.
+constexpr uint32_t kHeads = 4;
 __global__ void __launch_bounds__(256)
 k_pages_fork(ane_paged_cache c, const uint32_t* src, const uint32_t* dst, PagesWs w) {
-    const uint32_t i = blockIdx.x, len = w.req_len[i];
+    constexpr uint32_t kVecs = 2;
+    const uint32_t i = blockIdx.x, len = w.req_len[i], fresh = w.req_page[i], from_seq = src[i];
     if (len == 0) return;
-    const uint32_t whole = len / c.page_size, part = len % c.page_size, fresh = w.req_page[i];
-    const uint32_t* from = c.page_table + (uint64_t)src[i] * c.max_pages;
+    const uint32_t whole = len / c.page_size, part = len % c.page_size;
+    const uint32_t* from = c.page_table + (uint64_t)from_seq * c.max_pages;
     if (blockIdx.y == 0) {
-        uint32_t* row = c.page_table + (uint64_t)dst[i] * c.max_pages;
+        const uint32_t to = dst[i];
+        uint32_t* row = c.page_table + (uint64_t)to * c.max_pages;
         for (uint32_t j = threadIdx.x; j < whole + (part ? 1 : 0); j += 256) {
             const uint32_t p = j < whole ? from[j] : fresh;
             row[j] = p;
             if (p < c.n_pages) atomicAdd(&c.page_refs[p], 1u);
         }
-        if (threadIdx.x == 0) c.kv_len[dst[i]] = len;
+        if (threadIdx.x == 0) c.kv_len[to] = len;
     }
     if (!part) return;
     const uint32_t old = from[whole];
     if (old >= c.n_pages || fresh >= c.n_pages) return;
     const uint32_t lane = threadIdx.x & 63, hv = c.head_dim / 8;  // 16-byte vectors a row
-    const uint32_t jobs = c.n_layers * 2 * c.n_kv_heads, vecs = part * hv;
+    const uint32_t quads = (c.n_kv_heads + kHeads - 1) / kHeads, jobs = c.n_layers * 2 * quads, run = part * hv;
+    const uint64_t head = (uint64_t)c.page_size * hv, page = head * c.n_kv_heads;
     for (uint32_t j = blockIdx.y * 4 + (threadIdx.x >> 6); j < jobs; j += gridDim.y * 4) {
-        const uint32_t g = j % c.n_kv_heads, kv = j / c.n_kv_heads % 2, l = j / c.n_kv_heads / 2;
-        uint4* pool = reinterpret_cast<uint4*>(kv ? c.v_pages : c.k_pages);
-        const uint64_t head = (uint64_t)c.page_size * hv, base = (uint64_t)l * c.n_pages * c.n_kv_heads;
-        const uint4* a = pool + (base + (uint64_t)old * c.n_kv_heads + g) * head;
-        uint4* b = pool + (base + (uint64_t)fresh * c.n_kv_heads + g) * head;
-        for (uint32_t e = lane; e < vecs; e += 256) {
-            uint4 t[4];
+        const uint32_t g0 = j % quads * kHeads, kv = j / quads & 1, l = j / quads / 2;
+        v4u* pool = reinterpret_cast<v4u*>(kv ? c.v_pages : c.k_pages) + (uint64_t)l * c.n_pages * page + g0 * head;
+        const v4u* a = pool + old * page;
+        v4u* b = pool + fresh * page;
+        for (uint32_t e = lane; e < run; e += kVecs * 64) {
+            // unconditional loads (a vector past the end or a head past the last
+            // reads one of its own again): all in flight before the first store
+            v4u t[kHeads][kVecs];
 #pragma unroll
-            for (uint32_t k = 0; k < 4; k++)
-                if (e + k * 64 < vecs) t[k] = a[e + k * 64];
+            for (uint32_t h = 0; h < kHeads; h++)
 #pragma unroll
-            for (uint32_t k = 0; k < 4; k++)
-                if (e + k * 64 < vecs) b[e + k * 64] = t[k];
+                for (uint32_t k = 0; k < kVecs; k++) t[h][k] = a[min(h, c.n_kv_heads - 1 - g0) * head + min(e + k * 64, run - 1)];
+#pragma unroll
+            for (uint32_t h = 0; h < kHeads; h++)
+#pragma unroll
+                for (uint32_t k = 0; k < kVecs; k++)
+                    if (g0 + h < c.n_kv_heads && e + k * 64 < run) b[h * head + e + k * 64] = t[h][k];
         }
     }
 }
@@ -398,19 +427,23 @@ __global__ void __launch_bounds__(256) k_pages_free(ane_paged_cache c, const uin
 // the r-th free one before it; the counts and the numbers that follow.
 __global__ void __launch_bounds__(kPlanThreads)
 k_pages_compact_plan(ane_paged_cache c, uint32_t* refs_out, uint32_t* n_live, PagesWs w) {
-    __shared__ uint64_t sh[kPlanWaves];
+    __shared__ uint32_t list_lds[kLdsList], before_lds[kPlanThreads];
+    __shared__ uint64_t bits[kPlanThreads];
     const uint32_t* refs = c.page_refs;
-    auto live = [](uint32_t r) { return r != 0; };
-    const uint32_t n = (uint32_t)pick_pages(refs, 0, c.n_pages, ~0ull, sh, live, [](uint64_t, uint32_t) {});
-    const uint32_t holes = (uint32_t)pick_pages(refs, 0, n, ~0ull, sh, [](uint32_t r) { return r == 0; },
-                                                [&](uint64_t rank, uint32_t i) { w.list[rank] = i; });
+    const Pool pool = {refs, c.n_pages, bits, before_lds};
+    pool.look(0);
+    const uint32_t n = pool.pick(false, 0, c.n_pages, ~0u, [](uint32_t, uint32_t) {});
+    const uint32_t holes = pool.pick(true, 0, n, ~0u, [&](uint32_t rank, uint32_t i) {
+        w.list[rank] = i;
+        if (rank < kLdsList) list_lds[rank] = i;
+    });
     // numbers at or past the live count: a live page's new one, another's own
     for (uint64_t i = n + threadIdx.x; i < c.n_pages; i += kPlanThreads) w.map[i] = (uint32_t)i;
     if (refs_out != refs)
         for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) refs_out[i] = refs[i];
     __syncthreads();
-    pick_pages(refs, n, c.n_pages, ~0ull, sh, live, [&](uint64_t rank, uint32_t i) {
-        const uint32_t to = w.list[rank];
+    pool.pick(false, n, c.n_pages, ~0u, [&](uint32_t rank, uint32_t i) {
+        const uint32_t to = rank < kLdsList ? list_lds[rank] : w.list[rank];
         w.movers[rank] = i;
         w.map[i] = to;
         refs_out[to] = refs[i];
@@ -434,10 +467,10 @@ __device__ __forceinline__ void copy_pages(const ane_paged_cache& c, uint32_t n,
         const uint32_t kv = r & 1, l = (uint32_t)(r / 2 % c.n_layers), i = (uint32_t)(r / 2 / c.n_layers);
         const uint32_t a = src[i], b = dst[i];
         if (a >= c.n_pages || b >= c.n_pages || a == b) continue;
-        uint4* pool = reinterpret_cast<uint4*>(kv ? c.v_pages : c.k_pages) + (uint64_t)l * c.n_pages * vecs;
-        const uint4* from = pool + a * vecs;
-        uint4* to = pool + b * vecs;
-        uint4 t[4];
+        v4u* pool = reinterpret_cast<v4u*>(kv ? c.v_pages : c.k_pages) + (uint64_t)l * c.n_pages * vecs;
+        const v4u* from = pool + a * vecs;
+        v4u* to = pool + b * vecs;
+        v4u t[4];
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++) {
             const uint64_t e = st * kCopyVecs + k * 256 + threadIdx.x;
@@ -547,8 +580,9 @@ extern "C" int ane_hip_pages_fork(const ane_paged_cache* cache, uint32_t n, cons
     pages_layout(cache, workspace, &w);
     hipStream_t s = (hipStream_t)stream;
     hipLaunchKernelGGL(k_pages_fork_plan, dim3(1), dim3(kPlanThreads), 0, s, *cache, n, src, dst, served, w);
-    // four waves a workgroup, one (layer, K or V, kv head) a wave; at most 4096 workgroups more than the forks
-    const uint64_t jobs = ((uint64_t)cache->n_layers * 2 * cache->n_kv_heads + 3) / 4, room = 4096 / n + 1;
+    // four jobs a workgroup; at most 4096 workgroups more than the forks
+    const uint64_t quads = (cache->n_kv_heads + kHeads - 1) / kHeads, jobs = ((uint64_t)cache->n_layers * 2 * quads + 3) / 4;
+    const uint64_t room = 4096 / n + 1;
     hipLaunchKernelGGL(k_pages_fork, dim3(n, (uint32_t)(jobs < room ? jobs : room)), dim3(256), 0, s, *cache, src, dst, w);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;

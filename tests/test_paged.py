@@ -820,6 +820,35 @@ def test_many_requests(ane):
     m.check()
 
 
+@pytest.mark.gpu
+def test_pools_past_one_look(ane):
+    """More pages than the planning workgroup looks at at a time (65536)."""
+    P = 140001
+    c = filled_cache(n_layers=1, n_heads=1, n_kv_heads=1, head_dim=64, page_size=16, n_pages=P, n_seqs=9, max_pages=60000)
+    m, ws = Model(c), ane.pages_workspace(c)
+    n = [16 * 60000 - 7, 16 * 50000, 16 * 29990 + 1, 3]
+    got = i32([0] * 4)
+    ane.pages_reserve(c, i32([3, 0, 8, 5]), i32(n), got, workspace=ws)
+    assert got.tolist() == m.reserve([3, 0, 8, 5], n) == [1, 1, 1, 1]
+    ane.pages_free(c, i32([3]))
+    m.free([3])
+    got = i32([0] * 3)
+    ane.pages_fork(c, i32([8, 5, 0]), i32([1, 2, 4]), got, workspace=ws)
+    assert got.tolist() == m.fork([8, 5, 0], [1, 2, 4]) == [1, 1, 1]
+    m.check()
+    live = i32([0])
+    ane.pages_compact(c, n_live=live, workspace=ws)
+    assert int(live) == sum(r > 0 for r in m.refs)
+    moves = [p for p in range(int(live), P) if m.refs[p]]
+    holes = [p for p in range(int(live)) if not m.refs[p]]
+    to = dict(zip(moves, holes))
+    for a, b in to.items():
+        m.refs[b], m.refs[a] = m.refs[a], 0
+    m.k[:, holes], m.v[:, holes] = m.k[:, moves], m.v[:, moves]
+    m.table = [[to.get(p, p) for p in row] for row in m.table]
+    m.check()
+
+
 # ------------------------------------------------------------------ together
 @pytest.mark.gpu
 @pytest.mark.parametrize("ty", ["f32", "f16"])
