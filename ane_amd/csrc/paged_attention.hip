@@ -29,6 +29,7 @@ namespace ane {
 namespace {
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __fp16 hh2 __attribute__((ext_vector_type(2)));  // (what the dot product's builtin takes)
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -36,6 +37,21 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4* lds_s4;
 
 enum Mode { kPrompt, kPrefix, kOwn };
+
+// x / d for x < 2^30 and d <= 2^16 as (x * magic) >> shift: with shift = 30 +
+// ceil(log2 d) and magic = ceil(2^shift / d), at most 2^31, the excess magic * d -
+// 2^shift is below d <= 2^(shift - 30), so x * excess < 2^shift and the floor is
+// exact.  (A division the compiler spells out is some 40 instructions before a
+// workgroup's first load.)
+struct Div {
+    uint32_t magic, shift;
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)((uint64_t)x * magic >> shift); }
+};
+Div div_by(uint32_t d) {
+    uint32_t lg = 0;
+    while ((1u << lg) < d) lg++;
+    return Div{(uint32_t)(((1ull << (30 + lg)) + d - 1) / d), 30 + lg};
+}
 
 struct AttnArgs {
     const void* q;
@@ -45,7 +61,7 @@ struct AttnArgs {
     const uint32_t *table, *kv_len, *seqs, *q_start, *group_start, *prefix;
     uint64_t q_stride, out_stride;
     uint32_t n, n_tokens, n_groups, n_heads, n_kv, G, ps, n_pages, max_pages, n_seqs;
-    uint32_t div_magic, div_shift;                // 16-position group -> page, see page_div
+    Div by_page, by_G, by_kv;      // 16-position group -> page, row -> token, workgroup -> row tile
     struct Parts {
         uint32_t chunk, n, first;  // keys a part, parts, number of the first
     } own, pre;                    // of a row's own keys (all of a prompt's), of the shared prefix
@@ -56,23 +72,13 @@ struct AttnArgs {
     __device__ __forceinline__ const Parts& parts() const { return MODE == kPrefix ? pre : own; }
 };
 
-// u / (ps / 16) for u < 2^27 as (u * magic) >> shift: with shift = 27 +
-// ceil(log2 d), magic = ceil(2^shift / d) <= 2^28, the excess magic * d - 2^shift
-// is below d <= 2^(shift - 27), so u * excess < 2^shift and the floor is exact.
-void page_div(uint32_t ps, uint32_t* magic, uint32_t* shift) {
-    const uint32_t d = ps / 16;
-    uint32_t lg = 0;
-    while ((1u << lg) < d) lg++;
-    *shift = 27 + lg;
-    *magic = (uint32_t)(((1ull << *shift) + d - 1) / d);
-}
-
 // No branches: a load in flight next to the others costs less than its test.
 __device__ __forceinline__ uint32_t seq_id(const AttnArgs& a, uint32_t s) { return a.seqs ? a.seqs[s] : s; }
-__device__ __forceinline__ uint32_t seq_len(const AttnArgs& a, uint32_t id) {
-    const uint32_t len = a.kv_len[min(id, a.n_seqs - 1)];
-    return id < a.n_seqs ? (uint32_t)min((uint64_t)len, (uint64_t)a.max_pages * a.ps) : 0;
+__device__ __forceinline__ uint32_t raw_len(const AttnArgs& a, uint32_t id) { return a.kv_len[min(id, a.n_seqs - 1)]; }
+__device__ __forceinline__ uint32_t seq_len(const AttnArgs& a, uint32_t id, uint32_t raw) {
+    return id < a.n_seqs ? (uint32_t)min((uint64_t)raw, (uint64_t)a.max_pages * a.ps) : 0;
 }
+__device__ __forceinline__ uint32_t seq_len(const AttnArgs& a, uint32_t id) { return seq_len(a, id, raw_len(a, id)); }
 __device__ __forceinline__ uint32_t lane_of(uint32_t x, uint32_t lane) { return __builtin_amdgcn_readlane(x, lane); }
 __device__ __forceinline__ uint32_t last_lane(bool yes) {  // the last lane that says yes, 0 if none
     const uint64_t m = __ballot(yes);
@@ -87,6 +93,7 @@ struct Work {
     uint32_t s, id, tok0, toks, row0, rows;  // batch row or group, sequence, first token, tokens, first row, rows in all
     int32_t kbeg, kend, lo, len;             // lo: keys before it are masked (kbeg rounds it down to 16)
     bool alone;                              // kOwn: no group has the row
+    uint32_t raw, prefix;                    // as loaded: the sequence's length, the group's prefix
 };
 
 __device__ __forceinline__ void uniform(uint32_t& x) { x = __builtin_amdgcn_readfirstlane(x); }
@@ -123,6 +130,8 @@ __device__ __forceinline__ bool find_rows(const AttnArgs& a, uint32_t slot, Work
     w.row0 = tile * BM;
     if (tile >= (1u << 24) || w.row0 >= w.rows) return false;
     w.id = seq_id(a, MODE == kPrefix ? w.tok0 : w.s);
+    w.raw = raw_len(a, w.id);
+    if (MODE == kPrefix) w.prefix = a.prefix[w.s];
     uniform(w.s), uniform(w.id), uniform(w.tok0), uniform(w.toks), uniform(w.row0), uniform(w.rows);
     return true;
 }
@@ -147,15 +156,15 @@ __device__ __forceinline__ uint32_t shared_len(const AttnArgs& a, uint32_t s, ui
 // The keys of part `part`; at: its first position, where the work has any.
 template <int MODE>
 __device__ __forceinline__ void find_keys(const AttnArgs& a, uint32_t bm, uint32_t part, Work& w) {
-    w.len = (int32_t)seq_len(a, w.id);
+    w.len = (int32_t)seq_len(a, w.id, w.raw);
     w.kbeg = w.lo = 0;
     w.kend = w.len;
     w.alone = true;
     if (MODE == kPrompt) {
-        const int32_t last = (int32_t)((min(w.row0 + bm, w.rows) - 1) / a.G);
+        const int32_t last = (int32_t)a.by_G(min(w.row0 + bm, w.rows) - 1);
         w.kend = min(w.len, w.len - (int32_t)w.toks + last + 1);
     } else if (MODE == kPrefix) {
-        w.kend = (int32_t)min(a.prefix[w.s], (uint32_t)w.len);
+        w.kend = (int32_t)min(w.prefix, (uint32_t)w.len);
     } else {
         w.lo = (int32_t)shared_len(a, w.s, (uint32_t)w.len, w.alone);
         w.kbeg = w.lo & ~15;
@@ -206,7 +215,7 @@ struct Loader {
         }
     }
     __device__ __forceinline__ uint32_t page(const AttnArgs& a, uint32_t u) const {
-        return (uint32_t)((uint64_t)u * a.div_magic >> a.div_shift);
+        return a.by_page(u);
     }
     // u: this lane's 16-position group
     __device__ __forceinline__ void lookup(const AttnArgs& a, uint32_t id, uint32_t u) {
@@ -254,6 +263,15 @@ __device__ __forceinline__ h8 as_h8(v4i x) {
 // copy to LDS in flight first.
 __device__ __forceinline__ s4 read_tr(const uint8_t* __restrict__ p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
+}
+
+// x as two fp16 parts, 22 bits in all.
+__device__ __forceinline__ void split(f2 x, h2& hi, h2& lw) {
+    hi = __builtin_convertvector(x, h2);
+    f2 rest;  // x - hi, with hi read as fp16: one instruction a value
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest.x) : "v"(hi), "v"(x.x));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rest.y) : "v"(hi), "v"(x.y));
+    lw = __builtin_convertvector(rest, h2);
 }
 
 // The running maximum may lag by kLag (in log2) before O and l are rescaled;
@@ -326,23 +344,25 @@ struct Rows {
 #pragma unroll
             for (int e = 0; e < 8; e++) ql[0][e] = (_Float16)0.0f;
         } else {
-            uint32_t top = 0;
+            float top = 0.0f;
 #pragma unroll
             for (int s = 0; s < 2 * NS; s++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) top = max(top, (uint32_t)w.x[s][k] & 0x7fffffffu);
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+                for (int k = 0; k < 4; k++) top = fmaxf(top, fabsf(__int_as_float(w.x[s][k])));
+            top = other_max(top);
             // 2^(140 - ex) brings the largest |q| (exponent field ex) to [2^13, 2^14)
-            const uint32_t ex = max(top >> 23, 20u);
+            const uint32_t ex = max(__float_as_uint(top) >> 23, 20u);
             const float up = __uint_as_float((267 - ex) << 23);
             c *= __uint_as_float((ex - 13) << 23);
 #pragma unroll
             for (int s = 0; s < NS; s++)
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float v = __int_as_float(w.x[2 * s + k / 4][k % 4]) * up;
-                    qh[s][k] = (_Float16)v;
-                    ql[s][k] = (_Float16)(v - (float)qh[s][k]);
+                for (int k = 0; k < 8; k += 2) {
+                    const f2 v = {__int_as_float(w.x[2 * s + k / 4][k % 4]) * up, __int_as_float(w.x[2 * s + k / 4][k % 4 + 1]) * up};
+                    h2 hi, lw;
+                    split(v, hi, lw);
+                    qh[s][k] = hi.x, qh[s][k + 1] = hi.y;
+                    ql[s][k] = lw.x, ql[s][k + 1] = lw.y;
                 }
         }
     }
@@ -426,19 +446,19 @@ struct Rows {
             for (int r = 0; r < 16; r += 2) {
                 const f2 x = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], c, b)),
                               __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + 1], c, b))};
-                l += x.x + x.y;
-                asm volatile("" : "+v"(l));  // here: put off, the sums would keep all weights alive
-                const h2 hi = __builtin_convertvector(x, h2);
-                p.h[2 * t + r / 8][r % 8] = hi.x;
-                p.h[2 * t + r / 8][r % 8 + 1] = hi.y;
+                h2 hi, lw;
                 if constexpr (F32) {
-                    f2 rest;  // x - hi, with hi read as fp16: one instruction a weight
-                    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest.x) : "v"(hi), "v"(x.x));
-                    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rest.y) : "v"(hi), "v"(x.y));
-                    const h2 lw = __builtin_convertvector(rest, h2);
+                    split(x, hi, lw);
                     p.l[2 * t + r / 8][r % 8] = lw.x;
                     p.l[2 * t + r / 8][r % 8 + 1] = lw.y;
+                    l += x.x + x.y;
+                } else {  // the sum of the weights as they enter the product
+                    hi = __builtin_convertvector(x, h2);
+                    l = __builtin_amdgcn_fdot2(__builtin_bit_cast(hh2, hi), hh2{(__fp16)1.0f, (__fp16)1.0f}, l, false);
                 }
+                asm volatile("" : "+v"(l));  // here: put off, the sums would keep all weights alive
+                p.h[2 * t + r / 8][r % 8] = hi.x;
+                p.h[2 * t + r / 8][r % 8 + 1] = hi.y;
             }
     }
     __device__ __forceinline__ void first_values(const uint8_t* v, h8 (&vf)[kAhead]) const {
@@ -471,7 +491,7 @@ struct Rows {
     __device__ __forceinline__ void add_nonfinite(const AttnArgs& a, const Work& w, uint32_t g, int32_t from, int32_t to) {
 #pragma unroll 1
         for (int32_t key = max(from, w.lo); key < min(to, w.kend); key++) {
-            const uint32_t p = (uint32_t)((uint64_t)((uint32_t)key / 16) * a.div_magic >> a.div_shift);
+            const uint32_t p = a.by_page((uint32_t)key / 16);
             const uint32_t id = p < a.max_pages ? a.table[(uint64_t)w.id * a.max_pages + p] : ANE_NO_PAGE;
             if (id >= a.n_pages) continue;
             const uint16_t* v = a.vp + (((uint64_t)id * a.n_kv + g) * a.ps + (uint32_t)key - p * a.ps) * HD + 4 * half;
@@ -537,7 +557,8 @@ __device__ __forceinline__ void no_prefix(const AttnArgs& a, const Work& w, uint
     const uint64_t all = (uint64_t)a.n_tokens * a.n_heads;
     for (uint32_t i = threadIdx.x; i < a.pre.n * rows; i += 256) {
         const uint32_t r = w.row0 + i % rows;
-        const uint64_t pr = i / rows * all + (uint64_t)(w.tok0 + r / a.G) * a.n_heads + g * a.G + r % a.G;
+        const uint32_t t = a.by_G(r);
+        const uint64_t pr = i / rows * all + (uint64_t)(w.tok0 + t) * a.n_heads + g * a.G + r - t * a.G;
         *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(-INFINITY, 0.0f);
     }
 }
@@ -556,9 +577,10 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
     __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kT + 48];
     int32_t* least = reinterpret_cast<int32_t*>(smem + 4 * kT);
     int32_t *odd = least + 4, odd_from = 0x7fffffff, odd_to = 0;
-    const uint32_t wave = block_wave(), lane = threadIdx.x & 63, g = blockIdx.x % a.n_kv;
+    const uint32_t wave = block_wave(), lane = threadIdx.x & 63, tile = a.by_kv(blockIdx.x);
+    const uint32_t g = blockIdx.x - tile * a.n_kv;
     // a causal prompt's last tiles have the most keys: they start first
-    const uint32_t slot = slots - 1 - blockIdx.x / a.n_kv, part = blockIdx.y;
+    const uint32_t slot = slots - 1 - tile, part = blockIdx.y;
     Work w;
     if (!find_rows<MODE, 128>(a, slot, w)) return;
 
@@ -568,8 +590,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
     if (early_keys<MODE>(a)) ld.lookup(a, w.id, u0 + lane * 4);
     Rows<HD, F32> r;
     typename Rows<HD, F32>::Raw raw;
-    const uint32_t row = w.row0 + wave * 32 + (lane & 31), tok = min(row, w.rows - 1) / a.G;
-    const uint32_t head = g * a.G + min(row, w.rows - 1) % a.G;
+    const uint32_t row = w.row0 + wave * 32 + (lane & 31), tok = a.by_G(min(row, w.rows - 1));
+    const uint32_t head = g * a.G + min(row, w.rows - 1) - tok * a.G;
     const bool live = row < w.rows;
     r.fetch_q(a.q, (w.tok0 + tok) * a.q_stride + head * HD, live, raw);
     find_keys<MODE>(a, 128, part, w);
@@ -654,14 +676,14 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
 // copied once the scores have read this one's, V once the sums have, so that two
 // workgroups fit a CU and one's start hides behind the other.
 template <int HD>
-constexpr uint32_t few_lds() {  // K and V of four waves, or their merge
-    return std::max<uint32_t>(8 * 32 * HD * 2, (4 * 32 * (HD + 4) + 256) * 4);
+constexpr uint32_t few_lds() {  // K and V of four waves (or their sums), and their maxima and sums of weights
+    return 8 * 32 * HD * 2 + 1024;
 }
 template <int HD, bool F32, int MODE>
 __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint32_t part, uint32_t g, uint8_t* smem) {
-    constexpr uint32_t kT = 32 * HD * 2, kPad = HD + 4, kC = 2 * Loader<HD>::kCopies;
-    float* oo = reinterpret_cast<float*>(smem);
-    float *sm = oo + 4 * 32 * kPad, *sl = sm + 128;
+    constexpr uint32_t kT = 32 * HD * 2, kC = 2 * Loader<HD>::kCopies;
+    float4* oo = reinterpret_cast<float4*>(smem);
+    float *sm = reinterpret_cast<float*>(smem + 8 * kT), *sl = sm + 128;
     const uint32_t wave = block_wave(), lane = threadIdx.x & 63;
     Work w;
     if (!find_rows<MODE, 32>(a, slot, w)) return;
@@ -671,8 +693,8 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
     if (early_keys<MODE>(a)) ld.lookup(a, w.id, u0 + lane / 2 * 8 + (lane & 1));
     Rows<HD, F32> r;
     typename Rows<HD, F32>::Raw raw;
-    const uint32_t row = w.row0 + (lane & 31), tok = min(row, w.rows - 1) / a.G;
-    const uint32_t head = g * a.G + min(row, w.rows - 1) % a.G;
+    const uint32_t row = w.row0 + (lane & 31), tok = a.by_G(min(row, w.rows - 1));
+    const uint32_t head = g * a.G + min(row, w.rows - 1) - tok * a.G;
     const bool live = row < w.rows;
     r.fetch_q(a.q, (w.tok0 + tok) * a.q_stride + head * HD, live, raw);
     find_keys<MODE>(a, 32, part, w);
@@ -729,44 +751,46 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
     // (this wave's keys of that range only: the other waves add their own)
     for (int32_t t0 = odd_from; t0 < odd_to; t0 += 128) r.add_nonfinite(a, w, g, t0, t0 + 32);
 
-    // merge the four waves: rows of HD + 4 floats keep 16-byte stores of
-    // neighbouring rows on different banks
+    // Merge the four waves: each puts its sums into LDS as its lanes hold them
+    // (a unit of four dimensions is 1 KB, so nothing conflicts) and takes a
+    // quarter of the units of all four back.
+    constexpr int kUnits = HD / 8, kMine = kUnits / 4;
     const float l = other_sum(r.l);
     __syncthreads();
     if (r.half == 0) sm[wave * 32 + lane] = r.m, sl[wave * 32 + lane] = l;
 #pragma unroll
-    for (int d = 0; d < HD / 32; d++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            *reinterpret_cast<float4*>(oo + (wave * 32 + (lane & 31)) * kPad + d * 32 + 8 * e + 4 * r.half) =
-                make_float4(r.o[d][4 * e], r.o[d][4 * e + 1], r.o[d][4 * e + 2], r.o[d][4 * e + 3]);
+    for (int u = 0; u < kUnits; u++)
+        oo[(wave * kUnits + u) * 64 + lane] = make_float4(r.o[u / 4][u % 4 * 4], r.o[u / 4][u % 4 * 4 + 1],
+                                                         r.o[u / 4][u % 4 * 4 + 2], r.o[u / 4][u % 4 * 4 + 3]);
     __syncthreads();
-    const uint32_t rows = min(w.rows - w.row0, 32u);
-    if (MODE == kOwn) no_prefix(a, w, g, part, rows);
-    for (uint32_t e = threadIdx.x; e < rows * (HD / 4); e += 256) {
-        const uint32_t i = e / (HD / 4), d = e % (HD / 4) * 4;
-        const float M = fmaxf(fmaxf(sm[i], sm[32 + i]), fmaxf(sm[64 + i], sm[96 + i]));
-        float L = 0.0f;
+    if (MODE == kOwn) no_prefix(a, w, g, part, min(w.rows - w.row0, 32u));
+    if (!live) return;
+    const uint32_t i = lane & 31;
+    const float M = fmaxf(fmaxf(sm[i], sm[32 + i]), fmaxf(sm[64 + i], sm[96 + i]));
+    float L = 0.0f, f[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float m = sm[k * 32 + i], l1 = sl[k * 32 + i];
+        f[k] = m == -INFINITY && l1 == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - M);  // 0: no key of this row
+        L = __builtin_fmaf(l1, f[k], L);
+    }
+    const uint64_t pr = (uint64_t)(a.parts<MODE>().first + part) * a.n_tokens * a.n_heads + (uint64_t)(w.tok0 + tok) * a.n_heads + head;
+    const bool whole = a.parts_total == 1;
+    if (!whole && wave == 0 && r.half == 0) *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(M, L);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const uint64_t at = (w.tok0 + tok) * a.out_stride + head * HD;
+#pragma unroll
+    for (int j = 0; j < kMine; j++) {
+        const uint32_t u = wave * kMine + j, d = u / 4 * 32 + u % 4 * 8 + 4 * r.half;
         float4 x = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const float m = sm[k * 32 + i], l1 = sl[k * 32 + i];
-            if (m == -INFINITY && l1 == 0.0f) continue;  // no key of this row
-            const float f = __builtin_amdgcn_exp2f(m - M);
-            const float4 y = *reinterpret_cast<const float4*>(oo + (k * 32 + i) * kPad + d);
-            L = __builtin_fmaf(l1, f, L);
-            x.x = __builtin_fmaf(y.x, f, x.x), x.y = __builtin_fmaf(y.y, f, x.y);
-            x.z = __builtin_fmaf(y.z, f, x.z), x.w = __builtin_fmaf(y.w, f, x.w);
+            const float4 y = oo[(k * kUnits + u) * 64 + lane];
+            x.x = __builtin_fmaf(y.x, f[k], x.x), x.y = __builtin_fmaf(y.y, f[k], x.y);
+            x.z = __builtin_fmaf(y.z, f[k], x.z), x.w = __builtin_fmaf(y.w, f[k], x.w);
         }
-        const uint32_t t = (w.row0 + i) / a.G, h = g * a.G + (w.row0 + i) % a.G;
-        if (a.parts_total == 1) {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            put4<F32>(a.out, (w.tok0 + t) * a.out_stride + h * HD + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-        } else {
-            const uint64_t pr = (uint64_t)(a.parts<MODE>().first + part) * a.n_tokens * a.n_heads + (uint64_t)(w.tok0 + t) * a.n_heads + h;
-            if (d == 0) *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(M, L);
-            if (L != 0.0f) put4<true>(a.po, pr * HD + d, x);
-        }
+        if (whole) put4<F32>(a.out, at + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+        else if (L != 0.0f) put4<true>(a.po, pr * HD + d, x);
     }
 }
 
@@ -780,7 +804,8 @@ __device__ __forceinline__ float wave_max_all(float x) {
 template <int HD, bool F32, int MODE>
 __global__ void __launch_bounds__(256, 2) k_attn_few(AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
-    attn_few<HD, F32, MODE>(a, blockIdx.x / a.n_kv, blockIdx.y, blockIdx.x % a.n_kv, smem);
+    const uint32_t slot = a.by_kv(blockIdx.x);
+    attn_few<HD, F32, MODE>(a, slot, blockIdx.y, blockIdx.x - slot * a.n_kv, smem);
 }
 // A batch with few rows a group: prefix and own keys in one launch, the prefix's
 // workgroups, which have more keys, first (64 rows behind 8192 shared positions:
@@ -788,7 +813,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_few(AttnArgs a) {
 template <int HD, bool F32>
 __global__ void __launch_bounds__(256, 2) k_attn_shared(AttnArgs a, uint32_t prefix_slots, uint32_t prefix_blocks) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
-    const uint32_t b = blockIdx.x / a.n_kv, g = blockIdx.x % a.n_kv;
+    const uint32_t b = a.by_kv(blockIdx.x), g = blockIdx.x - b * a.n_kv;
     if (b < prefix_blocks) attn_few<HD, F32, kPrefix>(a, b % prefix_slots, b / prefix_slots, g, smem);
     else attn_few<HD, F32, kOwn>(a, (b - prefix_blocks) / a.own.n, (b - prefix_blocks) % a.own.n, g, smem);
 }
@@ -945,7 +970,7 @@ AttnArgs attn_args(const ane_paged_cache* c, uint32_t layer, const uint32_t* seq
     a.q_stride = q_stride, a.out_stride = out_stride;
     a.n = n, a.n_tokens = n_tokens, a.n_heads = c->n_heads, a.n_kv = c->n_kv_heads, a.G = c->n_heads / c->n_kv_heads;
     a.ps = c->page_size, a.n_pages = c->n_pages, a.max_pages = c->max_pages, a.n_seqs = c->n_seqs;
-    page_div(a.ps, &a.div_magic, &a.div_shift);
+    a.by_page = div_by(a.ps / 16), a.by_G = div_by(a.G), a.by_kv = div_by(a.n_kv);
     a.scale_log2e = (float)((double)scale * 1.4426950408889634);
     return a;
 }
