@@ -903,7 +903,7 @@ struct Launch {
 
 // units: sequences (groups) of the launch, tokens: rows before the heads of a
 // group are counted; single: one token each.
-Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len) {
+Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len, bool beside = false) {
     Launch l;
     const uint64_t G = c->n_heads / c->n_kv_heads, rows = tokens * G;
     l.few = rows <= 1024 * units || rows * c->n_kv_heads <= 256 * 128;
@@ -911,7 +911,7 @@ Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool sing
     l.slots = single ? units * ((G + bm - 1) / bm) : rows / bm + units;
     const uint64_t wgs = (rows + units * bm - 1) / (units * bm) * units * c->n_kv_heads;  // of equally long sequences
     const uint64_t step = l.few ? 128 : 64, least = l.few ? 256 : 512;
-    uint64_t parts = (l.few ? 512 : 256) / wgs;
+    uint64_t parts = (l.few && !beside ? 512 : 256) / wgs;
     parts = std::max<uint64_t>(1, std::min(parts, (max_len + least - 1) / least));
     l.chunk = (uint32_t)(((max_len + parts - 1) / parts + step - 1) / step * step);
     l.parts = (uint32_t)((max_len + l.chunk - 1) / l.chunk);
@@ -1025,7 +1025,7 @@ struct SharedPlan {
 SharedPlan shared_plan(const ane_paged_cache* c, uint32_t n, uint32_t n_groups, uint32_t max_prefix, uint32_t max_len) {
     SharedPlan p = {};
     p.own = plan(c, n, n, true, bound_len(c, max_len));
-    if (n_groups) p.prefix = plan(c, n_groups, n, false, bound_len(c, max_prefix));
+    if (n_groups) p.prefix = plan(c, n_groups, n, false, bound_len(c, max_prefix), true);
     p.parts = p.prefix.parts + p.own.parts;
     return p;
 }
