@@ -575,8 +575,14 @@ __device__ __forceinline__ void no_prefix(const AttnArgs& a, const Work& w, uint
 
 __device__ __forceinline__ uint32_t block_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-// 128 rows a workgroup, 32 a wave; the four waves share tiles of 64 keys on a
-// 2-stage LDS ring (each wave copies one 16-key group of K and V a tile).
+// 128 rows a workgroup, 32 a wave, all their keys; the four waves share tiles of
+// 64 keys on a 2-stage LDS ring (each wave copies one 16-key group of K and V a
+// tile).  Two workgroups a CU: while one wave of a SIMD is in its weights (some 650
+// vector cycles a 32-key block), the other is in its products (512 matrix cycles,
+// fp32 1024).  8192 tokens x 32 heads fp16: 550-570 us, 0.96-1.0 PFLOP/s, at the
+// 1.85 GHz the clock holds then (a library fp16 product of 8192^3: 1.1); fp32:
+// 0.59, so 1.18 of matrix work.  Weights between the products of the other half
+// in one wave measured slower (584), a ring of fragments of 2, 3 or 6 the same.
 template <int HD, bool F32, int MODE>
 __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slots) {
     constexpr uint32_t kT = 64 * HD * 2;
@@ -590,33 +596,27 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
     const uint32_t wave = block_wave(), lane = threadIdx.x & 63, tile = a.by_kv(blockIdx.x);
     const uint32_t g = blockIdx.x - tile * a.n_kv;
     // a causal prompt's last tiles have the most keys: they start first
-    const uint32_t slot = slots - 1 - tile, part = blockIdx.y;
     Work w;
-    if (!find_rows<MODE, 128>(a, slot, w)) return;
+    if (!find_rows<MODE, 128>(a, slots - 1 - tile, w)) return;
 
     // page numbers, length and q are under way together; then the first copies
     Loader<HD> ld;
-    uint32_t u0 = part * (a.parts<MODE>().chunk / 16) + wave;
-    if (early_keys<MODE>(a)) ld.lookup(a, w.id, u0 + lane * 4);
+    ld.lookup(a, w.id, wave + lane * 4);
     Rows<HD, F32> r;
     typename Rows<HD, F32>::Raw raw;
     const uint32_t row = w.row0 + wave * 32 + (lane & 31), tok = a.by_G(min(row, w.rows - 1));
     const uint32_t head = g * a.G + min(row, w.rows - 1) - tok * a.G;
     const bool live = row < w.rows;
     r.fetch_q(a.q, (w.tok0 + tok) * a.q_stride + head * HD, live, raw);
-    find_keys<MODE>(a, 128, part, w);
-    if (!early_keys<MODE>(a)) {
-        u0 = (uint32_t)w.kbeg / 16 + wave;
-        ld.lookup(a, w.id, u0 + lane * 4);
-    }
+    find_keys<MODE>(a, 128, 0, w);
     ld.settle();
     ld.init();
-    const uint32_t tiles = w.kend > w.kbeg ? (uint32_t)(w.kend - w.kbeg + 63) / 64 : 0;
+    const uint32_t tiles = w.kend > 0 ? (uint32_t)(w.kend + 63) / 64 : 0;
     auto issue = [&](uint32_t t) {
-        if (t && (t & 63) == 0) ld.lookup(a, w.id, u0 + (t + lane) * 4), ld.settle();
+        if (t && (t & 63) == 0) ld.lookup(a, w.id, wave + (t + lane) * 4), ld.settle();
         uint8_t* st = smem + (t & 1) * 2 * kT + wave * (kT / 4);
-        ld.copy(a, a.kp, w, g, u0 + t * 4, t & 63, st);
-        ld.copy(a, a.vp, w, g, u0 + t * 4, t & 63, st + kT);
+        ld.copy(a, a.kp, w, g, wave + t * 4, t & 63, st);
+        ld.copy(a, a.vp, w, g, wave + t * 4, t & 63, st + kT);
     };
     if (tiles) issue(0);
     r.init(a.scale_log2e, row_limit<MODE>(a, w, tok), live);
@@ -628,37 +628,34 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
     wait_lgkmcnt0();
     lds_barrier();
     const int32_t wg_min = min(min(least[0], least[1]), min(least[2], least[3]));
-    {
-        for (uint32_t t = 0; t < tiles; t++) {
-            const int32_t t0 = w.kbeg + (int32_t)t * 64;
-            const uint8_t* st = smem + (t & 1) * 2 * kT;
-            const bool masked = t0 + 64 > wg_min || t0 < w.lo;
-            wait_vmcnt<0>();  // this wave's copies of tile t
-            int32_t* flag = odd + (t & 1) * 4;
-            if (masked) {
-                const bool bad = tidy<HD>(smem + (t & 1) * 2 * kT + kT + wave * (kT / 4));
-                if (lane == 0) flag[wave] = bad;
-            }
-            wait_lgkmcnt0();  // and its reads of tile t - 1
-            lds_barrier();    // everybody's
-            if (t + 1 < tiles) issue(t + 1);
-            if (masked && __builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3]))
-                odd_from = min(odd_from, t0), odd_to = t0 + 64;
-            if constexpr (F32) {  // 32 keys at a time: the two parts of q and of 64 weights do not fit 256 registers
+    for (uint32_t t = 0; t < tiles; t++) {
+        const int32_t t0 = (int32_t)t * 64;
+        uint8_t* st = smem + (t & 1) * 2 * kT;
+        int32_t* flag = odd + (t & 1) * 4;
+        const bool masked = t0 + 64 > wg_min;
+        wait_vmcnt<0>();  // this wave's copies of tile t
+        if (masked) {
+            const bool bad = tidy<HD>(st + kT + wave * (kT / 4));
+            if (lane == 0) flag[wave] = bad;
+        }
+        wait_lgkmcnt0();  // and its reads of tile t - 1
+        lds_barrier();    // everybody's
+        if (t + 1 < tiles) issue(t + 1);
+        if (masked && __builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3]))
+            odd_from = min(odd_from, t0), odd_to = t0 + 64;
+        if constexpr (F32) {  // 32 keys at a time: the two parts of q and of 64 weights do not fit 256 registers
 #pragma unroll 1
-                for (int h = 0; h < 2; h++)
-                    if (t0 + 32 * h < r.wmax) r.template step<1>(st + h * (kT / 2), st + kT + h * (kT / 2), t0 + 32 * h, w.lo);
-            } else {
-                if (t0 < r.wmax) r.template step<2>(st, st + kT, t0, w.lo);
-            }
+            for (int h = 0; h < 2; h++)
+                if (t0 + 32 * h < r.wmax) r.template step<1>(st + h * (kT / 2), st + kT + h * (kT / 2), t0 + 32 * h, 0);
+        } else {
+            if (t0 < r.wmax) r.template step<2>(st, st + kT, t0, 0);
         }
     }
     if (odd_from < odd_to) r.add_nonfinite(a, w, g, odd_from, odd_to);
 
-    if (MODE == kOwn) no_prefix(a, w, g, part, min(w.rows - w.row0, 128u));
     if (!live) return;
     const float l = other_sum(r.l);
-    if (a.parts_total == 1) {
+    if (MODE == kPrompt) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const uint64_t at = (w.tok0 + tok) * a.out_stride + head * HD + 4 * r.half;
 #pragma unroll
@@ -667,8 +664,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
             for (int e = 0; e < 4; e++)
                 put4<F32>(a.out, at + d * 32 + 8 * e, make_float4(r.o[d][4 * e] * inv, r.o[d][4 * e + 1] * inv,
                                                                  r.o[d][4 * e + 2] * inv, r.o[d][4 * e + 3] * inv));
-    } else {
-        const uint64_t pr = (uint64_t)(a.parts<MODE>().first + part) * a.n_tokens * a.n_heads + (uint64_t)(w.tok0 + tok) * a.n_heads + head;
+    } else {  // part 0 of a batch
+        const uint64_t pr = (uint64_t)(w.tok0 + tok) * a.n_heads + head;
         if (r.half == 0) *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(r.m, l);
         if (l == 0.0f) return;
 #pragma unroll
@@ -894,7 +891,7 @@ int attention_status(const ane_paged_cache* c, uint32_t layer, uint32_t n, uint3
     const uint32_t size = type == ANE_TYPE_F32 ? 4 : 2;
     const uint64_t width = (uint64_t)c->n_heads * c->head_dim;
     if (layer >= c->n_layers || n_tokens > kMaxTokens || n > kMaxTokens ||
-        (type != ANE_TYPE_F32 && type != ANE_TYPE_F16) || !(scale > 0.0f) || !isfinite(scale))
+        (type != ANE_TYPE_F32 && type != ANE_TYPE_F16) || !(scale > 0.0f) || !(scale < 1e30f))
         return ANE_ERR_INVALID_ARG;
     if (n == 0 || n_tokens == 0) return ANE_OK;
     if (!q || !out) return ANE_ERR_BAD_POINTER;
@@ -911,8 +908,17 @@ struct Launch {
     uint32_t chunk, parts;
 };
 
-// units: sequences (groups) of the launch, tokens: rows before the heads of a
-// group are counted; single: one token each.
+// units: sequences (groups) of the launch; tokens: theirs in all; single: one
+// token each; beside: shares its launch with the batch's own keys.
+//
+// 32 rows a workgroup up to 1024 rows a sequence on average, and wherever 128 rows
+// a workgroup would leave CUs without one (512 tokens x 32 heads 23.5 us, 29 with
+// 128; 16 chunks of 64 tokens after 2000 positions 55, 68; 2048 tokens 108, 89,
+// since the four waves read every K and V tile for themselves).  Few rows and many
+// keys: the keys in parts, as many as fill the 512 places (two workgroups a CU) at
+// once but not more: a second, part-filled round costs more than the longer
+// parts (200 tokens after 4000 positions 51 us, in 1.5 times the parts 63).
+// 128-row workgroups are then more than the CUs, and their keys stay whole.
 Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len, bool beside = false) {
     Launch l;
     const uint64_t G = c->n_heads / c->n_kv_heads, rows = tokens * G;
@@ -920,10 +926,8 @@ Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool sing
     const uint64_t bm = l.few ? 32 : 128;
     l.slots = single ? units * ((G + bm - 1) / bm) : rows / bm + units;
     const uint64_t wgs = (rows + units * bm - 1) / (units * bm) * units * c->n_kv_heads;  // of equally long sequences
-    const uint64_t step = l.few ? 128 : 64, least = l.few ? 256 : 512;
-    uint64_t parts = (l.few && !beside ? 512 : 256) / wgs;
-    parts = std::max<uint64_t>(1, std::min(parts, (max_len + least - 1) / least));
-    l.chunk = (uint32_t)(((max_len + parts - 1) / parts + step - 1) / step * step);
+    const uint64_t fit = l.few ? std::min((beside ? 256 : 512) / wgs, (max_len + 255) / 256) : 1, n = std::max<uint64_t>(1, fit);
+    l.chunk = (uint32_t)(((max_len + n - 1) / n + 127) / 128 * 128);
     l.parts = (uint32_t)((max_len + l.chunk - 1) / l.chunk);
     return l;
 }
@@ -940,22 +944,22 @@ size_t parts_bytes(const ane_paged_cache* c, uint32_t n_tokens, uint32_t parts, 
     return o + ceil_to(rows * 8, 256);
 }
 
-template <int HD, bool F32, int MODE>
-void launch(const AttnArgs& a, const Launch& l, hipStream_t s) {
+template <int HD, bool F32>
+void launch_prompt(const AttnArgs& a, const Launch& l, hipStream_t s) {
     const dim3 grid((uint32_t)(l.slots * a.n_kv), l.parts);
-    if (l.few) hipLaunchKernelGGL((k_attn_few<HD, F32, MODE>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_block<HD, F32, MODE>), grid, dim3(256), 0, s, a, (uint32_t)l.slots);
+    if (l.few) hipLaunchKernelGGL((k_attn_few<HD, F32, kPrompt>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_block<HD, F32, kPrompt>), grid, dim3(256), 0, s, a, (uint32_t)l.slots);
 }
-template <int MODE>
-void launch_as(const AttnArgs& a, const Launch& l, uint32_t hd, int type, hipStream_t s) {
-    if (hd == 128) type == ANE_TYPE_F32 ? launch<128, true, MODE>(a, l, s) : launch<128, false, MODE>(a, l, s);
-    else type == ANE_TYPE_F32 ? launch<64, true, MODE>(a, l, s) : launch<64, false, MODE>(a, l, s);
-}
-void both_as(const AttnArgs& a, const Launch& pre, const Launch& own, uint32_t hd, int type, hipStream_t s) {
-    auto* f = hd == 128 ? (type == ANE_TYPE_F32 ? k_attn_shared<128, true> : k_attn_shared<128, false>)
-                        : (type == ANE_TYPE_F32 ? k_attn_shared<64, true> : k_attn_shared<64, false>);
+template <int HD, bool F32>
+void launch_shared(const AttnArgs& a, const Launch& pre, const Launch& own, hipStream_t s) {
     const uint32_t pb = (uint32_t)(pre.slots * pre.parts), ob = (uint32_t)(own.slots * own.parts);
-    hipLaunchKernelGGL(f, dim3((pb + ob) * a.n_kv), dim3(256), 0, s, a, (uint32_t)pre.slots, pb);
+    if (a.n_groups && pre.few) {
+        hipLaunchKernelGGL((k_attn_shared<HD, F32>), dim3((pb + ob) * a.n_kv), dim3(256), 0, s, a, (uint32_t)pre.slots, pb);
+        return;
+    }
+    if (a.n_groups)
+        hipLaunchKernelGGL((k_attn_block<HD, F32, kPrefix>), dim3(pb * a.n_kv), dim3(256), 0, s, a, (uint32_t)pre.slots);
+    hipLaunchKernelGGL((k_attn_few<HD, F32, kOwn>), dim3((uint32_t)(own.slots * a.n_kv), own.parts), dim3(256), 0, s, a);
 }
 void join_as(const AttnArgs& a, uint32_t hd, int type, hipStream_t s) {
     auto pick = [&](auto few, auto many) { return a.parts_total <= 4 ? few : many; };
@@ -1021,7 +1025,8 @@ extern "C" int ane_hip_attention_prompt(const ane_paged_cache* cache, uint32_t l
     a.pml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ml);
     a.own = {l.chunk, l.parts, 0}, a.parts_total = l.parts;
     hipStream_t s = (hipStream_t)stream;
-    launch_as<kPrompt>(a, l, cache->head_dim, type, s);
+    if (cache->head_dim == 128) type == ANE_TYPE_F32 ? launch_prompt<128, true>(a, l, s) : launch_prompt<128, false>(a, l, s);
+    else type == ANE_TYPE_F32 ? launch_prompt<64, true>(a, l, s) : launch_prompt<64, false>(a, l, s);
     if (l.parts > 1) join_as(a, cache->head_dim, type, s);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;
@@ -1067,12 +1072,10 @@ extern "C" int ane_hip_attention_shared(const ane_paged_cache* cache, uint32_t l
     a.parts_total = p.parts;
     a.pre = {p.prefix.chunk, p.prefix.parts, 0}, a.own = {p.own.chunk, p.own.parts, p.prefix.parts};
     hipStream_t s = (hipStream_t)stream;
-    if (n_groups && p.prefix.few && p.own.few) {
-        both_as(a, p.prefix, p.own, cache->head_dim, type, s);
-    } else {
-        if (n_groups) launch_as<kPrefix>(a, p.prefix, cache->head_dim, type, s);
-        launch_as<kOwn>(a, p.own, cache->head_dim, type, s);
-    }
+    if (cache->head_dim == 128)
+        type == ANE_TYPE_F32 ? launch_shared<128, true>(a, p.prefix, p.own, s) : launch_shared<128, false>(a, p.prefix, p.own, s);
+    else
+        type == ANE_TYPE_F32 ? launch_shared<64, true>(a, p.prefix, p.own, s) : launch_shared<64, false>(a, p.prefix, p.own, s);
     if (p.parts > 1) join_as(a, cache->head_dim, type, s);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;

@@ -249,8 +249,9 @@ struct ane_paged_cache {
  * NULL: k and v only.  rope_table NULL: no rotation; else fp32 [rope_len]
  * [head_dim/2][2].  A token whose position is negative, past its sequence's
  * pages or not below rope_len is not appended and its q_out row is zeros.
- * kv_len counts the new tokens already (ane_hip_pages_reserve); appending to a
- * page that two sequences hold changes both. */
+ * kv_len counts the new tokens already (ane_hip_pages_reserve).  A sequence may
+ * be in the batch once; appending to a page that two sequences hold changes
+ * both. */
 int ane_hip_paged_rope_append(const struct ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
                               const uint32_t* q_start, uint32_t n_tokens, int in_type, const void* q,
                               uint64_t q_stride, const void* k, const void* v, uint64_t kv_stride,
@@ -263,8 +264,8 @@ int ane_hip_paged_rope_append(const struct ane_paged_cache* cache, uint32_t laye
  * Keys a token does not see never touch its result, whatever they hold.
  * type: of q and out.  F32: products of fp32 accuracy (q and the softmax
  * weights enter the matrix cores as two fp16 parts each); F16: q and the
- * weights are fp16.  Scores, softmax and sums are fp32 in both.  scale: finite
- * and positive.  max_len: a bound on the lengths, which sizes the workspace and
+ * weights are fp16.  Scores, softmax and sums are fp32 in both.  scale: positive,
+ * below 1e30.  max_len: a bound on the lengths, which sizes the workspace and
  * the split of long rows (longer sequences are still computed whole); 0 stands
  * for max_pages * page_size.  out may be q when the strides agree.  The
  * workspace (256-byte aligned; NULL when its size is 0) belongs to the call

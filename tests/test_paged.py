@@ -110,7 +110,7 @@ def test_argument_refusals():
         assert c_append(c, **kw) == want, kw
     for call in (c_prompt, c_shared):
         for kw, want in [(dict(layer=2), 1), (dict(ty=2), 1), (dict(scale=0.0), 1), (dict(scale=-0.1), 1),
-                         (dict(scale=math.inf), 1), (dict(scale=math.nan), 1), (dict(q=None), 2), (dict(out=None), 2),
+                         (dict(scale=math.inf), 1), (dict(scale=math.nan), 1), (dict(scale=2e30), 1), (dict(q=None), 2), (dict(out=None), 2),
                          (dict(q=P + 8), 1), (dict(out=P + 8), 1), (dict(qstr=1022), 1), (dict(qstr=1020), 1),
                          (dict(ostr=1020), 1), (dict(ostr=1026), 1), (dict(n=0), 0)]:
             assert call(c, **kw) == want, (call.__name__, kw)
@@ -382,6 +382,12 @@ SHAPES = [
     ("f32", 128, 8, 8, 1024, [90], [800]),
     ("f32", 128, 4, 1, 16, [9, 2], [5000, 7001]),
     ("f16", 64, 8, 2, 32, [5], [9000]),
+    # enough rows for the kernel of 128 a workgroup (over 1024 a sequence, over 32768 in all)
+    ("f32", 128, 32, 8, 16, [1500, 30, 700], [0, 5, 300]),
+    ("f16", 128, 32, 8, 64, [2100], [0]),
+    ("f32", 64, 32, 8, 48, [1300, 900], [14, 333]),
+    ("f16", 64, 40, 8, 32, [1700, 3], [1, 0]),
+    ("f16", 128, 36, 12, 16, [1001], [4200]),
 ]
 
 
@@ -423,20 +429,21 @@ def test_prompt_strides_order_scale_and_bound(ane, ty):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("ty,hd", [("f32", 128), ("f16", 128), ("f32", 64), ("f16", 64)])
-@pytest.mark.parametrize("new,old", [([200], [0]), ([40, 90], [300, 10]), ([2, 3], [600, 700])])
-def test_prompt_masked_places_hold_anything(ane, ty, hd, new, old):
+@pytest.mark.parametrize("heads,kv,new,old", [(8, 2, [200], [0]), (8, 2, [40, 90], [300, 10]), (8, 2, [2, 3], [600, 700]),
+                                              (32, 8, [1100, 90], [70, 10]), (32, 8, [1040], [0])])
+def test_prompt_masked_places_hold_anything(ane, ty, hd, heads, kv, new, old):
     """NaN and infinities in keys and values a row does not see never reach it;
     make_cache fills every unused row of every page with NaN as well."""
     import torch
 
     lens = [a + b for a, b in zip(new, old)]
-    c = make_cache(lens, 8, 2, hd, 16, seed=3)
+    c = make_cache(lens, heads, kv, hd, 16, seed=3)
     for s, (n, bad) in enumerate(zip(lens, (math.nan, -math.inf))):
         for j, val in ((n - 1, bad), (n - 2, math.inf)):  # seen by the last tokens only
             page = int(c.page_table[s, j // 16])
             c.v_pages[0, page, 0, j % 16, 3:40] = val
             c.k_pages[0, page, 1, j % 16, 5] = val
-    q = randq(sum(new), 8, hd, dt(ty))
+    q = randq(sum(new), heads, hd, dt(ty))
     out = torch.zeros_like(q)
     start = run_prompt(c, new, q, out)
     for i, n in enumerate(new):
@@ -450,29 +457,31 @@ def test_prompt_masked_places_hold_anything(ane, ty, hd, new, old):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("ty", ["f32", "f16"])
-def test_prompt_rows_without_keys(ane, ty):
+@pytest.mark.parametrize("heads,kv,many", [(4, 1, 60), (32, 8, 5300)])
+def test_prompt_rows_without_keys(ane, ty, heads, kv, many):
     """More new tokens than positions, empty sequences and unknown ones: zeros."""
     import torch
 
-    c = make_cache([3, 0, 40], 4, 1, 128, 16)
-    q = randq(100, 4, 128, dt(ty))
+    c = make_cache([3, 0, 40], heads, kv, 128, 16)
+    q = randq(many + 40, heads, 128, dt(ty))
     out = torch.full_like(q, 5.0)
-    ane.attention_prompt(c, 0, i32([0, 60, 70, 70, 80, 100]), q, out, seqs=i32([0, 1, 2, 99, 2]))
-    assert not out[:57].any() and not out[60:80].any()
-    check_rows(c, 0, 0, q[57:60], out[57:60], [1, 2, 3], 128 ** -0.5)
-    check_rows(c, 0, 2, q[80:], out[80:], [21 + t for t in range(20)], 128 ** -0.5)
+    start = [0, many, many + 10, many + 10, many + 20, many + 40]
+    ane.attention_prompt(c, 0, i32(start), q, out, seqs=i32([0, 1, 2, 99, 2]))
+    assert not out[:many - 3].any() and not out[many:many + 20].any()
+    check_rows(c, 0, 0, q[many - 3:many], out[many - 3:many], [1, 2, 3], 128 ** -0.5)
+    check_rows(c, 0, 2, q[many + 20:], out[many + 20:], [21 + t for t in range(20)], 128 ** -0.5)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("new", [[4], [150]])
-def test_broken_page_numbers_read_as_zeros(ane, new):
+@pytest.mark.parametrize("heads,kv,new", [(4, 1, [4]), (4, 1, [150]), (40, 8, [1200])])
+def test_broken_page_numbers_read_as_zeros(ane, heads, kv, new):
     import torch
 
-    c = make_cache([500], 4, 1, 128, 16, extra=1)
+    c = make_cache([max(500, new[0])], heads, kv, 128, 16, extra=1)
     zero = max(set(range(c.n_pages)) - set(c.page_table[0].tolist()))
     c.k_pages[0, zero] = 0
     c.v_pages[0, zero] = 0
-    q = randq(new[0], 4, 128, dt("f32"))
+    q = randq(new[0], heads, 128, dt("f32"))
     a, b = torch.zeros_like(q), torch.zeros_like(q)
     for j, bad in ((3, c.n_pages), (17, NO_PAGE), (30, 0x7fffffff)):
         c.page_table[0, j] = zero
@@ -488,19 +497,19 @@ def test_broken_page_numbers_read_as_zeros(ane, new):
 
 
 @pytest.mark.gpu
-def test_extreme_queries(ane):
+@pytest.mark.parametrize("heads,kv,n", [(4, 2, 40), (40, 8, 1100)])
+def test_extreme_queries(ane, heads, kv, n):
     """fp32 queries far outside fp16's range, and tiny ones, keep fp32 accuracy."""
     import torch
 
-    c = make_cache([300], 4, 2, 128, 16, seed=2)
-    q = randq(40, 4, 128, dt("f32"))
+    c = make_cache([n + 260], heads, kv, 128, 16, seed=2)
+    q = randq(n, heads, 128, dt("f32"))
     q[:10] *= 1e6
     q[10:20] *= 1e-6
     q[20:30, :, ::2] *= 1e4
-    scale = torch.ones(1).item() * 1e-2
     out = torch.zeros_like(q)
-    start = run_prompt(c, [40], q, out, scale=scale)
-    check_prompt(c, [40], q, out, start, scale=scale)
+    start = run_prompt(c, [n], q, out, scale=1e-2)
+    check_prompt(c, [n], q, out, start, scale=1e-2)
 
 
 @pytest.mark.gpu
@@ -577,6 +586,27 @@ def test_shared(ane, ty, hd, heads, kv, ps, lens, bounds, prefixes):
         ane.attention_shared(c, 1, q, out, **kw, **more)
         for s, n in enumerate(lens):
             check_rows(c, 1, s, q[s:s + 1], out[s:s + 1], [n], hd ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty,hd,prefix,apart", [("f32", 128, 150, 0), ("f16", 64, 77, 9), ("f16", 128, 16, 299)])
+def test_shared_by_a_large_group(ane, ty, hd, prefix, apart):
+    """300 rows of 8 query heads a kv head: the prefix on 128 rows a workgroup.
+    The first `apart` rows are in no group; two rows are shorter than the
+    prefix."""
+    import torch
+
+    n, heads, kv = 300, 128, 16
+    lens = [prefix + 3 + i % 40 for i in range(n)]
+    lens[40], lens[299] = prefix - 5, 1
+    c = make_cache(lens, heads, kv, hd, 16, seed=6)
+    share(c, [apart, n], [prefix])
+    q = randq(n, heads, hd, dt(ty))
+    out = torch.full_like(q, 5.0)
+    ane.attention_shared(c, 0, q, out, group_start=i32([apart, n]), prefix_len=i32([prefix]), max_len=prefix + 50,
+                         max_prefix=prefix)
+    for s in (0, 1, 8, 9, 15, 16, 17, 40, 150, 255, 256, 298, 299):
+        check_rows(c, 0, s, q[s:s + 1], out[s:s + 1], [lens[s]], hd ** -0.5)
 
 
 @pytest.mark.gpu
