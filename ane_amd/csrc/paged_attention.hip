@@ -918,7 +918,9 @@ struct Launch {
 // keys: the keys in parts, as many as fill the 512 places (two workgroups a CU) at
 // once but not more: a second, part-filled round costs more than the longer
 // parts (200 tokens after 4000 positions 51 us, in 1.5 times the parts 63).
-// 128-row workgroups are then more than the CUs, and their keys stay whole.
+// A prefix beside its batch's own keys takes half the places (four 64-wide
+// workgroups fit a CU): 8 groups of 8 sequences 48 -> 42 us.  128-row workgroups
+// are more than the CUs as it is, and their keys stay whole.
 Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len, bool beside = false) {
     Launch l;
     const uint64_t G = c->n_heads / c->n_kv_heads, rows = tokens * G;
@@ -926,7 +928,8 @@ Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool sing
     const uint64_t bm = l.few ? 32 : 128;
     l.slots = single ? units * ((G + bm - 1) / bm) : rows / bm + units;
     const uint64_t wgs = (rows + units * bm - 1) / (units * bm) * units * c->n_kv_heads;  // of equally long sequences
-    const uint64_t fit = l.few ? std::min((beside ? 256 : 512) / wgs, (max_len + 255) / 256) : 1, n = std::max<uint64_t>(1, fit);
+    const uint64_t places = beside && c->head_dim == 128 ? 256 : 512;
+    const uint64_t n = std::max<uint64_t>(1, l.few ? std::min(places / wgs, (max_len + 255) / 256) : 1);
     l.chunk = (uint32_t)(((max_len + n - 1) / n + 127) / 128 * 128);
     l.parts = (uint32_t)((max_len + l.chunk - 1) / l.chunk);
     return l;
