@@ -264,7 +264,8 @@ struct Request {
 };
 
 // Passes over the requests: who names a sequence first, how many pages are asked
-// for, which are free, and then done(i, request, served, its pages).
+// for, which are free, and then done(i, request, served, its pages), by every
+// thread (not served from i = n on).
 template <class Look, class Done>
 __device__ __forceinline__ void serve(const ane_paged_cache& c, uint32_t n, PagesWs& w, Look look, Done done) {
     __shared__ uint32_t claim_lds[kLdsSeqs], list_lds[kLdsList], before_lds[kPlanThreads];
@@ -305,7 +306,7 @@ __device__ __forceinline__ void serve(const ane_paged_cache& c, uint32_t n, Page
         uint64_t all;
         const uint64_t r0 = before + block_scan<uint64_t>(ok ? r.need : 0, &all);
         before += all;
-        if (i < n) done(i, r, ok && r0 + r.need <= have, list + r0);
+        done(i, r, ok && r0 + r.need <= have, list + r0);
     }
 }
 
@@ -323,14 +324,33 @@ k_pages_reserve(ane_paged_cache c, uint32_t n, const uint32_t* seqs, const uint3
               return r;
           },
           [&](uint32_t i, const Request& r, bool yes, const uint32_t* pages) {
-              if (served) served[i] = yes;
-              if (!yes) return;
-              for (uint32_t j = 0; j < r.need; j++) {
-                  const uint32_t p = pages[j];
-                  c.page_table[(uint64_t)r.seq * c.max_pages + r.y + j] = p;
+              auto take = [&](uint32_t seq, uint32_t at, uint32_t p) {
+                  c.page_table[(uint64_t)seq * c.max_pages + at] = p;
                   c.page_refs[p] = 1;
+              };
+              if (served && i < n) served[i] = yes;
+              // a lane takes its own request's pages, one every 0.11 us, or the wave does
+              // it for a few long ones, one request after the other, 0.3 us and more each
+              // (one request for 8192 pages 906 -> 22 us, 32 for 256 each 55 -> 25; 1024
+              // for 8 pages 26 us, by waves 42)
+              const bool lengthy = yes && r.need > 16;
+              const bool wide = lengthy && r.need > 4u * (uint32_t)__popcll(__ballot(lengthy));
+              if (yes && !wide)
+                  for (uint32_t j = 0; j < r.need; j++) take(r.seq, r.y + j, pages[j]);
+              for (uint64_t m = __ballot(wide); m; m &= m - 1) {
+                  const uint32_t l = __builtin_ctzll(m), lane = threadIdx.x & 63;
+                  const uint32_t seq = __shfl(r.seq, l), at = __shfl(r.y, l), need = __shfl(r.need, l);
+                  const uint32_t* from = reinterpret_cast<const uint32_t*>(__shfl(reinterpret_cast<uintptr_t>(pages), l));
+                  for (uint32_t j = lane; j < need; j += 256) {
+                      uint32_t x[4];
+#pragma unroll
+                      for (uint32_t k = 0; k < 4; k++) x[k] = from[min(j + k * 64, need - 1)];
+#pragma unroll
+                      for (uint32_t k = 0; k < 4; k++)
+                          if (j + k * 64 < need) take(seq, at + j + k * 64, x[k]);
+                  }
               }
-              if (r.x > c.kv_len[r.seq]) c.kv_len[r.seq] = r.x;
+              if (yes && r.x > c.kv_len[r.seq]) c.kv_len[r.seq] = r.x;
           });
 }
 
@@ -348,6 +368,7 @@ k_pages_fork_plan(ane_paged_cache c, uint32_t n, const uint32_t* src, const uint
               return Request{b, len % c.page_size != 0, len, 0};
           },
           [&](uint32_t i, const Request& r, bool yes, const uint32_t* pages) {
+              if (i >= n) return;
               if (served) served[i] = yes;
               w.req_len[i] = yes ? r.x : 0;
               w.req_page[i] = yes && r.need ? pages[0] : ANE_NO_PAGE;

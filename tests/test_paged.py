@@ -851,6 +851,29 @@ def test_many_requests(ane):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("need", [[8192], [5000, 1, 17, 0, 300, 16, 2], [70] * 40 + [400], [18] * 64 + [65, 257, 1]])
+def test_reserve_long_rows(ane, need):
+    """Requests for many pages, among short ones: the pages of the pool in order."""
+    import torch
+
+    total, n, wide = sum(need), len(need), max(need)
+    c = PagedCache.empty(1, 1, 1, 64, 16, total + 40, n + 2, wide)
+    taken = random.Random(n).sample(range(total + 40), 40)
+    c.page_refs[i32(taken).long()] = 1
+    order = random.Random(n + 1).sample(range(n + 2), n)
+    served = i32([7] * n)
+    ane.pages_reserve(c, i32(order), i32([16 * m - (m > 0) for m in need]), served)
+    free = [p for p in range(total + 40) if p not in set(taken)]
+    want = np.full((n + 2, wide), NO_PAGE, np.int32)
+    for s, m in zip(order, need):
+        want[s, :m], free = free[:m], free[m:]
+    assert served.tolist() == [1] * n and not free
+    assert np.array_equal(c.page_table.cpu().numpy(), want)
+    assert bool((c.page_refs == 1).all())
+    assert [int(x) for x in c.kv_len.cpu()[order]] == [16 * m - (m > 0) for m in need]
+
+
+@pytest.mark.gpu
 def test_pools_past_one_look(ane):
     """More pages than the planning workgroup looks at at a time (65536)."""
     P = 140001
