@@ -20,10 +20,11 @@ inline int cache_status(const ane_paged_cache* c) {
         c->n_heads / c->n_kv_heads > 128 || c->n_kv_heads > 4096 || (c->head_dim != 64 && c->head_dim != 128) ||
         c->page_size == 0 || c->page_size % 16 != 0 || c->page_size > (1u << 20) || c->n_pages == 0 ||
         c->n_pages >= (1u << 31) || c->n_seqs == 0 || c->n_seqs >= (1u << 31) || c->max_pages == 0 ||
-        page_cap(c) >= (1ull << 31))
+        page_cap(c) > (1ull << 30))
         return ANE_ERR_INVALID_ARG;
     if (!c->k_pages || !c->v_pages || !c->page_table || !c->kv_len) return ANE_ERR_BAD_POINTER;
     if ((((uintptr_t)c->k_pages) | ((uintptr_t)c->v_pages)) & 15) return ANE_ERR_INVALID_ARG;
+    if ((((uintptr_t)c->page_table) | ((uintptr_t)c->kv_len) | ((uintptr_t)c->page_refs)) & 3) return ANE_ERR_INVALID_ARG;
     return ANE_OK;
 }
 

@@ -224,7 +224,7 @@ struct ane_paged_cache {
     uint32_t page_size;   /* positions a page: a multiple of 16, at most 2^20 */
     uint32_t n_pages;     /* pages in the pool, below 2^31 */
     uint32_t n_seqs;      /* rows of page_table */
-    uint32_t max_pages;   /* entries a row; max_pages * page_size below 2^31 */
+    uint32_t max_pages;   /* entries a row; max_pages * page_size at most 2^30 */
     uint16_t* k_pages;    /* fp16 [n_layers][n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned */
     uint16_t* v_pages;    /* the same shape */
     uint32_t* page_table; /* [n_seqs][max_pages] */

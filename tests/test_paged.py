@@ -91,6 +91,15 @@ def test_every_call_refuses_a_bad_cache(kw):
     assert L.ane_hip_attention_shared_workspace_size(b, 2, 0, 0, 0) == 0
 
 
+@pytest.mark.parametrize("kw", [dict(table_ptr=P + 2), dict(len_ptr=P + 1), dict(refs_ptr=P + 2),
+                                dict(max_pages=(1 << 26) + 1)], ids=["table", "lengths", "counts", "positions"])
+def test_misaligned_arrays_and_too_many_positions_are_refused(kw):
+    """Counts and lengths are changed by atomics, which need whole words; keys
+    are numbered in 31 bits with room for the tiles past the last."""
+    test_every_call_refuses_a_bad_cache(kw)
+    assert ane_amd.lib().ane_hip_pages_workspace_size(ctypes.byref(raw_cache(max_pages=1 << 26))) > 0
+
+
 @pytest.mark.parametrize("ptr", ["k_ptr", "v_ptr", "table_ptr", "len_ptr"])
 def test_missing_cache_arrays_are_refused(ptr):
     c = raw_cache(**{ptr: 0})
