@@ -353,7 +353,8 @@ struct Rows {
             // 2^(140 - ex) brings the largest |q| (exponent field ex) to [2^13, 2^14)
             const uint32_t ex = max(__float_as_uint(top) >> 23, 20u);
             const float up = __uint_as_float((267 - ex) << 23);
-            c *= __uint_as_float((ex - 13) << 23);
+            // (never 0 nor infinite: -inf, a masked score, and 0, that of a zero, times it stay as they are)
+            c = __builtin_amdgcn_fmed3f(c * __uint_as_float((ex - 13) << 23), 0x1p-126f, 0x1p127f);
 #pragma unroll
             for (int s = 0; s < NS; s++)
 #pragma unroll

@@ -522,6 +522,25 @@ def test_extreme_queries(ane, heads, kv, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,n", [(4, 1, 40), (32, 8, 1100)])
+def test_scales_at_the_ends(ane, heads, kv, n):
+    """Queries of zeros or of tiny values under a tiny scale, and large ones of
+    keys that are zeros under a large scale: every score is 0 (or as good as 0),
+    and masked keys stay masked."""
+    c = make_cache([n + 30], heads, kv, 64, 16, seed=n)
+    q = randq(n, heads, 64, dt("f32"), seed=2) * 1e-38
+    q[::2] = 0
+    out = q.new_empty(q.shape)
+    for scale in (1e-12, 1e-37):
+        start = run_prompt(c, [n], q, out, scale=scale)
+        check_prompt(c, [n], q, out, start, scale=scale)
+    c.k_pages.nan_to_num_(nan=0.0).mul_(0.0)
+    q = randq(n, heads, 64, dt("f32"), seed=3) * 2.0 ** 110
+    start = run_prompt(c, [n], q, out, scale=9e29)
+    check_prompt(c, [n], q, out, start, scale=9e29)
+
+
+@pytest.mark.gpu
 def test_pages_past_32_bit_offsets(ane):
     """A pool of more than 4 GiB: the pages in use sit at its end."""
     import torch
