@@ -1004,7 +1004,8 @@ class PagedCache(ctypes.Structure):
     """Mirror of struct ane_paged_cache (include/ane_decode.h), over device
     tensors that it keeps alive: k_pages, v_pages fp16 [layers][pages][kv heads]
     [page size][head dim], page_table int32 [sequences][max pages] (NO_PAGE in
-    unused entries), kv_len int32 [sequences], page_refs int32 [pages]."""
+    unused entries), kv_len int32 [sequences], page_refs int32 [pages].  Calls
+    go to these tensors: write into them, a new one needs a new PagedCache."""
 
     _fields_ = [(n, ctypes.c_uint32) for n in ("n_layers", "n_heads", "n_kv_heads", "head_dim", "page_size", "n_pages",
                                                 "n_seqs", "max_pages")] + [
@@ -1033,7 +1034,7 @@ class PagedCache(ctypes.Structure):
         self._at = ctypes.addressof(self)
         self._q, self._kv = (n_heads, head_dim), (n_kv, head_dim)
         self._scale = head_dim ** -0.5
-        self._device = k_pages.device.index if k_pages.device.type == "cuda" else None
+        self._device = k_pages.get_device()  # -1: not on a GPU, and no call takes it
         self._types = {torch.float32: 0, torch.float16: 1}
         self._int32 = torch.int32
         self._cuda = torch.cuda
@@ -1056,6 +1057,8 @@ def _rows(t, width, cache, what):
     tokens, *rest = t.shape
     if tuple(rest) != width:
         raise ValueError(f"{what} is [tokens][{width[0]}][{width[1]}]")
+    if t.get_device() != cache._device:
+        raise ValueError(f"{what} is on the cache's device")
     ty = cache._types.get(t.dtype)
     if ty is None:
         raise ValueError(f"{what} is float32 or float16")
@@ -1069,14 +1072,16 @@ def _ints(t, n, cache, what):
     """The pointer of a device array of at least n int32, or None."""
     if t is None:
         return None
-    if t.dtype != cache._int32 or not t.is_contiguous() or t.numel() < n:
-        raise ValueError(f"{what} is a contiguous int32 tensor of {n} entries")
+    if t.dtype != cache._int32 or not t.is_contiguous() or t.numel() < n or t.get_device() != cache._device:
+        raise ValueError(f"{what} is a contiguous int32 tensor of {n} entries on the cache's device")
     return t.data_ptr()
 
 
 def _launch(fn, cache, what, stream, args):
     """fn(*args, stream) on the cache's device and, unless given, its current stream."""
-    if cache._device is None or cache._device == cache._cuda.current_device():
+    if cache._device < 0:
+        raise ValueError("the cache is not in GPU memory")
+    if cache._device == cache._cuda.current_device():
         st = fn(*args, _stream_on(cache, stream))
     else:
         with cache._cuda.device(cache._device):
@@ -1086,7 +1091,7 @@ def _launch(fn, cache, what, stream, args):
 
 
 def _stream_on(cache, stream):
-    if stream is None and cache._device is not None:
+    if stream is None:
         import torch
 
         return torch._C._cuda_getCurrentRawStream(cache._device)
@@ -1104,8 +1109,12 @@ def _batch(q_start, seqs, rows, cache):
 def _work(cache, workspace, need, stream):
     """(workspace, pointer, bytes): the caller's, or a temporary one of need() bytes (the tensor has to
     live until the call is queued)."""
+    if cache._device < 0:
+        raise ValueError("the cache is not in GPU memory")
     if workspace is None:
         workspace = _scratch(need(), cache.k_pages.device, stream)
+    elif workspace.get_device() != cache._device or not workspace.is_contiguous():
+        raise ValueError("the workspace is contiguous, on the cache's device")
     return workspace, workspace.data_ptr(), workspace.nbytes
 
 
@@ -1132,8 +1141,9 @@ def paged_rope_append(cache, layer, q_start, q, k, v, table, q_out, seqs=None, s
     tp, positions = None, 0
     if table is not None:
         positions = table.shape[0]
-        if cache._types.get(table.dtype) != 0 or not table.is_contiguous() or table.numel() != positions * cache._q[1]:
-            raise ValueError("table is a contiguous float32 [positions][head_dim/2][2]")
+        if (cache._types.get(table.dtype) != 0 or not table.is_contiguous()
+                or table.numel() != positions * cache._q[1] or table.get_device() != cache._device):
+            raise ValueError("table is a contiguous float32 [positions][head_dim/2][2] on the cache's device")
         tp = table.data_ptr()
     _launch(lib().ane_hip_paged_rope_append, cache, "paged_rope_append", stream,
             (cache._at, layer, sq, n, qs, tokens, ty, qp, q0, kp, vp, ks, tp, positions, to, op, o0))

@@ -182,6 +182,23 @@ def test_wrappers_refuse_wrong_tensors():
         ane_amd.pages_fork(c, lens, lens[:2])
 
 
+def test_wrappers_refuse_a_cache_in_host_memory():
+    """An address of host memory never reaches a kernel."""
+    import torch
+
+    k = torch.zeros(1, 4, 2, 16, 64, dtype=torch.float16)
+    ints = [torch.zeros(n, dtype=torch.int32) for n in (3, 4)]
+    c = PagedCache(4, k, k, torch.zeros(3, 2, dtype=torch.int32), *ints)
+    q, qs = torch.zeros(5, 4, 64), torch.tensor([0, 2, 4, 5], dtype=torch.int32)
+    for call in (lambda: ane_amd.attention_prompt(c, 0, qs, q, q), lambda: ane_amd.attention_shared(c, 0, q, q),
+                 lambda: ane_amd.paged_rope_append(c, 0, qs, None, q[:, :2], q[:, 2:], None, None),
+                 lambda: ane_amd.pages_reserve(c, qs, qs), lambda: ane_amd.pages_fork(c, qs, qs),
+                 lambda: ane_amd.pages_free(c, qs), lambda: ane_amd.pages_copy(c, qs, qs),
+                 lambda: ane_amd.pages_compact(c)):
+        with pytest.raises(ValueError, match="not in GPU memory"):
+            call()
+
+
 # ------------------------------------------------------------------ helpers
 def i32(v):
     import torch
@@ -1054,6 +1071,31 @@ def test_captured_calls_follow_lengths_and_tables(ane):
         out.fill_(3.0)
         ane.attention_shared(c, 0, q, out, group_start=gs, prefix_len=pl, max_prefix=384, max_len=384)
         assert bool((out == got).all())
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_tensors_of_another_device(ane):
+    """A tensor in host memory among those of a cache on the GPU."""
+    import torch
+
+    c = make_cache([40, 20], 4, 2, 64, 16, fill_rest=0.0)
+    q, n2 = randq(3, 4, 64, dt("f32")), i32([0, 1])
+    qs, ws = i32([0, 2, 3]), torch.zeros(1 << 20, dtype=torch.uint8)
+    table = torch.zeros(64, 32, 2)
+    for call in (lambda: ane.attention_prompt(c, 0, qs.cpu(), q, q), lambda: ane.attention_prompt(c, 0, qs, q.cpu(), q),
+                 lambda: ane.attention_prompt(c, 0, qs, q, q.cpu()), lambda: ane.attention_prompt(c, 0, qs, q, q, workspace=ws),
+                 lambda: ane.attention_prompt(c, 0, qs, q, q, seqs=n2.cpu()),
+                 lambda: ane.attention_shared(c, 0, q, q, seqs=qs.cpu()),
+                 lambda: ane.attention_shared(c, 0, q, q, group_start=n2, prefix_len=n2.cpu()),
+                 lambda: ane.paged_rope_append(c, 0, qs, q, q[:, :2], q[:, 2:], table, q),
+                 lambda: ane.paged_rope_append(c, 0, qs, None, q[:, :2].cpu(), q[:, 2:].cpu(), None, None),
+                 lambda: ane.pages_reserve(c, n2, n2.cpu()), lambda: ane.pages_fork(c, n2, n2, n2.cpu()),
+                 lambda: ane.pages_free(c, n2.cpu()), lambda: ane.pages_copy(c, n2, n2.cpu()),
+                 lambda: ane.pages_compact(c, n_live=n2.cpu()), lambda: ane.pages_compact(c, workspace=ws)):
+        with pytest.raises(ValueError, match="device"):
+            call()
+    with pytest.raises(ValueError):
+        PagedCache(4, c.k_pages, c.v_pages, c.page_table.cpu(), c.kv_len)
 
 
 @pytest.mark.gpu
