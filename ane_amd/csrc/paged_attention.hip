@@ -225,22 +225,28 @@ struct Loader {
     // the wait for the numbers here, not before each copy that follows
     __device__ __forceinline__ void settle() { asm volatile("" : "+v"(ids)); }
     // 16 rows of x from group u (wave-uniform) on, whose page number is in lane `from`, of kv head g
-    // (nt: of keys no other workgroup reads)
-    template <bool NT = false>
-    __device__ __forceinline__ void copy(const AttnArgs& a, const uint16_t* x, const Work& w, uint32_t g, uint32_t u,
-                                         uint32_t from, uint8_t* dst) const {
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t group(const AttnArgs& a, const uint16_t* x, const Work& w, uint32_t g,
+                                                            uint32_t u, uint32_t from) const {
         const uint32_t id = __builtin_amdgcn_readlane(ids, from);
         const uint32_t row = u * 16 - page(a, u) * a.ps;
         const int32_t left = w.kend - (int32_t)(u * 16);
         // (a clamp goes through the vector ALU: back to a scalar, as above)
         const uint32_t bytes = __builtin_amdgcn_readfirstlane(id < a.n_pages ? (uint32_t)min(max(left, 0), 16) * RB : 0);
         const uint64_t at = (((uint64_t)(id < a.n_pages ? id : 0) * a.n_kv + g) * a.ps + row) * HD;
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(x + at, bytes);
+        return make_rsrc(x + at, bytes);
+    }
+    // 1 KB of such a group (nt: of keys no other workgroup reads)
+    template <bool NT = false>
+    __device__ __forceinline__ void copy(__amdgpu_buffer_rsrc_t r, uint32_t i, uint8_t* dst) const {
+        if constexpr (NT) copy16_to_lds_nt(r, dst + i * 1024, off[i]);
+        else copy16_to_lds(r, dst + i * 1024, off[i]);
+    }
+    template <bool NT = false>
+    __device__ __forceinline__ void copy(const AttnArgs& a, const uint16_t* x, const Work& w, uint32_t g, uint32_t u,
+                                         uint32_t from, uint8_t* dst) const {
+        const __amdgpu_buffer_rsrc_t r = group(a, x, w, g, u, from);
 #pragma unroll
-        for (uint32_t i = 0; i < kCopies; i++) {
-            if constexpr (NT) copy16_to_lds_nt(r, dst + i * 1024, off[i]);
-            else copy16_to_lds(r, dst + i * 1024, off[i]);
-        }
+        for (uint32_t i = 0; i < kCopies; i++) copy<NT>(r, i, dst);
     }
 };
 
@@ -394,8 +400,8 @@ struct Rows {
     struct Weights {  // of 32 KT keys: the B operands of 16-key products
         h8 h[2 * KT], l[F32 ? 2 * KT : 1];
     };
-    template <int KT>
-    __device__ __forceinline__ void scores(const uint8_t* k, f16v (&s)[KT]) const {
+    template <int KT, class Between>
+    __device__ __forceinline__ void scores(const uint8_t* k, f16v (&s)[KT], Between between) const {
         const uint32_t kx = swz<HD>(ka & 15);
         auto frag = [&](int i) {  // products in the order (chunk e, block t)
             const int e = i / KT, t = i % KT;
@@ -415,13 +421,14 @@ struct Rows {
             s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], qh[e], s[t], 0, 0, 0);
             if constexpr (F32) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % kAhead], ql[e], s[t], 0, 0, 0);
             if (i + kAhead < NS * KT) kf[i % kAhead] = frag(i + kAhead);
+            between(i);
             __builtin_amdgcn_sched_barrier(0);
         }
         products(false);
     }
     // Scores of keys from position t0 on to weights; keys before lo are masked.
-    template <int KT>
-    __device__ __forceinline__ void weights(f16v (&s)[KT], int32_t t0, int32_t lo, Weights<KT>& p) {
+    template <int KT, class Between>
+    __device__ __forceinline__ void weights(f16v (&s)[KT], int32_t t0, int32_t lo, Weights<KT>& p, Between between) {
         if (t0 + 32 * KT > wmin || t0 < lo) {  // uniform
             asm volatile("");  // a branch, not two selects a score in every tile
 #pragma unroll
@@ -468,6 +475,7 @@ struct Rows {
                 asm volatile("" : "+v"(l));  // here: put off, the sums would keep all weights alive
                 p.h[2 * t + r / 8][r % 8] = hi.x;
                 p.h[2 * t + r / 8][r % 8 + 1] = hi.y;
+                between(t * 8 + r / 2);
             }
     }
     __device__ __forceinline__ void first_values(const uint8_t* v, h8 (&vf)[kAhead]) const {
@@ -492,8 +500,8 @@ struct Rows {
         f16v s[KT];
         Weights<KT> p;
         h8 vf[kAhead];
-        scores<KT>(k, s);
-        weights<KT>(s, t0, lo, p);
+        scores<KT>(k, s, [](int) {});
+        weights<KT>(s, t0, lo, p, [](int) {});
         first_values(v, vf);
         values<KT>(v, vf, p);
     }
@@ -680,16 +688,21 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
 
 // Few rows: 32 a workgroup, all of them in every wave; the waves take every
 // fourth block of 32 keys each, through tiles of their own (no barrier until the
-// end), and are merged through LDS.  A tile has one stage: K of the next block is
-// copied once the scores have read this one's, V once the sums have, so that two
-// workgroups fit a CU and one's start hides behind the other.
+// end), and are merged through LDS.  A tile has one stage, so that two workgroups
+// fit a CU and one's start hides behind the other: V of a block is copied during
+// its scores, K of the next during its weights.  The copies go out one at a time
+// between those instructions: a CU takes 1 KB to LDS every 16 cycles, and a wave
+// that issued all eight at once, among seven others, stood 600 cycles a block
+// (2 chunks of 96 tokens after 8000 positions 59 -> 55 us, 64 sequences behind
+// 8192 shared positions 48.5 -> 45.5 in a graph).
 template <int HD>
 constexpr uint32_t few_lds() {  // K and V of four waves (or their sums), and their maxima and sums of weights
     return 8 * 32 * HD * 2 + 1024;
 }
 template <int HD, bool F32, int MODE>
 __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint32_t part, uint32_t g, uint8_t* smem) {
-    constexpr uint32_t kT = 32 * HD * 2, kC = 2 * Loader<HD>::kCopies;
+    constexpr uint32_t kT = 32 * HD * 2;
+    constexpr int kC = 2 * Loader<HD>::kCopies;
     float4* oo = reinterpret_cast<float4*>(smem);
     float *sm = reinterpret_cast<float*>(smem + 8 * kT), *sl = sm + 128;
     const uint32_t wave = block_wave(), lane = threadIdx.x & 63;
@@ -715,11 +728,20 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
     const int32_t first = w.kbeg + (int32_t)wave * 32;
     const uint32_t tiles = w.kend > first ? (uint32_t)(w.kend - first + 127) / 128 : 0;
     uint8_t *kt = smem + wave * 2 * kT, *vt = kt + kT;
-    auto issue = [&](const uint16_t* x, uint32_t t, uint8_t* dst) {
-#pragma unroll
-        for (uint32_t i = 0; i < 2; i++) ld.template copy<MODE == kOwn>(a, x, w, g, u0 + t * 8 + i, (t & 31) * 2 + i, dst + i * (kT / 2));
+    struct Next {  // a block's two groups
+        __amdgpu_buffer_rsrc_t g[2];
     };
-    if (tiles) issue(a.kp, 0, kt), issue(a.vp, 0, vt);
+    auto aim = [&](const uint16_t* x, uint32_t t) {
+        return Next{ld.group(a, x, w, g, u0 + t * 8, (t & 31) * 2), ld.group(a, x, w, g, u0 + t * 8 + 1, (t & 31) * 2 + 1)};
+    };
+    auto copy = [&](const Next& n, int i, uint8_t* dst) {
+        ld.template copy<MODE == kOwn>(n.g[2 * i / kC], i % (kC / 2), dst + 2 * i / kC * (kT / 2));
+    };
+    if (tiles) {
+        const Next n = aim(a.kp, 0);
+#pragma unroll
+        for (int i = 0; i < kC; i++) copy(n, i, kt);
+    }
     r.init(a.scale_log2e, row_limit<MODE>(a, w, tok), live);
     r.take_q(raw);
     __builtin_amdgcn_sched_barrier(0);
@@ -728,24 +750,24 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
     int32_t odd_from = 0x7fffffff, odd_to = 0;
     for (uint32_t t = 0; t < tiles; t++) {
         const int32_t t0 = first + (int32_t)t * 128;
-        const bool more = t + 1 < tiles;
         f16v s[1];
         h8 vf[Rows<HD, F32>::kAhead];
         typename Rows<HD, F32>::template Weights<1> p;
-        wait_vmcnt<kC>();  // K of this block has landed, V may be on its way
-        r.template scores<1>(kt, s);
+        wait_vmcnt<0>();  // K of this block
+        const Next vn = aim(a.vp, t);
+        r.template scores<1>(kt, s, [&](int i) {
+            if (i < kC) copy(vn, i, vt);
+        });
         wait_lgkmcnt0();
-        if (more) {
-            if (((t + 1) & 31) == 0) {
-                wait_vmcnt<0>();
-                ld.lookup(a, w.id, u0 + (t + 1 + lane / 2) * 8 + (lane & 1));
-                ld.settle();
-            }
-            issue(a.kp, t + 1, kt);
+        if (t + 1 < tiles && ((t + 1) & 31) == 0) {
+            ld.lookup(a, w.id, u0 + (t + 1 + lane / 2) * 8 + (lane & 1));
+            ld.settle();
         }
-        r.template weights<1>(s, t0, w.lo, p);
-        if (more) wait_vmcnt<kC>();
-        else wait_vmcnt<0>();
+        const Next kn = aim(a.kp, t + 1);  // past the last: no extent, zeros that nobody reads
+        r.template weights<1>(s, t0, w.lo, p, [&](int i) {
+            if (i < kC) copy(kn, i, kt);
+        });
+        wait_vmcnt<kC>();  // V of this block
         if (t0 + 32 > r.wmin || t0 < w.lo) {
             const bool b0 = tidy<HD>(vt), b1 = tidy<HD>(vt + kT / 2);
             if (b0 || b1) odd_from = min(odd_from, t0), odd_to = t0 + 32;
@@ -754,11 +776,11 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
         r.first_values(vt, vf);
         r.template values<1>(vt, vf, p);
         wait_lgkmcnt0();
-        if (more) issue(a.vp, t + 1, vt);
     }
     // (this wave's keys of that range only: the other waves add their own)
     for (int32_t t0 = odd_from; t0 < odd_to; t0 += 128) r.add_nonfinite(a, w, g, t0, t0 + 32);
 
+    wait_vmcnt<0>();
     // Merge the four waves: each puts its sums into LDS as its lanes hold them
     // (a unit of four dimensions is 1 KB, so nothing conflicts) and takes a
     // quarter of the units of all four back.
