@@ -934,25 +934,31 @@ struct Launch {
 // units: sequences (groups) of the launch; tokens: theirs in all; single: one
 // token each; beside: shares its launch with the batch's own keys.
 //
-// 32 rows a workgroup up to 1024 rows a sequence on average, and wherever 128 rows
-// a workgroup would leave CUs without one (512 tokens x 32 heads 23.5 us, 29 with
-// 128; 16 chunks of 64 tokens after 2000 positions 55, 68; 2048 tokens 108, 89,
-// since the four waves read every K and V tile for themselves).  Few rows and many
-// keys: the keys in parts, as many as fill the 512 places (two workgroups a CU) at
-// once but not more: a second, part-filled round costs more than the longer
-// parts (200 tokens after 4000 positions 51 us, in 1.5 times the parts 63).
-// A prefix beside its batch's own keys takes half the places (four 64-wide
-// workgroups fit a CU): 8 groups of 8 sequences 48 -> 42 us.  128-row workgroups
-// are more than the CUs as it is, and their keys stay whole.
+// 32 rows a workgroup as long as its workgroups have a place each (512 of them, two
+// a CU; four a CU 64-wide), half again as many for one sequence, where 128 rows a
+// workgroup would leave most CUs idle: 512 tokens x 32 heads fp32 23 us, 29 with
+// 128 rows; 768 tokens 32, 37; 8 chunks of 64 tokens after 1000 positions 35, 47.
+// Beyond that 128 rows, since the four waves of the other kernel read every K and
+// V tile for themselves: 2 x 400 tokens 26 us, 32 with 32 rows; 16 x 256 tokens
+// 49, 90.  Sequences of 64 rows and less would leave half of such a tile empty:
+// single tokens, and 64 chunks of 16 tokens after 1000 positions (87 us, with 128
+// rows 89).  Few rows and many keys: the keys in parts, as many as fill the
+// places at once but not more: a second, part-filled round costs more than the
+// longer parts (200 tokens after 4000 positions 51 us, in 1.5 times the parts 63).
+// A prefix beside its batch's own keys takes half the places (three or four
+// 64-wide workgroups fit a CU): 8 groups of 8 sequences 48 -> 42 us.  128-row
+// workgroups are more than the CUs as it is, and their keys stay whole.
 Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len, bool beside = false) {
     Launch l;
     const uint64_t G = c->n_heads / c->n_kv_heads, rows = tokens * G;
-    l.few = rows <= 1024 * units || rows * c->n_kv_heads <= 256 * 128;
+    // of equally long sequences
+    auto wgs = [&](uint64_t bm) { return (rows + units * bm - 1) / (units * bm) * units * c->n_kv_heads; };
+    const uint64_t room = 512 * 128 / c->head_dim;
+    l.few = single || wgs(32) <= (units == 1 ? room + room / 2 : room) || wgs(32) < 3 * wgs(128);
     const uint64_t bm = l.few ? 32 : 128;
     l.slots = single ? units * ((G + bm - 1) / bm) : rows / bm + units;
-    const uint64_t wgs = (rows + units * bm - 1) / (units * bm) * units * c->n_kv_heads;  // of equally long sequences
     const uint64_t places = beside && c->head_dim == 128 ? 256 : 512;
-    const uint64_t n = std::max<uint64_t>(1, l.few ? std::min(places / wgs, (max_len + 255) / 256) : 1);
+    const uint64_t n = std::max<uint64_t>(1, l.few ? std::min(places / wgs(32), (max_len + 255) / 256) : 1);
     l.chunk = (uint32_t)(((max_len + n - 1) / n + 127) / 128 * 128);
     l.parts = (uint32_t)((max_len + l.chunk - 1) / l.chunk);
     return l;

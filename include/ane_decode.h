@@ -238,9 +238,11 @@ struct ane_paged_cache {
  * rows q_start[i] .. q_start[i+1]-1 of the activations (ascending, q_start[n]
  * <= n_tokens), its last positions: token t of m sits at kv_len - m + t.
  * q_start NULL: one new token a row.  Rows from q_start[n] on are left as they
- * were.  At most 2^23 tokens a call.  Strides are in elements from one token
- * to the next; a token's heads are contiguous.  q, k, v, q_out and out are
- * 16-byte aligned and their strides multiples of 16 bytes. */
+ * were.  At most 2^23 tokens a call; attention also refuses a batch of more
+ * workgroups than a launch takes (2^23: some 2^20 sequences on 8 kv heads).
+ * Strides are in elements from one token to the next; a token's heads are
+ * contiguous.  q, k, v, q_out and out are 16-byte aligned and their strides
+ * multiples of 16 bytes. */
 
 /* RoPE of q and k (adjacent pairs, the fp32 operations of
  * ane_hip_rope_kv_append) and the append of k and v, rounded to fp16, to the
@@ -261,7 +263,8 @@ int ane_hip_paged_rope_append(const struct ane_paged_cache* cache, uint32_t laye
 /* Causal attention of packed prompts with grouped heads: for each new token at
  * position p, out[h] = softmax(scale * q[h] . K[g][0..p]^T) V[g][0..p],
  * g = h / (n_heads / n_kv_heads); zeros for a token at a negative position.
- * Keys a token does not see never touch its result, whatever they hold.
+ * Keys a token does not see never touch its result, whatever they hold; an
+ * infinity or NaN it does see may make its result infinite or NaN.
  * type: of q and out.  F32: products of fp32 accuracy (q and the softmax
  * weights enter the matrix cores as two fp16 parts each); F16: q and the
  * weights are fp16.  Scores, softmax and sums are fp32 in both.  scale: positive,

@@ -414,6 +414,10 @@ SHAPES = [
     ("f32", 64, 32, 8, 48, [1300, 900], [14, 333]),
     ("f16", 64, 40, 8, 32, [1700, 3], [1, 0]),
     ("f16", 128, 36, 12, 16, [1001], [4200]),
+    ("f32", 128, 32, 8, 16, [256] * 9, [0, 3, 0, 17, 0, 0, 200, 0, 1]),
+    ("f16", 64, 32, 8, 16, [200] * 11, [0, 3, 0, 17, 0, 0, 200, 0, 1, 0, 0]),
+    ("f32", 64, 32, 8, 32, [33, 1, 30] * 8, [0, 700, 64] * 8),
+    ("f16", 128, 32, 8, 16, [16, 17] * 32, [100, 0] * 32),
 ]
 
 
@@ -539,7 +543,7 @@ def test_extreme_queries(ane, heads, kv, n):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("heads,kv,n", [(4, 1, 40), (32, 8, 1100)])
+@pytest.mark.parametrize("heads,kv,n", [(4, 1, 40), (32, 8, 1100), (96, 8, 600)])
 def test_scales_at_the_ends(ane, heads, kv, n):
     """Queries of zeros or of tiny values under a tiny scale, and large ones of
     keys that are zeros under a large scale: every score is 0 (or as good as 0),
@@ -634,14 +638,15 @@ def test_shared(ane, ty, hd, heads, kv, ps, lens, bounds, prefixes):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("ty,hd,prefix,apart", [("f32", 128, 150, 0), ("f16", 64, 77, 9), ("f16", 128, 16, 299)])
-def test_shared_by_a_large_group(ane, ty, hd, prefix, apart):
-    """300 rows of 8 query heads a kv head: the prefix on 128 rows a workgroup.
+@pytest.mark.parametrize("ty,hd,prefix,apart,n", [("f32", 128, 150, 0, 300), ("f16", 64, 77, 9, 300), ("f16", 128, 16, 299, 300),
+                                                  ("f32", 64, 40, 0, 420), ("f16", 64, 200, 3, 420)])
+def test_shared_by_a_large_group(ane, ty, hd, prefix, apart, n):
+    """300 or 420 rows of 8 query heads a kv head: the prefix on 128 rows a workgroup.
     The first `apart` rows are in no group; two rows are shorter than the
     prefix."""
     import torch
 
-    n, heads, kv = 300, 128, 16
+    heads, kv = 128, 16
     lens = [prefix + 3 + i % 40 for i in range(n)]
     lens[40], lens[299] = prefix - 5, 1
     c = make_cache(lens, heads, kv, hd, 16, seed=6)
