@@ -588,10 +588,14 @@ __device__ __forceinline__ uint32_t block_wave() { return __builtin_amdgcn_readf
 // 64 keys on a 2-stage LDS ring (each wave copies one 16-key group of K and V a
 // tile).  Two workgroups a CU: while one wave of a SIMD is in its weights (some 650
 // vector cycles a 32-key block), the other is in its products (512 matrix cycles,
-// fp32 1024).  8192 tokens x 32 heads fp16: 550-570 us, 0.96-1.0 PFLOP/s, at the
-// 1.85 GHz the clock holds then (a library fp16 product of 8192^3: 1.1); fp32:
-// 0.59, so 1.18 of matrix work.  Weights between the products of the other half
-// in one wave measured slower (584), a ring of fragments of 2, 3 or 6 the same.
+// fp32 1024).  8192 tokens x 32 heads fp16: 560-590 us, 0.94-0.98 PFLOP/s, power
+// being the limit: on zeros it takes 436 us, and a library fp16 product of 8192^3
+// goes from 1.07 to 1.68 PFLOP/s; fp32: 0.59, so 1.18 of matrix work.  A workgroup
+// costs some 20000 cycles besides 5000 a tile and pair of workgroups (fp32), so
+// prompts of 250-1023 tokens take 120 us where their products alone would take 80.
+// Weights between the products of the other half in one wave measured slower
+// (584 us, 549 so), fragments 2, 3 or 6 ahead, the copies spread over the products,
+// and row tiles started in descending order of keys the same.
 template <int HD, bool F32, int MODE>
 __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slots) {
     constexpr uint32_t kT = 64 * HD * 2;
@@ -694,7 +698,10 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
 // between those instructions: a CU takes 1 KB to LDS every 16 cycles, and a wave
 // that issued all eight at once, among seven others, stood 600 cycles a block
 // (2 chunks of 96 tokens after 8000 positions 59 -> 55 us, 64 sequences behind
-// 8192 shared positions 48.5 -> 45.5 in a graph).
+// 8192 shared positions 48.5 -> 45.5 in a graph).  Single tokens are bound by
+// memory: 32 over 1000-4096 positions, 366 MB in 62 us, 5.9 TB/s; the others by
+// the chain of a block (copy, products, weights, products: some 2200 cycles, 3100
+// beside a second workgroup) and by 15000 cycles of start and merge.
 template <int HD>
 constexpr uint32_t few_lds() {  // K and V of four waves (or their sums), and their maxima and sums of weights
     return 8 * 32 * HD * 2 + 1024;
@@ -851,7 +858,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_shared(AttnArgs a, uint32_t pre
 // One wave per (token, head): the parts of its keys joined, o = sum o_c 2^(m_c - M).
 // Every part of every covered row has its (maximum, sum) written, (-inf, 0) where
 // it has no key, so nothing is looked up here: the pairs (one a lane) and the
-// first parts' sums are in flight at once.
+// first parts' sums are in flight at once.  Latency: 4-5 us, most of it the launch.
 template <int HD, bool F32, uint32_t kBatch>
 __global__ void __launch_bounds__(64) k_attn_join(AttnArgs a) {
     constexpr int E = HD / 64;
