@@ -1037,7 +1037,8 @@ class PagedCache(ctypes.Structure):
         self._device = k_pages.get_device()  # -1: not on a GPU, and no call takes it
         self._types = {torch.float32: 0, torch.float16: 1}
         self._int32 = torch.int32
-        self._cuda = torch.cuda
+        self._cuda, self._current = torch.cuda, torch._C._cuda_getDevice
+        self._raw_stream = torch._C._cuda_getCurrentRawStream
         self._pages_need = None
 
     @classmethod
@@ -1054,18 +1055,19 @@ class PagedCache(ctypes.Structure):
 
 def _rows(t, width, cache, what):
     """(pointer, type, tokens, row stride) of activations [tokens][heads][head_dim] whose heads are contiguous."""
-    tokens, *rest = t.shape
-    if tuple(rest) != width:
-        raise ValueError(f"{what} is [tokens][{width[0]}][{width[1]}]")
-    if t.get_device() != cache._device:
-        raise ValueError(f"{what} is on the cache's device")
+    heads, dim = width
+    tokens, h, d = t.shape if t.dim() == 3 else (0, 0, 0)
+    if h != heads or d != dim:
+        raise ValueError(f"{what} is [tokens][{heads}][{dim}]")
     ty = cache._types.get(t.dtype)
     if ty is None:
         raise ValueError(f"{what} is float32 or float16")
+    if t.get_device() != cache._device:
+        raise ValueError(f"{what} is on the cache's device")
     s0, s1, s2 = t.stride()
-    if (s2 != 1 or (s1 != width[1] and width[0] > 1)) and tokens:
+    if (s2 != 1 or (s1 != dim and heads > 1)) and tokens:
         raise ValueError(f"the heads of a token of {what} are contiguous")
-    return t.data_ptr(), ty, tokens, s0 if tokens > 1 else width[0] * width[1]
+    return t.data_ptr(), ty, tokens, s0 if tokens > 1 else heads * dim
 
 
 def _ints(t, n, cache, what):
@@ -1081,21 +1083,13 @@ def _launch(fn, cache, what, stream, args):
     """fn(*args, stream) on the cache's device and, unless given, its current stream."""
     if cache._device < 0:
         raise ValueError("the cache is not in GPU memory")
-    if cache._device == cache._cuda.current_device():
-        st = fn(*args, _stream_on(cache, stream))
+    if cache._device == cache._current():
+        st = fn(*args, cache._raw_stream(cache._device) if stream is None else _stream_handle(stream))
     else:
         with cache._cuda.device(cache._device):
-            st = fn(*args, _stream_on(cache, stream))
+            st = fn(*args, cache._raw_stream(cache._device) if stream is None else _stream_handle(stream))
     if st:
         check(st, what)
-
-
-def _stream_on(cache, stream):
-    if stream is None:
-        import torch
-
-        return torch._C._cuda_getCurrentRawStream(cache._device)
-    return _stream_handle(stream)
 
 
 def _batch(q_start, seqs, rows, cache):
