@@ -340,6 +340,42 @@ struct Rows {
 #pragma unroll
             for (auto& x : w.x) x = v4i{0, 0, 0, 0};
     }
+    // The same by whole rows: the loads above touch 64 cache lines each, with 16 bytes
+    // of every one.  Load i takes RB bytes of kRows rows, for each of the P parts of
+    // a row; at: the byte offset of lane & 31's row.
+    static constexpr uint32_t kRows = 1024 / RB, kLoads = 32 / kRows, P = F32 ? 2 : 1;
+    __device__ __forceinline__ void fetch_rows(const void* q, uint64_t at, Raw& w) const {
+        const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; i++) {
+            const uint32_t r = i * kRows + lane / (RB / 16);
+            const uint64_t row = (uint64_t)__shfl((uint32_t)(at >> 32), r, 64) << 32 | __shfl((uint32_t)at, r, 64);
+            const uint8_t* p = static_cast<const uint8_t*>(q) + row + lane % (RB / 16) * 16;
+#pragma unroll
+            for (uint32_t k = 0; k < P; k++) w.x[k * kLoads + i] = *reinterpret_cast<const v4i*>(p + k * RB);
+        }
+    }
+    // and through a tile of LDS to the lanes they belong to
+    __device__ __forceinline__ void turn_rows(uint8_t* st, bool live, Raw& w) const {
+        const uint32_t lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (uint32_t k = 0; k < P; k++) {
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; i++) {
+                const uint32_t x = i * kRows + lane / (RB / 16);
+                *reinterpret_cast<v4i*>(st + x * RB + (((lane % (RB / 16)) ^ swz<HD>(x & 15)) << 4)) = w.x[k * kLoads + i];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kLoads; j++) {
+                const uint32_t c = F32 ? 4 * (j / 2) + 2 * h + j % 2 : 2 * j + h;
+                w.x[k * kLoads + j] = *reinterpret_cast<const v4i*>(st + r * RB + ((c ^ swz<HD>(r & 15)) << 4));
+            }
+        }
+        wait_lgkmcnt0();
+        if (!live)
+#pragma unroll
+            for (auto& x : w.x) x = v4i{0, 0, 0, 0};
+    }
     __device__ __forceinline__ void take_q(const Raw& w) {
         if constexpr (!F32) {
 #pragma unroll
@@ -724,7 +760,9 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
     const uint32_t row = w.row0 + (lane & 31), tok = a.by_G(min(row, w.rows - 1));
     const uint32_t head = g * a.G + min(row, w.rows - 1) - tok * a.G;
     const bool live = row < w.rows;
-    r.fetch_q(a.q, (w.tok0 + tok) * a.q_stride + head * HD, live, raw);
+    const uint64_t at_q = (w.tok0 + tok) * a.q_stride + head * HD;
+    if constexpr (MODE == kOwn) r.fetch_q(a.q, at_q, live, raw);
+    else r.fetch_rows(a.q, at_q * (F32 ? 4 : 2), raw);
     find_keys<MODE>(a, 32, part, w);
     if (!early_keys<MODE>(a)) {
         u0 = (uint32_t)w.kbeg / 16 + wave * 2;
@@ -750,6 +788,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
         for (int i = 0; i < kC; i++) copy(n, i, kt);
     }
     r.init(a.scale_log2e, row_limit<MODE>(a, w, tok), live);
+    if constexpr (MODE != kOwn) r.turn_rows(vt, live, raw);
     r.take_q(raw);
     __builtin_amdgcn_sched_barrier(0);
     r.clear();
