@@ -131,32 +131,41 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a) {
 // -------------------------------------------------------- assigning pages
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kLook = 1 << 16;
 
-// Exclusive prefix sums over the workgroup's 1024 threads; *total: the sum.
-template <class T>
-__device__ __forceinline__ T block_scan(T v, T* total) {
-    __shared__ T sums[kPlanWaves];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    auto scan = [&](T x, int n) {
-        for (int off = 1; off < n; off <<= 1) {
-            const T o = __shfl_up(x, off, 64);
-            if (lane >= (uint32_t)off) x += o;
-        }
-        return x;
-    };
-    const T s = scan(v, 64);
+// Prefix sums over the workgroup's 1024 threads, this thread's value included;
+// *total: the sum.  Sums stop at kMany, more than any pool's pages.  Within a
+// wave by DPP shifts (a row of 16 lanes, then row 0 into 1 and 2 into 3, then the
+// first half into the second): as shuffles the three of a plan took 1.5 us.
+constexpr uint32_t kMany = 0x7fffffff;
+__device__ __forceinline__ uint32_t add_up(uint32_t a, uint32_t b) { return min(a + b, kMany); }
+template <int ctrl, int rows>
+__device__ __forceinline__ uint32_t add_shifted(uint32_t v) {
+    return add_up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = add_shifted<0x111, 0xf>(v);  // row_shr:1
+    v = add_shifted<0x112, 0xf>(v);
+    v = add_shifted<0x114, 0xf>(v);
+    v = add_shifted<0x118, 0xf>(v);
+    v = add_shifted<0x142, 0xa>(v);  // row_bcast:15
+    return add_shifted<0x143, 0xc>(v);  // row_bcast:31
+}
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* total) {
+    __shared__ uint32_t sums[kPlanWaves];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t s = wave_scan(v);
     if (lane == 63) sums[wave] = s;
     __syncthreads();
-    const T t = scan(lane < kPlanWaves ? sums[lane] : 0, kPlanWaves);  // the waves' sums, scanned by every wave
-    const T before = wave ? __shfl(t, wave - 1, 64) : 0;
-    *total = __shfl(t, kPlanWaves - 1, 64);
+    const uint32_t t = wave_scan(lane < kPlanWaves ? sums[lane] : 0);  // the waves' sums, scanned by every wave
+    const uint32_t before = wave ? __builtin_amdgcn_readlane(t, wave - 1) : 0;
+    *total = __builtin_amdgcn_readlane(t, kPlanWaves - 1);
     __syncthreads();
-    return before + s - v;
+    return add_up(before, s);
 }
 
 // The free pages as bits in LDS, 65536 pages a look: a smaller pool is looked at
 // once, however many passes a call makes over it.  Short loops on purpose: one
 // workgroup runs them once, and what it waits for is mostly code and the few
-// loads (unrolled over registers, the plan of a compaction took 13 us, not 7).
+// loads (unrolled over registers, the plan of a compaction took 13 us, not 6).
 struct Pool {
     const uint32_t* refs;
     uint32_t pages;
@@ -200,7 +209,7 @@ struct Pool {
             };
             uint32_t all;
             const uint32_t mine = threadIdx.x < masks ? __popcll(mask(threadIdx.x)) : 0;
-            before[threadIdx.x] = block_scan(mine, &all);
+            before[threadIdx.x] = block_scan(mine, &all) - mine;
             __syncthreads();
             for (uint32_t j = threadIdx.x >> 6; j < masks; j += kPlanWaves) {
                 const uint64_t m = mask(j);
@@ -274,29 +283,30 @@ __device__ __forceinline__ void serve(const ane_paged_cache& c, uint32_t n, Page
     __shared__ uint64_t bits[kPlanThreads];
     const uint32_t tid = threadIdx.x;
     const Pool pool = {c.page_refs, c.n_pages, bits, before_lds};
-    pool.look(0);
+    // (waves without a request are at the counts meanwhile)
     const Request mine = tid < n ? look(tid) : Request{ANE_NO_PAGE, 0, 0, 0};
+    pool.look(0);
     auto request = [&](uint32_t i) { return i == tid ? mine : look(i); };
     uint32_t* claim = c.n_seqs <= kLdsSeqs ? claim_lds : w.claim;
     claim_first(n, claim, [&](uint32_t i) { return request(i).seq; });
     auto valid = [&](uint32_t i, const Request& r) {
         return r.seq != ANE_NO_PAGE && __atomic_load_n(&claim[r.seq], __ATOMIC_RELAXED) == i;
     };
-    uint64_t total = 0;
+    uint32_t total = 0;
     for (uint32_t base = 0; base < n; base += kPlanThreads) {
         const uint32_t i = base + tid;
-        uint64_t k = 0, all;
+        uint32_t k = 0, all;
         if (i < n) {
             const Request r = request(i);
             if (valid(i, r)) k = r.need;
         }
         block_scan(k, &all);
-        total += all;
+        total = add_up(total, all);
     }
-    const uint32_t want = (uint32_t)min(total, (uint64_t)c.n_pages);
+    const uint32_t want = min(total, c.n_pages);
     uint32_t* list = want <= kLdsList ? list_lds : w.list;
     const uint32_t have = pool.pick(true, 0, c.n_pages, want, [&](uint32_t rank, uint32_t i) { list[rank] = i; });
-    uint64_t before = 0;
+    uint32_t before = 0;
     for (uint32_t base = 0; base < n; base += kPlanThreads) {
         const uint32_t i = base + tid;
         Request r = {ANE_NO_PAGE, 0, 0, 0};
@@ -305,10 +315,10 @@ __device__ __forceinline__ void serve(const ane_paged_cache& c, uint32_t n, Page
             r = request(i);
             ok = valid(i, r);
         }
-        uint64_t all;
-        const uint64_t r0 = before + block_scan<uint64_t>(ok ? r.need : 0, &all);
-        before += all;
-        done(i, r, ok && r0 + r.need <= have, list + r0);
+        uint32_t all;
+        const uint32_t end = add_up(before, block_scan(ok ? r.need : 0, &all));
+        before = add_up(before, all);
+        done(i, r, ok && end <= have && end < kMany, list + (end - (ok ? r.need : 0)));
     }
 }
 
@@ -333,8 +343,8 @@ k_pages_reserve(ane_paged_cache c, uint32_t n, const uint32_t* seqs, const uint3
               if (served && i < n) served[i] = yes;
               // a lane takes its own request's pages, one every 0.11 us, or the wave does
               // it for a few long ones, one request after the other, 0.3 us and more each
-              // (one request for 8192 pages 906 -> 22 us, 32 for 256 each 55 -> 25; 1024
-              // for 8 pages 26 us, by waves 42)
+              // (one request for 8192 pages 906 -> 20 us, 32 for 256 each 55 -> 23; 1024
+              // for 8 pages 24 us, by waves 42)
               const bool lengthy = yes && r.need > 16;
               const bool wide = lengthy && r.need > 4u * (uint32_t)__popcll(__ballot(lengthy));
               if (yes && !wide)

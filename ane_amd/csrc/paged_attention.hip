@@ -341,8 +341,11 @@ struct Rows {
             for (auto& x : w.x) x = v4i{0, 0, 0, 0};
     }
     // The same by whole rows: the loads above touch 64 cache lines each, with 16 bytes
-    // of every one.  Load i takes RB bytes of kRows rows, for each of the P parts of
-    // a row; at: the byte offset of lane & 31's row.
+    // of every one, and all four waves of 32-row workgroups make them (a prompt of 128
+    // tokens 13.6 -> 12.9 us in a graph; the few rows of single tokens share their
+    // lines, and beside a busy second workgroup 128 rows take as long either way).
+    // Load i takes RB bytes of kRows rows, for each of the P parts of a row; at: the
+    // byte offset of lane & 31's row.
     static constexpr uint32_t kRows = 1024 / RB, kLoads = 32 / kRows, P = F32 ? 2 : 1;
     __device__ __forceinline__ void fetch_rows(const void* q, uint64_t at, Raw& w) const {
         const uint32_t lane = threadIdx.x & 63;

@@ -924,6 +924,22 @@ def test_reserve_long_rows(ane, need):
 
 
 @pytest.mark.gpu
+def test_reserve_more_pages_than_32_bits_count(ane):
+    """Requests for 2^26 pages each, 40 of them behind two small ones."""
+    import torch
+
+    k = torch.zeros(1, 100, 1, 16, 64, dtype=torch.float16, device="cuda")
+    table = torch.empty(44, 1 << 26, dtype=torch.int32, device="cuda")
+    table[:, :8] = NO_PAGE
+    c = PagedCache(1, k, k.clone(), table, i32([0] * 44), i32([0] * 100))
+    served = i32([7] * 43)
+    ane.pages_reserve(c, i32(range(43)), i32([33, 5] + [1 << 30] * 40 + [1]), served)
+    assert served.tolist() == [1, 1] + [0] * 41
+    assert table[:2, :4].tolist() == [[0, 1, 2, -1], [3, -1, -1, -1]] and bool((table[2:, :8] == -1).all())
+    assert c.kv_len.tolist() == [33, 5] + [0] * 42 and int(c.page_refs.sum()) == 4
+
+
+@pytest.mark.gpu
 def test_pools_past_one_look(ane):
     """More pages than the planning workgroup looks at at a time (65536)."""
     P = 140001
