@@ -610,10 +610,11 @@ __device__ __forceinline__ void put4(void* out, uint64_t at, float4 x) {
 }
 
 // A row that no group has: nobody else writes its parts of the prefix launch.
-__device__ __forceinline__ void no_prefix(const AttnArgs& a, const Work& w, uint32_t g, uint32_t part, uint32_t rows) {
+__device__ __forceinline__ void no_prefix(const AttnArgs& a, const Work& w, uint32_t g, uint32_t part, uint32_t rows,
+                                          uint32_t thread, uint32_t threads) {
     if (part != 0 || !w.alone) return;
     const uint64_t all = (uint64_t)a.n_tokens * a.n_heads;
-    for (uint32_t i = threadIdx.x; i < a.pre.n * rows; i += 256) {
+    for (uint32_t i = thread; i < a.pre.n * rows; i += threads) {
         const uint32_t r = w.row0 + i % rows;
         const uint32_t t = a.by_G(r);
         const uint64_t pr = i / rows * all + (uint64_t)(w.tok0 + t) * a.n_heads + g * a.G + r - t * a.G;
@@ -745,19 +746,22 @@ template <int HD>
 constexpr uint32_t few_lds() {  // K and V of four waves (or their sums), and their maxima and sums of weights
     return 8 * 32 * HD * 2 + 1024;
 }
-template <int HD, bool F32, int MODE>
+// EACH: every wave has rows and keys of its own (slot and g differ by wave), so
+// there is nothing to merge.
+template <int HD, bool F32, int MODE, bool EACH = false>
 __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint32_t part, uint32_t g, uint8_t* smem) {
     constexpr uint32_t kT = 32 * HD * 2;
     constexpr int kC = 2 * Loader<HD>::kCopies;
     float4* oo = reinterpret_cast<float4*>(smem);
     float *sm = reinterpret_cast<float*>(smem + 8 * kT), *sl = sm + 128;
-    const uint32_t wave = block_wave(), lane = threadIdx.x & 63;
+    constexpr uint32_t kWaves = EACH ? 1 : 4;  // that share the keys, in turn a block of 32 each
+    const uint32_t wave = block_wave(), turn = EACH ? 0 : wave, lane = threadIdx.x & 63;
     Work w;
     if (!find_rows<MODE, 32>(a, slot, w)) return;
 
     Loader<HD> ld;
-    uint32_t u0 = part * (a.parts<MODE>().chunk / 16) + wave * 2;
-    if (early_keys<MODE>(a)) ld.lookup(a, w.id, u0 + lane / 2 * 8 + (lane & 1));
+    uint32_t u0 = part * (a.parts<MODE>().chunk / 16) + turn * 2;
+    if (early_keys<MODE>(a)) ld.lookup(a, w.id, u0 + lane / 2 * (2 * kWaves) + (lane & 1));
     Rows<HD, F32> r;
     typename Rows<HD, F32>::Raw raw;
     const uint32_t row = w.row0 + (lane & 31), tok = a.by_G(min(row, w.rows - 1));
@@ -768,19 +772,21 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
     else r.fetch_rows(a.q, at_q * (F32 ? 4 : 2), raw);
     find_keys<MODE>(a, 32, part, w);
     if (!early_keys<MODE>(a)) {
-        u0 = (uint32_t)w.kbeg / 16 + wave * 2;
-        ld.lookup(a, w.id, u0 + lane / 2 * 8 + (lane & 1));
+        u0 = (uint32_t)w.kbeg / 16 + turn * 2;
+        ld.lookup(a, w.id, u0 + lane / 2 * (2 * kWaves) + (lane & 1));
     }
     ld.settle();
     ld.init();
-    const int32_t first = w.kbeg + (int32_t)wave * 32;
-    const uint32_t tiles = w.kend > first ? (uint32_t)(w.kend - first + 127) / 128 : 0;
+    constexpr int32_t kStep = 32 * kWaves;
+    const int32_t first = w.kbeg + (int32_t)turn * 32;
+    const uint32_t tiles = w.kend > first ? (uint32_t)(w.kend - first + kStep - 1) / kStep : 0;
     uint8_t *kt = smem + wave * 2 * kT, *vt = kt + kT;
     struct Next {  // a block's two groups
         __amdgpu_buffer_rsrc_t g[2];
     };
     auto aim = [&](const uint16_t* x, uint32_t t) {
-        return Next{ld.group(a, x, w, g, u0 + t * 8, (t & 31) * 2), ld.group(a, x, w, g, u0 + t * 8 + 1, (t & 31) * 2 + 1)};
+        const uint32_t u = u0 + t * (2 * kWaves), from = (t & 31) * 2;
+        return Next{ld.group(a, x, w, g, u, from), ld.group(a, x, w, g, u + 1, from + 1)};
     };
     auto copy = [&](const Next& n, int i, uint8_t* dst) {
         ld.template copy<MODE == kOwn>(n.g[2 * i / kC], i % (kC / 2), dst + 2 * i / kC * (kT / 2));
@@ -798,7 +804,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
 
     int32_t odd_from = 0x7fffffff, odd_to = 0;
     for (uint32_t t = 0; t < tiles; t++) {
-        const int32_t t0 = first + (int32_t)t * 128;
+        const int32_t t0 = first + (int32_t)t * kStep;
         f16v s[1];
         h8 vf[Rows<HD, F32>::kAhead];
         typename Rows<HD, F32>::template Weights<1> p;
@@ -809,7 +815,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
         });
         wait_lgkmcnt0();
         if (t + 1 < tiles && ((t + 1) & 31) == 0) {
-            ld.lookup(a, w.id, u0 + (t + 1 + lane / 2) * 8 + (lane & 1));
+            ld.lookup(a, w.id, u0 + (t + 1 + lane / 2) * (2 * kWaves) + (lane & 1));
             ld.settle();
         }
         const Next kn = aim(a.kp, t + 1);  // past the last: no extent, zeros that nobody reads
@@ -827,14 +833,33 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
         wait_lgkmcnt0();
     }
     // (this wave's keys of that range only: the other waves add their own)
-    for (int32_t t0 = odd_from; t0 < odd_to; t0 += 128) r.add_nonfinite(a, w, g, t0, t0 + 32);
+    for (int32_t t0 = odd_from; t0 < odd_to; t0 += kStep) r.add_nonfinite(a, w, g, t0, t0 + 32);
 
     wait_vmcnt<0>();
+    const bool whole = a.parts_total == 1;
+    const uint64_t pr = (uint64_t)(a.parts<MODE>().first + part) * a.n_tokens * a.n_heads + (uint64_t)(w.tok0 + tok) * a.n_heads + head;
+    const uint64_t at = (w.tok0 + tok) * a.out_stride + head * HD;
+    const float l = other_sum(r.l);
+    if constexpr (EACH) {
+        no_prefix(a, w, g, part, min(w.rows - w.row0, 32u), lane, 64);
+        if (!live) return;
+        if (!whole && r.half == 0) *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(r.m, l);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float4 x = make_float4(r.o[d][4 * e], r.o[d][4 * e + 1], r.o[d][4 * e + 2], r.o[d][4 * e + 3]);
+                const uint32_t to = d * 32 + 8 * e + 4 * r.half;
+                if (whole) put4<F32>(a.out, at + to, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+                else put4<true>(a.po, pr * HD + to, x);
+            }
+        return;
+    }
     // Merge the four waves: each puts its sums into LDS as its lanes hold them
     // (a unit of four dimensions is 1 KB, so nothing conflicts) and takes a
     // quarter of the units of all four back.
     constexpr int kUnits = HD / 8, kMine = kUnits / 4;
-    const float l = other_sum(r.l);
     __syncthreads();
     if (r.half == 0) sm[wave * 32 + lane] = r.m, sl[wave * 32 + lane] = l;
 #pragma unroll
@@ -842,7 +867,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
         oo[(wave * kUnits + u) * 64 + lane] = make_float4(r.o[u / 4][u % 4 * 4], r.o[u / 4][u % 4 * 4 + 1],
                                                          r.o[u / 4][u % 4 * 4 + 2], r.o[u / 4][u % 4 * 4 + 3]);
     __syncthreads();
-    if (MODE == kOwn) no_prefix(a, w, g, part, min(w.rows - w.row0, 32u));
+    if (MODE == kOwn) no_prefix(a, w, g, part, min(w.rows - w.row0, 32u), threadIdx.x, 256);
     if (!live) return;
     const uint32_t i = lane & 31;
     const float M = fmaxf(fmaxf(sm[i], sm[32 + i]), fmaxf(sm[64 + i], sm[96 + i]));
@@ -853,11 +878,8 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
         f[k] = m == -INFINITY && l1 == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - M);  // 0: no key of this row
         L = __builtin_fmaf(l1, f[k], L);
     }
-    const uint64_t pr = (uint64_t)(a.parts<MODE>().first + part) * a.n_tokens * a.n_heads + (uint64_t)(w.tok0 + tok) * a.n_heads + head;
-    const bool whole = a.parts_total == 1;
     if (!whole && wave == 0 && r.half == 0) *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(M, L);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    const uint64_t at = (w.tok0 + tok) * a.out_stride + head * HD;
 #pragma unroll
     for (int j = 0; j < kMine; j++) {
         const uint32_t u = wave * kMine + j, d = u / 4 * 32 + u % 4 * 8 + 4 * r.half;
@@ -879,22 +901,35 @@ __device__ __forceinline__ float wave_max_all(float x) {
     return x;
 }
 
-// (one LDS array in both kernels, as above)
+// (one LDS array in all of them, as above)
 template <int HD, bool F32, int MODE>
 __global__ void __launch_bounds__(256, 2) k_attn_few(AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
     const uint32_t slot = a.by_kv(blockIdx.x);
     attn_few<HD, F32, MODE>(a, slot, blockIdx.y, blockIdx.x - slot * a.n_kv, smem);
 }
+// Single tokens with few keys, a wave each.
+template <int HD, bool F32>
+__global__ void __launch_bounds__(256, 2) k_attn_each(AttnArgs a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
+    const uint32_t job = blockIdx.x * 4 + block_wave(), slot = a.by_kv(job);
+    attn_few<HD, F32, kOwn, true>(a, slot, 0, job - slot * a.n_kv, smem);
+}
 // A batch with few rows a group: prefix and own keys in one launch, the prefix's
 // workgroups, which have more keys, first (64 sequences behind 8192 shared
 // positions, prefix and own one after the other 58 us with the join, 49 so).
-template <int HD, bool F32>
+template <int HD, bool F32, bool EACH>
 __global__ void __launch_bounds__(256, 2) k_attn_shared(AttnArgs a, uint32_t prefix_slots, uint32_t prefix_blocks) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
     const uint32_t b = a.by_kv(blockIdx.x), g = blockIdx.x - b * a.n_kv;
-    if (b < prefix_blocks) attn_few<HD, F32, kPrefix>(a, b % prefix_slots, b / prefix_slots, g, smem);
-    else attn_few<HD, F32, kOwn>(a, (b - prefix_blocks) / a.own.n, (b - prefix_blocks) % a.own.n, g, smem);
+    if (b < prefix_blocks) {
+        attn_few<HD, F32, kPrefix>(a, b % prefix_slots, b / prefix_slots, g, smem);
+    } else if constexpr (EACH) {
+        const uint32_t job = (blockIdx.x - prefix_blocks * a.n_kv) * 4 + block_wave(), slot = a.by_kv(job);
+        attn_few<HD, F32, kOwn, true>(a, slot, 0, job - slot * a.n_kv, smem);
+    } else {
+        attn_few<HD, F32, kOwn>(a, (b - prefix_blocks) / a.own.n, (b - prefix_blocks) % a.own.n, g, smem);
+    }
 }
 
 // One wave per (token, head): the parts of its keys joined, o = sum o_c 2^(m_c - M).
@@ -1031,16 +1066,37 @@ void launch_prompt(const AttnArgs& a, const Launch& l, hipStream_t s) {
     if (l.few) hipLaunchKernelGGL((k_attn_few<HD, F32, kPrompt>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_attn_block<HD, F32, kPrompt>), grid, dim3(256), 0, s, a, (uint32_t)l.slots);
 }
+// A batch of single tokens.  each: a wave a (token, kv head), without a merge,
+// where there are 1024 of them and more and few keys each: 512 tokens over 30-100
+// positions 64 -> 37 us, 256 over 300 51 -> 44; over 1000 121 -> 126.
+struct SharedPlan {
+    Launch prefix, own;
+    uint32_t parts;
+    bool each;
+};
+SharedPlan shared_plan(const ane_paged_cache* c, uint32_t n, uint32_t n_groups, uint32_t max_prefix, uint32_t max_len) {
+    SharedPlan p = {};
+    const uint64_t len = bound_len(c, max_len), prefix = n_groups ? std::min(len, bound_len(c, max_prefix)) : 0;
+    p.own = plan(c, n, n, true, len);
+    if (n_groups) p.prefix = plan(c, n_groups, n, false, bound_len(c, max_prefix), true);
+    p.parts = p.prefix.parts + p.own.parts;
+    p.each = p.own.parts == 1 && p.own.slots * c->n_kv_heads >= 1024 && len - prefix <= 512;
+    return p;
+}
 template <int HD, bool F32>
-void launch_shared(const AttnArgs& a, const Launch& pre, const Launch& own, hipStream_t s) {
+void launch_shared(const AttnArgs& a, const SharedPlan& p, hipStream_t s) {
+    const Launch &pre = p.prefix, &own = p.own;
     const uint32_t pb = (uint32_t)(pre.slots * pre.parts), ob = (uint32_t)(own.slots * own.parts);
+    const uint32_t own_wgs = p.each ? (uint32_t)((own.slots * a.n_kv + 3) / 4) : ob * a.n_kv;
     if (a.n_groups && pre.few) {
-        hipLaunchKernelGGL((k_attn_shared<HD, F32>), dim3((pb + ob) * a.n_kv), dim3(256), 0, s, a, (uint32_t)pre.slots, pb);
+        auto* f = p.each ? k_attn_shared<HD, F32, true> : k_attn_shared<HD, F32, false>;
+        hipLaunchKernelGGL(f, dim3(pb * a.n_kv + own_wgs), dim3(256), 0, s, a, (uint32_t)pre.slots, pb);
         return;
     }
     if (a.n_groups)
         hipLaunchKernelGGL((k_attn_block<HD, F32, kPrefix>), dim3(pb * a.n_kv), dim3(256), 0, s, a, (uint32_t)pre.slots);
-    hipLaunchKernelGGL((k_attn_few<HD, F32, kOwn>), dim3((uint32_t)(own.slots * a.n_kv), own.parts), dim3(256), 0, s, a);
+    if (p.each) hipLaunchKernelGGL((k_attn_each<HD, F32>), dim3(own_wgs), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_few<HD, F32, kOwn>), dim3((uint32_t)(own.slots * a.n_kv), own.parts), dim3(256), 0, s, a);
 }
 void join_as(const AttnArgs& a, uint32_t hd, int type, hipStream_t s) {
     auto pick = [&](auto few, auto many) { return a.parts_total <= 4 ? few : many; };
@@ -1113,20 +1169,6 @@ extern "C" int ane_hip_attention_prompt(const ane_paged_cache* cache, uint32_t l
     return ANE_OK;
 }
 
-namespace {
-struct SharedPlan {
-    Launch prefix, own;
-    uint32_t parts;
-};
-SharedPlan shared_plan(const ane_paged_cache* c, uint32_t n, uint32_t n_groups, uint32_t max_prefix, uint32_t max_len) {
-    SharedPlan p = {};
-    p.own = plan(c, n, n, true, bound_len(c, max_len));
-    if (n_groups) p.prefix = plan(c, n_groups, n, false, bound_len(c, max_prefix), true);
-    p.parts = p.prefix.parts + p.own.parts;
-    return p;
-}
-}  // namespace
-
 extern "C" size_t ane_hip_attention_shared_workspace_size(const ane_paged_cache* cache, uint32_t n, uint32_t n_groups,
                                                           uint32_t max_prefix, uint32_t max_len) {
     if (cache_status(cache) || n == 0 || n > kMaxTokens || n_groups > n) return 0;
@@ -1154,9 +1196,9 @@ extern "C" int ane_hip_attention_shared(const ane_paged_cache* cache, uint32_t l
     a.pre = {p.prefix.chunk, p.prefix.parts, 0}, a.own = {p.own.chunk, p.own.parts, p.prefix.parts};
     hipStream_t s = (hipStream_t)stream;
     if (cache->head_dim == 128)
-        type == ANE_TYPE_F32 ? launch_shared<128, true>(a, p.prefix, p.own, s) : launch_shared<128, false>(a, p.prefix, p.own, s);
+        type == ANE_TYPE_F32 ? launch_shared<128, true>(a, p, s) : launch_shared<128, false>(a, p, s);
     else
-        type == ANE_TYPE_F32 ? launch_shared<64, true>(a, p.prefix, p.own, s) : launch_shared<64, false>(a, p.prefix, p.own, s);
+        type == ANE_TYPE_F32 ? launch_shared<64, true>(a, p, s) : launch_shared<64, false>(a, p, s);
     if (p.parts > 1) join_as(a, cache->head_dim, type, s);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;

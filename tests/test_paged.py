@@ -660,6 +660,33 @@ def test_shared_by_a_large_group(ane, ty, hd, prefix, apart, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ty,hd,heads,kv", [("f32", 128, 32, 8), ("f16", 128, 8, 8), ("f32", 64, 24, 8), ("f16", 64, 36, 9),
+                                            ("f32", 128, 320, 8)])
+@pytest.mark.parametrize("prefix", [0, 100])
+def test_shared_many_short(ane, ty, hd, heads, kv, prefix):
+    """1024 (token, kv head) pairs and more over few keys each, the last
+    workgroup with some to spare, with a prefix for two groups, rows in none."""
+    import torch
+
+    n = 131
+    lens = [(i * 37) % 300 + (prefix if 20 <= i < 110 else 0) for i in range(n)]
+    lens[7], lens[8], lens[30], lens[130] = 0, 1, prefix - 3 if prefix else 5, 299
+    c = make_cache(lens, heads, kv, hd, 16, seed=8)
+    kw = {}
+    if prefix:
+        share(c, [20, 64, 110], [prefix, prefix])
+        kw = dict(group_start=i32([20, 64, 110]), prefix_len=i32([prefix, prefix]), max_prefix=prefix)
+    page = int(c.page_table[10, 1])  # seen values that are not finite stay in their rows
+    c.v_pages[0, page, 0, 3, 5] = math.inf
+    q = randq(n, heads, hd, dt(ty))
+    out = torch.full_like(q, 5.0)
+    ane.attention_shared(c, 0, q, out, max_len=400, **kw)
+    for s in [s for s in range(n) if s % 6 == 0 or s in (7, 8, 20, 30, 63, 64, 109, 110, 129, 130)]:
+        check_rows(c, 0, s, q[s:s + 1], out[s:s + 1], [lens[s]], hd ** -0.5)
+    assert not torch.isfinite(out[10, :heads // kv, 5]).any() and bool(torch.isfinite(out[11]).all())
+
+
+@pytest.mark.gpu
 def test_shared_odd_groups(ane):
     """Prefixes longer than a row or than the first row, groups of none and of
     one, an unknown sequence, sequences by number, strided rows."""
