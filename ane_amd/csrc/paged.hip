@@ -81,10 +81,10 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a) {
     int64_t pos = -1;
     uint32_t page = ANE_NO_PAGE, row = 0;
     if (id < a.n_seqs) {
-        pos = (int64_t)a.kv_len[id] - (int64_t)(last - t);
-        const uint64_t pi = pos < 0 ? a.max_pages : (uint64_t)pos / a.ps;
-        if (pi < a.max_pages && (!a.rope || pos < a.rope_len)) {
-            page = a.table[(uint64_t)id * a.max_pages + pi];
+        // (the length as attention counts it, or a row would see another token's keys)
+        pos = (int64_t)min((uint64_t)a.kv_len[id], (uint64_t)a.max_pages * a.ps) - (int64_t)(last - t);
+        if (pos >= 0 && (!a.rope || pos < a.rope_len)) {
+            page = a.table[(uint64_t)id * a.max_pages + (uint32_t)pos / a.ps];
             row = (uint32_t)pos % a.ps;
         } else {
             pos = -1;

@@ -249,8 +249,8 @@ struct ane_paged_cache {
  * pages of one layer.  in_type: of q, k and v; q_out: the rotated q in
  * q_out_type (may be q itself when the types and strides agree).  q and q_out
  * NULL: k and v only.  rope_table NULL: no rotation; else fp32 [rope_len]
- * [head_dim/2][2].  A token whose position is negative, past its sequence's
- * pages or not below rope_len is not appended and its q_out row is zeros.
+ * [head_dim/2][2].  A token whose position is negative or not below rope_len is
+ * not appended and its q_out row is zeros.
  * kv_len counts the new tokens already (ane_hip_pages_reserve).  A sequence may
  * be in the batch once; appending to a page that two sequences hold changes
  * both. */

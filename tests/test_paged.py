@@ -391,6 +391,35 @@ def test_append_leaves_what_has_no_place(ane):
         assert bool((c2.k_pages[0, page, :, p % 16] == k[s].half()).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("over", [0, 1, 3, 10, 50, 2 ** 31 - 1 - 80])
+@pytest.mark.parametrize("rope", [True, False])
+def test_append_and_attention_count_an_overlong_length_alike(ane, over, rope):
+    """A length past max_pages * page_size counts as that many positions, for
+    the append as for the attention: the new tokens are the last of those, and
+    each sees itself."""
+    import torch
+
+    cap, new = 80, 10
+    c = make_cache([cap], 4, 2, 64, 16, fill_rest=0.0)
+    qkv = randq(new, 8, 64, dt("f32"), seed=over % 97)
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    rot, out = torch.full((new, 4, 64), 5.0, device="cuda"), torch.zeros((new, 4, 64), device="cuda")
+    cs = ane.rope_table(cap, 64)
+    before = c.k_pages.clone(), c.v_pages.clone()
+    c.kv_len[0] = cap + over
+    ane.paged_rope_append(c, 0, i32([0, new]), q, k, v, torch.from_numpy(cs).cuda() if rope else None, rot)
+    ane.attention_prompt(c, 0, i32([0, new]), rot, out)
+    row = c.page_table[0, cap // 16 - 1]
+    at = [cap - new + t for t in range(new)]  # within the last page
+    turn = (lambda x: np_turn(x.cpu().numpy(), cs[at][:, None])) if rope else lambda x: x.cpu().numpy()
+    for x, old, want in ((c.k_pages, before[0], turn(k)), (c.v_pages, before[1], v.cpu().numpy())):
+        old[0, row, :, 16 - new:] = torch.from_numpy(want.astype(np.float16)).cuda().transpose(0, 1)
+        assert bool((x == old).all())
+    assert np.array_equal(rot.cpu().numpy(), turn(q))
+    check_rows(c, 0, 0, rot, out, [p + 1 for p in at], 64 ** -0.5)
+
+
 # ------------------------------------------------------------------ prompts
 SHAPES = [
     # type, hd, heads, kv, page, new tokens, cached positions
