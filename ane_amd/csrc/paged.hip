@@ -228,7 +228,7 @@ struct PagesWs {
     uint32_t *list, *movers, *map;  // [n_pages] each
     uint32_t* claim;                // [n_seqs]
     uint32_t *req_len, *req_page;   // [kMaxRequests]
-    uint32_t* count;                // [1]
+    uint32_t* count;                // [2]: pages to move, live pages
 };
 
 size_t pages_layout(const ane_paged_cache* c, void* base, PagesWs* w) {
@@ -245,7 +245,7 @@ size_t pages_layout(const ane_paged_cache* c, void* base, PagesWs* w) {
     p.claim = take(c->n_seqs);
     p.req_len = take(kMaxRequests);
     p.req_page = take(kMaxRequests);
-    p.count = take(1);
+    p.count = take(2);
     if (w) *w = p;
     return off;
 }
