@@ -20,7 +20,7 @@ struct AppendArgs {
     uint16_t *kp, *vp;  // this layer's pages
     const uint32_t *table, *kv_len, *seqs, *q_start;
     uint64_t q_stride, kv_stride, q_out_stride;
-    uint32_t n, n_tokens, rope_len, n_heads, n_kv, hd, ps, n_pages, max_pages, n_seqs;
+    uint32_t n, rope_len, n_heads, n_kv, hd, ps, n_pages, max_pages, n_seqs;
 };
 
 template <class T>
@@ -574,7 +574,7 @@ extern "C" int ane_hip_paged_rope_append(const ane_paged_cache* cache, uint32_t 
     a.kp = cache->k_pages + lo, a.vp = cache->v_pages + lo;
     a.table = cache->page_table, a.kv_len = cache->kv_len, a.seqs = seqs, a.q_start = q_start;
     a.q_stride = q_stride, a.kv_stride = kv_stride, a.q_out_stride = q_out_stride;
-    a.n = n, a.n_tokens = n_tokens, a.rope_len = rope_len, a.n_heads = cache->n_heads, a.n_kv = cache->n_kv_heads;
+    a.n = n, a.rope_len = rope_len, a.n_heads = cache->n_heads, a.n_kv = cache->n_kv_heads;
     a.hd = cache->head_dim, a.ps = cache->page_size, a.n_pages = cache->n_pages, a.max_pages = cache->max_pages;
     a.n_seqs = cache->n_seqs;
     auto* f = in_type == ANE_TYPE_F32
