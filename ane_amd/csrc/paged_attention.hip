@@ -34,6 +34,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s4* lds_s4;
 
 enum Mode { kPrompt, kPrefix, kOwn };
@@ -153,7 +154,7 @@ __device__ __forceinline__ uint32_t shared_len(const AttnArgs& a, uint32_t s, ui
     return min(min(lane_of(p, l), len), seq_len(a, seq_id(a, first)));
 }
 
-// The keys of part `part`; at: its first position, where the work has any.
+// The keys of part `part`.
 template <int MODE>
 __device__ __forceinline__ void find_keys(const AttnArgs& a, uint32_t bm, uint32_t part, Work& w) {
     w.len = (int32_t)seq_len(a, w.id, w.raw);
@@ -271,19 +272,44 @@ __device__ __forceinline__ s4 read_tr(const uint8_t* __restrict__ p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
 }
 
-// x as two fp16 parts, 22 bits in all.
-__device__ __forceinline__ void split(f2 x, h2& hi, h2& lw) {
+// x as two fp16 parts, 22 bits in all; rest: x - hi.
+__device__ __forceinline__ void split(f2 x, h2& hi, h2& lw, f2& rest) {
     hi = __builtin_convertvector(x, h2);
-    f2 rest;  // x - hi, with hi read as fp16: one instruction a value
+    // with hi read as fp16: one instruction a value
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest.x) : "v"(hi), "v"(x.x));
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rest.y) : "v"(hi), "v"(x.y));
     lw = __builtin_convertvector(rest, h2);
 }
+__device__ __forceinline__ void split(f2 x, h2& hi, h2& lw) {
+    f2 rest;
+    split(x, hi, lw, rest);
+}
 
-// The running maximum may lag by kLag (in log2) before O and l are rescaled;
-// weights are e^s 2^kLift relative to it, at most 2^(kLag + kLift) = 2^14, so that
-// fp16 keeps weights 2^-20 of the largest with full precision.
-constexpr float kLag = 8.0f, kLift = 6.0f;
+// Weights are e^s 2^kLift relative to a reference m, a maximum that may lag by
+// kLag (in log2) before O and l are rescaled: at most 2^(kLag + kLift) = 2^14 in
+// fp16 mode, 2^15 in fp32 mode.
+//
+// fp16 mode: a weight is rounded to fp16 once, with full precision down to 2^-20 of
+// the largest and as a multiple of 2^-30 of it below.
+//
+// fp32 mode: two parts hold 22 bits of a weight of 2^-3 and more, below that a
+// multiple of 2^-24, which is enough for fp32 accuracy as long as larger weights
+// carry the row.  They need not: a key far above the others may hold a value of
+// zeros.  So
+// - the reference also goes down, to the maximum of a tile kDrop below it, but not
+//   more than kDeep below the largest seen (O grows by as much);
+// - a tile with weights below 2^kThin is looked at again: where 2^-25 a key and its
+//   largest value are not below 2^-19 of what the row has summed up, what the two
+//   parts left of the weights goes through the matrix cores too, 2^kAgain larger.
+// Weights that matter so keep 18 bits down to 2^-56 of the row's largest, and are
+// multiples of 2^-73 of it below.  O stays below 2^(15 + kDeep + kAgain) 2^16 a key:
+// 2^30 keys fit fp32.
+// The price (prompts of 250-1023 tokens x 32 heads, in a graph): 128 -> 133 us with
+// scores of deviation 1.5, 122 -> 137 with a key 14 above the others, and with scores
+// of deviation 3, where most tiles have such weights, 128 -> 163; with all of those
+// through the matrix cores 192.  A lag of 3 instead of 4 rescales O so often that
+// the first takes 137.
+constexpr float kDrop = 8.0f, kDeep = 24.0f, kThin = -7.0f, kAgain = 38.0f;
 
 // 32 rows of a wave: lane & 31 is the row, lane >> 5 the half of its keys (of its
 // dimensions in q and O).
@@ -292,8 +318,11 @@ struct Rows {
     static constexpr int NS = HD / 16, ND = HD / 32;
     static constexpr uint32_t RB = HD * 2;
     h8 qh[NS], ql[F32 ? NS : 1];  // q, its low part
+    static constexpr float kLag = F32 ? 4.0f : 8.0f, kLift = F32 ? 11.0f : 6.0f;
     f16v o[ND];
-    float m, l, c;  // maximum (log2, lagging), this half's sum, score factor
+    float m, l, c;  // reference (log2), this half's sum, score factor
+    float peak, bottom;  // fp32: the largest reference so far; a tile's maximum below it takes the reference down
+    float lost;          // fp32: largest value times keys, of the small weights left in two parts
     int32_t lim;    // keys below it are seen
     int32_t wmin, wmax;
     uint32_t half, ka, va[2 * ND];
@@ -310,7 +339,7 @@ struct Rows {
                 const uint32_t hi = HD == 128 ? d ^ (i >> 2) : d ^ (i >> 3);
                 va[j * ND + d] = (4 * half + 8 * j + (i >> 2)) * RB + (((hi << 2) | (low ^ (half + 2 * j))) << 4) + (i & 1) * 8;
             }
-        m = -INFINITY, l = 0.0f, c = scale_log2e;
+        m = peak = bottom = -INFINITY, lost = 0.0f, l = 0.0f, c = scale_log2e;
         lim = live ? limit : 0;
         wmin = live ? limit : 0x7fffffff, wmax = lim;
 #pragma unroll
@@ -465,18 +494,35 @@ struct Rows {
         }
         products(false);
     }
+    template <int KT>
+    __device__ __forceinline__ void mask(f16v (&s)[KT], int32_t t0, int32_t lo) const {
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int32_t key = t0 + t * 32 + 8 * (r >> 2) + 4 * (int32_t)half + (r & 3);
+                if (key >= lim || key < lo) s[t][r] = -INFINITY;
+            }
+    }
     // Scores of keys from position t0 on to weights; keys before lo are masked.
+    // Whether this lane has some so small that carried() has to look at them.
     template <int KT, class Between>
-    __device__ __forceinline__ void weights(f16v (&s)[KT], int32_t t0, int32_t lo, Weights<KT>& p, Between between) {
+    __device__ __forceinline__ bool weights(f16v (&s)[KT], int32_t t0, int32_t lo, Weights<KT>& p, Between between) {
+        float low = INFINITY;  // (of the masked too, which costs a second round at worst)
+        auto least = [&] {
+            if constexpr (F32) {
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) low = fminf(low, s[t][r]);
+            }
+        };
         if (t0 + 32 * KT > wmin || t0 < lo) {  // uniform
             asm volatile("");  // a branch, not two selects a score in every tile
-#pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int32_t key = t0 + t * 32 + 8 * (r >> 2) + 4 * (int32_t)half + (r & 3);
-                    if (key >= lim || key < lo) s[t][r] = -INFINITY;
-                }
+            least();
+            mask<KT>(s, t0, lo);
+        } else {
+            least();
         }
         float top = -INFINITY;
 #pragma unroll
@@ -484,15 +530,18 @@ struct Rows {
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[t][r]);
         top = other_max(top) * c;
-        if (__any(top > m + kLag)) {
-            const float mn = top > m + kLag ? top : m;
+        if (__any(top > m + kLag || (F32 && top < bottom))) {
+            float mn = top > m + kLag ? top : m;
+            if constexpr (F32) {
+                if (top < bottom && top != -INFINITY) mn = fmaxf(top, peak - kDeep);
+                peak = fmaxf(peak, mn);
+                bottom = mn > peak - kDeep ? mn - kDrop : -INFINITY;
+            }
             const float w = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= w;
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) o[d][r] *= w;
+            if constexpr (F32) lost *= w;
+            scale_o(w);
         }
         const float b = kLift - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
@@ -516,6 +565,71 @@ struct Rows {
                 p.h[2 * t + r / 8][r % 8 + 1] = hi.y;
                 between(t * 8 + r / 2);
             }
+        return F32 && __builtin_fmaf(low, c, b) < kThin;
+    }
+    // Whether the sums of each row with small weights (thin) are so large that what two
+    // parts leave of those, over the 32 keys of v, is below 2^-19 of them.
+    __device__ __forceinline__ bool carried(const uint8_t* v, bool thin) {
+        us2 x = {0, 0};
+        const v4u* p = reinterpret_cast<const v4u*>(v) + (threadIdx.x & 63);
+#pragma unroll 2
+        for (int i = 0; i < HD / 16; i++) {
+            const v4u y = p[i * 64];
+#pragma unroll
+            for (int k = 0; k < 4; k++) x = __builtin_elementwise_max(x, __builtin_bit_cast(us2, y[k] & 0x7fff7fffu));
+        }
+        uint32_t most = max(x.x, x.y);  // (fp16 magnitudes order as integers, NaN above all)
+        most = max8_u32(most);
+        most = max(most, dpp_u32<kDppRowMirror>(most));
+        most = max(max(lane_of(most, 0), lane_of(most, 16)), max(lane_of(most, 32), lane_of(most, 48)));
+        float sum = 0.0f;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) sum = fmaxf(sum, fabsf(o[d][r]));
+        const float more = __builtin_fmaf(half_bits_to_float(most), 32.0f, lost);
+        if (__any(thin && !(other_max(sum) >= more * 0x1p-6f))) return false;
+        lost = more;
+        return true;
+    }
+    // What the two parts of weights below 2^-3 left of them (of a larger one less than
+    // 2^-22), from the masked scores of 32 keys: added to O, 2^kAgain larger on the way.
+    __device__ __forceinline__ void leftovers(const uint8_t* v, const f16v& s) {
+        const float up = __builtin_ldexpf(1.0f, (int)kAgain);
+        float b = kLift - (m == -INFINITY ? 0.0f : m);
+        asm volatile("" : "+v"(b));  // not the weights kept since weights(): registers
+        scale_o(up);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            h8 ph, pl;
+#pragma unroll
+            for (int r = 0; r < 8; r += 2) {
+                const f2 x = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * e + r], c, b)),
+                              __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * e + r + 1], c, b))};
+                h2 hi, lw;
+                f2 rest;
+                split(x, hi, lw, rest);
+                rest.x = x.x < 0.125f ? (rest.x - (float)lw.x) * up : 0.0f;
+                rest.y = x.y < 0.125f ? (rest.y - (float)lw.y) * up : 0.0f;
+                split(rest, hi, lw);
+                ph[r] = hi.x, ph[r + 1] = hi.y;
+                pl[r] = lw.x, pl[r + 1] = lw.y;
+            }
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const h8 vf = as_h8(vfrag(v, e, d));
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[d], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        scale_o(1.0f / up);
+    }
+    __device__ __forceinline__ void scale_o(float w) {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] *= w;
     }
     __device__ __forceinline__ void first_values(const uint8_t* v, h8 (&vf)[kAhead]) const {
 #pragma unroll
@@ -540,9 +654,13 @@ struct Rows {
         Weights<KT> p;
         h8 vf[kAhead];
         scores<KT>(k, s, [](int) {});
-        weights<KT>(s, t0, lo, p, [](int) {});
+        const bool thin = weights<KT>(s, t0, lo, p, [](int) {});
         first_values(v, vf);
         values<KT>(v, vf, p);
+        if constexpr (F32) {
+            static_assert(KT == 1);
+            if (__any(thin) && !carried(v, thin)) leftovers(v, s[0]);
+        }
     }
     // Values that are not finite and that a row sees, added to its sums (whatever
     // their weight): keys [from, to).  tidy() took them out of the products.
@@ -819,7 +937,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
             ld.settle();
         }
         const Next kn = aim(a.kp, t + 1);  // past the last: no extent, zeros that nobody reads
-        r.template weights<1>(s, t0, w.lo, p, [&](int i) {
+        const bool thin = r.template weights<1>(s, t0, w.lo, p, [&](int i) {
             if (i < kC) copy(kn, i, kt);
         });
         wait_vmcnt<kC>();  // V of this block
@@ -830,6 +948,9 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
         }
         r.first_values(vt, vf);
         r.template values<1>(vt, vf, p);
+        if constexpr (F32) {
+            if (__any(thin) && !r.carried(vt, thin)) r.leftovers(vt, s[0]);
+        }
         wait_lgkmcnt0();
     }
     // (this wave's keys of that range only: the other waves add their own)
@@ -901,16 +1022,16 @@ __device__ __forceinline__ float wave_max_all(float x) {
     return x;
 }
 
-// (one LDS array in all of them, as above)
+// (one LDS array in all of them, as above; 64-wide heads three workgroups a CU)
 template <int HD, bool F32, int MODE>
-__global__ void __launch_bounds__(256, 2) k_attn_few(AttnArgs a) {
+__global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) k_attn_few(AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
     const uint32_t slot = a.by_kv(blockIdx.x);
     attn_few<HD, F32, MODE>(a, slot, blockIdx.y, blockIdx.x - slot * a.n_kv, smem);
 }
 // Single tokens with few keys, a wave each.
 template <int HD, bool F32>
-__global__ void __launch_bounds__(256, 2) k_attn_each(AttnArgs a) {
+__global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) k_attn_each(AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
     const uint32_t job = blockIdx.x * 4 + block_wave(), slot = a.by_kv(job);
     attn_few<HD, F32, kOwn, true>(a, slot, 0, job - slot * a.n_kv, smem);
@@ -919,7 +1040,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_each(AttnArgs a) {
 // workgroups, which have more keys, first (64 sequences behind 8192 shared
 // positions, prefix and own one after the other 58 us with the join, 49 so).
 template <int HD, bool F32, bool EACH>
-__global__ void __launch_bounds__(256, 2) k_attn_shared(AttnArgs a, uint32_t prefix_slots, uint32_t prefix_blocks) {
+__global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) k_attn_shared(AttnArgs a, uint32_t prefix_slots, uint32_t prefix_blocks) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
     const uint32_t b = a.by_kv(blockIdx.x), g = blockIdx.x - b * a.n_kv;
     if (b < prefix_blocks) {

@@ -265,9 +265,13 @@ int ane_hip_paged_rope_append(const struct ane_paged_cache* cache, uint32_t laye
  * g = h / (n_heads / n_kv_heads); zeros for a token at a negative position.
  * Keys a token does not see never touch its result, whatever they hold; an
  * infinity or NaN it does see may make its result infinite or NaN.
- * type: of q and out.  F32: products of fp32 accuracy (q and the softmax
- * weights enter the matrix cores as two fp16 parts each); F16: q and the
- * weights are fp16.  Scores, softmax and sums are fp32 in both.  scale: positive,
+ * type: of q and out.  F32: products of fp32 accuracy: q and the softmax
+ * weights enter the matrix cores in fp16 parts that hold 22 bits of q and of
+ * the weights that carry a row, and at least 18 of any that matters to it down to
+ * 2^-56 of its largest (smaller ones count as multiples of 2^-73 of that).  F16:
+ * q and the weights are rounded to fp16 once, the weights to multiples of 2^-30
+ * of a row's largest below 2^-20 of it.  Scores, softmax and sums are fp32 in
+ * both.  scale: positive,
  * below 1e30.  max_len: a bound on the lengths, which sizes the workspace and
  * the split of long rows (longer sequences are still computed whole); 0 stands
  * for max_pages * page_size.  out may be q when the strides agree.  The

@@ -181,3 +181,83 @@ def test_single_tokens(ane, hd, heads, kv, ps, lens, bounds, prefixes, std, marg
     ane.attention_shared(c, 0, q, out, max_len=max(lens), **kw)
     for s in sorted({0, 1, len(lens) // 2, len(lens) - 1} & set(range(len(lens)))):
         check_heads(c, 0, s, q[s:s + 1], out[s:s + 1], [lens[s]], margin)
+
+
+# ------------------------------------------------------------------ one key far above the others
+def with_sink(c, s, at, margin, value=0.0):
+    """Position `at` of sequence s scores `margin` above the mean of the others, for
+    queries whose dimension 0 is 4, and its value is made `value` times as large."""
+    n, ps = int(c.kv_len[s]), c.page_size
+    for j in range(-(-n // ps)):
+        c.k_pages[:, int(c.page_table[s, j]), :, :min(ps, n - j * ps), 0] = 0
+    page, row = int(c.page_table[s, at // ps]), at % ps
+    c.k_pages[:, page, :, row] = 0
+    c.k_pages[:, page, :, row, 0] = margin * c.head_dim ** 0.5 / 4
+    c.v_pages[:, page, :, row] *= value
+
+
+SINKS = [
+    # head_dim, heads, kv heads, new tokens, cached positions
+    (128, 8, 2, 4, 16), (64, 8, 2, 3, 30), (128, 4, 1, 30, 700), (64, 4, 1, 9, 5000), (128, 32, 8, 1, 4095),
+    (128, 32, 8, 1100, 70), (64, 32, 8, 2100, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("margin", [12, 14, 16, 18, 20, 22, 30])
+@pytest.mark.parametrize("hd,heads,kv,new,old", SINKS)
+def test_one_key_far_above_the_others(ane, hd, heads, kv, new, old, margin):
+    """The weights that carry the result are e^-margin of the largest, whose value is
+    zeros; the large key is the first, one in the middle or the last that every row
+    sees."""
+    import torch
+
+    for at in sorted({0, old // 2, old}):
+        c = make_cache([old + new], heads, kv, hd, 16, seed=13 + at)
+        with_sink(c, 0, at, margin)
+        q = randq(new, heads, hd, torch.float32, seed=at, std=1.0)
+        q[:, :, 0] = 4.0
+        out = torch.zeros_like(q)
+        ane.attention_prompt(c, 0, i32([0, new]), q, out, max_len=old + new)
+        rows = torch.arange(0 if old else 1, new, 1 + new // 50, device="cuda")  # (a row that sees it alone is zeros)
+        check_heads(c, 0, 0, q[rows], out[rows], [old + int(t) + 1 for t in rows], margin)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [1e-6, 1e-4, 1e-2])
+@pytest.mark.parametrize("margin", [10, 14, 18])
+@pytest.mark.parametrize("hd,heads,kv,new,old", [(128, 8, 2, 4, 16), (64, 4, 1, 9, 700), (128, 32, 8, 1100, 0)])
+def test_one_key_far_above_the_others_of_a_small_value(ane, hd, heads, kv, new, old, margin, value):
+    """Its share of the result is smaller, as large and larger than the others'."""
+    import torch
+
+    c = make_cache([old + new], heads, kv, hd, 16, seed=16)
+    with_sink(c, 0, 0, margin, value)
+    q = randq(new, heads, hd, torch.float32, seed=17, std=1.0)
+    q[:, :, 0] = 4.0
+    out = torch.zeros_like(q)
+    ane.attention_prompt(c, 0, i32([0, new]), q, out, max_len=old + new)
+    rows = torch.arange(0 if old else 1, new, 1 + new // 50, device="cuda")
+    check_heads(c, 0, 0, q[rows], out[rows], [old + int(t) + 1 for t in rows], margin)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("margin", [14, 18, 22, 30])
+@pytest.mark.parametrize("hd,heads,kv,n,prefix", [(128, 8, 2, 9, 300), (64, 8, 2, 5, 2000), (128, 32, 8, 140, 100),
+                                                  (128, 128, 16, 300, 150)])
+def test_one_key_far_above_the_others_in_a_prefix(ane, hd, heads, kv, n, prefix, margin):
+    """The large key at the start of a shared prefix, as a model's first token often
+    is: the prefix's sums and each row's own are joined."""
+    import torch
+
+    c = make_cache([prefix + 20 + i % 30 for i in range(n)], heads, kv, hd, 16, seed=14)
+    share(c, [0, n], [prefix])
+    for s in range(n):
+        with_sink(c, s, 0, margin)
+    q = randq(n, heads, hd, torch.float32, seed=15, std=1.0)
+    q[:, :, 0] = 4.0
+    out = torch.zeros_like(q)
+    ane.attention_shared(c, 0, q, out, group_start=i32([0, n]), prefix_len=i32([prefix]), max_len=prefix + 50,
+                         max_prefix=prefix)
+    for s in (0, n // 2, n - 1):
+        check_heads(c, 0, s, q[s:s + 1], out[s:s + 1], [prefix + 20 + s % 30], margin)
