@@ -70,7 +70,12 @@ inline uint64_t bound_len(const ane_paged_cache* c, uint32_t max_len) {
 
 // A batch of single tokens.  each: a wave a (token, kv head), without a merge,
 // where there are 1024 of them and more and few keys each: 512 tokens over 30-100
-// positions 64 -> 37 us, 256 over 300 51 -> 44; over 1000 121 -> 126.
+// positions 64 -> 37 us, 256 over 300 51 -> 44; over 1000 121 -> 126.  Behind a prefix
+// the bounds say how few keys a row may have of its own, not how many: one in no group
+// has all of max_len, one wave after the other 32 of them.  So also max_len is at most
+// 1536, where that costs as much as it saves (256 sequences with 100 own positions
+// behind 1024 56 -> 40 us; 120 such and 8 alone with 1024 44 -> 57, behind 2048 54 ->
+// 96, behind 8192 128 -> 328).
 struct SharedPlan {
     Launch prefix, own;
     uint32_t parts;
@@ -82,7 +87,7 @@ inline SharedPlan shared_plan(const ane_paged_cache* c, uint32_t n, uint32_t n_g
     p.own = plan(c, n, n, true, len);
     if (n_groups) p.prefix = plan(c, n_groups, n, false, bound_len(c, max_prefix), true);
     p.parts = p.prefix.parts + p.own.parts;
-    p.each = p.own.parts == 1 && p.own.slots * c->n_kv_heads >= 1024 && len - prefix <= 512;
+    p.each = p.own.parts == 1 && p.own.slots * c->n_kv_heads >= 1024 && len - prefix <= 512 && len <= 1536;
     return p;
 }
 

@@ -716,6 +716,46 @@ def test_shared_many_short(ane, ty, hd, heads, kv, prefix):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ty,hd,heads,kv", [("f32", 128, 32, 8), ("f16", 64, 24, 8), ("f32", 64, 16, 8)])
+@pytest.mark.parametrize("given", [True, False])
+def test_shared_short_rows_and_a_few_long(ane, ty, hd, heads, kv, given):
+    """As above, behind bounds that leave a row's own keys open: rows of 512 own
+    keys, one more, and many, in groups and in none."""
+    import torch
+
+    n, prefix = 140, [600, 40]
+    lens = [7 + (i * 37) % 300 + (prefix[0] if 10 <= i < 60 else prefix[1] if 60 <= i < 110 else 0) for i in range(n)]
+    lens[3], lens[4], lens[5], lens[139], lens[138] = 512, 513, 1500, 2200, 0
+    lens[11], lens[12], lens[59], lens[60], lens[61] = 600 + 512, 600 + 513, 590, 40 + 1300, 39
+    c = make_cache(lens, heads, kv, hd, 16, seed=21)
+    share(c, [10, 60, 110], prefix)
+    q = randq(n, heads, hd, dt(ty))
+    out = torch.full_like(q, 5.0)
+    kw = dict(max_prefix=1200, max_len=1500) if given else dict(max_len=2200)  # (a wave a row, or four)
+    ane.attention_shared(c, 0, q, out, group_start=i32([10, 60, 110]), prefix_len=i32(prefix), **kw)
+    for s in sorted({3, 4, 5, 10, 11, 12, 13, 58, 59, 60, 61, 62, 109, 110, 137, 138, 139} | set(range(0, n, 9))):
+        check_rows(c, 0, s, q[s:s + 1], out[s:s + 1], [lens[s]], hd ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty,hd", [("f32", 128), ("f16", 64)])
+def test_shared_by_a_large_group_and_a_few_long(ane, ty, hd):
+    """The same beside a prefix on 128 rows a workgroup."""
+    import torch
+
+    heads, kv, n, prefix = 128, 16, 420, 150
+    lens = [prefix + 3 + i % 40 for i in range(n)]
+    lens[0], lens[1], lens[50], lens[51], lens[52], lens[419] = 900, 512, prefix + 513, prefix + 512, 1600, 1
+    c = make_cache(lens, heads, kv, hd, 16, seed=22)
+    share(c, [2, n], [prefix])
+    q = randq(n, heads, hd, dt(ty))
+    out = torch.full_like(q, 5.0)
+    ane.attention_shared(c, 0, q, out, group_start=i32([2, n]), prefix_len=i32([prefix]), max_len=1500, max_prefix=1200)
+    for s in (0, 1, 2, 3, 49, 50, 51, 52, 53, 200, 418, 419):
+        check_rows(c, 0, s, q[s:s + 1], out[s:s + 1], [lens[s]], hd ** -0.5)
+
+
+@pytest.mark.gpu
 def test_shared_odd_groups(ane):
     """Prefixes longer than a row or than the first row, groups of none and of
     one, an unknown sequence, sequences by number, strided rows."""

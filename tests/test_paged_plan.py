@@ -59,3 +59,17 @@ def test_multiplied_division(program):
     """Page, token and row-tile numbers, as the kernels work them out."""
     got = subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout
     assert int(got) == 0
+
+
+@pytest.mark.parametrize("n,groups,max_prefix,max_len,each", [
+    (128, 0, 0, 512, True), (512, 0, 0, 100, True), (127, 0, 0, 100, False),  # 1024 (token, kv head) pairs and more
+    (128, 0, 0, 513, False), (128, 0, 512, 1000, False),  # no groups, no prefix
+    (128, 1, 400, 512, True), (128, 1, 488, 1000, True), (128, 1, 487, 1000, False), (128, 1, 1024, 1536, True),
+    # a row in no group, or in one with a shorter prefix, may have max_len keys of its own
+    (128, 1, 1025, 1537, False), (128, 1, 8192, 8192, False), (128, 1, 8000, 8300, False), (140, 3, 2000, 2200, False),
+    # no bound on the prefixes, none at all
+    (128, 1, 0, 4000, False), (128, 1, 0, 500, True), (128, 1, 0, 0, False)])
+def test_a_wave_a_row_only_where_no_row_can_be_long(program, n, groups, max_prefix, max_len, each):
+    got = subprocess.run([str(program), "plan"], input=f"32 8 128 1024 {n} {groups} {max_prefix} {max_len}\n", check=True,
+                         capture_output=True, text=True).stdout
+    assert bool(int(got)) is each
