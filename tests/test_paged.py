@@ -420,6 +420,40 @@ def test_append_and_attention_count_an_overlong_length_alike(ane, over, rope):
     check_rows(c, 0, 0, rot, out, [p + 1 for p in at], 64 ** -0.5)
 
 
+def wide_batch(n, most, seed):
+    """New tokens and cached positions of n sequences, some with none of either."""
+    r = random.Random(seed)
+    return [r.choice([0, 1, 1, r.randrange(most + 1)]) for _ in range(n)], [r.choice([0, 5, r.randrange(60)]) for _ in range(n)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [64, 65, 130, 1000, 4097])
+def test_append_wide_batch(ane, n):
+    """More sequences than a wave looks through in one step (64) and in two (4096)."""
+    import torch
+
+    new, old = wide_batch(n, 4, n)
+    c = make_cache([a + b for a, b in zip(new, old)], 2, 1, 64, 16, seed=n, fill_rest=0.0)
+    T, lead, behind = sum(new), 3, 2  # rows before the first sequence and behind the last
+    qkv = randq(lead + T + behind, 4, 64, dt("f32"), seed=n)
+    q, k, v = qkv[:, :2], qkv[:, 2:3], qkv[:, 3:]
+    out = torch.full((lead + T + behind, 2, 64), 5.0, device="cuda")
+    start = lead + np.concatenate([[0], np.cumsum(new)])
+    cs = ane.rope_table(80, 64)
+    seq = np.repeat(np.arange(n), new)
+    pos = np.asarray(old)[seq] + np.arange(T) - (start[:-1] - lead)[seq]
+    want_k, want_v = c.k_pages.cpu().numpy().copy(), c.v_pages.cpu().numpy().copy()
+    page, live = c.page_table.cpu().numpy()[seq, pos // 16], slice(lead, lead + T)
+    qf, kf, vf = (x.cpu().numpy() for x in (q, k, v))
+    want_k[0, page, 0, pos % 16] = np_turn(kf[live, 0], cs[pos]).astype(np.float16)
+    want_v[0, page, 0, pos % 16] = vf[live, 0].astype(np.float16)
+    ane.paged_rope_append(c, 0, i32(start.tolist()), q, k, v, torch.from_numpy(cs).cuda(), out)
+    got = out.cpu().numpy()
+    assert np.array_equal(got[live], np_turn(qf[live], cs[pos][:, None]))
+    assert (got[:lead] == 5.0).all() and (got[lead + T:] == 5.0).all()
+    assert np.array_equal(c.k_pages.cpu().numpy(), want_k) and np.array_equal(c.v_pages.cpu().numpy(), want_v)
+
+
 # ------------------------------------------------------------------ prompts
 SHAPES = [
     # type, hd, heads, kv, page, new tokens, cached positions
@@ -461,6 +495,31 @@ def test_prompt(ane, ty, hd, heads, kv, ps, new, old):
     start = run_prompt(c, new, q, out, layer=1)
     check_prompt(c, new, q, out, start, layer=1)
     assert bool((out[sum(new):] == 5.0).all())  # rows behind the last sequence
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty,hd,heads,kv,n,most", [
+    ("f32", 128, 4, 2, 64, 40), ("f32", 64, 4, 1, 65, 70), ("f16", 128, 8, 2, 130, 40), ("f32", 128, 2, 1, 1000, 9),
+    ("f16", 64, 2, 2, 4097, 4), ("f32", 128, 32, 8, 130, 250), ("f16", 64, 40, 8, 200, 300)])  # the last two: 128 rows a workgroup
+def test_prompt_wide_batch(ane, ty, hd, heads, kv, n, most):
+    """More sequences than a wave looks through in one step (64) and in two (4096),
+    empty ones among them, rows before the first and behind the last left as they were."""
+    import torch
+
+    new, old = wide_batch(n, most, n)
+    new[n // 2], new[-1], old[-1] = most, 3, 0
+    c = make_cache([a + b for a, b in zip(new, old)], heads, kv, hd, 16, seed=n)
+    T, lead, behind = sum(new), 3, 2
+    q = randq(lead + T + behind, heads, hd, dt(ty), seed=n)
+    out = torch.full_like(q, 5.0)
+    start = [lead]
+    for m in new:
+        start.append(start[-1] + m)
+    ane.attention_prompt(c, 0, i32(start), q, out, max_len=max(a + b for a, b in zip(new, old)))
+    assert bool((out[:lead] == 5.0).all()) and bool((out[lead + T:] == 5.0).all()) and not (out[lead:lead + T] == 5.0).all(2).any()
+    for i in sorted({0, 1, 31, 32, 62, 63, 64, n // 2, n - 2, n - 1} & set(range(n)) | set(range(0, n, 1 + n // 25))):
+        check_rows(c, 0, i, q[start[i]:start[i + 1]], out[start[i]:start[i + 1]], [old[i] + t + 1 for t in range(new[i])],
+                   hd ** -0.5)
 
 
 @pytest.mark.gpu
@@ -713,6 +772,45 @@ def test_shared_many_short(ane, ty, hd, heads, kv, prefix):
     for s in [s for s in range(n) if s % 6 == 0 or s in (7, 8, 20, 30, 63, 64, 109, 110, 129, 130)]:
         check_rows(c, 0, s, q[s:s + 1], out[s:s + 1], [lens[s]], hd ** -0.5)
     assert not torch.isfinite(out[10, :heads // kv, 5]).any() and bool(torch.isfinite(out[11]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty,hd,heads,kv,groups,each", [
+    ("f32", 128, 4, 2, 63, 3), ("f32", 64, 4, 1, 64, 2), ("f16", 128, 8, 2, 65, 3), ("f32", 128, 8, 8, 130, 3),
+    ("f16", 64, 2, 1, 1000, 2), ("f32", 64, 1, 1, 4097, 1), ("f32", 128, 128, 1, 70, 60)])
+def test_shared_by_many_groups(ane, ty, hd, heads, kv, groups, each):
+    """More groups than a wave looks through in one step (63) and in two, empty ones
+    and rows in none (before the first group and behind the last) among them."""
+    import torch
+
+    r = random.Random(groups)
+    bounds = [2]
+    for _ in range(groups):
+        bounds.append(bounds[-1] + r.choice([0, 1, each, each + 1]))
+    n = bounds[-1] + 3
+    prefix = [r.randrange(60) for _ in range(groups)]
+    lens = [r.randrange(40) for _ in range(n)]
+    for a, b, p in zip(bounds, bounds[1:], prefix):
+        for s in range(a, b):
+            lens[s] += p if r.random() < 0.9 else 0
+    c = make_cache(lens, heads, kv, hd, 16, seed=groups)
+    table = c.page_table.cpu()
+    for a, b, p in zip(bounds, bounds[1:], prefix):  # as share() does, and no further than the first row reaches
+        for s in range(a + 1, b):
+            m = min(p, lens[s], lens[a])
+            table[s, :m // 16] = table[a, :m // 16]
+            if m % 16:
+                for x in (c.k_pages, c.v_pages):
+                    x[:, int(table[s, m // 16]), :, :m % 16] = x[:, int(table[a, m // 16]), :, :m % 16].clone()
+    c.page_table.copy_(table)
+    q = randq(n, heads, hd, dt(ty), seed=groups)
+    out = torch.full_like(q, 5.0)
+    ane.attention_shared(c, 0, q, out, group_start=i32(bounds), prefix_len=i32(prefix), max_prefix=60, max_len=100)
+    assert not (out == 5.0).all(2).any()
+    few = {0, 1, 2, 3, n - 4, n - 3, n - 2, n - 1} | {bounds[g] + d for g in (1, 31, 32, 61, 62, 63, 64, groups // 2, groups - 1)
+                                                      if g < groups for d in (-1, 0, 1)} | set(range(0, n, 1 + n // 60))
+    for s in sorted(few & set(range(n))):
+        check_rows(c, 0, s, q[s:s + 1], out[s:s + 1], [lens[s]], hd ** -0.5)
 
 
 @pytest.mark.gpu
