@@ -731,11 +731,12 @@ __device__ __forceinline__ uint32_t block_wave() { return __builtin_amdgcn_readf
 // 64 keys on a 2-stage LDS ring (each wave copies one 16-key group of K and V a
 // tile).  Two workgroups a CU: while one wave of a SIMD is in its weights (some 650
 // vector cycles a 32-key block), the other is in its products (512 matrix cycles,
-// fp32 1024).  8192 tokens x 32 heads fp16: 560-590 us, 0.94-0.98 PFLOP/s, power
+// fp32 1024).  8192 tokens x 32 heads fp16: 560-615 us, 0.89-0.98 PFLOP/s, power
 // being the limit: on zeros it takes 436 us, and a library fp16 product of 8192^3
-// goes from 1.07 to 1.68 PFLOP/s; fp32: 0.59, so 1.18 of matrix work.  A workgroup
-// costs some 20000 cycles besides 5000 a tile and pair of workgroups (fp32), so
-// prompts of 250-1023 tokens take 120 us where their products alone would take 80.
+// goes from 1.07 to 1.68 PFLOP/s; fp32: 930-1040 us, 0.53-0.59, so up to 1.18 of
+// matrix work.  A workgroup costs some 20000 cycles besides 5000 a tile and pair of
+// workgroups (fp32), so prompts of 250-1023 tokens take 127-134 us where their
+// products alone would take 80.
 // Weights between the products of the other half in one wave measured slower
 // (584 us, 549 so), fragments 2, 3 or 6 ahead, the copies spread over the products,
 // and row tiles started in descending order of keys the same.
@@ -1007,7 +1008,7 @@ __device__ __forceinline__ float wave_max_all(float x) {
     return x;
 }
 
-// (one LDS array in all of them, as above; 64-wide heads three workgroups a CU)
+// (one LDS array in all of them, as above; of 64-wide heads at least three workgroups a CU)
 template <int HD, bool F32, int MODE>
 __global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) k_attn_few(AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];

@@ -35,14 +35,15 @@ struct Launch {
 // token each; beside: shares its launch with the batch's own keys.
 //
 // 32 rows a workgroup as long as its workgroups have a place each (512 of them, two
-// a CU; four a CU 64-wide), half again as many for one sequence, where 128 rows a
-// workgroup would leave most CUs idle: 512 tokens x 32 heads fp32 23 us, 29 with
-// 128 rows; 768 tokens 32, 37; 8 chunks of 64 tokens after 1000 positions 35, 47.
+// a CU; 64-wide four a CU, three in fp32), half again as many for one sequence,
+// where 128 rows a workgroup would leave most CUs idle: 512 tokens x 32 heads fp32
+// 22 us, 31 with 128 rows; 768 tokens 33, 39; 8 chunks of 64 tokens after 1000
+// positions 36, 50.
 // Beyond that 128 rows, since the four waves of the other kernel read every K and
-// V tile for themselves: 2 x 400 tokens 26 us, 32 with 32 rows; 16 x 256 tokens
-// 49, 90.  Sequences of 64 rows and less would leave half of such a tile empty:
-// single tokens, and 64 chunks of 16 tokens after 1000 positions (87 us, with 128
-// rows 89).  Few rows and many keys: the keys in parts, as many as fill the
+// V tile for themselves: 2 x 400 tokens 27 us, 30 with 32 rows; 16 x 256 tokens
+// 49, 81.  Sequences of 64 rows and less would leave half of such a tile empty:
+// single tokens, and 64 chunks of 16 tokens after 1000 positions (79 us, with 128
+// rows 93).  Few rows and many keys: the keys in parts, as many as fill the
 // places at once but not more: a second, part-filled round costs more than the
 // longer parts (200 tokens after 4000 positions 51 us, in 1.5 times the parts 63).
 // A prefix beside its batch's own keys takes half the places (three or four
