@@ -165,6 +165,10 @@ EXPORTS = (
     "ane_hip_pages_free",
     "ane_hip_pages_copy",
     "ane_hip_pages_compact",
+    "ane_hip_quantize_tokens",
+    "ane_hip_dense_i8_scaled",
+    "ane_hip_linear_i8_workspace_size",
+    "ane_hip_linear_i8",
 )
 
 _lib: ctypes.CDLL | None = None
@@ -273,6 +277,15 @@ _SIGS: dict[str, tuple[Any, list[Any]]] = {
     "ane_hip_pages_free": (_c.c_int, [_P, _c.c_uint32, _P, _P]),
     "ane_hip_pages_copy": (_c.c_int, [_P, _c.c_uint32, _P, _P, _P]),
     "ane_hip_pages_compact": (_c.c_int, [_P, _P, _P, _P, _P, _c.c_size_t, _P]),
+    "ane_hip_quantize_tokens": (
+        _c.c_int, [_c.c_uint32, _c.c_uint32, _c.c_int, _P, _c.c_uint64, _P, _c.c_float, _P, _c.c_uint64, _P, _P]),
+    "ane_hip_dense_i8_scaled": (
+        _c.c_int, [_c.c_uint32, _c.c_uint32, _c.c_uint32, _P, _c.c_uint64, _P, _P, _c.c_uint64, _P, _P, _P, _c.c_uint64,
+                   _c.c_int, _P, _c.c_uint64, _P]),
+    "ane_hip_linear_i8_workspace_size": (_c.c_size_t, [_c.c_uint32, _c.c_uint32, _c.c_uint32]),
+    "ane_hip_linear_i8": (
+        _c.c_int, [_c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_int, _P, _c.c_uint64, _P, _c.c_float, _P, _c.c_uint64, _P,
+                   _P, _P, _c.c_uint64, _c.c_int, _P, _c.c_uint64, _P, _c.c_size_t, _P]),
 }
 
 
@@ -1252,3 +1265,134 @@ def pages_compact(cache, table_out=None, refs_out=None, n_live=None, workspace=N
     r, l = _ints(refs_out, cache.k_pages.shape[1], cache, "refs_out"), _ints(n_live, 1, cache, "n_live")
     workspace, wp, size = _work(cache, workspace, lambda: _pages_need(cache), stream)
     _launch(lib().ane_hip_pages_compact, cache, "pages_compact", stream, (cache._at, t, r, l, wp, size))
+
+
+# ---------------------------------------------------------------- int8 linear layers of a batch
+def _act_types():
+    global _ACT_TYPES
+    if _ACT_TYPES is None:
+        import torch
+
+        _ACT_TYPES = {torch.float32: 0, torch.float16: 1}
+    return _ACT_TYPES
+
+
+_ACT_TYPES = None
+
+
+def _tokens(t, dev, what):
+    """(pointer, type, tokens, values, row stride) of activations [tokens][values] whose values are contiguous."""
+    ty = _act_types().get(t.dtype)
+    if ty is None or t.dim() != 2:
+        raise ValueError(f"{what} is a float32 or float16 tensor [tokens][values]")
+    (n, k), (s0, s1) = t.shape, t.stride()
+    if t.get_device() != dev:
+        raise ValueError(f"{what} is on the device of the others")
+    if s1 != 1 and k > 1:
+        raise ValueError(f"the values of a token of {what} are contiguous")
+    if n > 1 and s0 < k:
+        raise ValueError(f"the tokens of {what} do not overlap")
+    return t.data_ptr(), ty, n, k, s0 if n > 1 else k
+
+
+def _vector(t, n, dev, what):
+    """The pointer of n contiguous float32, or None."""
+    if t is None:
+        return None
+    if _act_types().get(t.dtype) != 0 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{what} is a contiguous float32 tensor of {n} values on the device of the others")
+    return t.data_ptr()
+
+
+def _int8_rows(t, k, dev, what):
+    """(pointer, rows, row stride) of int8 rows of k values that can be read up to k rounded up to 16."""
+    import torch
+
+    if t.dtype != torch.int8 or t.dim() != 2 or t.shape[1] != k or (k > 1 and t.stride(1) != 1) or t.get_device() != dev:
+        raise ValueError(f"{what} is an int8 tensor [rows][{k}] on the device of the others, its rows contiguous")
+    n, kp = t.shape[0], (k + 15) // 16 * 16
+    s0 = t.stride(0) if n > 1 else kp
+    p = t.data_ptr()
+    if p % 16 or s0 % 16 or s0 < kp:
+        raise ValueError(f"the rows of {what} start on 16 bytes (a view [:, :k] of rows of {kp} bytes will do)")
+    if n and t.storage_offset() + (n - 1) * s0 + kp > t.untyped_storage().nbytes():
+        raise ValueError(f"the last row of {what} can be read up to {kp} bytes")
+    return p, n, s0
+
+
+def _on(dev, fn, what, stream, args):
+    """fn(*args, stream) on device dev and, unless given, its current stream."""
+    import torch
+
+    if dev < 0:
+        raise ValueError("the tensors are not in GPU memory")
+    if dev == torch._C._cuda_getDevice():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream_handle(stream))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream_handle(stream))
+    if st:
+        check(st, what)
+
+
+def quantize_tokens(x, q, scales, norm_w=None, eps=1e-5, stream=None):
+    """q, scales of activations x [tokens][values], each token on its own, after an RMSNorm where norm_w is given.
+    q is int8 [tokens][values], its rows starting on 16 bytes; values past the last up to the next 16 are zeroed."""
+    dev = x.get_device()
+    xp, ty, n, k, xs = _tokens(x, dev, "x")
+    qp, rows, qs = _int8_rows(q, k, dev, "q")
+    if rows != n:
+        raise ValueError("q has the shape of x")
+    sp, wp = _vector(scales, n, dev, "scales"), _vector(norm_w, k, dev, "norm_w")
+    _on(dev, lib().ane_hip_quantize_tokens, "quantize_tokens", stream, (n, k, ty, xp, xs, wp, eps, qp, qs, sp))
+
+
+def _product(n, k, dev, w, w_scales, out, bias, residual):
+    wp, rows, ws = _int8_rows(w, k, dev, "w")
+    op, ty, no, width, os_ = _tokens(out, dev, "out")
+    if no != n or width != rows:
+        raise ValueError("out is [tokens][rows of w]")
+    rp, rs = None, 0
+    if residual is not None:
+        rp, tr, nr, wr, rs = _tokens(residual, dev, "residual")
+        if (tr, nr, wr) != (ty, no, width):
+            raise ValueError("residual has the shape and type of out")
+    return rows, wp, ws, _vector(w_scales, rows, dev, "w_scales"), _vector(bias, rows, dev, "bias"), rp, rs, ty, op, os_
+
+
+def dense_i8_scaled(q, q_scales, w, w_scales, out, bias=None, residual=None, stream=None):
+    """out [tokens][rows of w] = the product of int8 tokens q and int8 weights w, times the scales of token and row,
+    plus bias [rows of w] and residual (out's shape and type; may be out).  Rows of q hold zeros from their last value
+    up to the next 16 (quantize_tokens writes them)."""
+    dev = q.get_device()
+    k = q.shape[-1]
+    qp, n, qs = _int8_rows(q, k, dev, "q")
+    rows, wp, ws, cp, bp, rp, rs, ty, op, os_ = _product(n, k, dev, w, w_scales, out, bias, residual)
+    _on(dev, lib().ane_hip_dense_i8_scaled, "dense_i8_scaled", stream,
+        (n, rows, k, qp, qs, _vector(q_scales, n, dev, "q_scales"), wp, ws, cp, bp, rp, rs, ty, op, os_))
+
+
+def linear_i8_workspace_size(T, N, K) -> int:
+    return int(lib().ane_hip_linear_i8_workspace_size(T, N, K))
+
+
+def linear_i8_workspace(T, N, K, device="cuda"):
+    """A workspace for linear_i8 calls of these sizes, for callers that keep one."""
+    return _scratch(linear_i8_workspace_size(T, N, K), device)
+
+
+def linear_i8(x, w, w_scales, out, norm_w=None, eps=1e-5, bias=None, residual=None, workspace=None, stream=None):
+    """out [tokens][rows of w]: activations x [tokens][values] quantized a token at a time (after an RMSNorm where
+    norm_w is given), times int8 weights w [rows][values] with a scale a row, plus bias and residual."""
+    dev = x.get_device()
+    xp, ty, n, k, xs = _tokens(x, dev, "x")
+    rows, wp, ws, cp, bp, rp, rs, to, op, os_ = _product(n, k, dev, w, w_scales, out, bias, residual)
+    np_ = _vector(norm_w, k, dev, "norm_w")
+    if workspace is None:
+        if dev < 0:
+            raise ValueError("the tensors are not in GPU memory")
+        workspace = _scratch(linear_i8_workspace_size(n, rows, k), x.device, stream)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("the workspace is contiguous, on the device of the others")
+    _on(dev, lib().ane_hip_linear_i8, "linear_i8", stream,
+        (n, rows, k, ty, xp, xs, np_, eps, wp, ws, cp, bp, rp, rs, to, op, os_, workspace.data_ptr(), workspace.nbytes))

@@ -31,7 +31,7 @@ __device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t chunk) {
     return row * kBK + ((chunk ^ ((row ^ (row >> 3)) & 7)) << 4);
 }
 
-template <int BL, bool AU8>
+template <int BL, bool AU8, bool SC = false>
 __global__ void __launch_bounds__(kGThreads)
 k_gemm_i8(GemmParams p) {
     __shared__ __attribute__((aligned(16))) int8_t sA[kBM * kBK];
@@ -143,6 +143,7 @@ k_gemm_i8(GemmParams p) {
         const uint32_t j = col0 + wc0 + ni * 32 + (lane & 31);
         if (j >= p.Nout) continue;
         const float bj = p.bias ? p.bias[j] : 0.0f;
+        const float cj = SC ? p.cs[j] : 0.0f;
 #pragma unroll
         for (int mi = 0; mi < 2; mi++) {
 #pragma unroll
@@ -151,7 +152,9 @@ k_gemm_i8(GemmParams p) {
                 if (i >= p.Mout) continue;
                 int32_t v = acc[mi][ni][r];
                 if (AU8) v = (int32_t)((uint32_t)v + 128u * (uint32_t)colsum[ni]);
-                if (p.Craw) {
+                if (SC) {
+                    sc_put(p, i, j, sc_out(v, p.rs[i], cj, bj));
+                } else if (p.Craw) {
                     p.Craw[(uint64_t)i * p.ldc + j] = v;
                 } else if (p.ig) {
                     p.C[(uint64_t)i * p.ldc + j] =
@@ -221,6 +224,11 @@ static int launch_gemm(const GemmParams& p, hipStream_t s) {
     }
     dim3 grid((p.Nout + kBN - 1) / kBN, (p.Mout + kBM - 1) / kBM);
     if (grid.y > 65535) return ANE_ERR_INVALID_ARG;
+    if (BL == kBTransposed && !AU8 && p.rs) {
+        hipLaunchKernelGGL((k_gemm_i8<kBTransposed, false, true>), grid, dim3(kGThreads), 0, s, p);
+        ANE_HIP_CHECK_LAUNCH();
+        return ANE_OK;
+    }
     hipLaunchKernelGGL((k_gemm_i8<BL, AU8>), grid, dim3(kGThreads), 0, s, p);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;

@@ -30,7 +30,29 @@ struct GemmParams {
     const int32_t* igc;
     const int32_t* igr;
     uint32_t nsum, corr;
+    // Scaled epilogue (linear_i8.hip) where rs is given: C = fl(fl((float)acc *
+    // rs[i]) * cs[j]) + bias[j] + res[i][j], each step rounded, C and res fp16
+    // where half; C and ldc as below, in elements.
+    const float* rs;      // fp32[Mout]
+    const float* cs;      // fp32[Nout]
+    const void* res;      // or nullptr
+    uint64_t ldr;
+    bool half;
 };
+
+__device__ __forceinline__ float sc_out(int32_t acc, float rs, float cs, float bias) {
+    return __fadd_rn(__fmul_rn(__fmul_rn((float)acc, rs), cs), bias);
+}
+// One output of the scaled epilogue: the residual added, stored in its type.
+__device__ __forceinline__ void sc_put(const GemmParams& p, uint64_t i, uint64_t j, float f) {
+    if (p.half) {
+        if (p.res) f = __fadd_rn(f, (float)static_cast<const _Float16*>(p.res)[i * p.ldr + j]);
+        reinterpret_cast<_Float16*>(p.C)[i * p.ldc + j] = (_Float16)f;
+    } else {
+        if (p.res) f = __fadd_rn(f, static_cast<const float*>(p.res)[i * p.ldr + j]);
+        p.C[i * p.ldc + j] = f;
+    }
+}
 
 // Partials per column or row, at most: each reader adds them up, so they pay
 // only while they are few (igemm.hip).

@@ -39,7 +39,7 @@ namespace {
 // lane's 16 bytes of column n0 + l%16 are dword l%16 of four consecutive
 // 64-byte groups.  AU8: uint8 A enters as a - 128 and 128 * (column sum of B)
 // is added back.
-template <int MB, bool PANEL = false, bool AU8 = false>
+template <int MB, bool PANEL = false, bool AU8 = false, bool SC = false>
 __global__ void __launch_bounds__(256) k_gemm_skinny(GemmParams p) {
     __shared__ v4i red[4][MB][64];
     __shared__ int csum[AU8 ? 4 : 1][16];
@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(256) k_gemm_skinny(GemmParams p) {
     if (p.sdev) s = __fmul_rn(__fmul_rn(p.sdev[0], p.sdev[1]), p.smul);
     const uint32_t j = n0 + c16;
     const float bj = (p.bias && j < p.Nout) ? p.bias[j] : 0.0f;
+    const float cj = SC && j < p.Nout ? p.cs[j] : 0.0f;
     const uint32_t igc = p.ig ? ig_sum(p.igc, p.nsum, p.Nout, j) : 0u;
     for (uint32_t r = wave; r < (uint32_t)MB; r += 4) {
         v4i t = red[0][r][lane] + red[1][r][lane] + red[2][r][lane] + red[3][r][lane];
@@ -137,7 +138,9 @@ __global__ void __launch_bounds__(256) k_gemm_skinny(GemmParams p) {
         for (int i = 0; i < 4; i++) {
             const uint32_t row = m0 + 16 * r + 4 * g + i;
             if (row >= p.Mout || j >= p.Nout) continue;
-            if (p.Craw) {
+            if (SC) {
+                sc_put(p, row, j, sc_out(t[i], p.rs[row], cj, bj));
+            } else if (p.Craw) {
                 p.Craw[(uint64_t)row * p.ldc + j] = t[i];
             } else if (p.ig) {
                 p.C[(uint64_t)row * p.ldc + j] = ig_out(p, t[i], igc, ig_sum(p.igr, p.nsum, p.Mout, row));
@@ -173,20 +176,22 @@ bool skinny_eligible(const GemmParams& p, uint64_t wgs_max) {
     return true;
 }
 
-template <bool PANEL, bool AU8>
+template <bool PANEL, bool AU8, bool SC = false>
 static int launch_skinny(const GemmParams& p, hipStream_t s) {
     const uint32_t mb = p.Mout > 128 ? 4 : (p.Mout + 15) / 16;
     const dim3 grid((p.Nout + 15) / 16, p.Mout > 128 ? (p.Mout + 63) / 64 : 1);
-    const auto fn = mb == 1   ? k_gemm_skinny<1, PANEL, AU8>
-                    : mb == 2 ? k_gemm_skinny<2, PANEL, AU8>
-                    : mb <= 4 ? k_gemm_skinny<4, PANEL, AU8>
-                              : k_gemm_skinny<8, PANEL, AU8>;
+    const auto fn = mb == 1   ? k_gemm_skinny<1, PANEL, AU8, SC>
+                    : mb == 2 ? k_gemm_skinny<2, PANEL, AU8, SC>
+                    : mb <= 4 ? k_gemm_skinny<4, PANEL, AU8, SC>
+                              : k_gemm_skinny<8, PANEL, AU8, SC>;
     hipLaunchKernelGGL(fn, grid, dim3(256), 0, s, p);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;
 }
 
-int launch_gemm_skinny(const GemmParams& p, hipStream_t s) { return launch_skinny<false, false>(p, s); }
+int launch_gemm_skinny(const GemmParams& p, hipStream_t s) {
+    return p.rs ? launch_skinny<false, false, true>(p, s) : launch_skinny<false, false>(p, s);
+}
 
 bool panel_skinny_eligible(const GemmParams& p, uint64_t wgs_max) {
     if (p.Mout == 0 || !rows_ok(p, wgs_max) || p.Nout == 0 || p.Kp == 0 || (p.Kp & 63) || p.ldb * 4 != p.Kp) return false;

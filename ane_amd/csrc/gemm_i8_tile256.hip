@@ -268,11 +268,37 @@ __device__ __forceinline__ void store16_sc1(uint32_t* dst, v4i v) {
     asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 0" ::"v"(dst), "v"(v) : "memory");
 }
 
+// Four outputs of the scaled epilogue (sc_put), at element `at` of C and `ar`
+// of the residual.
+__device__ __forceinline__ void sc_put4(const GemmParams& p, uint64_t at, uint64_t ar, v4i v) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    if (p.half) {
+        h4 o;
+        if (p.res) {
+            const h4 r = *reinterpret_cast<const h4*>(static_cast<const _Float16*>(p.res) + ar);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = __float_as_int(__fadd_rn(__int_as_float(v[e]), (float)r[e]));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = (_Float16)__int_as_float(v[e]);
+        *reinterpret_cast<h4*>(reinterpret_cast<_Float16*>(p.C) + at) = o;
+        return;
+    }
+    if (p.res) {
+        const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(p.res) + ar);
+        v[0] = __float_as_int(__fadd_rn(__int_as_float(v[0]), r.x));
+        v[1] = __float_as_int(__fadd_rn(__int_as_float(v[1]), r.y));
+        v[2] = __float_as_int(__fadd_rn(__int_as_float(v[2]), r.z));
+        v[3] = __float_as_int(__fadd_rn(__int_as_float(v[3]), r.w));
+    }
+    store16_sc1(reinterpret_cast<uint32_t*>(p.C) + at, v);
+}
+
 #if ANE_TILE_PANEL
 template <bool AU8>
 #else
 constexpr bool AU8 = false;
-template <bool IG>  // the integer GEMM epilogue (GemmParams::ig)
+template <bool IG, bool SC = false>  // the integer GEMM's epilogue (GemmParams::ig), the scaled one (rs)
 #endif
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu)))
 ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
@@ -319,7 +345,7 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
     if (p.sdev) s = __fmul_rn(__fmul_rn(p.sdev[0], p.sdev[1]), p.smul);
 
 #if ANE_TILE_PANEL
-    constexpr bool IG = false;
+    constexpr bool IG = false, SC = false;
 #endif
     const uint32_t wr0 = (wave / WN) * (FM * 32);
     const uint32_t wc0 = (wave % WN) * (FN * 32);
@@ -432,11 +458,19 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
         __syncthreads();
     }
 #endif
-    float bj[FN];
+    float bj[FN], cj[SC ? FN : 1];
 #pragma unroll
     for (int ni = 0; ni < FN; ni++) {
         const uint32_t j = col0 + wc0 + ni * 32 + (lane & 31);
         bj[ni] = (p.bias && j < p.Nout) ? p.bias[j] : 0.0f;
+        if constexpr (SC) cj[ni] = p.cs[j < p.Nout ? j : p.Nout - 1];
+    }
+    // SC: the scales of the tile's rows, past the staging
+    const float* const rsc = reinterpret_cast<const float*>(smem + NW * kEpiWaveBytes);
+    if constexpr (SC) {
+        static_assert(NW * kEpiWaveBytes + TM * 4 <= kLdsBytes && TM <= kThreads, "room for the scales");
+        if (tid < (uint32_t)TM) const_cast<float*>(rsc)[tid] = p.rs[row0 + tid < p.Mout ? row0 + tid : p.Mout - 1];
+        __syncthreads();
     }
     // IG: 128 x the sums of the tile's columns, then of its rows, past the staging
     uint32_t igc[FN];
@@ -456,7 +490,9 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
         for (int ni = 0; ni < FN; ni++) igc[ni] = isum[wc0 + ni * 32 + (lane & 31)];
     }
     int8_t* epi = smem + wave * kEpiWaveBytes;
-    const bool vec_ok = (((uintptr_t)(craw ? (void*)craw : (void*)p.C)) & 15) == 0 && (p.ldc & 3) == 0;
+    const bool vec_ok = SC && p.half ? ((((uintptr_t)p.C) | ((uintptr_t)p.res)) & 7) == 0 && ((p.ldc | p.ldr) & 3) == 0
+                        : SC ? ((((uintptr_t)p.C) | ((uintptr_t)p.res)) & 15) == 0 && ((p.ldc | p.ldr) & 3) == 0
+                             : (((uintptr_t)(craw ? (void*)craw : (void*)p.C)) & 15) == 0 && (p.ldc & 3) == 0;
 
 #pragma unroll
     for (int mi = 0; mi < FM; mi++) {
@@ -476,7 +512,9 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
 #if ANE_TILE_PANEL
                     if (AU8) av = (int32_t)((uint32_t)av + 128u * (uint32_t)csj[ni]);
 #endif
-                    if (craw) {
+                    if constexpr (SC) {
+                        bitsv = __float_as_uint(sc_out(av, rsc[wr0 + mi * 32 + h * EPR + lr], cj[ni], bj[ni]));
+                    } else if (craw) {
                         bitsv = (uint32_t)av;
                     } else if (IG) {
                         bitsv = __float_as_uint(ig_out(p, av, igc[ni], isum[TN + wr0 + mi * 32 + h * EPR + lr]));
@@ -498,6 +536,16 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
                 const uint32_t i = row0 + wr0 + mi * 32 + h * EPR + lr;
                 const uint32_t j = col0 + wc0 + lc;
                 if (i >= p.Mout) continue;
+                if constexpr (SC) {
+                    if (vec_ok && j + 3 < p.Nout) {
+                        sc_put4(p, (uint64_t)i * p.ldc + j, (uint64_t)i * p.ldr + j, v);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (j + e < p.Nout) sc_put(p, i, j + e, __int_as_float(v[e]));
+                    }
+                    continue;
+                }
                 uint32_t* dst = craw ? reinterpret_cast<uint32_t*>(craw) + (uint64_t)i * p.ldc + j
                                      : reinterpret_cast<uint32_t*>(p.C) + (uint64_t)i * p.ldc + j;
                 if (vec_ok && j + 3 < p.Nout) {
@@ -539,7 +587,7 @@ int ANE_TILE_LAUNCH(const GemmParams& p, bool a_unsigned, hipStream_t s) {
 #else
 bool ANE_TILE_ELIGIBLE(const GemmParams& p, bool any_rows) {
     if ((!any_rows && p.Mout < TM) || p.Nout < TN) return false;
-    if (p.Kp == 0 || (p.Kp % 64) != 0) return false;
+    if (p.Kp == 0 || (p.Kp % (p.rs ? 16 : 64)) != 0) return false;  // (a slice's tail is masked 16 bytes at a time)
     if ((p.lda & 15) || (p.ldb & 15)) return false;
     if ((((uintptr_t)p.A) & 15) || (((uintptr_t)p.B) & 15)) return false;
     if (p.rowsA < p.Mout || p.colsB < p.Nout) return false;
@@ -558,7 +606,7 @@ int ANE_TILE_LAUNCH(const GemmParams& p, hipStream_t s, uint32_t ksplit) {
     if (total > 0x7fffffffull || ksplit == 0 || ksplit > 65535) return ANE_ERR_INVALID_ARG;
     if (ksplit > 1 && !p.Craw) return ANE_ERR_INVALID_ARG;  // split K writes int32 planes
     if (p.ig && p.nsum > kIgParts) return ANE_ERR_INVALID_ARG;
-    const auto fn = p.ig ? ANE_TILE_KERNEL<true> : ANE_TILE_KERNEL<false>;
+    const auto fn = p.rs ? ANE_TILE_KERNEL<false, true> : p.ig ? ANE_TILE_KERNEL<true> : ANE_TILE_KERNEL<false>;
     hipLaunchKernelGGL(fn, dim3((uint32_t)total, ksplit), dim3(kThreads), 0, s, p, tiles_m, tiles_n);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;

@@ -341,6 +341,44 @@ int ane_hip_pages_copy(const struct ane_paged_cache* cache, uint32_t n, const ui
 int ane_hip_pages_compact(const struct ane_paged_cache* cache, uint32_t* page_table_out, uint32_t* page_refs_out,
                           uint32_t* n_live, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------ int8 linear layers of a batch
+ *
+ * out = (q . w^T) with a scale for each token and each output channel, for T
+ * tokens of K values and N output channels.  No counterpart in the reference,
+ * whose int8 products have one scale a tensor.  Types are ANE_TYPE_F32 or
+ * ANE_TYPE_F16; strides are in elements from one token (row of w) to the next,
+ * the values of one are contiguous.  1 <= K < 2^17, T and N at most 65535 * 128,
+ * T * N below 2^38.  All calls are asynchronous on stream; pointers must belong
+ * to the current device and be aligned to their elements, q and w (and their
+ * strides, which are bytes) to 16 bytes.
+ *
+ * Weights: int8 rows [N][w_stride], w_stride >= K, each readable up to K rounded
+ * up to 16; what stands there past K does not matter.
+ * Quantized tokens: int8 rows [T][q_stride], q_stride >= K rounded up to 16,
+ * zeros from K up to there.
+ *
+ * quantize_tokens: y = x, or with norm_w (fp32 [K]) y = fl(fl(x * inv) * norm_w),
+ * inv as ane_hip_rms_norm has it; scales[t] = fl(max|y| / 127), q = y * fl(127 /
+ * max|y|) rounded to even, at most 127 in magnitude.  A token of zeros has scale
+ * 1; one whose y holds an infinity or NaN a scale that is not finite, and its row
+ * of any product is NaN.
+ * dense_i8_scaled: out[t][n] = fl(fl((float)sum q w * q_scales[t]) * w_scales[n])
+ * + bias[n] + residual[t][n], one rounding a step, the sum exact; bias (fp32 [N])
+ * and residual (out's type; may be out itself with its stride) may be NULL.
+ * linear_i8: both, q and scales in the workspace (256-byte aligned; it belongs to
+ * the call until it has run).  The same bits as the two calls. */
+int ane_hip_quantize_tokens(uint32_t T, uint32_t K, int type, const void* x, uint64_t x_stride, const float* norm_w,
+                            float eps, int8_t* q, uint64_t q_stride, float* scales, void* stream);
+int ane_hip_dense_i8_scaled(uint32_t T, uint32_t N, uint32_t K, const int8_t* q, uint64_t q_stride,
+                            const float* q_scales, const int8_t* w, uint64_t w_stride, const float* w_scales,
+                            const float* bias, const void* residual, uint64_t residual_stride, int out_type, void* out,
+                            uint64_t out_stride, void* stream);
+size_t ane_hip_linear_i8_workspace_size(uint32_t T, uint32_t N, uint32_t K);
+int ane_hip_linear_i8(uint32_t T, uint32_t N, uint32_t K, int type, const void* x, uint64_t x_stride,
+                      const float* norm_w, float eps, const int8_t* w, uint64_t w_stride, const float* w_scales,
+                      const float* bias, const void* residual, uint64_t residual_stride, int out_type, void* out,
+                      uint64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
