@@ -165,6 +165,7 @@ EXPORTS = (
     "ane_hip_pages_free",
     "ane_hip_pages_copy",
     "ane_hip_pages_compact",
+    "ane_hip_paged_norm_rope_append",
     "ane_hip_quantize_tokens",
     "ane_hip_dense_i8_scaled",
     "ane_hip_linear_i8_workspace_size",
@@ -277,6 +278,9 @@ _SIGS: dict[str, tuple[Any, list[Any]]] = {
     "ane_hip_pages_free": (_c.c_int, [_P, _c.c_uint32, _P, _P]),
     "ane_hip_pages_copy": (_c.c_int, [_P, _c.c_uint32, _P, _P, _P]),
     "ane_hip_pages_compact": (_c.c_int, [_P, _P, _P, _P, _P, _c.c_size_t, _P]),
+    "ane_hip_paged_norm_rope_append": (
+        _c.c_int, [_P, _c.c_uint32, _P, _c.c_uint32, _P, _c.c_uint32, _c.c_int, _P, _c.c_uint64, _P, _P, _c.c_uint64,
+                   _P, _P, _P, _c.c_float, _c.c_int, _P, _c.c_uint64, _P]),
     "ane_hip_quantize_tokens": (
         _c.c_int, [_c.c_uint32, _c.c_uint32, _c.c_int, _P, _c.c_uint64, _P, _c.c_float, _P, _c.c_uint64, _P, _P]),
     "ane_hip_dense_i8_scaled": (
@@ -1154,6 +1158,87 @@ def paged_rope_append(cache, layer, q_start, q, k, v, table, q_out, seqs=None, s
         tp = table.data_ptr()
     _launch(lib().ane_hip_paged_rope_append, cache, "paged_rope_append", stream,
             (cache._at, layer, sq, n, qs, tokens, ty, qp, q0, kp, vp, ks, tp, positions, to, op, o0))
+
+
+def rope_freqs(rot_dim, base=10000.0, factor=1.0, scaling=None, context=8192, low=1.0, high=4.0):
+    """(radians a position of each of the rot_dim/2 pairs in float64, the factor of cos and sin) for Rope: base^(-2i /
+    rot_dim), for a context `factor` times the one of `context` positions the model was trained on scaled by
+
+    None       not at all;
+    "linear"   all of them divided by factor;
+    "base"     base raised so that the slowest pair is divided by factor and the fastest kept;
+    "turns"    divided by factor below `low` turns within the old context, kept from `high` turns on, blended by the
+               number of turns in between;
+    "index"    the same borders (usually low=1, high=32), blended by the pair's index, and cos and sin times
+               0.1 ln(factor) + 1."""
+    import numpy as np
+
+    if rot_dim <= 0 or rot_dim % 2 or base <= 0 or factor <= 0 or context <= 0:
+        raise ValueError("rot_dim is even, base, factor and context are positive")
+    if scaling not in (None, "linear", "base", "turns", "index"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    i = np.arange(rot_dim // 2, dtype=np.float64)
+    if scaling == "base" and rot_dim > 2:
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    f = np.power(float(base), -2.0 * i / rot_dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling in ("turns", "index"):
+        if not 0 < low < high:
+            raise ValueError("0 < low < high")
+        if scaling == "turns":
+            keep = (context * f / (2 * np.pi) - low) / (high - low)
+        else:
+            at = [rot_dim * np.log(context / (2 * np.pi * t)) / (2 * np.log(base)) for t in (high, low)]
+            first, last = max(np.floor(at[0]), 0), min(np.ceil(at[1]), rot_dim - 1)
+            keep = 1.0 - (i - first) / max(last - first, 1e-3)
+        keep = np.clip(keep, 0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+    return f, (0.1 * np.log(factor) + 1.0 if scaling == "index" and factor > 1 else 1.0)
+
+
+class Rope(ctypes.Structure):
+    """Mirror of struct ane_rope (include/ane_decode.h) over a float64 device tensor of radians a position, which it
+    keeps alive (rope_freqs makes the values); half: pairs (i, i + n) of a head's first 2 n values, else (2i, 2i + 1);
+    factor multiplies cosines and sines."""
+
+    _fields_ = [("rot_dim", ctypes.c_uint32), ("halves", ctypes.c_uint32), ("freqs_ptr", ctypes.c_void_p),
+                ("factor", ctypes.c_double)]
+
+    def __init__(self, freqs, half=False, factor=1.0):
+        import torch
+
+        if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
+            raise ValueError("freqs is a contiguous float64 tensor of a value a pair")
+        self.freqs = freqs
+        super().__init__(2 * freqs.numel(), int(bool(half)), _p(freqs), factor)
+        self._at, self._device = ctypes.addressof(self), freqs.get_device()
+
+
+def paged_norm_rope_append(cache, layer, q_start, q, k, v, rope, q_out, q_norm=None, k_norm=None, eps=1e-6, seqs=None,
+                           stream=None):
+    """RMSNorm of each q and k head (float32 weights [head_dim]; None: none), the rotation of `rope` (a Rope; None: none)
+    and the append of k and v to the pages of one layer; the rest as paged_rope_append."""
+    kp, ty, tokens, ks = _rows(k, cache._kv, cache, "k")
+    vp, tv, nv, vs = _rows(v, cache._kv, cache, "v")
+    if (ty, tokens, ks) != (tv, nv, vs):
+        raise ValueError("k and v have the same shape, strides and type")
+    n, qs, sq = _batch(q_start, seqs, tokens, cache)
+    qp = op = None
+    q0 = o0 = to = 0
+    if q is not None and q_out is not None:
+        qp, tq, nq, q0 = _rows(q, cache._q, cache, "q")
+        op, to, no, o0 = _rows(q_out, cache._q, cache, "q_out")
+        if tq != ty or nq != tokens or no < tokens:
+            raise ValueError("q has the tokens and type of k, q_out room for them")
+    elif q is not None or q_out is not None:
+        raise ValueError("q and q_out go together")
+    if rope is not None and rope._device != cache._device:
+        raise ValueError("the rope's frequencies are on the cache's device")
+    _launch(lib().ane_hip_paged_norm_rope_append, cache, "paged_norm_rope_append", stream,
+            (cache._at, layer, sq, n, qs, tokens, ty, qp, q0, kp, vp, ks, None if rope is None else rope._at,
+             _vector(q_norm, cache._q[1], cache._device, "q_norm"), _vector(k_norm, cache._q[1], cache._device, "k_norm"),
+             eps, to, op, o0))
 
 
 def _attention_rows(cache, q, out):

@@ -10,8 +10,6 @@
 namespace ane {
 namespace {
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-
 // ------------------------------------------------------------ RoPE + append
 struct AppendArgs {
     const void *q, *k, *v;
@@ -22,32 +20,6 @@ struct AppendArgs {
     uint64_t q_stride, kv_stride, q_out_stride;
     uint32_t n, rope_len, n_heads, n_kv, hd, ps, n_pages, max_pages, n_seqs;
 };
-
-template <class T>
-__device__ __forceinline__ void load8(const void* p, uint64_t i, float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const h8 a = *reinterpret_cast<const h8*>(static_cast<const _Float16*>(p) + i);
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = (float)a[e];
-    }
-}
-template <class T>
-__device__ __forceinline__ void store8(void* p, uint64_t i, const float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        float* o = static_cast<float*>(p) + i;
-        *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(o + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-        h8 a;
-#pragma unroll
-        for (int e = 0; e < 8; e++) a[e] = (_Float16)x[e];
-        *reinterpret_cast<h8*>(static_cast<_Float16*>(p) + i) = a;
-    }
-}
 
 // One workgroup per token; a thread takes 8 values (4 pairs) of one head at a
 // time: [q heads | k heads | v heads] x hd/8 units.  The values of the first

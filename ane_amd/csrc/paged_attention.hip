@@ -30,7 +30,6 @@ namespace {
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __fp16 hh2 __attribute__((ext_vector_type(2)));  // (what the dot product's builtin takes)
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef short s4 __attribute__((ext_vector_type(4)));

@@ -260,6 +260,27 @@ int ane_hip_paged_rope_append(const struct ane_paged_cache* cache, uint32_t laye
                               const float* rope_table, uint32_t rope_len, int q_out_type, void* q_out,
                               uint64_t q_out_stride, void* stream);
 
+/* The same for models that normalise each q and k head, rotate halves or part of
+ * a head, or scale the rotation for long contexts: with q_norm and k_norm (fp32
+ * [head_dim], each may be NULL) a head becomes x / sqrt(mean(x^2) + eps) * w
+ * first; then pair i of its leading rot_dim values (a, b) becomes (a c - b s,
+ * a s + b c), c and s = factor * (cos, sin)(position * freqs[i]).  The angle is
+ * formed in fp64, its cosine and sine exact to fp32, the rest in fp32; there is no
+ * table and no bound on positions but the cache's.  rope NULL or rot_dim 0: no
+ * rotation.  A token at a negative position is not appended and its q_out row is
+ * zeros.  Everything else as above. */
+struct ane_rope {
+    uint32_t rot_dim;    /* a multiple of 16, at most head_dim */
+    uint32_t halves;     /* 0: pairs (2i, 2i + 1); else (i, i + rot_dim / 2) */
+    const double* freqs; /* device, [rot_dim / 2]: radians a position */
+    double factor;       /* above 0, below 1e30; 1 for most models */
+};
+int ane_hip_paged_norm_rope_append(const struct ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
+                                   const uint32_t* q_start, uint32_t n_tokens, int in_type, const void* q,
+                                   uint64_t q_stride, const void* k, const void* v, uint64_t kv_stride,
+                                   const struct ane_rope* rope, const float* q_norm, const float* k_norm, float eps,
+                                   int q_out_type, void* q_out, uint64_t q_out_stride, void* stream);
+
 /* Causal attention of packed prompts with grouped heads: for each new token at
  * position p, out[h] = softmax(scale * q[h] . K[g][0..p]^T) V[g][0..p],
  * g = h / (n_heads / n_kv_heads); zeros for a token at a negative position.
