@@ -166,6 +166,8 @@ EXPORTS = (
     "ane_hip_pages_copy",
     "ane_hip_pages_compact",
     "ane_hip_paged_norm_rope_append",
+    "ane_hip_attention_rule_workspace_size",
+    "ane_hip_attention_rule",
     "ane_hip_quantize_tokens",
     "ane_hip_dense_i8_scaled",
     "ane_hip_linear_i8_workspace_size",
@@ -281,6 +283,10 @@ _SIGS: dict[str, tuple[Any, list[Any]]] = {
     "ane_hip_paged_norm_rope_append": (
         _c.c_int, [_P, _c.c_uint32, _P, _c.c_uint32, _P, _c.c_uint32, _c.c_int, _P, _c.c_uint64, _P, _P, _c.c_uint64,
                    _P, _P, _P, _c.c_float, _c.c_int, _P, _c.c_uint64, _P]),
+    "ane_hip_attention_rule_workspace_size": (_c.c_size_t, [_P, _c.c_uint32, _c.c_uint32, _c.c_uint32, _P]),
+    "ane_hip_attention_rule": (
+        _c.c_int, [_P, _c.c_uint32, _P, _c.c_uint32, _P, _c.c_uint32, _c.c_uint32, _P, _c.c_int, _P, _c.c_uint64,
+                   _c.c_float, _P, _c.c_uint64, _P, _c.c_size_t, _P]),
     "ane_hip_quantize_tokens": (
         _c.c_int, [_c.c_uint32, _c.c_uint32, _c.c_int, _P, _c.c_uint64, _P, _c.c_float, _P, _c.c_uint64, _P, _P]),
     "ane_hip_dense_i8_scaled": (
@@ -1249,28 +1255,76 @@ def _attention_rows(cache, q, out):
     return ty, tokens, qp, q0, op, o0
 
 
-def attention_prompt_workspace_size(cache, n, n_tokens, max_len=None) -> int:
+class AttentionRule(ctypes.Structure):
+    """Mirror of struct ane_attention_rule (include/ane_decode.h), over device tensors that it keeps alive: scores capped
+    at softcap by a tanh (0: not), lowered by slopes (float32 [heads]) times the distance, keys window and more positions
+    back not seen (0: all), none before first (int32 [tokens]: where each new token's document begins), all below prefix
+    (int32 [rows of the batch]) seen from both sides.  A call reads the tensors when it runs."""
+
+    _fields_ = [("softcap", ctypes.c_float), ("window", ctypes.c_uint32), ("slopes_ptr", ctypes.c_void_p),
+                ("first_ptr", ctypes.c_void_p), ("prefix_ptr", ctypes.c_void_p)]
+
+    def __init__(self, softcap=0.0, slopes=None, window=0, first=None, prefix=None):
+        import torch
+
+        given = [t for t in (slopes, first, prefix) if t is not None]
+        if slopes is not None and slopes.dtype != torch.float32:
+            raise ValueError("slopes is a float32 tensor of a value a head")
+        if any(t.dtype != torch.int32 for t in (first, prefix) if t is not None):
+            raise ValueError("first and prefix are int32 tensors")
+        if not all(t.dim() == 1 and t.is_contiguous() and t.get_device() == given[0].get_device() for t in given):
+            raise ValueError("the rule's tensors are contiguous vectors on one device")
+        if not 0 <= window < 1 << 32:
+            raise ValueError("window is a number of positions")
+        self.slopes, self.first, self.prefix = slopes, first, prefix
+        super().__init__(softcap, window, _p(slopes) or None, _p(first) or None, _p(prefix) or None)
+        self._at, self._device = ctypes.addressof(self), given[0].get_device() if given else None
+        self._need = [None if t is None else t.numel() for t in (slopes, first, prefix)]
+
+
+def _rule(rule, cache, tokens, n):
+    """The rule's address, its tensors long enough for the call."""
+    heads, first, prefix = rule._need
+    if heads is not None and heads != cache._q[0]:
+        raise ValueError("slopes has a value for each head")
+    if (first is not None and first < tokens) or (prefix is not None and prefix < n):
+        raise ValueError("first has an entry for each token, prefix one for each row of the batch")
+    if rule._device is not None and rule._device != cache._device:
+        raise ValueError("the rule's tensors are on the cache's device")
+    return rule._at
+
+
+def attention_prompt_workspace_size(cache, n, n_tokens, max_len=None, rule=None) -> int:
+    if rule is not None:
+        return int(lib().ane_hip_attention_rule_workspace_size(cache._at, n, n_tokens, max_len or 0, rule._at))
     return int(lib().ane_hip_attention_prompt_workspace_size(cache._at, n, n_tokens, max_len or 0))
 
 
-def attention_prompt_workspace(cache, n, n_tokens, max_len=None):
+def attention_prompt_workspace(cache, n, n_tokens, max_len=None, rule=None):
     """A workspace for attention_prompt calls of these sizes, for callers that keep one."""
-    return _scratch(attention_prompt_workspace_size(cache, n, n_tokens, max_len), cache.k_pages.device)
+    return _scratch(attention_prompt_workspace_size(cache, n, n_tokens, max_len, rule), cache.k_pages.device)
 
 
-def attention_prompt(cache, layer, q_start, q, out, max_len=None, scale=None, seqs=None, workspace=None, stream=None):
+def attention_prompt(cache, layer, q_start, q, out, max_len=None, scale=None, seqs=None, workspace=None, stream=None,
+                     rule=None):
     """Causal attention of packed prompts over the pages of one layer: q and out
     [tokens][heads][head_dim] float32 or float16, the new tokens of batch row i
     (its sequence's last positions, already appended) in rows q_start[i] ..
-    q_start[i+1]-1.  max_len bounds the sequences' lengths; scale None:
-    1/sqrt(head_dim)."""
+    q_start[i+1]-1 (q_start None: one each).  max_len bounds the sequences'
+    lengths; scale None: 1/sqrt(head_dim); rule: an AttentionRule, for scores
+    that are capped or lowered with the distance and for other masks."""
     ty, tokens, qp, q0, op, o0 = _attention_rows(cache, q, out)
     n, qs, sq = _batch(q_start, seqs, tokens, cache)
     workspace, wp, size = _work(cache, workspace,
-                                lambda: attention_prompt_workspace_size(cache, n, tokens, max_len), stream)
+                                lambda: attention_prompt_workspace_size(cache, n, tokens, max_len, rule), stream)
+    scale = cache._scale if scale is None else scale
+    if rule is not None:
+        _launch(lib().ane_hip_attention_rule, cache, "attention_prompt", stream,
+                (cache._at, layer, sq, n, qs, tokens, max_len or 0, _rule(rule, cache, tokens, n), ty, qp, q0, scale, op, o0,
+                 wp, size))
+        return
     _launch(lib().ane_hip_attention_prompt, cache, "attention_prompt", stream,
-            (cache._at, layer, sq, n, qs, tokens, max_len or 0, ty, qp, q0, cache._scale if scale is None else scale, op,
-             o0, wp, size))
+            (cache._at, layer, sq, n, qs, tokens, max_len or 0, ty, qp, q0, scale, op, o0, wp, size))
 
 
 def attention_shared_workspace_size(cache, n, n_groups=0, max_prefix=None, max_len=None) -> int:

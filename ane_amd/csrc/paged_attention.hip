@@ -52,6 +52,13 @@ struct AttnArgs {
     } own, pre;                    // of a row's own keys (all of a prompt's), of the shared prefix
     uint32_t parts_total;
     float scale_log2e;
+    // A rule (ane_decode.h), in kernels with RULE: cap and 1 / cap in log2 units
+    // (0: none), slopes by head, window (0: none), the first position each token
+    // sees, the prefix each batch row sees whole (null: none).
+    float cap, inv_cap;
+    uint32_t window;
+    const float* slopes;
+    const uint32_t *first, *seen;
 
     template <int MODE>
     __device__ __forceinline__ const Parts& parts() const { return MODE == kPrefix ? pre : own; }
@@ -138,8 +145,20 @@ __device__ __forceinline__ uint32_t shared_len(const AttnArgs& a, uint32_t s, ui
     return min(min(lane_of(p, l), len), seq_len(a, seq_id(a, first)));
 }
 
+// The first position token t of the work's sees under a rule.
+__device__ __forceinline__ int32_t rule_first(const AttnArgs& a, const Work& w, uint32_t t) {
+    const int32_t pos = w.len - (int32_t)w.toks + (int32_t)t;
+    int32_t lo = a.window ? max(pos + 1 - (int32_t)a.window, 0) : 0;
+    if (a.first) lo = max(lo, (int32_t)min(a.first[w.tok0 + t], 0x7fffffffu));
+    return lo;
+}
+// The end of what they see, whatever the token.
+__device__ __forceinline__ int32_t rule_seen(const AttnArgs& a, const Work& w) {
+    return a.seen ? (int32_t)min(a.seen[w.s], (uint32_t)w.len) : 0;
+}
+
 // The keys of part `part`.
-template <int MODE>
+template <int MODE, bool RULE = false>
 __device__ __forceinline__ void find_keys(const AttnArgs& a, uint32_t bm, uint32_t part, Work& w) {
     w.len = (int32_t)seq_len(a, w.id, w.raw);
     w.kbeg = w.lo = 0;
@@ -148,6 +167,19 @@ __device__ __forceinline__ void find_keys(const AttnArgs& a, uint32_t bm, uint32
     if (MODE == kPrompt) {
         const int32_t last = (int32_t)a.by_G(min(w.row0 + bm, w.rows) - 1);
         w.kend = min(w.len, w.len - (int32_t)w.toks + last + 1);
+        if constexpr (RULE) {
+            const int32_t tok = (int32_t)a.by_G(w.row0);
+            if (w.kend > 0) w.kend = max(w.kend, rule_seen(a, w));
+            int32_t lo = a.window ? max(w.len - (int32_t)w.toks + tok + 1 - (int32_t)a.window, 0) : 0;
+            if (a.first) {  // the least of the tile's tokens (at most 128): what none of them sees is not read
+                uint32_t f = 0xffffffffu;
+                for (int32_t t = tok + (int32_t)(threadIdx.x & 63); t <= last; t += 64) f = min(f, a.first[w.tok0 + t]);
+#pragma unroll
+                for (int x = 32; x >= 1; x >>= 1) f = min(f, (uint32_t)__shfl_xor((int)f, x, 64));
+                lo = max(lo, (int32_t)min(f, 0x7fffffffu));
+            }
+            w.kbeg = min(lo, max(w.kend, 0)) & ~15;
+        }
     } else if (MODE == kPrefix) {
         w.kend = (int32_t)min(w.prefix, (uint32_t)w.len);
     } else {
@@ -161,14 +193,15 @@ __device__ __forceinline__ void find_keys(const AttnArgs& a, uint32_t bm, uint32
     uniform(w.kbeg), uniform(w.kend), uniform(w.lo), uniform(w.len);
 }
 // Whether the first key's position is known before any length is.
-template <int MODE>
-__device__ __forceinline__ bool early_keys(const AttnArgs& a) { return MODE != kOwn || a.n_groups == 0; }
+template <int MODE, bool RULE = false>
+__device__ __forceinline__ bool early_keys(const AttnArgs& a) { return !RULE && (MODE != kOwn || a.n_groups == 0); }
 
 // Keys of the work a row (token t of the work's) sees: those below.
-template <int MODE>
+template <int MODE, bool RULE = false>
 __device__ __forceinline__ int32_t row_limit(const AttnArgs& a, const Work& w, uint32_t t) {
     int32_t l = w.len;
     if (MODE == kPrompt) l += (int32_t)t + 1 - (int32_t)w.toks;
+    if (RULE && l > 0) l = max(l, rule_seen(a, w));
     if (MODE == kPrefix) l = (int32_t)seq_len(a, seq_id(a, w.tok0 + t));
     return min(l, w.kend);
 }
@@ -295,9 +328,42 @@ __device__ __forceinline__ void split(f2 x, h2& hi, h2& lw) {
 // the first takes 137.
 constexpr float kDrop = 8.0f, kDeep = 24.0f, kThin = -7.0f, kAgain = 38.0f;
 
+// tanh(y) = y + y z P(z), z = y^2, up to |y| = kSmall (P fitted here for the least
+// relative error: 2^-23.8 with five coefficients to 0.6, in fp32 arithmetic; 2^-20.4
+// with four to 0.75, below what fp16 weights are rounded by), beyond that as 1 - 2 /
+// (1 + e^2y), there exact to 2^-22.  A cap is chosen well above most scores, so most
+// tiles are all small, and P costs half of what exponential and reciprocal do.
+template <bool F32>
+struct Tanh {
+    static constexpr float kSmall = F32 ? 0.6f : 0.75f;
+    static __device__ __forceinline__ float small(float y) {
+        const float z = y * y;
+        float p;
+        if constexpr (F32) {
+            p = -0.0058951363f;
+            p = __builtin_fmaf(p, z, 0.02079595252f);
+            p = __builtin_fmaf(p, z, -0.0537838228f);
+            p = __builtin_fmaf(p, z, 0.13331924378f);
+            p = __builtin_fmaf(p, z, -0.3333329856f);
+        } else {
+            p = 0.01310574356f;
+            p = __builtin_fmaf(p, z, -0.0502778515f);
+            p = __builtin_fmaf(p, z, 0.13268233835f);
+            p = __builtin_fmaf(p, z, -0.3332966864f);
+        }
+        return __builtin_fmaf(p * z, y, y);
+    }
+    static __device__ __forceinline__ float any(float y) {
+        const float e = __builtin_amdgcn_exp2f(y * 2.88539008177792681f);
+        const float t = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+        return fabsf(y) > kSmall ? t : small(y);
+    }
+};
+
 // 32 rows of a wave: lane & 31 is the row, lane >> 5 the half of its keys (of its
-// dimensions in q and O).
-template <int HD, bool F32>
+// dimensions in q and O).  RULE: scores capped, lowered with the distance, keys before
+// a row's own first one masked (ane_decode.h).
+template <int HD, bool F32, bool RULE = false>
 struct Rows {
     static constexpr int NS = HD / 16, ND = HD / 32;
     static constexpr uint32_t RB = HD * 2;
@@ -310,6 +376,69 @@ struct Rows {
     int32_t lim;    // keys below it are seen
     int32_t wmin, wmax;
     uint32_t half, ka, va[2 * ND];
+    // RULE: keys before `begin` are masked (least and largest of the rows below), the
+    // row's position and slope (log2 units); scores times cin, then capped and lowered,
+    // are in log2 units already, and c is 1 (bent: they are).
+    int32_t begin, fmin, fmax, pos;
+    float slope, cin, cap;
+    bool bent, sloped;
+
+    __device__ __forceinline__ void init_rule(const AttnArgs& a, const Work& w, uint32_t t, uint32_t head, bool live) {
+        pos = w.len - (int32_t)w.toks + (int32_t)t;
+        begin = rule_first(a, w, t);
+        fmin = live ? begin : 0x7fffffff, fmax = live ? begin : 0;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            fmin = min(fmin, __shfl_xor(fmin, x, 64));
+            fmax = max(fmax, __shfl_xor(fmax, x, 64));
+        }
+        fmin = __builtin_amdgcn_readfirstlane(fmin);
+        fmax = __builtin_amdgcn_readfirstlane(fmax);
+        slope = a.slopes ? a.slopes[head] * 1.44269504088896341f : 0.0f;
+        cap = a.cap;
+        sloped = a.slopes;
+        bent = sloped || cap != 0.0f;
+    }
+    // after take_q
+    __device__ __forceinline__ void bend_scale(const AttnArgs& a) {
+        if (!bent) return;
+        // (as c in take_q: never 0 nor infinite)
+        cin = a.cap != 0.0f ? __builtin_amdgcn_fmed3f(c * a.inv_cap, 0x1p-126f, 0x1p127f) : c;
+        c = 1.0f;
+    }
+    template <int KT>
+    __device__ __forceinline__ void bend(f16v (&s)[KT], int32_t t0) const {
+        float top = 0.0f;
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[t][r] *= cin;
+        if (cap != 0.0f) {  // uniform, as the next one
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, fabsf(s[t][r])), fabsf(s[t][r + 1]));
+            if (__any(top > Tanh<F32>::kSmall)) {
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[t][r] = Tanh<F32>::any(s[t][r]) * cap;
+            } else {
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[t][r] = Tanh<F32>::small(s[t][r]) * cap;
+            }
+        }
+        if (sloped) {
+            const float at = (float)(pos - t0 - 4 * (int32_t)half);
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    s[t][r] = __builtin_fmaf(-slope, fabsf(at - (float)(t * 32 + 8 * (r >> 2) + (r & 3))), s[t][r]);
+        }
+    }
 
     __device__ __forceinline__ void init(float scale_log2e, int32_t limit, bool live) {
         const uint32_t lane = threadIdx.x & 63, i = lane & 15, grp = lane >> 4;
@@ -485,13 +614,16 @@ struct Rows {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int32_t key = t0 + t * 32 + 8 * (r >> 2) + 4 * (int32_t)half + (r & 3);
-                if (key >= lim || key < lo) s[t][r] = -INFINITY;
+                if (key >= lim || key < lo || (RULE && key < begin)) s[t][r] = -INFINITY;
             }
     }
     // Scores of keys from position t0 on to weights; keys before lo are masked.
     // Whether this lane has some so small that carried() has to look at them.
     template <int KT, class Between>
     __device__ __forceinline__ bool weights(f16v (&s)[KT], int32_t t0, int32_t lo, Weights<KT>& p, Between between) {
+        if constexpr (RULE) {
+            if (bent) bend<KT>(s, t0);
+        }
         float low = INFINITY;  // (of the masked too, which costs a second round at worst)
         auto least = [&] {
             if constexpr (F32) {
@@ -501,7 +633,7 @@ struct Rows {
                     for (int r = 0; r < 16; r++) low = fminf(low, s[t][r]);
             }
         };
-        if (t0 + 32 * KT > wmin || t0 < lo) {  // uniform
+        if (t0 + 32 * KT > wmin || t0 < lo || (RULE && t0 < fmax)) {  // uniform
             asm volatile("");  // a branch, not two selects a score in every tile
             least();
             mask<KT>(s, t0, lo);
@@ -655,7 +787,7 @@ struct Rows {
             const uint32_t id = p < a.max_pages ? a.table[(uint64_t)w.id * a.max_pages + p] : ANE_NO_PAGE;
             if (id >= a.n_pages) continue;
             const uint16_t* v = a.vp + (((uint64_t)id * a.n_kv + g) * a.ps + (uint32_t)key - p * a.ps) * HD + 4 * half;
-            const bool sees = key < lim;
+            const bool sees = key < lim && !(RULE && key < begin);
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -739,56 +871,64 @@ __device__ __forceinline__ uint32_t block_wave() { return __builtin_amdgcn_readf
 // Weights between the products of the other half in one wave measured slower
 // (584 us, 549 so), fragments 2, 3 or 6 ahead, the copies spread over the products,
 // and row tiles started in descending order of keys the same.
-template <int HD, bool F32, int MODE>
+template <int HD, bool F32, int MODE, bool RULE = false>
 __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slots) {
     constexpr uint32_t kT = 64 * HD * 2;
     // K, V of each stage, then one word a wave: its rows' least limit, and whether
     // its group of a tile of each parity holds a value that is not finite.  One
     // array on purpose: with several, the compiler tells LDS accesses apart, and
     // then waits for all copies in flight before it reads what they may alias.
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kT + 48];
-    int32_t* least = reinterpret_cast<int32_t*>(smem + 4 * kT);
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kT + (RULE ? 64 : 48)];
+    int32_t *least = reinterpret_cast<int32_t*>(smem + 4 * kT), *most = least + 12;
     int32_t *odd = least + 4, odd_from = 0x7fffffff, odd_to = 0;
     const uint32_t wave = block_wave(), lane = threadIdx.x & 63, tile = a.by_kv(blockIdx.x);
     const uint32_t g = blockIdx.x - tile * a.n_kv;
     // a causal prompt's last tiles have the most keys: they start first
     Work w;
     if (!find_rows<MODE, 128>(a, slots - 1 - tile, w)) return;
+    if constexpr (RULE) uniform(w.row0), uniform(w.rows), uniform(w.tok0), uniform(w.toks);  // (again: else held as vectors)
 
     // page numbers, length and q are under way together; then the first copies
     Loader<HD> ld;
-    ld.lookup(a, w.id, wave + lane * 4);
-    Rows<HD, F32> r;
-    typename Rows<HD, F32>::Raw raw;
-    const uint32_t row = w.row0 + wave * 32 + (lane & 31), tok = a.by_G(min(row, w.rows - 1));
-    const uint32_t head = g * a.G + min(row, w.rows - 1) - tok * a.G;
-    const bool live = row < w.rows;
+    if (!RULE) ld.lookup(a, w.id, wave + lane * 4);
+    Rows<HD, F32, RULE> r;
+    typename Rows<HD, F32, RULE>::Raw raw;
+    uint32_t row = w.row0 + wave * 32 + (lane & 31), tok = a.by_G(min(row, w.rows - 1));
+    uint32_t head = g * a.G + min(row, w.rows - 1) - tok * a.G;
+    bool live = row < w.rows;
     r.fetch_q(a.q, (w.tok0 + tok) * a.q_stride + head * HD, live, raw);
-    find_keys<MODE>(a, 128, 0, w);
+    find_keys<MODE, RULE>(a, 128, 0, w);
+    const int32_t base = RULE ? w.kbeg : 0;  // the first tile's first key
+    const uint32_t u0 = (uint32_t)base / 16 + wave;
+    if (RULE) ld.lookup(a, w.id, u0 + lane * 4);
     ld.settle();
     ld.init();
-    const uint32_t tiles = w.kend > 0 ? (uint32_t)(w.kend + 63) / 64 : 0;
+    const uint32_t tiles = w.kend > base ? (uint32_t)(w.kend - base + 63) / 64 : 0;
     auto issue = [&](uint32_t t) {
-        if (t && (t & 63) == 0) ld.lookup(a, w.id, wave + (t + lane) * 4), ld.settle();
+        if (t && (t & 63) == 0) ld.lookup(a, w.id, u0 + (t + lane) * 4), ld.settle();
         uint8_t* st = smem + (t & 1) * 2 * kT + wave * (kT / 4);
-        ld.copy(a, a.kp, w, g, wave + t * 4, t & 63, st);
-        ld.copy(a, a.vp, w, g, wave + t * 4, t & 63, st + kT);
+        ld.copy(a, a.kp, w, g, u0 + t * 4, t & 63, st);
+        ld.copy(a, a.vp, w, g, u0 + t * 4, t & 63, st + kT);
     };
     if (tiles) issue(0);
-    r.init(a.scale_log2e, row_limit<MODE>(a, w, tok), live);
+    r.init(a.scale_log2e, row_limit<MODE, RULE>(a, w, tok), live);
+    if constexpr (RULE) r.init_rule(a, w, tok, head, live);
     r.take_q(raw);
+    if constexpr (RULE) r.bend_scale(a);
     __builtin_amdgcn_sched_barrier(0);
     r.clear();
 
     if (lane == 0) least[wave] = r.wmin;
+    if (RULE && lane == 0) most[wave] = r.fmax;
     wait_lgkmcnt0();
     lds_barrier();
     const int32_t wg_min = min(min(least[0], least[1]), min(least[2], least[3]));
+    const int32_t wg_from = RULE ? max(max(most[0], most[1]), max(most[2], most[3])) : 0;
     for (uint32_t t = 0; t < tiles; t++) {
-        const int32_t t0 = (int32_t)t * 64;
+        const int32_t t0 = base + (int32_t)t * 64;
         uint8_t* st = smem + (t & 1) * 2 * kT;
         int32_t* flag = odd + (t & 1) * 4;
-        const bool masked = t0 + 64 > wg_min;
+        const bool masked = t0 + 64 > wg_min || (RULE && t0 < wg_from);
         wait_vmcnt<0>();  // this wave's copies of tile t
         if (masked) {
             const bool bad = tidy<HD>(st + kT + wave * (kT / 4));
@@ -802,13 +942,19 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
         if constexpr (F32) {  // 32 keys at a time: the two parts of q and of 64 weights do not fit 256 registers
 #pragma unroll 1
             for (int h = 0; h < 2; h++)
-                if (t0 + 32 * h < r.wmax) r.template step<1>(st + h * (kT / 2), st + kT + h * (kT / 2), t0 + 32 * h, 0);
+                if (t0 + 32 * h < r.wmax && !(RULE && t0 + 32 * h + 32 <= r.fmin)) r.template step<1>(st + h * (kT / 2), st + kT + h * (kT / 2), t0 + 32 * h, 0);
         } else {
-            if (t0 < r.wmax) r.template step<2>(st, st + kT, t0, 0);
+            if (t0 < r.wmax && !(RULE && t0 + 64 <= r.fmin)) r.template step<2>(st, st + kT, t0, 0);
         }
     }
     if (odd_from < odd_to) r.add_nonfinite(a, w, g, odd_from, odd_to);
 
+    if constexpr (RULE) {  // worked out again: kept through the loop, they spill
+        uint32_t i = lane;
+        asm volatile("" : "+v"(i));
+        row = w.row0 + wave * 32 + (i & 31), tok = a.by_G(min(row, w.rows - 1));
+        head = g * a.G + min(row, w.rows - 1) - tok * a.G, live = row < w.rows;
+    }
     if (!live) return;
     const float l = other_sum(r.l);
     if (MODE == kPrompt) {
@@ -851,7 +997,7 @@ constexpr uint32_t few_lds() {  // K and V of four waves (or their sums), and th
 }
 // EACH: every wave has rows and keys of its own (slot and g differ by wave), so
 // there is nothing to merge.
-template <int HD, bool F32, int MODE, bool EACH = false>
+template <int HD, bool F32, int MODE, bool EACH = false, bool RULE = false>
 __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint32_t part, uint32_t g, uint8_t* smem) {
     constexpr uint32_t kT = 32 * HD * 2;
     constexpr int kC = 2 * Loader<HD>::kCopies;
@@ -864,17 +1010,17 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
 
     Loader<HD> ld;
     uint32_t u0 = part * (a.parts<MODE>().chunk / 16) + turn * 2;
-    if (early_keys<MODE>(a)) ld.lookup(a, w.id, u0 + lane / 2 * (2 * kWaves) + (lane & 1));
-    Rows<HD, F32> r;
-    typename Rows<HD, F32>::Raw raw;
+    if (early_keys<MODE, RULE>(a)) ld.lookup(a, w.id, u0 + lane / 2 * (2 * kWaves) + (lane & 1));
+    Rows<HD, F32, RULE> r;
+    typename Rows<HD, F32, RULE>::Raw raw;
     const uint32_t row = w.row0 + (lane & 31), tok = a.by_G(min(row, w.rows - 1));
     const uint32_t head = g * a.G + min(row, w.rows - 1) - tok * a.G;
     const bool live = row < w.rows;
     const uint64_t at_q = (w.tok0 + tok) * a.q_stride + head * HD;
     if constexpr (MODE == kOwn) r.fetch_q(a.q, at_q, live, raw);
     else r.fetch_rows(a.q, at_q * (F32 ? 4 : 2), raw);
-    find_keys<MODE>(a, 32, part, w);
-    if (!early_keys<MODE>(a)) {
+    find_keys<MODE, RULE>(a, 32, part, w);
+    if (!early_keys<MODE, RULE>(a)) {
         u0 = (uint32_t)w.kbeg / 16 + turn * 2;
         ld.lookup(a, w.id, u0 + lane / 2 * (2 * kWaves) + (lane & 1));
     }
@@ -899,9 +1045,11 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
 #pragma unroll
         for (int i = 0; i < kC; i++) copy(n, i, kt);
     }
-    r.init(a.scale_log2e, row_limit<MODE>(a, w, tok), live);
+    r.init(a.scale_log2e, row_limit<MODE, RULE>(a, w, tok), live);
+    if constexpr (RULE) r.init_rule(a, w, tok, head, live);
     if constexpr (MODE != kOwn) r.turn_rows(vt, live, raw);
     r.take_q(raw);
+    if constexpr (RULE) r.bend_scale(a);
     __builtin_amdgcn_sched_barrier(0);
     r.clear();
 
@@ -909,8 +1057,8 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
     for (uint32_t t = 0; t < tiles; t++) {
         const int32_t t0 = first + (int32_t)t * kStep;
         f16v s[1];
-        h8 vf[Rows<HD, F32>::kAhead];
-        typename Rows<HD, F32>::template Weights<1> p;
+        h8 vf[Rows<HD, F32, RULE>::kAhead];
+        typename Rows<HD, F32, RULE>::template Weights<1> p;
         wait_vmcnt<0>();  // K of this block
         const Next vn = aim(a.vp, t);
         r.template scores<1>(kt, s, [&](int i) {
@@ -926,7 +1074,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
             if (i < kC) copy(kn, i, kt);
         });
         wait_vmcnt<kC>();  // V of this block
-        if (t0 + 32 > r.wmin || t0 < w.lo) {
+        if (t0 + 32 > r.wmin || t0 < w.lo || (RULE && t0 < r.fmax)) {
             const bool b0 = tidy<HD>(vt), b1 = tidy<HD>(vt + kT / 2);
             if (b0 || b1) odd_from = min(odd_from, t0), odd_to = t0 + 32;
             wait_lgkmcnt0();
@@ -1008,11 +1156,11 @@ __device__ __forceinline__ float wave_max_all(float x) {
 }
 
 // (one LDS array in all of them, as above; of 64-wide heads at least three workgroups a CU)
-template <int HD, bool F32, int MODE>
+template <int HD, bool F32, int MODE, bool RULE = false>
 __global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) k_attn_few(AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
     const uint32_t slot = a.by_kv(blockIdx.x);
-    attn_few<HD, F32, MODE>(a, slot, blockIdx.y, blockIdx.x - slot * a.n_kv, smem);
+    attn_few<HD, F32, MODE, false, RULE>(a, slot, blockIdx.y, blockIdx.x - slot * a.n_kv, smem);
 }
 // Single tokens with few keys, a wave each.
 template <int HD, bool F32>
@@ -1122,11 +1270,11 @@ size_t parts_bytes(const ane_paged_cache* c, uint32_t n_tokens, uint32_t parts, 
     return o + ceil_to(rows * 8, 256);
 }
 
-template <int HD, bool F32>
+template <int HD, bool F32, bool RULE = false>
 void launch_prompt(const AttnArgs& a, const Launch& l, hipStream_t s) {
     const dim3 grid((uint32_t)(l.slots * a.n_kv), l.parts);
-    if (l.few) hipLaunchKernelGGL((k_attn_few<HD, F32, kPrompt>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_block<HD, F32, kPrompt>), grid, dim3(256), 0, s, a, (uint32_t)l.slots);
+    if (l.few) hipLaunchKernelGGL((k_attn_few<HD, F32, kPrompt, RULE>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_block<HD, F32, kPrompt, RULE>), grid, dim3(256), 0, s, a, (uint32_t)l.slots);
 }
 template <int HD, bool F32>
 void launch_shared(const AttnArgs& a, const SharedPlan& p, hipStream_t s) {
@@ -1180,24 +1328,33 @@ bool bad_workspace(const void* ws, size_t bytes, size_t need) {
 
 using namespace ane;
 
-extern "C" size_t ane_hip_attention_prompt_workspace_size(const ane_paged_cache* cache, uint32_t n, uint32_t n_tokens,
-                                                          uint32_t max_len) {
+// A bound on the keys that a row tile's rows see under a rule: with a window, and
+// nothing seen past a token's own position, no more than window and tile.
+static uint64_t rule_len(const ane_paged_cache* c, const ane_attention_rule* r, uint32_t max_len) {
+    const uint64_t len = bound_len(c, max_len);
+    return r && r->window && !r->prefix ? std::min<uint64_t>(len, (uint64_t)r->window + 32 + 16) : len;
+}
+
+static size_t prompt_workspace(const ane_paged_cache* cache, const ane_attention_rule* rule, uint32_t n, uint32_t n_tokens,
+                               uint32_t max_len) {
     if (cache_status(cache) || n == 0 || n_tokens == 0 || n > kMaxTokens || n_tokens > kMaxTokens) return 0;
     // the same for a batch of single tokens with and without q_start
-    const Launch l = plan(cache, n, n_tokens, false, bound_len(cache, max_len));
-    const Launch one = plan(cache, n, n_tokens, true, bound_len(cache, max_len));
+    const Launch l = plan(cache, n, n_tokens, false, rule_len(cache, rule, max_len));
+    const Launch one = plan(cache, n, n_tokens, true, rule_len(cache, rule, max_len));
     return parts_bytes(cache, n_tokens, n_tokens == n ? std::max(l.parts, one.parts) : l.parts, nullptr);
 }
 
-extern "C" int ane_hip_attention_prompt(const ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
-                                        const uint32_t* q_start, uint32_t n_tokens, uint32_t max_len, int type,
-                                        const void* q, uint64_t q_stride, float scale, void* out, uint64_t out_stride,
-                                        void* workspace, size_t workspace_bytes, void* stream) {
+static int prompt(const ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n, const uint32_t* q_start,
+                  uint32_t n_tokens, uint32_t max_len, const ane_attention_rule* rule, int type, const void* q,
+                  uint64_t q_stride, float scale, void* out, uint64_t out_stride, void* workspace, size_t workspace_bytes,
+                  void* stream) {
     const int st = attention_status(cache, layer, n, n_tokens, type, q, q_stride, scale, out, out_stride);
     if (st) return st;
     if (!q_start && n_tokens != n) return ANE_ERR_INVALID_ARG;
+    if (rule && !(rule->softcap == 0.0f || (rule->softcap >= 0x1p-20f && rule->softcap <= 0x1p20f))) return ANE_ERR_INVALID_ARG;
+    if (rule && ((((uintptr_t)rule->slopes) | ((uintptr_t)rule->first) | ((uintptr_t)rule->prefix)) & 3)) return ANE_ERR_INVALID_ARG;
     if (n == 0 || n_tokens == 0) return ANE_OK;
-    const Launch l = plan(cache, n, n_tokens, !q_start, bound_len(cache, max_len));
+    const Launch l = plan(cache, n, n_tokens, !q_start, rule_len(cache, rule, max_len));
     if (!plan_fits(cache, l, n_tokens, l.parts)) return ANE_ERR_INVALID_ARG;
     size_t ml = 0;
     if (bad_workspace(workspace, workspace_bytes, parts_bytes(cache, n_tokens, l.parts, &ml))) return ANE_ERR_WORKSPACE;
@@ -1207,11 +1364,48 @@ extern "C" int ane_hip_attention_prompt(const ane_paged_cache* cache, uint32_t l
     a.pml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ml);
     a.own = {l.chunk, l.parts, 0}, a.parts_total = l.parts;
     hipStream_t s = (hipStream_t)stream;
-    if (cache->head_dim == 128) type == ANE_TYPE_F32 ? launch_prompt<128, true>(a, l, s) : launch_prompt<128, false>(a, l, s);
-    else type == ANE_TYPE_F32 ? launch_prompt<64, true>(a, l, s) : launch_prompt<64, false>(a, l, s);
+    const bool f32 = type == ANE_TYPE_F32;
+    if (rule) {
+        const double cap = (double)rule->softcap * 1.4426950408889634;
+        a.cap = (float)cap, a.inv_cap = cap != 0.0 ? (float)(1.0 / cap) : 0.0f;
+        a.slopes = rule->slopes, a.window = std::min(rule->window, 1u << 30), a.first = rule->first, a.seen = rule->prefix;
+        if (cache->head_dim == 128) f32 ? launch_prompt<128, true, true>(a, l, s) : launch_prompt<128, false, true>(a, l, s);
+        else f32 ? launch_prompt<64, true, true>(a, l, s) : launch_prompt<64, false, true>(a, l, s);
+    } else {
+        if (cache->head_dim == 128) f32 ? launch_prompt<128, true>(a, l, s) : launch_prompt<128, false>(a, l, s);
+        else f32 ? launch_prompt<64, true>(a, l, s) : launch_prompt<64, false>(a, l, s);
+    }
     if (l.parts > 1) join_as(a, cache->head_dim, type, s);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;
+}
+
+extern "C" size_t ane_hip_attention_prompt_workspace_size(const ane_paged_cache* cache, uint32_t n, uint32_t n_tokens,
+                                                          uint32_t max_len) {
+    return prompt_workspace(cache, nullptr, n, n_tokens, max_len);
+}
+
+extern "C" int ane_hip_attention_prompt(const ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
+                                        const uint32_t* q_start, uint32_t n_tokens, uint32_t max_len, int type,
+                                        const void* q, uint64_t q_stride, float scale, void* out, uint64_t out_stride,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+    return prompt(cache, layer, seqs, n, q_start, n_tokens, max_len, nullptr, type, q, q_stride, scale, out, out_stride,
+                  workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t ane_hip_attention_rule_workspace_size(const ane_paged_cache* cache, uint32_t n, uint32_t n_tokens,
+                                                        uint32_t max_len, const ane_attention_rule* rule) {
+    return prompt_workspace(cache, rule, n, n_tokens, max_len);
+}
+
+extern "C" int ane_hip_attention_rule(const ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
+                                      const uint32_t* q_start, uint32_t n_tokens, uint32_t max_len,
+                                      const ane_attention_rule* rule, int type, const void* q, uint64_t q_stride,
+                                      float scale, void* out, uint64_t out_stride, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
+    if (!rule) return ANE_ERR_BAD_POINTER;
+    return prompt(cache, layer, seqs, n, q_start, n_tokens, max_len, rule, type, q, q_stride, scale, out, out_stride,
+                  workspace, workspace_bytes, stream);
 }
 
 extern "C" size_t ane_hip_attention_shared_workspace_size(const ane_paged_cache* cache, uint32_t n, uint32_t n_groups,

@@ -305,6 +305,34 @@ int ane_hip_attention_prompt(const struct ane_paged_cache* cache, uint32_t layer
                              uint64_t q_stride, float scale, void* out, uint64_t out_stride, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* ane_hip_attention_prompt for models that are not plainly causal.  The new
+ * token t of batch row i, at position p, sees the keys j of its sequence with
+ *   j <= p, or j < prefix[i]       (prefix NULL: j <= p; a prefix seen from both sides)
+ *   j >= first[t]                  (first NULL: all; the first position of t's document)
+ *   p - j < window                 (window 0: all)
+ * all three holding, and its score of one is
+ *   s = scale * q[h] . K[g][j];  s = softcap * tanh(s / softcap) (softcap 0: as it
+ *   is);  s - slopes[h] * |p - j| (slopes NULL: as it is).
+ * A token that sees nothing gets zeros; a token at a negative position sees
+ * nothing.  first is indexed by packed row, prefix by batch row; a prefix past
+ * the length counts as the length, keys that no token of a tile sees are not read.
+ * softcap: 0, or 2^-20 to 2^20.  Single tokens (q_start NULL) are the decode step.
+ * Types, accuracy (of the score before the cap, in fp32) and everything else as
+ * above; the workspace is that of the rule (with a window fewer keys are split). */
+struct ane_attention_rule {
+    float softcap;
+    uint32_t window;
+    const float* slopes;    /* device, [n_heads], or NULL */
+    const uint32_t* first;  /* device, [n_tokens], or NULL */
+    const uint32_t* prefix; /* device, [n], or NULL */
+};
+size_t ane_hip_attention_rule_workspace_size(const struct ane_paged_cache* cache, uint32_t n, uint32_t n_tokens,
+                                             uint32_t max_len, const struct ane_attention_rule* rule);
+int ane_hip_attention_rule(const struct ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
+                           const uint32_t* q_start, uint32_t n_tokens, uint32_t max_len,
+                           const struct ane_attention_rule* rule, int type, const void* q, uint64_t q_stride, float scale,
+                           void* out, uint64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
 /* One new token of each of n sequences (row i of q and out), attending to
  * positions 0 .. kv_len-1 of its sequence; zeros where there are none.
  * With n_groups > 0, batch rows group_start[g] .. group_start[g+1]-1 (device,
