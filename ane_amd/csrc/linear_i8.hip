@@ -3,7 +3,7 @@
 // and output channel applied as it is written.
 //
 //   y = x, or fl(fl(x * inv) * norm_w) with inv as ane_hip_rms_norm's
-//   q[t][k] = rint(y * 127 / max|y_t|),  qs[t] = max|y_t| / 127
+//   q[t][k] = rint(y * fl(fl(1 / max|y_t|) * 127)),  qs[t] = max|y_t| / 127
 //   out[t][n] = fl(fl((float)sum_k q[t][k] w[n][k] * qs[t]) * ws[n]) + bias[n] + residual[t][n]
 //
 // The sum is an exact int32 (K below 2^17), so no split of K and no order of
@@ -120,11 +120,9 @@ __global__ void __launch_bounds__(256) k_quantize_tokens(QuantArgs a) {
         __syncthreads();
         top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
     }
-    // (a maximum below 2^-96 is brought up first: 127 over it would not be finite)
-    const float up = top < 0x0f800000u ? 0x1p96f : 1.0f;
-    float scale, per;
-    quant_params(__uint_as_float(top) * up, scale, per);
-    if (top == 0) scale = up;  // 1 in the end
+    // (a maximum below 2^-96 is brought up first: its reciprocal would not be finite)
+    const float up = top < 0x0f800000u ? 0x1p96f : 1.0f, m = __uint_as_float(top) * up;
+    const float scale = top == 0 ? up : m / 127.0f, per = top == 0 ? 127.0f : __fmul_rn(1.0f / m, 127.0f);
     if (wave % NW == 0 && lane == 0) a.scales[t] = scale / up;
     const uint32_t Kp = (a.K + 15) & ~15u;  // zeros up to here
     auto put = [&](uint32_t r, const float(&y)[8]) {

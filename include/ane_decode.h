@@ -407,8 +407,8 @@ int ane_hip_pages_compact(const struct ane_paged_cache* cache, uint32_t* page_ta
  * zeros from K up to there.
  *
  * quantize_tokens: y = x, or with norm_w (fp32 [K]) y = fl(fl(x * inv) * norm_w),
- * inv as ane_hip_rms_norm has it; scales[t] = fl(max|y| / 127), q = y * fl(127 /
- * max|y|) rounded to even, at most 127 in magnitude.  A token of zeros has scale
+ * inv as ane_hip_rms_norm has it; scales[t] = fl(max|y| / 127), q = y *
+ * fl(fl(1 / max|y|) * 127) rounded to even, at most 127 in magnitude.  A token of zeros has scale
  * 1; one whose y holds an infinity or NaN a scale that is not finite, and its row
  * of any product is NaN.
  * dense_i8_scaled: out[t][n] = fl(fl((float)sum q w * q_scales[t]) * w_scales[n])

@@ -29,7 +29,7 @@ def quantized(x, norm_w=None, eps=1e-5):
         top = np.abs(y).max(axis=1)  # (NaN where there is one)
         up = np.where(top < np.float32(2.0 ** -96), np.float32(2.0 ** 96), np.float32(1))
         scale = np.where(top == 0, np.float32(1), top * up / np.float32(127) / up)
-        per = np.where(top == 0, np.float32(127), np.float32(127) / (top * up))
+        per = np.where(top == 0, np.float32(127), np.float32(1) / (top * up) * np.float32(127))
         t = (y * up[:, None]) * per[:, None]
         q = np.rint(np.clip(np.where(np.isnan(t), 0, t), -127, 127)).astype(np.int8)
     return q, scale.astype(np.float32)
