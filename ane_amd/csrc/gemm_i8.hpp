@@ -38,6 +38,11 @@ struct GemmParams {
     const void* res;      // or nullptr
     uint64_t ldr;
     bool half;
+    // K split over several workgroups a tile, the scaled epilogue in the last one to
+    // arrive: int32 partials [split][Mout][Nout rounded up to 4], 16-byte aligned, and
+    // a count a tile, zero before the launch.
+    int32_t* planes;
+    uint32_t* counts;
 };
 
 __device__ __forceinline__ float sc_out(int32_t acc, float rs, float cs, float bias) {
@@ -83,6 +88,17 @@ __device__ __forceinline__ float ig_out(const GemmParams& p, int32_t acc, uint32
 // (gemm_i8.hip chooses the kernel).
 int launch_gemm_rows(const GemmParams& p, hipStream_t s);
 
+// The kernel of the scaled epilogue for sizes, and over how many workgroups a tile its
+// K is split (with p.planes and p.counts, kScaledCounts words zero before the launch).
+enum ScaledKernel { kScaledFew, kScaled64, kScaled128d, kScaled128, kScaled256 };
+struct ScaledPlan {
+    ScaledKernel kernel;
+    uint32_t split;
+};
+constexpr uint32_t kScaledCounts = 256;
+ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split);
+int launch_gemm_scaled(const GemmParams& p, ScaledPlan plan, hipStream_t s);
+
 // dense_fused_i8 operand preparation (quantize_fused.hip): absmax partials
 // (kFusedPartials per tensor), qA (M x Kp), qBt (N x Kp), scales {sa, sb},
 // and the launch's wait record wstatus: wstatus[0] = the number of
@@ -123,7 +139,7 @@ bool resident_mixed_bit(uint32_t bits);
 // reasonably.
 // any_rows: also fewer rows than one tile (rows past Mout read as zeros).
 // ksplit > 1 splits K over gridDim.y workgroups per tile, each writing its
-// int32 plane y of Craw (Mout x ldc): raw output only.
+// int32 plane y of Craw (Mout x ldc), or with the scaled epilogue of planes.
 bool tile256_eligible(const GemmParams& p, bool any_rows = false);
 int launch_gemm_tile256(const GemmParams& p, hipStream_t s, uint32_t ksplit = 1);
 

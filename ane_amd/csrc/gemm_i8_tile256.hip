@@ -298,7 +298,9 @@ __device__ __forceinline__ void sc_put4(const GemmParams& p, uint64_t at, uint64
 template <bool AU8>
 #else
 constexpr bool AU8 = false;
-template <bool IG, bool SC = false>  // the integer GEMM's epilogue (GemmParams::ig), the scaled one (rs)
+// the integer GEMM's epilogue (GemmParams::ig), the scaled one (rs), that one behind
+// a split K (planes)
+template <bool IG, bool SC = false, bool SPLIT = false>
 #endif
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu)))
 ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
@@ -345,7 +347,7 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
     if (p.sdev) s = __fmul_rn(__fmul_rn(p.sdev[0], p.sdev[1]), p.smul);
 
 #if ANE_TILE_PANEL
-    constexpr bool IG = false, SC = false;
+    constexpr bool IG = false, SC = false, SPLIT = false;
 #endif
     const uint32_t wr0 = (wave / WN) * (FM * 32);
     const uint32_t wc0 = (wave % WN) * (FN * 32);
@@ -490,6 +492,57 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
         for (int ni = 0; ni < FN; ni++) igc[ni] = isum[wc0 + ni * 32 + (lane & 31)];
     }
     int8_t* epi = smem + wave * kEpiWaveBytes;
+    // Split K behind the scaled epilogue: each workgroup writes its sums (exact in any
+    // order), then counts itself; the last one of a tile adds them up.  Stores and loads
+    // of the sums and the count are all at agent scope (sc1: through the L2 of each XCD),
+    // and the stores have been waited for before the count, so the last one sees them
+    // all.  (Fences instead write back and drop whole L2s: 23 us for 32 x 4096 over 14336
+    // in four parts, not 15; added by a launch of their own the sums take 16.4.)
+    const uint32_t ldp = (p.Nout + 3) & ~3u;
+    int32_t* const plane = SPLIT ? p.planes + (uint64_t)blockIdx.y * p.Mout * ldp : nullptr;
+    const uint32_t lc4 = 4 * (lane % kLanesPerRow), j4 = col0 + wc0 + lc4;  // this lane's columns of a staged row
+    float cj4[SPLIT ? 4 : 1], bj4[SPLIT ? 4 : 1];
+    if constexpr (SPLIT) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+            const uint32_t j = j4 + e < p.Nout ? j4 + e : p.Nout - 1;
+            cj4[e] = p.cs[j], bj4[e] = p.bias ? p.bias[j] : 0.0f;
+        }
+#pragma unroll
+        for (int mi = 0; mi < FM; mi++) {
+#pragma unroll
+            for (int h = 0; h < 32 / EPR; h++) {
+                if (row0 + wr0 + mi * 32 + h * EPR >= p.Mout) continue;  // uniform: nothing to write
+#pragma unroll
+                for (int ni = 0; ni < FN; ni++)
+#pragma unroll
+                    for (int r = h * EPR / 2; r < (h + 1) * EPR / 2; r++) {
+                        const uint32_t lr = 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) - h * EPR;
+                        *reinterpret_cast<int32_t*>(epi + lr * kEpiRowBytes + (ni * 32 + (lane & 31)) * 4) = acc[mi][ni][r];
+                    }
+                wait_lgkmcnt0();
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int q = 0; q < EPR / kRowsPerStore; q++) {
+                    const uint32_t lr = kRowsPerStore * q + lane / kLanesPerRow;
+                    const v4i v = *reinterpret_cast<const v4i*>(epi + lr * kEpiRowBytes + lc4 * 4);
+                    const uint32_t i = row0 + wr0 + mi * 32 + h * EPR + lr;
+                    if (i < p.Mout && j4 < p.Nout) store16_sc1(reinterpret_cast<uint32_t*>(plane) + (uint64_t)i * ldp + j4, v);
+                }
+                wait_lgkmcnt0();
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        wait_vmcnt<0>();
+        __syncthreads();
+        uint32_t* const last = reinterpret_cast<uint32_t*>(smem + NW * kEpiWaveBytes + TM * 4);
+        static_assert(NW * kEpiWaveBytes + TM * 4 + 4 <= kLdsBytes, "room for the word");
+        if (tid == 0)
+            *last = __hip_atomic_fetch_add(p.counts + logical, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.y;
+        __syncthreads();
+        if (!*last) return;
+    }
+    const __amdgpu_buffer_rsrc_t rp = make_rsrc(p.planes, SPLIT ? gridDim.y * p.Mout * ldp * 4 : 0);
     const bool vec_ok = SC && p.half ? ((((uintptr_t)p.C) | ((uintptr_t)p.res)) & 7) == 0 && ((p.ldc | p.ldr) & 3) == 0
                         : SC ? ((((uintptr_t)p.C) | ((uintptr_t)p.res)) & 15) == 0 && ((p.ldc | p.ldr) & 3) == 0
                              : (((uintptr_t)(craw ? (void*)craw : (void*)p.C)) & 15) == 0 && (p.ldc & 3) == 0;
@@ -512,7 +565,9 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
 #if ANE_TILE_PANEL
                     if (AU8) av = (int32_t)((uint32_t)av + 128u * (uint32_t)csj[ni]);
 #endif
-                    if constexpr (SC) {
+                    if constexpr (SPLIT) {
+                        bitsv = (uint32_t)av;
+                    } else if constexpr (SC) {
                         bitsv = __float_as_uint(sc_out(av, rsc[wr0 + mi * 32 + h * EPR + lr], cj[ni], bj[ni]));
                     } else if (craw) {
                         bitsv = (uint32_t)av;
@@ -525,6 +580,34 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
                     *reinterpret_cast<uint32_t*>(epi + lr * kEpiRowBytes + lc * 4) = bitsv;
                 }
             }
+            // SPLIT: the other workgroups' sums, four of them in flight at a time
+            constexpr int kQ = EPR / kRowsPerStore;
+            v4i others[SPLIT ? kQ : 1];
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int q = 0; q < kQ; q++) others[q] = v4i{0, 0, 0, 0};
+                for (uint32_t y0 = 0; y0 < gridDim.y; y0 += 4) {
+                    v4i o[4][kQ];
+#pragma unroll
+                    for (uint32_t y = 0; y < 4; y++) {
+                        const uint32_t from = (y0 + y < gridDim.y ? y0 + y : y0) * p.Mout;
+#pragma unroll
+                        for (int q = 0; q < kQ; q++) {
+                            const uint32_t i = row0 + wr0 + mi * 32 + h * EPR + kRowsPerStore * q + lane / kLanesPerRow;
+                            const uint32_t at = (from + (i < p.Mout ? i : 0)) * ldp + (j4 < p.Nout ? j4 : 0);
+                            o[y][q] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rp, at * 4, 0, kCpolSc1));
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t y = 0; y < 4; y++) {
+                        const int use = y0 + y < gridDim.y && y0 + y != blockIdx.y ? -1 : 0;
+#pragma unroll
+                        for (int q = 0; q < kQ; q++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) others[q][e] = (int)((uint32_t)others[q][e] + (uint32_t)(o[y][q][e] & use));
+                    }
+                }
+            }
             wait_lgkmcnt0();
             __builtin_amdgcn_wave_barrier();
             // 16 B per lane: kLanesPerRow lanes cover one staged row
@@ -532,10 +615,16 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
             for (int q = 0; q < EPR / kRowsPerStore; q++) {
                 const uint32_t lr = kRowsPerStore * q + lane / kLanesPerRow;
                 const uint32_t lc = 4 * (lane % kLanesPerRow);
-                const v4i v = *reinterpret_cast<const v4i*>(epi + lr * kEpiRowBytes + lc * 4);
+                v4i v = *reinterpret_cast<const v4i*>(epi + lr * kEpiRowBytes + lc * 4);
                 const uint32_t i = row0 + wr0 + mi * 32 + h * EPR + lr;
                 const uint32_t j = col0 + wc0 + lc;
                 if (i >= p.Mout) continue;
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        v[e] = __float_as_int(sc_out((int)((uint32_t)v[e] + (uint32_t)others[q][e]),
+                                                     rsc[wr0 + mi * 32 + h * EPR + lr], cj4[e], bj4[e]));
+                }
                 if constexpr (SC) {
                     if (vec_ok && j + 3 < p.Nout) {
                         sc_put4(p, (uint64_t)i * p.ldc + j, (uint64_t)i * p.ldr + j, v);
@@ -604,9 +693,10 @@ int ANE_TILE_LAUNCH(const GemmParams& p, hipStream_t s, uint32_t ksplit) {
     const uint32_t tiles_n = (p.Nout + TN - 1) / TN;
     const uint64_t total = (uint64_t)tiles_m * tiles_n;
     if (total > 0x7fffffffull || ksplit == 0 || ksplit > 65535) return ANE_ERR_INVALID_ARG;
-    if (ksplit > 1 && !p.Craw) return ANE_ERR_INVALID_ARG;  // split K writes int32 planes
+    if (ksplit > 1 && !p.Craw && !(p.rs && p.planes)) return ANE_ERR_INVALID_ARG;  // split K writes int32 planes
     if (p.ig && p.nsum > kIgParts) return ANE_ERR_INVALID_ARG;
-    const auto fn = p.rs ? ANE_TILE_KERNEL<false, true> : p.ig ? ANE_TILE_KERNEL<true> : ANE_TILE_KERNEL<false>;
+    const auto fn = p.rs && ksplit > 1 ? ANE_TILE_KERNEL<false, true, true>
+                    : p.rs ? ANE_TILE_KERNEL<false, true> : p.ig ? ANE_TILE_KERNEL<true> : ANE_TILE_KERNEL<false>;
     hipLaunchKernelGGL(fn, dim3((uint32_t)total, ksplit), dim3(kThreads), 0, s, p, tiles_m, tiles_n);
     ANE_HIP_CHECK_LAUNCH();
     return ANE_OK;

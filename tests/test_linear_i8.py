@@ -341,3 +341,68 @@ def test_zero_sizes_leave_outputs(ane):
     with pytest.raises((AneError, ValueError)):
         ane.linear_i8(torch.zeros((2, 0), device="cuda"), torch.zeros((8, 0), dtype=torch.int8, device="cuda"), ws,
                       torch.zeros((2, 8), device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [100, 777, 1777, 4096, 5000, 14336, 20000])
+@pytest.mark.parametrize("half", [False, True])
+def test_a_token_does_not_depend_on_its_batch(ane, K, half):
+    """The integers, the scale and the row of the product have the same bits alone and in batches of every size, whichever
+    kernels they go through; the norm is ane_hip_rms_norm's."""
+    import torch
+
+    N, T = 200, 1100
+    x, w, ws, norm, bias, _ = inputs(T, N, K, seed=9, half_in=half)
+    X, W, S, nw, B = dev(x), rows16(w), dev(ws), dev(norm), dev(bias)
+    q0 = torch.zeros((T, (K + 15) // 16 * 16), dtype=torch.int8, device="cuda")[:, :K]
+    s0, out0 = torch.zeros(T, device="cuda"), torch.zeros((T, N), device="cuda")
+    ane.quantize_tokens(X, q0, s0, norm_w=nw)
+    ane.linear_i8(X, W, S, out0, norm_w=nw, bias=B)
+    for n in (1, 2, 16, 40, 64, 100, 257, 600):
+        q, s, out = torch.zeros_like(q0)[:n], torch.zeros(n, device="cuda"), torch.zeros((n, N), device="cuda")
+        ane.quantize_tokens(X[:n], q, s, norm_w=nw)
+        ane.linear_i8(X[:n], W, S, out, norm_w=nw, bias=B)
+        assert torch.equal(q, q0[:n]) and torch.equal(s, s0[:n]) and torch.equal(out, out0[:n])
+        ane.dense_i8_scaled(q, s, W, S, out.zero_(), bias=B)
+        assert torch.equal(out, out0[:n])
+    if K % 32 == 0 and not half:
+        y, one = torch.zeros(K, device="cuda"), torch.zeros(1, device="cuda")
+        ane.rms_norm(K, X[3].contiguous(), nw, 1e-5, y)
+        qy = torch.zeros((1, K), dtype=torch.int8, device="cuda")
+        ane.quantize_tokens(y[None], qy, one)
+        assert torch.equal(qy[0], q0[3]) and torch.equal(one[0], s0[3])
+
+
+@pytest.mark.gpu
+def test_one_token_over_very_many_rows(ane):
+    """More rows than 64 a wave on two workgroups a CU."""
+    import torch
+
+    N, K = 300_001, 48
+    x, w, ws, _, bias, _ = inputs(1, N, K, seed=10)
+    out = torch.zeros((1, N), device="cuda")
+    ane.linear_i8(dev(x), rows16(w), dev(ws), out, bias=dev(bias))
+    same(out.cpu().numpy(), product(*quantized(x), w, ws, bias))
+
+
+def test_plans():
+    """Which kernel takes a product (ane::scaled_plan, gemm_i8.hip; 256 CUs), and the room for its parts of K."""
+    import ctypes
+
+    class Plan(ctypes.Structure):
+        _fields_ = [("kernel", ctypes.c_int), ("split", ctypes.c_uint32)]
+
+    f = ane_amd.lib()._FuncPtr(("_ZN3ane11scaled_planEjjjb", ane_amd.lib()))
+    f.restype, f.argtypes = Plan, [ctypes.c_uint32] * 3 + [ctypes.c_bool]
+    few, t64, t128d, t128, t256 = range(5)
+    for T, N, K, may, want in ((16, 4096, 4096, True, (few, 1)), (32, 4096, 4096, True, (t64, 4)), (32, 4096, 14336, True, (t64, 4)),
+                               (32, 4096, 14336, False, (few, 1)), (64, 28672, 4096, True, (t64, 1)),
+                               (192, 4096, 14336, True, (t128d, 4)), (512, 4096, 14336, True, (t128d, 2)),
+                               (512, 4096, 14336, False, (t64, 1)), (512, 6144, 4096, True, (t128d, 1)),
+                               (768, 6144, 4096, True, (t128, 1)), (4096, 28672, 4096, True, (t256, 1))):
+        p = f(T, N, K, may)
+        assert (p.kernel, p.split) == want, (T, N, K)
+    for T, N, K in ((32, 4096, 14336), (192, 4095, 14336), (64, 4001, 4096)):
+        split = f(T, N, K, True).split
+        need = T * (-(-K // 128) * 128) + 4 * T + 1024 + split * T * (-(-N // 4) * 4) * 4
+        assert split > 1 and need <= ane_amd.lib().ane_hip_linear_i8_workspace_size(T, N, K) <= need + 1024
