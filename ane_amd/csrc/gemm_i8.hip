@@ -232,6 +232,10 @@ static int launch_gemm(const GemmParams& p, hipStream_t s) {
 int launch_gemm_rows(const GemmParams& p, hipStream_t s) { return launch_gemm<kBTransposed, false>(p, s); }
 
 // Measured as T x N x K in us, for 256 CUs (n = CUs, t = tiles):
+// - up to 64 tokens the few-row kernel, which reads x again for every 16 columns, while
+//   that is little: 16 x 4096 x 4096 7.1, in 64-tiles 7.3; 32 x 4096 x 4096 9.2, 7.8;
+//   8 x 28672 x 4096 28.6, 27.4.  Where K cannot be split the 64-tiles need more
+//   columns: 32 x 4096 x 14336 26, in whole 64-tiles 33.
 // - 256-tiles from 3n/4: 384 x 28672 x 4096 67, in 128-tiles 71; 2048 x 6144 x 4096 60,
 //   70; with n/2 of them 2048 x 4096 x 4096 45, 38.
 // - above n/2 128-tiles, on the deep ring up to n: 512 x 6144 x 4096 22.5, in 64-tiles
@@ -242,18 +246,17 @@ int launch_gemm_rows(const GemmParams& p, hipStream_t s) { return launch_gemm<kB
 // - 64-tiles with K in as many parts as fill the CUs, at most 4, of 8 steps at least:
 //   64 x 4096 x 4096 8.3 in four, 10.6 whole; 32 x 4096 x 14336 15, 33; 64 x 2003 x 1792
 //   7.5 in three, 7.4 whole.
-// - the few-row kernel, which reads x again for every 16 columns, up to 64 tokens while
-//   that is little: 16 x 4096 x 4096 7.1, in 64-tiles 7.3; 32 x 4096 x 4096 9.2, 7.8;
-//   1 x 28672 x 4096 24, 26; 8 x 28672 x 4096 28.6, 27.4.  Where K cannot be split the
-//   64-tiles need more columns: 32 x 4096 x 14336 26, in whole 64-tiles 33.
 ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split) {
     const uint64_t n = tile256_min_tiles(), nk = ((uint64_t)K + 127) / 128;
     auto tiles = [&](uint64_t b) { return (T + b - 1) / b * ((N + b - 1) / b); };
     const uint64_t t64 = tiles(64), t128 = tiles(128);
-    if (tiles(256) * 4 >= n * 3) return {kScaled256, 1};
-    if (t128 * 2 > n) return {t128 <= n ? kScaled128d : kScaled128, 1};
-    if (may_split && nk >= 64 && t128 * 16 >= n * 3) return {kScaled128d, (uint32_t)(n / t128)};
-    if (T <= 64 && (may_split ? (uint64_t)T * N * K < 300000000ull : t64 * T < 3000)) return {kScaledFew, 1};
+    if (T <= 64) {
+        if (may_split ? (uint64_t)T * N * K < 300000000ull : t64 * T < 3000) return {kScaledFew, 1};
+    } else {
+        if (T > 128 && tiles(256) * 4 >= n * 3) return {kScaled256, 1};
+        if (t128 * 2 > n) return {t128 <= n ? kScaled128d : kScaled128, 1};
+        if (may_split && nk >= 64 && t128 * 16 >= n * 3) return {kScaled128d, (uint32_t)(n / t128)};
+    }
     uint64_t split = may_split ? n / t64 : 1;
     if (split > 4) split = 4;
     if (split > nk / 8) split = nk / 8;

@@ -359,7 +359,7 @@ def test_a_token_does_not_depend_on_its_batch(ane, K, half):
     ane.quantize_tokens(X, q0, s0, norm_w=nw)
     ane.linear_i8(X, W, S, out0, norm_w=nw, bias=B)
     for n in (1, 2, 16, 40, 64, 100, 257, 600):
-        q, s, out = torch.zeros_like(q0)[:n], torch.zeros(n, device="cuda"), torch.zeros((n, N), device="cuda")
+        q, s, out = rows16(np.zeros((n, K), np.int8), fill=0), torch.zeros(n, device="cuda"), torch.zeros((n, N), device="cuda")
         ane.quantize_tokens(X[:n], q, s, norm_w=nw)
         ane.linear_i8(X[:n], W, S, out, norm_w=nw, bias=B)
         assert torch.equal(q, q0[:n]) and torch.equal(s, s0[:n]) and torch.equal(out, out0[:n])
@@ -398,7 +398,8 @@ def test_plans():
     for T, N, K, may, want in ((16, 4096, 4096, True, (few, 1)), (32, 4096, 4096, True, (t64, 4)), (32, 4096, 14336, True, (t64, 4)),
                                (32, 4096, 14336, False, (few, 1)), (64, 28672, 4096, True, (t64, 1)),
                                (192, 4096, 14336, True, (t128d, 4)), (512, 4096, 14336, True, (t128d, 2)),
-                               (512, 4096, 14336, False, (t64, 1)), (512, 6144, 4096, True, (t128d, 1)),
+                               (512, 4096, 14336, False, (t64, 1)), (16, 65536, 4096, True, (t64, 1)),
+                               (128, 65536, 4096, True, (t128, 1)), (512, 6144, 4096, True, (t128d, 1)),
                                (768, 6144, 4096, True, (t128, 1)), (4096, 28672, 4096, True, (t256, 1))):
         p = f(T, N, K, may)
         assert (p.kernel, p.split) == want, (T, N, K)
