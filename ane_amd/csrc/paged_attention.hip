@@ -336,6 +336,7 @@ constexpr float kDrop = 8.0f, kDeep = 24.0f, kThin = -7.0f, kAgain = 38.0f;
 template <bool F32>
 struct Tanh {
     static constexpr float kSmall = F32 ? 0.6f : 0.75f;
+    // tanh(y) / y - 1
     static __device__ __forceinline__ float small(float y) {
         const float z = y * y;
         float p;
@@ -351,12 +352,11 @@ struct Tanh {
             p = __builtin_fmaf(p, z, 0.13268233835f);
             p = __builtin_fmaf(p, z, -0.3332966864f);
         }
-        return __builtin_fmaf(p * z, y, y);
+        return p * z;
     }
-    static __device__ __forceinline__ float any(float y) {
+    static __device__ __forceinline__ float large(float y) {
         const float e = __builtin_amdgcn_exp2f(y * 2.88539008177792681f);
-        const float t = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
-        return fabsf(y) > kSmall ? t : small(y);
+        return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
     }
 };
 
@@ -377,11 +377,10 @@ struct Rows {
     int32_t wmin, wmax;
     uint32_t half, ka, va[2 * ND];
     // RULE: keys before `begin` are masked (least and largest of the rows below), the
-    // row's position and slope (log2 units); scores times cin, then capped and lowered,
-    // are in log2 units already, and c is 1 (bent: they are).
+    // row's position and slope (log2 units), the score factor: c is 1 where there are
+    // slopes, scores then are in log2 units already.
     int32_t begin, fmin, fmax, pos;
-    float slope, cin, cap;
-    bool bent, sloped;
+    float slope, factor;
 
     __device__ __forceinline__ void init_rule(const AttnArgs& a, const Work& w, uint32_t t, uint32_t head, bool live) {
         pos = w.len - (int32_t)w.toks + (int32_t)t;
@@ -395,48 +394,55 @@ struct Rows {
         fmin = __builtin_amdgcn_readfirstlane(fmin);
         fmax = __builtin_amdgcn_readfirstlane(fmax);
         slope = a.slopes ? a.slopes[head] * 1.44269504088896341f : 0.0f;
-        cap = a.cap;
-        sloped = a.slopes;
-        bent = sloped || cap != 0.0f;
     }
     // after take_q
-    __device__ __forceinline__ void bend_scale(const AttnArgs& a) {
-        if (!bent) return;
-        // (as c in take_q: never 0 nor infinite)
-        cin = a.cap != 0.0f ? __builtin_amdgcn_fmed3f(c * a.inv_cap, 0x1p-126f, 0x1p127f) : c;
-        c = 1.0f;
+    __device__ __forceinline__ void init_factor(const AttnArgs& a) {
+        factor = c;
+        if (a.slopes) c = 1.0f;
     }
+    // Scores as the products give them, capped: s tanh(y) / y with y = s factor / cap, in
+    // the same units; then lowered with the distance, in log2 units.
     template <int KT>
-    __device__ __forceinline__ void bend(f16v (&s)[KT], int32_t t0) const {
-        float top = 0.0f;
-#pragma unroll
-        for (int t = 0; t < KT; t++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[t][r] *= cin;
-        if (cap != 0.0f) {  // uniform, as the next one
+    __device__ __forceinline__ void bend(const AttnArgs& a, f16v (&s)[KT], int32_t t0) const {
+        if (a.cap != 0.0f) {  // uniform, as the next ones
+            // (as c in take_q: never 0 nor infinite)
+            const float down = __builtin_amdgcn_fmed3f(factor * a.inv_cap, 0x1p-126f, 0x1p127f);
+            float top = 0.0f;
 #pragma unroll
             for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, fabsf(s[t][r])), fabsf(s[t][r + 1]));
-            if (__any(top > Tanh<F32>::kSmall)) {
+            if (__any(top * down > Tanh<F32>::kSmall)) {
+                const float up = __builtin_amdgcn_rcpf(down);
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[t][r] = Tanh<F32>::any(s[t][r]) * cap;
+                    for (int r = 0; r < 16; r++) {
+                        const float y = s[t][r] * down, l = Tanh<F32>::large(y) * up;
+                        s[t][r] = fabsf(y) > Tanh<F32>::kSmall ? l : __builtin_fmaf(Tanh<F32>::small(y), s[t][r], s[t][r]);
+                    }
             } else {
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[t][r] = Tanh<F32>::small(s[t][r]) * cap;
+                    for (int r = 0; r < 16; r++) s[t][r] = __builtin_fmaf(Tanh<F32>::small(s[t][r] * down), s[t][r], s[t][r]);
             }
         }
-        if (sloped) {
+        if (!a.slopes) return;
+        if (a.seen) {  // keys on both sides of a row
             const float at = (float)(pos - t0 - 4 * (int32_t)half);
 #pragma unroll
             for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int r = 0; r < 16; r++)
-                    s[t][r] = __builtin_fmaf(-slope, fabsf(at - (float)(t * 32 + 8 * (r >> 2) + (r & 3))), s[t][r]);
+                    s[t][r] = __builtin_fmaf(-slope, fabsf(at - (float)(t * 32 + 8 * (r >> 2) + (r & 3))), s[t][r] * factor);
+        } else {
+            const float at = slope * (float)(t0 + 4 * (int32_t)half - pos);
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    s[t][r] = __builtin_fmaf(s[t][r], factor, __builtin_fmaf(slope, (float)(t * 32 + 8 * (r >> 2) + (r & 3)), at));
         }
     }
 
@@ -620,10 +626,8 @@ struct Rows {
     // Scores of keys from position t0 on to weights; keys before lo are masked.
     // Whether this lane has some so small that carried() has to look at them.
     template <int KT, class Between>
-    __device__ __forceinline__ bool weights(f16v (&s)[KT], int32_t t0, int32_t lo, Weights<KT>& p, Between between) {
-        if constexpr (RULE) {
-            if (bent) bend<KT>(s, t0);
-        }
+    __device__ __forceinline__ bool weights(const AttnArgs& a, f16v (&s)[KT], int32_t t0, int32_t lo, Weights<KT>& p, Between between) {
+        if constexpr (RULE) bend<KT>(a, s, t0);
         float low = INFINITY;  // (of the masked too, which costs a second round at worst)
         auto least = [&] {
             if constexpr (F32) {
@@ -765,12 +769,12 @@ struct Rows {
         products(false);
     }
     template <int KT>
-    __device__ __forceinline__ void step(const uint8_t* k, const uint8_t* v, int32_t t0, int32_t lo) {
+    __device__ __forceinline__ void step(const AttnArgs& a, const uint8_t* k, const uint8_t* v, int32_t t0, int32_t lo) {
         f16v s[KT];
         Weights<KT> p;
         h8 vf[kAhead];
         scores<KT>(k, s, [](int) {});
-        const bool thin = weights<KT>(s, t0, lo, p, [](int) {});
+        const bool thin = weights<KT>(a, s, t0, lo, p, [](int) {});
         first_values(v, vf);
         values<KT>(v, vf, p);
         if constexpr (F32) {
@@ -914,7 +918,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
     r.init(a.scale_log2e, row_limit<MODE, RULE>(a, w, tok), live);
     if constexpr (RULE) r.init_rule(a, w, tok, head, live);
     r.take_q(raw);
-    if constexpr (RULE) r.bend_scale(a);
+    if constexpr (RULE) r.init_factor(a);
     __builtin_amdgcn_sched_barrier(0);
     r.clear();
 
@@ -942,9 +946,9 @@ __global__ void __launch_bounds__(256, 2) k_attn_block(AttnArgs a, uint32_t slot
         if constexpr (F32) {  // 32 keys at a time: the two parts of q and of 64 weights do not fit 256 registers
 #pragma unroll 1
             for (int h = 0; h < 2; h++)
-                if (t0 + 32 * h < r.wmax && !(RULE && t0 + 32 * h + 32 <= r.fmin)) r.template step<1>(st + h * (kT / 2), st + kT + h * (kT / 2), t0 + 32 * h, 0);
+                if (t0 + 32 * h < r.wmax && !(RULE && t0 + 32 * h + 32 <= r.fmin)) r.template step<1>(a, st + h * (kT / 2), st + kT + h * (kT / 2), t0 + 32 * h, 0);
         } else {
-            if (t0 < r.wmax && !(RULE && t0 + 64 <= r.fmin)) r.template step<2>(st, st + kT, t0, 0);
+            if (t0 < r.wmax && !(RULE && t0 + 64 <= r.fmin)) r.template step<2>(a, st, st + kT, t0, 0);
         }
     }
     if (odd_from < odd_to) r.add_nonfinite(a, w, g, odd_from, odd_to);
@@ -1049,7 +1053,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
     if constexpr (RULE) r.init_rule(a, w, tok, head, live);
     if constexpr (MODE != kOwn) r.turn_rows(vt, live, raw);
     r.take_q(raw);
-    if constexpr (RULE) r.bend_scale(a);
+    if constexpr (RULE) r.init_factor(a);
     __builtin_amdgcn_sched_barrier(0);
     r.clear();
 
@@ -1070,7 +1074,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
             ld.settle();
         }
         const Next kn = aim(a.kp, t + 1);  // past the last: no extent, zeros that nobody reads
-        const bool thin = r.template weights<1>(s, t0, w.lo, p, [&](int i) {
+        const bool thin = r.template weights<1>(a, s, t0, w.lo, p, [&](int i) {
             if (i < kC) copy(kn, i, kt);
         });
         wait_vmcnt<kC>();  // V of this block
@@ -1335,12 +1339,17 @@ static uint64_t rule_len(const ane_paged_cache* c, const ane_attention_rule* r, 
     return r && r->window && !r->prefix ? std::min<uint64_t>(len, (uint64_t)r->window + 32 + 16) : len;
 }
 
+static Launch prompt_plan(const ane_paged_cache* c, const ane_attention_rule* r, uint32_t n, uint32_t n_tokens, bool single,
+                          uint32_t max_len) {
+    return plan(c, n, n_tokens, single, rule_len(c, r, max_len), false, r && !r->window);
+}
+
 static size_t prompt_workspace(const ane_paged_cache* cache, const ane_attention_rule* rule, uint32_t n, uint32_t n_tokens,
                                uint32_t max_len) {
     if (cache_status(cache) || n == 0 || n_tokens == 0 || n > kMaxTokens || n_tokens > kMaxTokens) return 0;
     // the same for a batch of single tokens with and without q_start
-    const Launch l = plan(cache, n, n_tokens, false, rule_len(cache, rule, max_len));
-    const Launch one = plan(cache, n, n_tokens, true, rule_len(cache, rule, max_len));
+    const Launch l = prompt_plan(cache, rule, n, n_tokens, false, max_len);
+    const Launch one = prompt_plan(cache, rule, n, n_tokens, true, max_len);
     return parts_bytes(cache, n_tokens, n_tokens == n ? std::max(l.parts, one.parts) : l.parts, nullptr);
 }
 
@@ -1354,7 +1363,7 @@ static int prompt(const ane_paged_cache* cache, uint32_t layer, const uint32_t* 
     if (rule && !(rule->softcap == 0.0f || (rule->softcap >= 0x1p-20f && rule->softcap <= 0x1p20f))) return ANE_ERR_INVALID_ARG;
     if (rule && ((((uintptr_t)rule->slopes) | ((uintptr_t)rule->first) | ((uintptr_t)rule->prefix)) & 3)) return ANE_ERR_INVALID_ARG;
     if (n == 0 || n_tokens == 0) return ANE_OK;
-    const Launch l = plan(cache, n, n_tokens, !q_start, rule_len(cache, rule, max_len));
+    const Launch l = prompt_plan(cache, rule, n, n_tokens, !q_start, max_len);
     if (!plan_fits(cache, l, n_tokens, l.parts)) return ANE_ERR_INVALID_ARG;
     size_t ml = 0;
     if (bad_workspace(workspace, workspace_bytes, parts_bytes(cache, n_tokens, l.parts, &ml))) return ANE_ERR_WORKSPACE;

@@ -32,13 +32,17 @@ struct Launch {
 };
 
 // units: sequences (groups) of the launch; tokens: theirs in all; single: one
-// token each; beside: shares its launch with the batch's own keys.
+// token each; beside: shares its launch with the batch's own keys; bent: under a
+// rule without a window.
 //
 // 32 rows a workgroup as long as its workgroups have a place each (512 of them, two
 // a CU; 64-wide four a CU, three in fp32), half again as many for one sequence,
 // where 128 rows a workgroup would leave most CUs idle: 512 tokens x 32 heads fp32
 // 22 us, 31 with 128 rows; 768 tokens 33, 39; 8 chunks of 64 tokens after 1000
-// positions 36, 50.
+// positions 36, 50.  Under a rule scores cost the vector unit more, which one workgroup
+// of 128 rows a CU leaves idle between its waves' products: a quarter more places (2 x
+// 300 tokens after 3000, capped, fp32 151 -> 108; 64-wide, 3 x 400 after 3000, 159 ->
+// 119), but not where a window leaves few keys to share among the waves (20, 25).
 // Beyond that 128 rows, since the four waves of the other kernel read every K and
 // V tile for themselves: 2 x 400 tokens 27 us, 30 with 32 rows; 16 x 256 tokens
 // 49, 81.  Sequences of 64 rows and less would leave half of such a tile empty:
@@ -49,13 +53,14 @@ struct Launch {
 // A prefix beside its batch's own keys takes half the places (three or four
 // 64-wide workgroups fit a CU): 8 groups of 8 sequences 48 -> 42 us.  128-row
 // workgroups are more than the CUs as it is, and their keys stay whole.
-inline Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len, bool beside = false) {
+inline Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len, bool beside = false,
+                   bool bent = false) {
     Launch l;
     const uint64_t G = c->n_heads / c->n_kv_heads, rows = tokens * G;
     // of equally long sequences
     auto wgs = [&](uint64_t bm) { return (rows + units * bm - 1) / (units * bm) * units * c->n_kv_heads; };
     const uint64_t room = 512 * 128 / c->head_dim;
-    l.few = single || wgs(32) <= (units == 1 ? room + room / 2 : room) || wgs(32) < 3 * wgs(128);
+    l.few = single || wgs(32) <= (units == 1 ? room + room / 2 : bent ? room + room / 4 : room) || wgs(32) < 3 * wgs(128);
     const uint64_t bm = l.few ? 32 : 128;
     l.slots = single ? units * ((G + bm - 1) / bm) : rows / bm + units;
     const uint64_t places = beside && c->head_dim == 128 ? 256 : 512;
