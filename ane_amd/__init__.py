@@ -1407,21 +1407,30 @@ def pages_compact(cache, table_out=None, refs_out=None, n_live=None, workspace=N
 
 
 # ---------------------------------------------------------------- int8 linear layers of a batch
-def _act_types():
-    global _ACT_TYPES
-    if _ACT_TYPES is None:
+class _Torch:
+    """What every call below asks torch for, looked up once (an import statement costs as much as a tensor's check)."""
+
+    def __init__(self):
         import torch
 
-        _ACT_TYPES = {torch.float32: 0, torch.float16: 1}
-    return _ACT_TYPES
+        self.types = {torch.float32: 0, torch.float16: 1}
+        self.float32, self.int8, self.device = torch.float32, torch.int8, torch.cuda.device
+        self.current, self.raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-_ACT_TYPES = None
+_TORCH: _Torch | None = None
+
+
+def _torch() -> _Torch:
+    global _TORCH
+    if _TORCH is None:
+        _TORCH = _Torch()
+    return _TORCH
 
 
 def _tokens(t, dev, what):
     """(pointer, type, tokens, values, row stride) of activations [tokens][values] whose values are contiguous."""
-    ty = _act_types().get(t.dtype)
+    ty = (_TORCH or _torch()).types.get(t.dtype)
     if ty is None or t.dim() != 2:
         raise ValueError(f"{what} is a float32 or float16 tensor [tokens][values]")
     (n, k), (s0, s1) = t.shape, t.stride()
@@ -1429,47 +1438,49 @@ def _tokens(t, dev, what):
         raise ValueError(f"{what} is on the device of the others")
     if s1 != 1 and k > 1:
         raise ValueError(f"the values of a token of {what} are contiguous")
-    if n > 1 and s0 < k:
-        raise ValueError(f"the tokens of {what} do not overlap")
-    return t.data_ptr(), ty, n, k, s0 if n > 1 else k
+    if n > 1:
+        if s0 < k:
+            raise ValueError(f"the tokens of {what} do not overlap")
+        return t.data_ptr(), ty, n, k, s0
+    return t.data_ptr(), ty, n, k, k
 
 
 def _vector(t, n, dev, what):
     """The pointer of n contiguous float32, or None."""
     if t is None:
         return None
-    if _act_types().get(t.dtype) != 0 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
+    if t.dtype != (_TORCH or _torch()).float32 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
         raise ValueError(f"{what} is a contiguous float32 tensor of {n} values on the device of the others")
     return t.data_ptr()
 
 
 def _int8_rows(t, k, dev, what):
     """(pointer, rows, row stride) of int8 rows of k values that can be read up to k rounded up to 16."""
-    import torch
-
-    if t.dtype != torch.int8 or t.dim() != 2 or t.shape[1] != k or (k > 1 and t.stride(1) != 1) or t.get_device() != dev:
-        raise ValueError(f"{what} is an int8 tensor [rows][{k}] on the device of the others, its rows contiguous")
-    n, kp = t.shape[0], (k + 15) // 16 * 16
-    s0 = t.stride(0) if n > 1 else kp
-    p = t.data_ptr()
-    if p % 16 or s0 % 16 or s0 < kp:
+    if t.dtype != (_TORCH or _torch()).int8 or t.dim() != 2 or t.get_device() != dev:
+        raise ValueError(f"{what} is an int8 tensor [rows][{k}] on the device of the others")
+    (n, width), (s0, s1) = t.shape, t.stride()
+    if width != k or (s1 != 1 and k > 1):
+        raise ValueError(f"{what} is an int8 tensor [rows][{k}], its rows contiguous")
+    kp, p = (k + 15) // 16 * 16, t.data_ptr()
+    if n <= 1:
+        s0 = kp
+    if (p | s0) & 15 or s0 < kp:
         raise ValueError(f"the rows of {what} start on 16 bytes (a view [:, :k] of rows of {kp} bytes will do)")
-    if n and t.storage_offset() + (n - 1) * s0 + kp > t.untyped_storage().nbytes():
+    if kp != k and n and t.storage_offset() + (n - 1) * s0 + kp > t.untyped_storage().nbytes():
         raise ValueError(f"the last row of {what} can be read up to {kp} bytes")
     return p, n, s0
 
 
 def _on(dev, fn, what, stream, args):
     """fn(*args, stream) on device dev and, unless given, its current stream."""
-    import torch
-
     if dev < 0:
         raise ValueError("the tensors are not in GPU memory")
-    if dev == torch._C._cuda_getDevice():
-        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream_handle(stream))
+    t = _TORCH or _torch()
+    if dev == t.current():
+        st = fn(*args, t.raw_stream(dev) if stream is None else _stream_handle(stream))
     else:
-        with torch.cuda.device(dev):
-            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream_handle(stream))
+        with t.device(dev):
+            st = fn(*args, t.raw_stream(dev) if stream is None else _stream_handle(stream))
     if st:
         check(st, what)
 
