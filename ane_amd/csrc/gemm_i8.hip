@@ -232,9 +232,12 @@ static int launch_gemm(const GemmParams& p, hipStream_t s) {
 int launch_gemm_rows(const GemmParams& p, hipStream_t s) { return launch_gemm<kBTransposed, false>(p, s); }
 
 // Measured as T x N x K in us, for 256 CUs (n = CUs, t = tiles):
+// - up to 8 tokens over whole rows, while the tokens take at most 64 KB of LDS, so that
+//   two workgroups fit a CU: 4 x 28672 x 4096 22.9 with its quantizer, 29.1 before; 8 x
+//   28672 x 4096 27.2, 29.3; 8 x 4096 x 14336 (112 KB) 20.2, in 64-tiles 19.0.
 // - up to 64 tokens the few-row kernel, which reads x again for every 16 columns, while
-//   that is little: 16 x 4096 x 4096 7.1, in 64-tiles 7.3; 32 x 4096 x 4096 9.2, 7.8;
-//   8 x 28672 x 4096 28.6, 27.4.  Where K cannot be split the 64-tiles need more
+//   that is little: 16 x 4096 x 4096 7.1, in 64-tiles 7.3; 32 x 4096 x 4096 9.2, 7.8.
+//   Where K cannot be split the 64-tiles need more
 //   columns: 32 x 4096 x 14336 26, in whole 64-tiles 33.
 // - 256-tiles from 3n/4: 384 x 28672 x 4096 67, in 128-tiles 71; 2048 x 6144 x 4096 60,
 //   70; with n/2 of them 2048 x 4096 x 4096 45, 38.
@@ -250,6 +253,8 @@ ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split) {
     const uint64_t n = tile256_min_tiles(), nk = ((uint64_t)K + 127) / 128;
     auto tiles = [&](uint64_t b) { return (T + b - 1) / b * ((N + b - 1) / b); };
     const uint64_t t64 = tiles(64), t128 = tiles(128);
+    const uint64_t kb = ((uint64_t)K + 1023) / 1024;  // a token's room in LDS
+    if (T <= 8 && (T > 4 ? 8 : T > 2 ? 4 : T) * kb <= 64) return {kScaledRows, 1};
     if (T <= 64) {
         if (may_split ? (uint64_t)T * N * K < 300000000ull : t64 * T < 3000) return {kScaledFew, 1};
     } else {
@@ -266,6 +271,9 @@ ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split) {
 int launch_gemm_scaled(const GemmParams& p, ScaledPlan plan, hipStream_t s) {
     switch (plan.kernel) {
         case kScaledFew: break;
+        case kScaledRows:
+            if (gemm_dot_eligible(p)) return launch_gemm_dot(p, s);
+            break;
         case kScaled64:
             if (tile64_eligible(p, true)) return launch_gemm_tile64(p, s, plan.split);
             break;

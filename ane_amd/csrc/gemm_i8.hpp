@@ -90,7 +90,7 @@ int launch_gemm_rows(const GemmParams& p, hipStream_t s);
 
 // The kernel of the scaled epilogue for sizes, and over how many workgroups a tile its
 // K is split (with p.planes and p.counts, kScaledCounts words zero before the launch).
-enum ScaledKernel { kScaledFew, kScaled64, kScaled128d, kScaled128, kScaled256 };
+enum ScaledKernel { kScaledRows, kScaledFew, kScaled64, kScaled128d, kScaled128, kScaled256 };
 struct ScaledPlan {
     ScaledKernel kernel;
     uint32_t split;
@@ -98,6 +98,9 @@ struct ScaledPlan {
 constexpr uint32_t kScaledCounts = 256;
 ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split);
 int launch_gemm_scaled(const GemmParams& p, ScaledPlan plan, hipStream_t s);
+// kScaledRows: at most eight tokens, over whole rows of Bt (linear_i8.hip).
+bool gemm_dot_eligible(const GemmParams& p);
+int launch_gemm_dot(const GemmParams& p, hipStream_t s);
 
 // dense_fused_i8 operand preparation (quantize_fused.hip): absmax partials
 // (kFusedPartials per tensor), qA (M x Kp), qBt (N x Kp), scales {sa, sb},

@@ -358,7 +358,7 @@ def test_a_token_does_not_depend_on_its_batch(ane, K, half):
     s0, out0 = torch.zeros(T, device="cuda"), torch.zeros((T, N), device="cuda")
     ane.quantize_tokens(X, q0, s0, norm_w=nw)
     ane.linear_i8(X, W, S, out0, norm_w=nw, bias=B)
-    for n in (1, 2, 16, 40, 64, 100, 257, 600):
+    for n in (1, 2, 3, 8, 16, 40, 64, 100, 257, 600):
         q, s, out = rows16(np.zeros((n, K), np.int8), fill=0), torch.zeros(n, device="cuda"), torch.zeros((n, N), device="cuda")
         ane.quantize_tokens(X[:n], q, s, norm_w=nw)
         ane.linear_i8(X[:n], W, S, out, norm_w=nw, bias=B)
@@ -394,8 +394,9 @@ def test_plans():
 
     f = ane_amd.lib()._FuncPtr(("_ZN3ane11scaled_planEjjjb", ane_amd.lib()))
     f.restype, f.argtypes = Plan, [ctypes.c_uint32] * 3 + [ctypes.c_bool]
-    few, t64, t128d, t128, t256 = range(5)
-    for T, N, K, may, want in ((16, 4096, 4096, True, (few, 1)), (32, 4096, 4096, True, (t64, 4)), (32, 4096, 14336, True, (t64, 4)),
+    rows, few, t64, t128d, t128, t256 = range(6)
+    for T, N, K, may, want in ((4, 4096, 14336, True, (rows, 1)), (8, 4096, 14336, True, (t64, 4)), (5, 4096, 8192, False, (rows, 1)),
+                               (1, 99, 70000, False, (few, 1)), (16, 4096, 4096, True, (few, 1)), (32, 4096, 4096, True, (t64, 4)), (32, 4096, 14336, True, (t64, 4)),
                                (32, 4096, 14336, False, (few, 1)), (64, 28672, 4096, True, (t64, 1)),
                                (192, 4096, 14336, True, (t128d, 4)), (512, 4096, 14336, True, (t128d, 2)),
                                (512, 4096, 14336, False, (t64, 1)), (16, 65536, 4096, True, (t64, 1)),
