@@ -9,6 +9,8 @@
 // The angle is formed and reduced in fp64 and its cosine and sine are rounded
 // once, so far positions are as exact as near ones and no table of positions is
 // read.
+#include <algorithm>
+
 #include "paged.hpp"
 
 namespace ane {
@@ -68,7 +70,7 @@ template <class TI, class TQ, int HD, bool HALF>
 __global__ void __launch_bounds__(256) k_paged_rotate(RotateArgs a) {
     constexpr uint32_t per = HD / 8;
     __shared__ float2 turns[4][64];
-    const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, d = tid % per * 8;
+    const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, d = tid % per * 8, width = blockDim.x;
     const uint32_t qu = a.q ? a.n_heads * per : 0, ku = a.n_kv * per, units = qu + 2 * ku;
     auto load = [&](uint32_t u, float(&x)[8]) {
         if (u < qu) load8<TI>(a.q, t * a.q_stride + u * 8, x);
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(256) k_paged_rotate(RotateArgs a) {
     };
     float x[kAhead][8];
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; i++) load(tid + i * 256, x[i]);
+    for (uint32_t i = 0; i < kAhead; i++) load(tid + i * width, x[i]);
     float qw[8], kw[8];
     if (a.q_norm)
 #pragma unroll
@@ -174,10 +176,10 @@ __global__ void __launch_bounds__(256) k_paged_rotate(RotateArgs a) {
         }
     };
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; i++) put(tid + i * 256, x[i]);
-    for (uint32_t i = kAhead; i * 256 < units; i++) {  // (all lanes: they exchange values)
-        load(tid + i * 256, x[0]);
-        put(tid + i * 256, x[0]);
+    for (uint32_t i = 0; i < kAhead; i++) put(tid + i * width, x[i]);
+    for (uint32_t i = kAhead; i * width < units; i++) {  // (all lanes: they exchange values)
+        load(tid + i * width, x[0]);
+        put(tid + i * width, x[0]);
     }
 }
 
@@ -185,7 +187,8 @@ template <class TI, class TQ>
 void launch(const RotateArgs& a, uint32_t hd, bool half, uint32_t n_tokens, hipStream_t s) {
     const auto f = hd == 128 ? (half ? k_paged_rotate<TI, TQ, 128, true> : k_paged_rotate<TI, TQ, 128, false>)
                              : (half ? k_paged_rotate<TI, TQ, 64, true> : k_paged_rotate<TI, TQ, 64, false>);
-    hipLaunchKernelGGL(f, dim3(n_tokens), dim3(256), 0, s, a);
+    const uint32_t units = ((a.q ? a.n_heads : 0) + 2 * a.n_kv) * hd / 8;
+    hipLaunchKernelGGL(f, dim3(n_tokens), dim3(64 * std::min((units + 64 * kAhead - 1) / (64 * kAhead), 4u)), 0, s, a);
 }
 
 }  // namespace
