@@ -1341,7 +1341,7 @@ static uint64_t rule_len(const ane_paged_cache* c, const ane_attention_rule* r, 
 
 static Launch prompt_plan(const ane_paged_cache* c, const ane_attention_rule* r, uint32_t n, uint32_t n_tokens, bool single,
                           uint32_t max_len) {
-    return plan(c, n, n_tokens, single, rule_len(c, r, max_len), false, r && !r->window);
+    return plan(c, n, n_tokens, single, rule_len(c, r, max_len), false, r && !r->window, r && r->window);
 }
 
 static size_t prompt_workspace(const ane_paged_cache* cache, const ane_attention_rule* rule, uint32_t n, uint32_t n_tokens,

@@ -33,7 +33,8 @@ struct Launch {
 
 // units: sequences (groups) of the launch; tokens: theirs in all; single: one
 // token each; beside: shares its launch with the batch's own keys; bent: under a
-// rule without a window.
+// rule without a window; windowed: under one with, max_len then a bound on the keys that
+// a workgroup's rows see.
 //
 // 32 rows a workgroup as long as its workgroups have a place each (512 of them, two
 // a CU; 64-wide four a CU, three in fp32), half again as many for one sequence,
@@ -52,9 +53,13 @@ struct Launch {
 // longer parts (200 tokens after 4000 positions 51 us, in 1.5 times the parts 63).
 // A prefix beside its batch's own keys takes half the places (three or four
 // 64-wide workgroups fit a CU): 8 groups of 8 sequences 48 -> 42 us.  128-row
-// workgroups are more than the CUs as it is, and their keys stay whole.
+// workgroups are more than the CUs as it is, and their keys stay whole.  Behind a window
+// rows have equally many keys, so two parts spread nothing more evenly than one: single
+// tokens, which memory bounds, and short windows save the join (32 tokens behind 1024
+// 31.4 -> 29.7 us, behind 4096 98.7 -> 94.7; 2 x 96 tokens behind 1024 26.2 -> 23.8, but
+// 3 x 64 behind 4096 55 -> 62).
 inline Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len, bool beside = false,
-                   bool bent = false) {
+                   bool bent = false, bool windowed = false) {
     Launch l;
     const uint64_t G = c->n_heads / c->n_kv_heads, rows = tokens * G;
     // of equally long sequences
@@ -64,7 +69,8 @@ inline Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bo
     const uint64_t bm = l.few ? 32 : 128;
     l.slots = single ? units * ((G + bm - 1) / bm) : rows / bm + units;
     const uint64_t places = beside && c->head_dim == 128 ? 256 : 512;
-    const uint64_t n = std::max<uint64_t>(1, l.few ? std::min(places / wgs(32), (max_len + 255) / 256) : 1);
+    uint64_t n = std::max<uint64_t>(1, l.few ? std::min(places / wgs(32), (max_len + 255) / 256) : 1);
+    if (windowed && n == 2 && (single || max_len <= 2048)) n = 1;
     l.chunk = (uint32_t)(((max_len + n - 1) / n + 127) / 128 * 128);
     l.parts = (uint32_t)((max_len + l.chunk - 1) / l.chunk);
     return l;
