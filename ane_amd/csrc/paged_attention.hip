@@ -1042,7 +1042,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs& a, uint32_t slot, uint3
         return Next{ld.group(a, x, w, g, u, from), ld.group(a, x, w, g, u + 1, from + 1)};
     };
     auto copy = [&](const Next& n, int i, uint8_t* dst) {
-        ld.template copy<MODE == kOwn>(n.g[2 * i / kC], i % (kC / 2), dst + 2 * i / kC * (kT / 2));
+        ld.template copy<MODE == kOwn || EACH>(n.g[2 * i / kC], i % (kC / 2), dst + 2 * i / kC * (kT / 2));
     };
     if (tiles) {
         const Next n = aim(a.kp, 0);
@@ -1167,11 +1167,11 @@ __global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) k_attn_few(AttnArgs a) 
     attn_few<HD, F32, MODE, false, RULE>(a, slot, blockIdx.y, blockIdx.x - slot * a.n_kv, smem);
 }
 // Single tokens with few keys, a wave each.
-template <int HD, bool F32>
-__global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) k_attn_each(AttnArgs a) {
+template <int HD, bool F32, bool RULE = false>
+__global__ void __launch_bounds__(256, HD == 64 && !(RULE && F32) ? 3 : 2) k_attn_each(AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[few_lds<HD>()];
     const uint32_t job = blockIdx.x * 4 + block_wave(), slot = a.by_kv(job);
-    attn_few<HD, F32, kOwn, true>(a, slot, 0, job - slot * a.n_kv, smem);
+    attn_few<HD, F32, RULE ? kPrompt : kOwn, true, RULE>(a, slot, 0, job - slot * a.n_kv, smem);
 }
 // A batch with few rows a group: prefix and own keys in one launch, the prefix's
 // workgroups, which have more keys, first (64 sequences behind 8192 shared
@@ -1277,6 +1277,12 @@ size_t parts_bytes(const ane_paged_cache* c, uint32_t n_tokens, uint32_t parts, 
 template <int HD, bool F32, bool RULE = false>
 void launch_prompt(const AttnArgs& a, const Launch& l, hipStream_t s) {
     const dim3 grid((uint32_t)(l.slots * a.n_kv), l.parts);
+    if constexpr (RULE) {
+        if (l.each) {
+            hipLaunchKernelGGL((k_attn_each<HD, F32, true>), dim3((grid.x + 3) / 4), dim3(256), 0, s, a);
+            return;
+        }
+    }
     if (l.few) hipLaunchKernelGGL((k_attn_few<HD, F32, kPrompt, RULE>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_attn_block<HD, F32, kPrompt, RULE>), grid, dim3(256), 0, s, a, (uint32_t)l.slots);
 }
@@ -1341,7 +1347,9 @@ static uint64_t rule_len(const ane_paged_cache* c, const ane_attention_rule* r, 
 
 static Launch prompt_plan(const ane_paged_cache* c, const ane_attention_rule* r, uint32_t n, uint32_t n_tokens, bool single,
                           uint32_t max_len) {
-    return plan(c, n, n_tokens, single, rule_len(c, r, max_len), false, r && !r->window, r && r->window);
+    Launch l = plan(c, n, n_tokens, single, rule_len(c, r, max_len), false, r && !r->window, r && r->window);
+    l.each = r && single && each_pays(c, l, rule_len(c, r, max_len));
+    return l;
 }
 
 static size_t prompt_workspace(const ane_paged_cache* cache, const ane_attention_rule* rule, uint32_t n, uint32_t n_tokens,

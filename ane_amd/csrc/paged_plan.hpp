@@ -26,7 +26,7 @@ inline Div div_by(uint32_t d) {
 
 // One launch: which kernel, over how many row tiles, its keys in how many parts.
 struct Launch {
-    bool few;
+    bool few, each;  // each: single tokens under a rule, a wave a (token, kv head)
     uint64_t slots;
     uint32_t chunk, parts;
 };
@@ -60,7 +60,7 @@ struct Launch {
 // 3 x 64 behind 4096 55 -> 62).
 inline Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bool single, uint64_t max_len, bool beside = false,
                    bool bent = false, bool windowed = false) {
-    Launch l;
+    Launch l = {};
     const uint64_t G = c->n_heads / c->n_kv_heads, rows = tokens * G;
     // of equally long sequences
     auto wgs = [&](uint64_t bm) { return (rows + units * bm - 1) / (units * bm) * units * c->n_kv_heads; };
@@ -88,6 +88,9 @@ inline uint64_t bound_len(const ane_paged_cache* c, uint32_t max_len) {
 // 1536, where that costs as much as it saves (256 sequences with 100 own positions
 // behind 1024 56 -> 40 us; 120 such and 8 alone with 1024 44 -> 57, behind 2048 54 ->
 // 96, behind 8192 128 -> 328).
+inline bool each_pays(const ane_paged_cache* c, const Launch& l, uint64_t len) {
+    return l.parts == 1 && l.slots * c->n_kv_heads >= 1024 && len <= 512;
+}
 struct SharedPlan {
     Launch prefix, own;
     uint32_t parts;
@@ -99,7 +102,7 @@ inline SharedPlan shared_plan(const ane_paged_cache* c, uint32_t n, uint32_t n_g
     p.own = plan(c, n, n, true, len);
     if (n_groups) p.prefix = plan(c, n_groups, n, false, bound_len(c, max_prefix), true);
     p.parts = p.prefix.parts + p.own.parts;
-    p.each = p.own.parts == 1 && p.own.slots * c->n_kv_heads >= 1024 && len - prefix <= 512 && len <= 1536;
+    p.each = each_pays(c, p.own, len - prefix) && len <= 1536;
     return p;
 }
 

@@ -232,6 +232,28 @@ def test_single_tokens(ane, ty, hd, name, lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ty,hd", [("f32", 128), ("f16", 128), ("f32", 64), ("f16", 64)])
+@pytest.mark.parametrize("kw", [dict(cap=20.0), dict(slopes=True), dict(window=90), dict(window=300, cap=3.0), dict(prefix=True),
+                                dict(first=True)], ids=str)
+def test_many_single_tokens(ane, ty, hd, kw):
+    """Batches of which every (token, kv head) gets a wave: lengths from none to 400, a bound or a window of at most 512."""
+    heads, kv, n = 12, 4, 270
+    r = random.Random(hd)
+    lens = [r.choice([0, 1, 31, 32, 33, 64, r.randint(1, 400)]) for _ in range(n)]
+    kw = dict(kw)
+    if "slopes" in kw:
+        kw["slopes"] = alibi(heads)
+    if "first" in kw:
+        kw["first"] = [r.choice([0, max(0, m - 1), m, m // 2, 1 << 20]) for m in lens]
+    if "prefix" in kw:
+        kw["prefix"] = [r.randint(0, 500) for _ in lens]
+    c = make_cache(lens, heads, kv, hd, 16, seed=n)
+    run(c, [1] * n, ty, single=True, max_len=400, **kw)
+    if "window" in kw:
+        run(c, [1] * n, ty, single=True, max_len=None, **kw)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("ty", ["f32", "f16"])
 @pytest.mark.parametrize("many", [False, True])
 def test_tokens_that_see_nothing(ane, ty, many):
