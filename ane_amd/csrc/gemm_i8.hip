@@ -235,37 +235,42 @@ int launch_gemm_rows(const GemmParams& p, hipStream_t s) { return launch_gemm<kB
 // - up to 8 tokens over whole rows, while the tokens take at most 64 KB of LDS, so that
 //   two workgroups fit a CU: 4 x 28672 x 4096 22.9 with its quantizer, 29.1 before; 8 x
 //   28672 x 4096 27.2, 29.3; 8 x 4096 x 14336 (112 KB) 20.2, in 64-tiles 19.0.
-// - up to 64 tokens the few-row kernel, which reads x again for every 16 columns, while
-//   that is little: 16 x 4096 x 4096 7.1, in 64-tiles 7.3; 32 x 4096 x 4096 9.2, 7.8.
-//   Where K cannot be split the 64-tiles need more
-//   columns: 32 x 4096 x 14336 26, in whole 64-tiles 33.
-// - 256-tiles from 3n/4: 384 x 28672 x 4096 67, in 128-tiles 71; 2048 x 6144 x 4096 60,
-//   70; with n/2 of them 2048 x 4096 x 4096 45, 38.
+// - 256-tiles from 3n/4 of them or where 128-tiles would not all have a place (2n):
+//   384 x 28672 x 4096 67, in 128-tiles 71; 2048 x 6144 x 4096 60, 70; 1400 x 6784 x 896
+//   (162, 583 128-tiles) 19, 28; 2048 x 4096 x 4096 (128, 512) 45, 38.
 // - above n/2 128-tiles, on the deep ring up to n: 512 x 6144 x 4096 22.5, in 64-tiles
 //   31; 768 x 6144 x 4096 (288 tiles, two a CU) 35, on the deep ring 40.
-// - the others in 64-tiles; with K of 64 steps and more, and 3n/16 128-tiles, in
-//   128-tiles with K split: 512 x 4096 x 14336 47 in two parts, in 64-tiles 61; 192 x
-//   4096 x 14336 30 in four, 36.
-// - 64-tiles with K in as many parts as fill the CUs, at most 4, of 8 steps at least:
-//   64 x 4096 x 4096 8.3 in four, 10.6 whole; 32 x 4096 x 14336 15, 33; 64 x 2003 x 1792
-//   7.5 in three, 7.4 whole.
+// - with K of 64 steps and more, and 3n/16 128-tiles, in 128-tiles with K split: 512 x
+//   4096 x 14336 47 in two parts, in 64-tiles 61; 192 x 4096 x 14336 30 in four, 36.
+// - the others in 64-tiles with K in as many parts as fill the CUs, at most 8, of 8
+//   steps at least: 64 x 4096 x 4096 8.3 in four, 10.6 whole; 32 x 4096 x 14336 15, 33;
+//   32 x 512 x 14336 9.1 in eight, 11.2 in four; 64 x 2003 x 1792 7.5 in three, 7.4 whole.
+// - up to 64 tokens the few-row kernel instead, which reads x again for every 16
+//   columns, where that costs less by the fits below (in 10 ns): 16 x 4096 x 4096 7.1,
+//   in 64-tiles 7.3; 32 x 4096 x 4096 9.2, 7.8; 16 x 512 x 14336 16.4, 8.5; 32 x 1024 x
+//   1024 4.1, 4.8; 32 x 4096 x 14336 26, in whole 64-tiles 33.
 ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split) {
     const uint64_t n = tile256_min_tiles(), nk = ((uint64_t)K + 127) / 128;
     auto tiles = [&](uint64_t b) { return (T + b - 1) / b * ((N + b - 1) / b); };
     const uint64_t t64 = tiles(64), t128 = tiles(128);
     const uint64_t kb = ((uint64_t)K + 1023) / 1024;  // a token's room in LDS
     if (T <= 8 && (T > 4 ? 8 : T > 2 ? 4 : T) * kb <= 64) return {kScaledRows, 1};
-    if (T <= 64) {
-        if (may_split ? (uint64_t)T * N * K < 300000000ull : t64 * T < 3000) return {kScaledFew, 1};
-    } else {
-        if (T > 128 && tiles(256) * 4 >= n * 3) return {kScaled256, 1};
+    if (T > 64) {
+        if (T > 128 && (tiles(256) * 4 >= n * 3 || t128 > 2 * n)) return {kScaled256, 1};
         if (t128 * 2 > n) return {t128 <= n ? kScaled128d : kScaled128, 1};
         if (may_split && nk >= 64 && t128 * 16 >= n * 3) return {kScaled128d, (uint32_t)(n / t128)};
     }
     uint64_t split = may_split ? n / t64 : 1;
-    if (split > 4) split = 4;
+    if (split > 8) split = 8;
     if (split > nk / 8) split = nk / 8;
-    return {kScaled64, split > 1 ? (uint32_t)split : 1u};
+    if (split < 1) split = 1;
+    if (T <= 64) {
+        const uint64_t groups = (N + 15ull) / 16;
+        const uint64_t few = 250 + (nk + 3) / 4 * (17 + 32 * ((T + 15) / 16)) * ((groups + n - 1) / n);
+        const uint64_t tile = 220 + (nk + split - 1) / split * 30 * ((t64 * split + n - 1) / n) + (split > 1 ? 220 : 0);
+        if (few <= tile) return {kScaledFew, 1};
+    }
+    return {kScaled64, (uint32_t)split};
 }
 
 int launch_gemm_scaled(const GemmParams& p, ScaledPlan plan, hipStream_t s) {

@@ -675,7 +675,7 @@ int ANE_TILE_LAUNCH(const GemmParams& p, bool a_unsigned, hipStream_t s) {
 }
 #else
 bool ANE_TILE_ELIGIBLE(const GemmParams& p, bool any_rows) {
-    if ((!any_rows && p.Mout < TM) || p.Nout < TN) return false;
+    if ((!any_rows && p.Mout < TM) || (!p.rs && p.Nout < TN)) return false;
     if (p.Kp == 0 || (p.Kp % (p.rs ? 16 : 64)) != 0) return false;  // (a slice's tail is masked 16 bytes at a time)
     if ((p.lda & 15) || (p.ldb & 15)) return false;
     if ((((uintptr_t)p.A) & 15) || (((uintptr_t)p.B) & 15)) return false;
@@ -693,9 +693,10 @@ int ANE_TILE_LAUNCH(const GemmParams& p, hipStream_t s, uint32_t ksplit) {
     const uint32_t tiles_n = (p.Nout + TN - 1) / TN;
     const uint64_t total = (uint64_t)tiles_m * tiles_n;
     if (total > 0x7fffffffull || ksplit == 0 || ksplit > 65535) return ANE_ERR_INVALID_ARG;
-    if (ksplit > 1 && !p.Craw && !(p.rs && p.planes)) return ANE_ERR_INVALID_ARG;  // split K writes int32 planes
+    constexpr bool kAdds = TM == 64 || STAGES > 2;  // the tiles whose K the scaled epilogue splits
+    if (ksplit > 1 && !p.Craw && !(kAdds && p.rs && p.planes)) return ANE_ERR_INVALID_ARG;  // split K writes int32 planes
     if (p.ig && p.nsum > kIgParts) return ANE_ERR_INVALID_ARG;
-    const auto fn = p.rs && ksplit > 1 ? ANE_TILE_KERNEL<false, true, true>
+    const auto fn = p.rs && ksplit > 1 ? ANE_TILE_KERNEL<false, true, kAdds>
                     : p.rs ? ANE_TILE_KERNEL<false, true> : p.ig ? ANE_TILE_KERNEL<true> : ANE_TILE_KERNEL<false>;
     hipLaunchKernelGGL(fn, dim3((uint32_t)total, ksplit), dim3(kThreads), 0, s, p, tiles_m, tiles_n);
     ANE_HIP_CHECK_LAUNCH();

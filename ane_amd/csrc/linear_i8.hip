@@ -201,10 +201,16 @@ void launch_quantize(const QuantArgs& a, hipStream_t s) {
         if (a.K <= 16384) return go(k_quantize_tokens<T, 16, 2>, 16);
         return go(k_quantize_tokens<T, 16, 0>, 16);
     }
-    if (a.K <= 2048) return go(k_quantize_tokens<T, 4, 1>, 4);
-    if (a.K <= 4096) return go(k_quantize_tokens<T, 4, 2>, 4);
-    if (a.K <= 8192) return go(k_quantize_tokens<T, 4, 4>, 4);
-    go(k_quantize_tokens<T, 4, 8>, 4);
+    switch ((a.K + 2047) / 2048) {
+        case 1: return go(k_quantize_tokens<T, 4, 1>, 4);
+        case 2: return go(k_quantize_tokens<T, 4, 2>, 4);
+        case 3: return go(k_quantize_tokens<T, 4, 3>, 4);
+        case 4: return go(k_quantize_tokens<T, 4, 4>, 4);
+        case 5: return go(k_quantize_tokens<T, 4, 5>, 4);
+        case 6: return go(k_quantize_tokens<T, 4, 6>, 4);
+        case 7: return go(k_quantize_tokens<T, 4, 7>, 4);
+        default: return go(k_quantize_tokens<T, 4, 8>, 4);
+    }
 }
 
 __device__ __forceinline__ int wave_sum_i32(int v) {

@@ -220,7 +220,7 @@ def test_quantize_special_values(ane):
 SHAPES = [(1, 1, 1), (1, 6144, 4096), (1, 17, 31), (2, 100, 777), (3, 16, 16), (5, 33, 100), (15, 2003, 64), (16, 4096, 513),
           (17, 48, 1000), (32, 4096, 14336), (33, 500, 200), (64, 1000, 4096), (65, 129, 96), (100, 4096, 4096), (128, 640, 1777),
           (129, 300, 130), (200, 8192, 256), (256, 256, 64), (301, 2003, 1777), (512, 4096, 1040), (600, 5000, 1000),
-          (1000, 1536, 1000), (1024, 1024, 4096), (2048, 4096, 512), (4096, 4096, 144), (5000, 3000, 48), (9000, 130, 80),
+          (1000, 1536, 1000), (1024, 1024, 4096), (2048, 4096, 512), (4096, 4096, 144), (5000, 3000, 48), (9000, 130, 80), (76, 39, 7203), (300, 5, 400), (40, 20, 9000), (100, 61, 3000),
           (300, 28672, 192)]
 
 
@@ -396,7 +396,8 @@ def test_plans():
     f.restype, f.argtypes = Plan, [ctypes.c_uint32] * 3 + [ctypes.c_bool]
     rows, few, t64, t128d, t128, t256 = range(6)
     for T, N, K, may, want in ((4, 4096, 14336, True, (rows, 1)), (8, 4096, 14336, True, (t64, 4)), (5, 4096, 8192, False, (rows, 1)),
-                               (1, 99, 70000, False, (few, 1)), (16, 4096, 4096, True, (few, 1)), (32, 4096, 4096, True, (t64, 4)), (32, 4096, 14336, True, (t64, 4)),
+                               (1, 99, 70000, False, (few, 1)), (16, 4096, 4096, True, (few, 1)), (16, 6144, 4096, True, (t64, 2)), (32, 512, 14336, True, (t64, 8)),
+                               (32, 2003, 1777, True, (few, 1)), (100, 39, 7203, True, (t64, 7)), (1400, 6784, 896, True, (t256, 1)), (32, 4096, 4096, True, (t64, 4)), (32, 4096, 14336, True, (t64, 4)),
                                (32, 4096, 14336, False, (few, 1)), (64, 28672, 4096, True, (t64, 1)),
                                (192, 4096, 14336, True, (t128d, 4)), (512, 4096, 14336, True, (t128d, 2)),
                                (512, 4096, 14336, False, (t64, 1)), (16, 65536, 4096, True, (t64, 1)),
