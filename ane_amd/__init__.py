@@ -1533,7 +1533,8 @@ def linear_i8_workspace(T, N, K, device="cuda"):
 
 def linear_i8(x, w, w_scales, out, norm_w=None, eps=1e-5, bias=None, residual=None, workspace=None, stream=None):
     """out [tokens][rows of w]: activations x [tokens][values] quantized a token at a time (after an RMSNorm where
-    norm_w is given), times int8 weights w [rows][values] with a scale a row, plus bias and residual."""
+    norm_w is given), times int8 weights w [rows][values] with a scale a row, plus bias and residual (may be out; out may
+    be x)."""
     dev = x.get_device()
     xp, ty, n, k, xs = _tokens(x, dev, "x")
     rows, wp, ws, cp, bp, rp, rs, to, op, os_ = _product(n, k, dev, w, w_scales, out, bias, residual)

@@ -32,7 +32,7 @@ struct GemmParams {
     uint32_t nsum, corr;
     // Scaled epilogue (linear_i8.hip) where rs is given: C = fl(fl((float)acc *
     // rs[i]) * cs[j]) + bias[j] + res[i][j], each step rounded, C and res fp16
-    // where half; C and ldc as below, in elements.
+    // where half; ldc and ldr in elements.
     const float* rs;      // fp32[Mout]
     const float* cs;      // fp32[Nout]
     const void* res;      // or nullptr

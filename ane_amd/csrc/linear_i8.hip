@@ -523,7 +523,10 @@ extern "C" int ane_hip_linear_i8(uint32_t T, uint32_t N, uint32_t K, int type, c
         p.planes = reinterpret_cast<int32_t*>(q + l.planes);
     }
     const QuantArgs a{x, x_stride, row_bytes(K), norm_w, q, qs, T, K, eps, p.counts};
-    if (const uint32_t runs = linear_one_runs(p, K)) {
+    // (the one launch reads x in every workgroup, so an output in its place takes two)
+    const uintptr_t xa = (uintptr_t)x, oa = (uintptr_t)out;
+    const bool apart = xa + K * item_size(type) <= oa || oa + N * item_size(out_type) <= xa;
+    if (const uint32_t runs = apart ? linear_one_runs(p, K) : 0) {
         type == ANE_TYPE_F32 ? launch_one<float>(a, p, runs, (hipStream_t)stream) : launch_one<_Float16>(a, p, runs, (hipStream_t)stream);
         ANE_HIP_CHECK_LAUNCH();
         return ANE_OK;

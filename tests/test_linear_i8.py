@@ -332,6 +332,61 @@ def test_other_stream_and_graph(ane, T, N, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 2, 8, 40, 300])
+@pytest.mark.parametrize("half", [False, True])
+def test_output_in_place_of_the_input(ane, T, half):
+    """x = residual = out, as in a layer whose input nobody needs afterwards, with many workgroups that read a token."""
+    N = K = 8192
+    x, w, ws, norm, bias, _ = inputs(T, N, K, seed=9, half_in=half, half_out=half)
+    X, W, S, nw, b = dev(x), rows16(w), dev(ws), dev(norm), dev(bias)
+    for i in range(3):
+        want = product(*quantized(x, norm), w, ws, bias, x, half)
+        ane.linear_i8(X, W, S, X, norm_w=nw, bias=b, residual=X)
+        x = X.cpu().numpy()
+        same(x, want)
+    y = dev(inputs(T, N, K, seed=10, half_in=half)[0])
+    want = product(*quantized(y.cpu().numpy(), None), w[:-96], ws[:-96], None, None, half)
+    ane.linear_i8(y, W[:-96], S[:-96], y[:, 96:])  # behind its start
+    same(y[:, 96:].cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N", [(3, 300), (100, 600)])
+def test_tokens_past_32_bit_offsets(ane, T, N):
+    import torch
+
+    K, stride = 80, (1 << 31) // (T - 1) // 16 * 16 + 16
+    x, w, ws, _, bias, _ = inputs(T, N, K, seed=11)
+    q, qs = quantized(x)
+    far = torch.zeros((T, stride), dtype=torch.int8, device="cuda")  # up to 3.2 GB
+    far[:, :K] = dev(q)
+    out = torch.zeros((T, N), device="cuda")
+    ane.dense_i8_scaled(far[:, :K], dev(qs), rows16(w), dev(ws), out, bias=dev(bias))
+    same(out.cpu().numpy(), product(q, qs, w, ws, bias))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(ane):
+    """K in parts on two streams, each with its workspace, many calls in flight."""
+    import torch
+
+    T, N, K = 32, 4096, 14336
+    jobs = []
+    for seed in (12, 13):
+        x, w, ws, norm, _, _ = inputs(T, N, K, seed=seed)
+        jobs.append((torch.cuda.Stream(), dev(x), rows16(w), dev(ws), dev(norm), [torch.zeros((T, N), device="cuda") for _ in range(6)],
+                     ane.linear_i8_workspace(T, N, K), product(*quantized(x, norm), w, ws, None, None)))
+    torch.cuda.synchronize()
+    for i in range(6):
+        for st, X, W, S, nw, outs, work, _ in jobs:
+            ane.linear_i8(X, W, S, outs[i], norm_w=nw, workspace=work, stream=st)
+    torch.cuda.synchronize()
+    for *_, outs, _, want in jobs:
+        for o in outs:
+            same(o.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
 def test_zero_sizes_leave_outputs(ane):
     import torch
 
