@@ -397,6 +397,8 @@ struct Rows {
     }
     // after take_q
     __device__ __forceinline__ void init_factor(const AttnArgs& a) {
+        // (in reach of 1 / cap: scores of a factor above 2^100 caps are zero or at the cap)
+        if (a.cap != 0.0f) c = fminf(c, a.cap * 0x1p100f);
         factor = c;
         if (a.slopes) c = 1.0f;
     }
@@ -405,8 +407,7 @@ struct Rows {
     template <int KT>
     __device__ __forceinline__ void bend(const AttnArgs& a, f16v (&s)[KT], int32_t t0) const {
         if (a.cap != 0.0f) {  // uniform, as the next ones
-            // (as c in take_q: never 0 nor infinite)
-            const float down = __builtin_amdgcn_fmed3f(factor * a.inv_cap, 0x1p-126f, 0x1p127f);
+            const float down = fmaxf(factor * a.inv_cap, 0x1p-126f);  // (as c in take_q: never 0)
             float top = 0.0f;
 #pragma unroll
             for (int t = 0; t < KT; t++)

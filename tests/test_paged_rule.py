@@ -329,6 +329,26 @@ def test_caps_and_slopes_at_the_ends(ane, heads, kv, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,n", [(4, 2, 60), (32, 8, 800)])
+def test_least_cap_over_largest_scores(ane, heads, kv, n):
+    """|score| <= 2^-20: each weight is 1 / keys within a factor of e^(2^-19), whatever q."""
+    import torch
+
+    c = make_cache([n], heads, kv, 128, 16, seed=2)
+    v = seq_kv(c, 0, 0, n)[1].double()
+    for ty, std, scale in (("f32", 3e37, None), ("f32", 3e37, 9e29), ("f16", 3000.0, 9e29)):
+        q = randq(n, heads, 128, dt(ty), seed=3).clamp(-4, 4) * std
+        out = torch.full_like(q, 5.0)
+        ane.attention_prompt(c, 0, i32([0, n]), q, out, scale=scale, rule=AttentionRule(2.0 ** -20))
+        keys = torch.arange(1, n + 1, device="cuda", dtype=torch.float64)[:, None]
+        for h in range(heads):
+            x = v[h // (heads // kv)]
+            top = x.abs().amax()
+            tol = (1.01 * 2.0 ** -19 + (2 * n + 64) * U + 2 * 2.0 ** -10 * (ty == "f16")) * top
+            assert bool(((out[:, h].double() - x.cumsum(0) / keys).abs() <= tol).all()), (ty, scale, h)
+
+
+@pytest.mark.gpu
 def test_no_rule_at_all_is_the_plain_call(ane):
     """An empty rule gives attention_prompt's bits."""
     import torch
