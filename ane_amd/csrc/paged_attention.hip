@@ -56,6 +56,7 @@ struct AttnArgs {
     // (0: none), slopes by head, window (0: none), the first position each token
     // sees, the prefix each batch row sees whole (null: none).
     float cap, inv_cap;
+    float bend[3];  // fp16: Tanh's coefficients for scores as the products give them, or zeros
     uint32_t window;
     const float* slopes;
     const uint32_t *first, *seen;
@@ -329,13 +330,16 @@ __device__ __forceinline__ void split(f2 x, h2& hi, h2& lw) {
 constexpr float kDrop = 8.0f, kDeep = 24.0f, kThin = -7.0f, kAgain = 38.0f;
 
 // tanh(y) = y + y z P(z), z = y^2, up to |y| = kSmall (P fitted here for the least
-// relative error: 2^-23.8 with five coefficients to 0.6, in fp32 arithmetic; 2^-20.4
-// with four to 0.75, below what fp16 weights are rounded by), beyond that as 1 - 2 /
+// relative error: 2^-23.8 with five coefficients to 0.6, in fp32 arithmetic; 2^-20.5
+// with three to 0.5, below what fp16 weights are rounded by), beyond that as 1 - 2 /
 // (1 + e^2y), there exact to 2^-22.  A cap is chosen well above most scores, so most
-// tiles are all small, and P costs half of what exponential and reciprocal do.
+// tiles are all small, and P costs half of what exponential and reciprocal do.  fp16
+// rows share their factor, so P takes the scores as they are (8192 tokens x 32 heads
+// behind a window of 1024 207 -> 197 us, without a window 720 -> 674; uncapped 171, 570).
 template <bool F32>
 struct Tanh {
-    static constexpr float kSmall = F32 ? 0.6f : 0.75f;
+    static constexpr float kSmall = F32 ? 0.6f : 0.5f;
+    static constexpr float kHalf[3] = {-0.33328157663f, 0.13205355406f, -0.04475053400f};
     // tanh(y) / y - 1
     static __device__ __forceinline__ float small(float y) {
         const float z = y * y;
@@ -347,10 +351,8 @@ struct Tanh {
             p = __builtin_fmaf(p, z, 0.13331924378f);
             p = __builtin_fmaf(p, z, -0.3333329856f);
         } else {
-            p = 0.01310574356f;
-            p = __builtin_fmaf(p, z, -0.0502778515f);
-            p = __builtin_fmaf(p, z, 0.13268233835f);
-            p = __builtin_fmaf(p, z, -0.3332966864f);
+            p = __builtin_fmaf(kHalf[2], z, kHalf[1]);
+            p = __builtin_fmaf(p, z, kHalf[0]);
         }
         return p * z;
     }
@@ -413,7 +415,7 @@ struct Rows {
             for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, fabsf(s[t][r])), fabsf(s[t][r + 1]));
-            if (__any(top * down > Tanh<F32>::kSmall)) {
+            if (__any(top * down > Tanh<F32>::kSmall) || (!F32 && a.bend[0] == 0.0f)) {
                 const float up = __builtin_amdgcn_rcpf(down);
 #pragma unroll
                 for (int t = 0; t < KT; t++)
@@ -426,7 +428,15 @@ struct Rows {
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[t][r] = __builtin_fmaf(Tanh<F32>::small(s[t][r] * down), s[t][r], s[t][r]);
+                    for (int r = 0; r < 16; r++) {
+                        if constexpr (F32) {
+                            s[t][r] = __builtin_fmaf(Tanh<F32>::small(s[t][r] * down), s[t][r], s[t][r]);
+                        } else {  // (the factor is one for all rows)
+                            const float z = s[t][r] * s[t][r];
+                            const float p = __builtin_fmaf(__builtin_fmaf(a.bend[2], z, a.bend[1]), z, a.bend[0]);
+                            s[t][r] *= __builtin_fmaf(p, z, 1.0f);
+                        }
+                    }
             }
         }
         if (!a.slopes) return;
@@ -1386,6 +1396,10 @@ static int prompt(const ane_paged_cache* cache, uint32_t layer, const uint32_t* 
     if (rule) {
         const double cap = (double)rule->softcap * 1.4426950408889634;
         a.cap = (float)cap, a.inv_cap = cap != 0.0 ? (float)(1.0 / cap) : 0.0f;
+        // (neither these nor squares of scores below kSmall of the cap leave fp32's range then)
+        const double d = (double)a.scale_log2e * a.inv_cap;
+        const bool in_range = d >= 0x1p-20 && d <= 0x1p20;
+        for (int k = 0; k < 3; k++) a.bend[k] = in_range ? (float)(Tanh<false>::kHalf[k] * std::pow(d, 2 * k + 2)) : 0.0f;
         a.slopes = rule->slopes, a.window = std::min(rule->window, 1u << 30), a.first = rule->first, a.seen = rule->prefix;
         if (cache->head_dim == 128) f32 ? launch_prompt<128, true, true>(a, l, s) : launch_prompt<128, false, true>(a, l, s);
         else f32 ? launch_prompt<64, true, true>(a, l, s) : launch_prompt<64, false, true>(a, l, s);
