@@ -1358,8 +1358,10 @@ static uint64_t rule_len(const ane_paged_cache* c, const ane_attention_rule* r, 
 
 static Launch prompt_plan(const ane_paged_cache* c, const ane_attention_rule* r, uint32_t n, uint32_t n_tokens, bool single,
                           uint32_t max_len) {
-    Launch l = plan(c, n, n_tokens, single, rule_len(c, r, max_len), false, r && !r->window, r && r->window);
-    l.each = r && single && each_pays(c, l, rule_len(c, r, max_len));
+    const uint64_t len = rule_len(c, r, max_len);
+    const bool windowed = r && r->window && r->window < bound_len(c, max_len);
+    Launch l = plan(c, n, n_tokens, single, len, false, r && len > (windowed ? 1024 : 256), windowed);
+    l.each = r && single && each_pays(c, l, len);
     return l;
 }
 

@@ -33,17 +33,20 @@ struct Launch {
 
 // units: sequences (groups) of the launch; tokens: theirs in all; single: one
 // token each; beside: shares its launch with the batch's own keys; bent: under a
-// rule without a window; windowed: under one with, max_len then a bound on the keys that
-// a workgroup's rows see.
+// rule, its rows seeing many keys; windowed: its window leaves fewer keys than there are,
+// max_len then a bound on those that a workgroup's rows see.
 //
 // 32 rows a workgroup as long as its workgroups have a place each (512 of them, two
 // a CU; 64-wide four a CU, three in fp32), half again as many for one sequence,
 // where 128 rows a workgroup would leave most CUs idle: 512 tokens x 32 heads fp32
 // 22 us, 31 with 128 rows; 768 tokens 33, 39; 8 chunks of 64 tokens after 1000
 // positions 36, 50.  Under a rule scores cost the vector unit more, which one workgroup
-// of 128 rows a CU leaves idle between its waves' products: a quarter more places (2 x
-// 300 tokens after 3000, capped, fp32 151 -> 108; 64-wide, 3 x 400 after 3000, 159 ->
-// 119), but not where a window leaves few keys to share among the waves (20, 25).
+// of 128 rows a CU leaves idle between its waves' products: half again as many places (2
+// x 300 tokens after 3000, capped, fp32 151 -> 108; 64-wide, 3 x 900 after 2000, fp32
+// 135 -> 107, fp16 84 -> 75, behind a window of 1024 59 -> 53 and 38 -> 37; 3 x 500 31 ->
+// 28; 1.7 times the places 6 x 777 38, 39), but not where there are few keys to share
+// among the waves (2 x 1488 behind a window of 256 20, 24, behind 512 23, 25; 14 x 35
+// tokens over as many keys 14, 20).
 // Beyond that 128 rows, since the four waves of the other kernel read every K and
 // V tile for themselves: 2 x 400 tokens 27 us, 30 with 32 rows; 16 x 256 tokens
 // 49, 81.  Sequences of 64 rows and less would leave half of such a tile empty:
@@ -65,7 +68,7 @@ inline Launch plan(const ane_paged_cache* c, uint32_t units, uint64_t tokens, bo
     // of equally long sequences
     auto wgs = [&](uint64_t bm) { return (rows + units * bm - 1) / (units * bm) * units * c->n_kv_heads; };
     const uint64_t room = 512 * 128 / c->head_dim;
-    l.few = single || wgs(32) <= (units == 1 ? room + room / 2 : bent ? room + room / 4 : room) || wgs(32) < 3 * wgs(128);
+    l.few = single || wgs(32) <= (units == 1 || bent ? room + room / 2 : room) || wgs(32) < 3 * wgs(128);
     const uint64_t bm = l.few ? 32 : 128;
     l.slots = single ? units * ((G + bm - 1) / bm) : rows / bm + units;
     const uint64_t places = beside && c->head_dim == 128 ? 256 : 512;
