@@ -452,7 +452,7 @@ def test_plans():
     rows, few, t64, t128d, t128, t256 = range(6)
     for T, N, K, may, want in ((4, 4096, 14336, True, (rows, 1)), (8, 4096, 14336, True, (t64, 4)), (5, 4096, 8192, False, (rows, 1)),
                                (1, 99, 70000, False, (few, 1)), (16, 4096, 4096, True, (few, 1)), (16, 6144, 4096, True, (t64, 2)), (32, 512, 14336, True, (t64, 8)),
-                               (32, 2003, 1777, True, (few, 1)), (100, 39, 7203, True, (t64, 7)), (1400, 6784, 896, True, (t256, 1)), (32, 4096, 4096, True, (t64, 4)), (32, 4096, 14336, True, (t64, 4)),
+                               (32, 2003, 1777, True, (few, 1)), (100, 39, 7203, True, (t64, 7)), (1400, 6784, 896, True, (t256, 1)), (1879, 19392, 384, True, (t128, 1)), (32, 4096, 4096, True, (t64, 4)), (32, 4096, 14336, True, (t64, 4)),
                                (32, 4096, 14336, False, (few, 1)), (64, 28672, 4096, True, (t64, 1)),
                                (192, 4096, 14336, True, (t128d, 4)), (512, 4096, 14336, True, (t128d, 2)),
                                (512, 4096, 14336, False, (t64, 1)), (16, 65536, 4096, True, (t64, 1)),
