@@ -237,9 +237,10 @@ int launch_gemm_rows(const GemmParams& p, hipStream_t s) { return launch_gemm<kB
 //   28672 x 4096 27.2, 29.3; 8 x 4096 x 14336 (112 KB) 20.2, in 64-tiles 19.0.
 // - 256-tiles from 3n/4 of them or where 128-tiles would not all have a place (2n):
 //   384 x 28672 x 4096 67, in 128-tiles 71; 2048 x 6144 x 4096 60, 70; 1400 x 6784 x 896
-//   (162, 583 128-tiles) 19, 28; 2048 x 4096 x 4096 (128, 512) 45, 38.  Not up to 3n of
+//   (162, 583 128-tiles) 19, 28; 2048 x 4096 x 4096 (128, 512) 45, 38.  Not n to 3n of
 //   them over at most three steps of K, which two tiles a CU cover for each other: 1879
-//   x 19392 x 384 (608) 43, in 128-tiles 37; 7524 x 11024 x 187 (1320) 69, 81.
+//   x 19392 x 384 (608) 43, in 128-tiles 37; 1995 x 6144 x 384 (192) 16, 18; 7524 x 11024
+//   x 187 (1320) 69, 81.
 // - above n/2 128-tiles, on the deep ring up to n: 512 x 6144 x 4096 22.5, in 64-tiles
 //   31; 768 x 6144 x 4096 (288 tiles, two a CU) 35, on the deep ring 40.
 // - with K of 64 steps and more, and 3n/16 128-tiles, in 128-tiles with K split: 512 x
@@ -258,7 +259,7 @@ ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split) {
     const uint64_t kb = ((uint64_t)K + 1023) / 1024;  // a token's room in LDS
     if (T <= 8 && (T > 4 ? 8 : T > 2 ? 4 : T) * kb <= 64) return {kScaledRows, 1};
     if (T > 64) {
-        const bool brief = nk <= 3 && tiles(256) < 3 * n;
+        const bool brief = nk <= 3 && tiles(256) > n && tiles(256) < 3 * n;
         if (T > 128 && !brief && (tiles(256) * 4 >= n * 3 || t128 > 2 * n)) return {kScaled256, 1};
         if (t128 * 2 > n) return {t128 <= n ? kScaled128d : kScaled128, 1};
         if (may_split && nk >= 64 && t128 * 16 >= n * 3) return {kScaled128d, (uint32_t)(n / t128)};

@@ -1349,16 +1349,18 @@ bool bad_workspace(const void* ws, size_t bytes, size_t need) {
 
 using namespace ane;
 
-// A bound on the keys that a row tile's rows see under a rule: with a window, and
-// nothing seen past a token's own position, no more than window and tile.
-static uint64_t rule_len(const ane_paged_cache* c, const ane_attention_rule* r, uint32_t max_len) {
+// A bound on the keys from the first to the last that a row tile's rows see under a
+// rule: with a window no more than window and tile, and what a prefix lets a token see
+// past its own position, which is a new token's.
+static uint64_t rule_len(const ane_paged_cache* c, const ane_attention_rule* r, uint32_t n_tokens, bool single, uint32_t max_len) {
     const uint64_t len = bound_len(c, max_len);
-    return r && r->window && !r->prefix ? std::min<uint64_t>(len, (uint64_t)r->window + 32 + 16) : len;
+    if (!r || !r->window) return len;
+    return std::min<uint64_t>(len, (uint64_t)r->window + 32 + 16 + (r->prefix && !single ? n_tokens : 0));
 }
 
 static Launch prompt_plan(const ane_paged_cache* c, const ane_attention_rule* r, uint32_t n, uint32_t n_tokens, bool single,
                           uint32_t max_len) {
-    const uint64_t len = rule_len(c, r, max_len);
+    const uint64_t len = rule_len(c, r, n_tokens, single, max_len);
     const bool windowed = r && r->window && r->window < bound_len(c, max_len);
     Launch l = plan(c, n, n_tokens, single, len, false, r && len > (windowed ? 1024 : 256), windowed);
     l.each = r && single && each_pays(c, l, len);

@@ -78,7 +78,10 @@ def test_workspace():
     plain = ane_amd.lib().ane_hip_attention_prompt_workspace_size(ctypes.byref(c), 1, 1, 8192)
     assert f(ctypes.byref(c), 1, 1, 8192, none) == plain > 0
     assert f(ctypes.byref(c), 1, 1, 8192, ctypes.byref(raw_rule(window=64))) < plain
-    assert f(ctypes.byref(c), 1, 1, 8192, ctypes.byref(raw_rule(window=64, prefix=P))) == plain
+    both = raw_rule(window=64, prefix=P)  # a window's keys, and what may lie ahead of a chunk's first token
+    assert f(ctypes.byref(c), 1, 1, 8192, ctypes.byref(both)) < plain
+    many = ane_amd.lib().ane_hip_attention_prompt_workspace_size(ctypes.byref(c), 1, 4000, 4040)
+    assert f(ctypes.byref(c), 1, 4000, 4040, ctypes.byref(both)) == many
     assert call(c=c, n=1, qs=None, T=1, ml=8192, wsb=plain - 1) == WORKSPACE
     assert call(c=c, n=1, qs=None, T=1, ml=8192, ws=None) == WORKSPACE
 
@@ -229,6 +232,18 @@ def test_single_tokens(ane, ty, hd, name, lens):
     run(c, [1] * len(lens), ty, single=True, max_len=max(lens), **r)
     if len(lens) == 5:
         run(c, [1] * 3, ty, single=True, seqs=[4, 1, 3], **r)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty,hd", [("f32", 128), ("f16", 64)])
+def test_prefix_ahead_of_a_window(ane, ty, hd):
+    """Chunks far into a sequence whose prefix ends behind them, inside them, before them: keys in parts by the window."""
+    new, old = [45, 300, 7, 90], [4744, 900, 3000, 0]
+    c = make_cache([a + b for a, b in zip(new, old)], 4, 2, hd, 32, seed=4)
+    for prefix in ([4789, 1200, 3003, 90], [4750, 1000, 10, 45], [120, 950, 3010, 1]):
+        for window in (953, 60, 3000):
+            run(c, new, ty, prefix=prefix, window=window, cap=30.0)
+    run(c, [1] * 4, ty, single=True, prefix=[4789, 5, 3007, 90], window=953)
 
 
 @pytest.mark.gpu
