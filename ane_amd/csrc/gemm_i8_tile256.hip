@@ -268,28 +268,30 @@ __device__ __forceinline__ void store16_sc1(uint32_t* dst, v4i v) {
     asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 0" ::"v"(dst), "v"(v) : "memory");
 }
 
-// Four outputs of the scaled epilogue (sc_put), at element `at` of C and `ar`
-// of the residual.
-__device__ __forceinline__ void sc_put4(const GemmParams& p, uint64_t at, uint64_t ar, v4i v) {
-    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+// Four values of the residual at element `at` as they stand (scaled epilogue), and four
+// outputs with them added.
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ v4i sc_residual4(const GemmParams& p, uint64_t at) {
+    if (!p.half) return *reinterpret_cast<const v4i*>(static_cast<const float*>(p.res) + at);
+    const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const _Float16*>(p.res) + at);
+    return v4i{(int)r.x, (int)r.y, 0, 0};
+}
+__device__ __forceinline__ void sc_put4(const GemmParams& p, uint64_t at, v4i v, v4i r) {
     if (p.half) {
-        h4 o;
         if (p.res) {
-            const h4 r = *reinterpret_cast<const h4*>(static_cast<const _Float16*>(p.res) + ar);
+            const h4 x = __builtin_bit_cast(h4, make_uint2((uint32_t)r[0], (uint32_t)r[1]));
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = __float_as_int(__fadd_rn(__int_as_float(v[e]), (float)r[e]));
+            for (int e = 0; e < 4; e++) v[e] = __float_as_int(__fadd_rn(__int_as_float(v[e]), (float)x[e]));
         }
+        h4 o;
 #pragma unroll
         for (int e = 0; e < 4; e++) o[e] = (_Float16)__int_as_float(v[e]);
         *reinterpret_cast<h4*>(reinterpret_cast<_Float16*>(p.C) + at) = o;
         return;
     }
     if (p.res) {
-        const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(p.res) + ar);
-        v[0] = __float_as_int(__fadd_rn(__int_as_float(v[0]), r.x));
-        v[1] = __float_as_int(__fadd_rn(__int_as_float(v[1]), r.y));
-        v[2] = __float_as_int(__fadd_rn(__int_as_float(v[2]), r.z));
-        v[3] = __float_as_int(__fadd_rn(__int_as_float(v[3]), r.w));
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = __float_as_int(__fadd_rn(__int_as_float(v[e]), __int_as_float(r[e])));
     }
     store16_sc1(reinterpret_cast<uint32_t*>(p.C) + at, v);
 }
@@ -547,10 +549,28 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
                         : SC ? ((((uintptr_t)p.C) | ((uintptr_t)p.res)) & 15) == 0 && ((p.ldc | p.ldr) & 3) == 0
                              : (((uintptr_t)(craw ? (void*)craw : (void*)p.C)) & 15) == 0 && (p.ldc & 3) == 0;
 
+    constexpr int kQ = EPR / kRowsPerStore, kPasses = FM * 32 / EPR;
+    // SC: the residual of the next pass on its way while this one is stored, its loads
+    // all at once (each just before its store, as C may be the residual: 4096 x 28672 x
+    // 1024 fp16 291 us, 250 so, 6000 x 6784 x 896 fp32 129, 105; 4096^3 fp32 74, 76)
+    const bool ahead = SC && p.res && vec_ok && p.Nout >= 4;  // uniform
+    v4i res[2][SC ? kQ : 1];
+    auto fetch = [&](int pass, int to) {
+#pragma unroll
+        for (int q = 0; q < kQ; q++) {
+            const uint32_t i = row0 + wr0 + pass * EPR + kRowsPerStore * q + lane / kLanesPerRow;
+            const uint32_t i1 = i < p.Mout ? i : p.Mout - 1, j1 = j4 + 3 < p.Nout ? j4 : (p.Nout - 4) & ~3u;
+            res[SC ? to : 0][SC ? q : 0] = sc_residual4(p, (uint64_t)i1 * p.ldr + j1);
+        }
+    };
+    if constexpr (SC) {
+        if (ahead) fetch(0, 0);
+    }
 #pragma unroll
     for (int mi = 0; mi < FM; mi++) {
 #pragma unroll
         for (int h = 0; h < 32 / EPR; h++) {
+            const int pass = mi * (32 / EPR) + h;
             // rows [h*EPR, (h+1)*EPR) of the 32-row block mi -> LDS.  Lane l,
             // register r of a 32x32 MFMA block holds row 8(r/4) + 4(l/32) +
             // r%4, column l%32.
@@ -581,7 +601,6 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
                 }
             }
             // SPLIT: the other workgroups' sums, four of them in flight at a time
-            constexpr int kQ = EPR / kRowsPerStore;
             v4i others[SPLIT ? kQ : 1];
             if constexpr (SPLIT) {
 #pragma unroll
@@ -610,12 +629,25 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
             }
             wait_lgkmcnt0();
             __builtin_amdgcn_wave_barrier();
+            if constexpr (SC) {
+                if (ahead && pass + 1 < kPasses) {
+                    fetch(pass + 1, (pass + 1) & 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            v4i staged[SC ? kQ : 1];  // SC: read before this pass's residual is waited for
+            if constexpr (SC) {
+#pragma unroll
+                for (int q = 0; q < kQ; q++)
+                    staged[q] = *reinterpret_cast<const v4i*>(epi + (kRowsPerStore * q + lane / kLanesPerRow) * kEpiRowBytes + lc4 * 4);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             // 16 B per lane: kLanesPerRow lanes cover one staged row
 #pragma unroll
             for (int q = 0; q < EPR / kRowsPerStore; q++) {
                 const uint32_t lr = kRowsPerStore * q + lane / kLanesPerRow;
                 const uint32_t lc = 4 * (lane % kLanesPerRow);
-                v4i v = *reinterpret_cast<const v4i*>(epi + lr * kEpiRowBytes + lc * 4);
+                v4i v = SC ? staged[SC ? q : 0] : *reinterpret_cast<const v4i*>(epi + lr * kEpiRowBytes + lc * 4);
                 const uint32_t i = row0 + wr0 + mi * 32 + h * EPR + lr;
                 const uint32_t j = col0 + wc0 + lc;
                 if (i >= p.Mout) continue;
@@ -627,7 +659,7 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
                 }
                 if constexpr (SC) {
                     if (vec_ok && j + 3 < p.Nout) {
-                        sc_put4(p, (uint64_t)i * p.ldc + j, (uint64_t)i * p.ldr + j, v);
+                        sc_put4(p, (uint64_t)i * p.ldc + j, v, res[pass & 1][q]);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
