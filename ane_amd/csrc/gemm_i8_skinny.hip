@@ -35,6 +35,22 @@
 namespace ane {
 namespace {
 
+// The residual of one output as it stands (0 without), and the output stored with it.
+__device__ __forceinline__ uint32_t residual_bits(const GemmParams& p, uint32_t i, uint32_t j) {
+    if (!p.res) return 0;
+    const uint64_t at = i * p.ldr + j;
+    return p.half ? static_cast<const uint16_t*>(p.res)[at] : static_cast<const uint32_t*>(p.res)[at];
+}
+__device__ __forceinline__ void put(const GemmParams& p, uint32_t i, uint32_t j, float f, uint32_t res) {
+    const uint64_t at = i * p.ldc + j;
+    if (p.half) {
+        if (p.res) f = __fadd_rn(f, (float)__builtin_bit_cast(_Float16, (uint16_t)res));
+        reinterpret_cast<_Float16*>(p.C)[at] = (_Float16)f;
+    } else {
+        p.C[at] = p.res ? __fadd_rn(f, __uint_as_float(res)) : f;
+    }
+}
+
 // PANEL: B in the SMOPA panels of dense_i8 / dense_u8s8, workgroup = panel: a
 // lane's 16 bytes of column n0 + l%16 are dword l%16 of four consecutive
 // 64-byte groups.  AU8: uint8 A enters as a - 128 and 128 * (column sum of B)
@@ -99,6 +115,23 @@ __global__ void __launch_bounds__(256) k_gemm_skinny(GemmParams p) {
         }
     };
 
+    // SC: what this wave's outputs are scaled by and added to, on its way during the steps
+    // (20 x 1024 x 1024 with a residual 7.8 -> 7.1 us with its quantizer)
+    constexpr int kOut = SC ? (MB + 3) / 4 : 1;
+    float scr[kOut][4], scc = 0.0f, scb = 0.0f;
+    uint32_t scx[kOut][4];
+    if constexpr (SC) {
+        const uint32_t jc = n0 + c16 < p.Nout ? n0 + c16 : p.Nout - 1;
+        scc = p.cs[jc], scb = p.bias ? p.bias[jc] : 0.0f;
+#pragma unroll
+        for (int o = 0; o < kOut; o++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t row = min(m0 + 16 * (wave + 4 * o) + 4 * g + i, p.Mout - 1);
+                scr[o][i] = p.rs[row], scx[o][i] = residual_bits(p, row, jc);
+            }
+    }
+
     v4i acc[MB];
 #pragma unroll
     for (int r = 0; r < MB; r++) acc[r] = v4i{0, 0, 0, 0};
@@ -126,10 +159,12 @@ __global__ void __launch_bounds__(256) k_gemm_skinny(GemmParams p) {
     float s = p.s;
     if (p.sdev) s = __fmul_rn(__fmul_rn(p.sdev[0], p.sdev[1]), p.smul);
     const uint32_t j = n0 + c16;
-    const float bj = (p.bias && j < p.Nout) ? p.bias[j] : 0.0f;
-    const float cj = SC && j < p.Nout ? p.cs[j] : 0.0f;
+    const float bj = (!SC && p.bias && j < p.Nout) ? p.bias[j] : 0.0f;
     const uint32_t igc = p.ig ? ig_sum(p.igc, p.nsum, p.Nout, j) : 0u;
-    for (uint32_t r = wave; r < (uint32_t)MB; r += 4) {
+#pragma unroll
+    for (int o = 0; o < (MB + 3) / 4; o++) {
+        const uint32_t r = wave + 4 * o;
+        if (r >= (uint32_t)MB) break;
         v4i t = red[0][r][lane] + red[1][r][lane] + red[2][r][lane] + red[3][r][lane];
         if (AU8)
 #pragma unroll
@@ -139,7 +174,7 @@ __global__ void __launch_bounds__(256) k_gemm_skinny(GemmParams p) {
             const uint32_t row = m0 + 16 * r + 4 * g + i;
             if (row >= p.Mout || j >= p.Nout) continue;
             if (SC) {
-                sc_put(p, row, j, sc_out(t[i], p.rs[row], cj, bj));
+                put(p, row, j, sc_out(t[i], scr[SC ? o : 0][i], scc, scb), scx[SC ? o : 0][i]);
             } else if (p.Craw) {
                 p.Craw[(uint64_t)row * p.ldc + j] = t[i];
             } else if (p.ig) {
