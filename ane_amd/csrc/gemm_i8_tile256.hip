@@ -284,7 +284,12 @@ __device__ __forceinline__ v4i sc_residual4(const GemmParams& p, uint64_t at) {
     const uint64_t r = reinterpret_cast<const Halves4*>(static_cast<const _Float16*>(p.res) + at)->v;
     return v4i{(int)(uint32_t)r, (int)(uint32_t)(r >> 32), 0, 0};
 }
-__device__ __forceinline__ void sc_put4(const GemmParams& p, uint64_t at, v4i v, v4i r) {
+// fp16 is stored past the caches (nt), and fp32 where `past`: they then keep the operands
+// that other tiles read again (4096 x 28672 x 4096 fp16 460 -> 405 us; fp32 495 -> 448, but
+// 4096^3 64 -> 66 and 2000 x 6785 x 1000 24 -> 30) and the residual (1879 x 19392 x 384
+// fp32 73 -> 57).
+__device__ __forceinline__ bool sc_past(const GemmParams& p) { return p.res || (uint64_t)p.Mout * p.Nout >= 1u << 25; }
+__device__ __forceinline__ void sc_put4(const GemmParams& p, uint64_t at, v4i v, v4i r, bool past) {
     if (p.half) {
         if (p.res) {
             const h4 x = __builtin_bit_cast(h4, make_uint2((uint32_t)r[0], (uint32_t)r[1]));
@@ -294,14 +299,15 @@ __device__ __forceinline__ void sc_put4(const GemmParams& p, uint64_t at, v4i v,
         h4 o;
 #pragma unroll
         for (int e = 0; e < 4; e++) o[e] = (_Float16)__int_as_float(v[e]);
-        reinterpret_cast<Halves4*>(reinterpret_cast<_Float16*>(p.C) + at)->v = __builtin_bit_cast(uint64_t, o);
+        __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, o), &reinterpret_cast<Halves4*>(reinterpret_cast<_Float16*>(p.C) + at)->v);
         return;
     }
     if (p.res) {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = __float_as_int(__fadd_rn(__int_as_float(v[e]), __int_as_float(r[e])));
     }
-    store16_sc1(reinterpret_cast<uint32_t*>(p.C) + at, v);
+    if (past) __builtin_nontemporal_store(v, &reinterpret_cast<Floats4*>(p.C + at)->v);
+    else store16_sc1(reinterpret_cast<uint32_t*>(p.C) + at, v);
 }
 
 #if ANE_TILE_PANEL
@@ -559,7 +565,7 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
     // SC: the residual of the next pass on its way while this one is stored, its loads
     // all at once (each just before its store, as C may be the residual: 4096 x 28672 x
     // 1024 fp16 291 us, 250 so, 6000 x 6784 x 896 fp32 129, 105; 4096^3 fp32 74, 76)
-    const bool ahead = SC && p.res && p.Nout >= 4;  // uniform
+    const bool ahead = SC && p.res && p.Nout >= 4, past = SC && sc_past(p);  // uniform
     v4i res[2][SC ? kQ : 1];
     auto fetch = [&](int pass, int to) {
 #pragma unroll
@@ -665,7 +671,7 @@ ANE_TILE_KERNEL(GemmParams p, uint32_t tiles_m, uint32_t tiles_n) {
                 }
                 if constexpr (SC) {
                     if (j + 3 < p.Nout) {
-                        sc_put4(p, (uint64_t)i * p.ldc + j, v, res[pass & 1][q]);
+                        sc_put4(p, (uint64_t)i * p.ldc + j, v, res[pass & 1][q], past);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
