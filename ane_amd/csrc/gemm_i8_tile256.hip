@@ -285,9 +285,10 @@ __device__ __forceinline__ v4i sc_residual4(const GemmParams& p, uint64_t at) {
     return v4i{(int)(uint32_t)r, (int)(uint32_t)(r >> 32), 0, 0};
 }
 // fp16 is stored past the caches (nt), and fp32 where `past`: they then keep the operands
-// that other tiles read again (4096 x 28672 x 4096 fp16 460 -> 405 us; fp32 495 -> 448, but
-// 4096^3 64 -> 66 and 2000 x 6785 x 1000 24 -> 30) and the residual (1879 x 19392 x 384
-// fp32 73 -> 57).
+// that other tiles read again (calls one after the other on the same weights: 4096 x 28672
+// x 4096 fp16 460 -> 405 us; fp32 495 -> 448, but 4096^3 64 -> 66 and 2000 x 6785 x 1000
+// 24 -> 30; on weights from memory 455 -> 450) and the residual (1879 x 19392 x 384 fp32
+// 73 -> 57).
 __device__ __forceinline__ bool sc_past(const GemmParams& p) { return p.res || (uint64_t)p.Mout * p.Nout >= 1u << 25; }
 __device__ __forceinline__ void sc_put4(const GemmParams& p, uint64_t at, v4i v, v4i r, bool past) {
     if (p.half) {
