@@ -246,12 +246,13 @@ int launch_gemm_rows(const GemmParams& p, hipStream_t s) { return launch_gemm<kB
 // - with K of 64 steps and more, and 3n/16 128-tiles, in 128-tiles with K split: 512 x
 //   4096 x 14336 47 in two parts, in 64-tiles 61; 192 x 4096 x 14336 30 in four, 36.
 // - the others in 64-tiles with K in as many parts as fill the CUs, at most 8, of 8
-//   steps at least: 64 x 4096 x 4096 8.3 in four, 10.6 whole; 32 x 4096 x 14336 15, 33;
-//   32 x 512 x 14336 9.1 in eight, 11.2 in four; 64 x 2003 x 1792 7.5 in three, 7.4 whole.
+//   steps at least, where that costs less than K whole by the fits below (in 10 ns): 64 x
+//   4096 x 4096 8.3 in four, 10.6 whole; 32 x 4096 x 14336 15, 32; 32 x 512 x 14336 9.6 in
+//   eight, 11.5 in four; 358 x 209 x 2007 9.0 in two, 8.1 whole.
 // - up to 64 tokens the few-row kernel instead, which reads x again for every 16
-//   columns, where that costs less by the fits below (in 10 ns): 16 x 4096 x 4096 7.1,
-//   in 64-tiles 7.3; 32 x 4096 x 4096 9.2, 7.8; 16 x 512 x 14336 16.4, 8.5; 32 x 1024 x
-//   1024 4.1, 4.8; 32 x 4096 x 14336 26, in whole 64-tiles 33.
+//   columns, where that costs less: 16 x 4096 x 4096 6.3, in 64-tiles 7.8; 32 x 4096 x 4096
+//   8.1, 7.8; 16 x 512 x 14336 15.3, 9.0; 32 x 1024 x 1024 3.1, 4.5; 12 x 445 x 232 1.7, 2.9;
+//   32 x 4096 x 14336 25, in whole 64-tiles 32.
 ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split) {
     const uint64_t n = tile256_min_tiles(), nk = ((uint64_t)K + 127) / 128;
     auto tiles = [&](uint64_t b) { return (T + b - 1) / b * ((N + b - 1) / b); };
@@ -268,11 +269,12 @@ ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split) {
     if (split > 8) split = 8;
     if (split > nk / 8) split = nk / 8;
     if (split < 1) split = 1;
+    auto tile = [&](uint64_t s) { return 280 + (nk + s - 1) / s * 26 * ((t64 * s + n - 1) / n) + (s > 1 ? 300 : 0); };
+    if (tile(1) <= tile(split)) split = 1;
     if (T <= 64) {
         const uint64_t groups = (N + 15ull) / 16;
-        const uint64_t few = 250 + (nk + 3) / 4 * (17 + 32 * ((T + 15) / 16)) * ((groups + n - 1) / n);
-        const uint64_t tile = 220 + (nk + split - 1) / split * 30 * ((t64 * split + n - 1) / n) + (split > 1 ? 220 : 0);
-        if (few <= tile) return {kScaledFew, 1};
+        const uint64_t few = 140 + (nk + 3) / 4 * (29 + 28 * ((T + 15) / 16)) * ((groups + n - 1) / n);
+        if (few <= tile(split)) return {kScaledFew, 1};
     }
     return {kScaled64, (uint32_t)split};
 }
