@@ -1527,7 +1527,7 @@ def linear_i8_workspace_size(T, N, K) -> int:
 
 
 def linear_i8_workspace(T, N, K, device="cuda"):
-    """A workspace for linear_i8 calls of these sizes, for callers that keep one."""
+    """A workspace for linear_i8 calls of up to T tokens through weights [N][K], for callers that keep one."""
     return _scratch(linear_i8_workspace_size(T, N, K), device)
 
 

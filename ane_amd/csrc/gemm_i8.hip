@@ -17,6 +17,7 @@
 // the kernel of gemm_i8_skinny.hip, both also on SMOPA panels.
 #include "gemm_i8.hpp"
 
+#include <algorithm>
 #include <atomic>
 #include <vector>
 
@@ -266,7 +267,7 @@ ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split) {
         if (may_split && nk >= 64 && t128 * 16 >= n * 3) return {kScaled128d, (uint32_t)(n / t128)};
     }
     uint64_t split = may_split ? n / t64 : 1;
-    if (split > 8) split = 8;
+    if (split > kScaledMaxSplit) split = kScaledMaxSplit;
     if (split > nk / 8) split = nk / 8;
     if (split < 1) split = 1;
     auto tile = [&](uint64_t s) { return 280 + (nk + s - 1) / s * 26 * ((t64 * s + n - 1) / n) + (s > 1 ? 300 : 0); };
@@ -277,6 +278,23 @@ ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split) {
         if (few <= tile(split)) return {kScaledFew, 1};
     }
     return {kScaled64, (uint32_t)split};
+}
+
+// Parts times tiles are at most the CUs, so s parts mean at most CUs / (s * columns of
+// tiles) rows of tiles.
+uint64_t scaled_split_rows(uint32_t T, uint32_t N, uint32_t K) {
+    const uint64_t n = tile256_min_tiles(), nk = ((uint64_t)K + 127) / 128;
+    if (scaled_plan(T, N, K, true).kernel == kScaledRows) return 0;  // as for all fewer tokens
+    uint64_t rows = 0;
+    auto most = [&](uint64_t b, uint64_t parts) {
+        for (uint64_t s = 2; s <= parts; s++) {
+            const uint64_t r = n / (s * ((N + b - 1) / b)) * b;
+            rows = std::max(rows, s * std::min<uint64_t>(T, r));
+        }
+    };
+    most(64, std::min<uint64_t>(kScaledMaxSplit, nk / 8));
+    if (T > 64 && nk >= 64) most(128, 16 / 3);  // (from 3n/16 tiles on)
+    return rows;
 }
 
 int launch_gemm_scaled(const GemmParams& p, ScaledPlan plan, hipStream_t s) {

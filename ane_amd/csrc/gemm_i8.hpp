@@ -95,8 +95,10 @@ struct ScaledPlan {
     ScaledKernel kernel;
     uint32_t split;
 };
-constexpr uint32_t kScaledCounts = 256;
+constexpr uint32_t kScaledCounts = 256, kScaledMaxSplit = 8;
 ScaledPlan scaled_plan(uint32_t T, uint32_t N, uint32_t K, bool may_split);
+// A bound on split * tokens over all batches of at most T tokens whose K is split.
+uint64_t scaled_split_rows(uint32_t T, uint32_t N, uint32_t K);
 int launch_gemm_scaled(const GemmParams& p, ScaledPlan plan, hipStream_t s);
 // kScaledRows: at most eight tokens, over whole rows of Bt (linear_i8.hip).
 bool gemm_dot_eligible(const GemmParams& p);

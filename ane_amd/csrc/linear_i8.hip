@@ -438,13 +438,14 @@ struct LinearSpace {
     ScaledPlan plan;
     uint64_t scales, counts, planes, bytes;
 };
+uint64_t plane_bytes(uint64_t rows, uint32_t N) { return rows * ceil_to(N, 4) * 4; }  // of sums, over all parts
 LinearSpace linear_space(uint32_t T, uint32_t N, uint32_t K) {
     LinearSpace l;
     l.plan = scaled_plan(T, N, K, true);
     l.scales = q_bytes(T, K);
     l.counts = l.scales + ceil_to((uint64_t)T * 4, 256);
     l.planes = l.counts + (l.plan.split > 1 ? kScaledCounts * 4 : 0);
-    l.bytes = l.planes + (l.plan.split > 1 ? (uint64_t)l.plan.split * T * ceil_to(N, 4) * 4 : 0);
+    l.bytes = l.planes + (l.plan.split > 1 ? plane_bytes((uint64_t)l.plan.split * T, N) : 0);
     return l;
 }
 
@@ -502,7 +503,9 @@ extern "C" int ane_hip_dense_i8_scaled(uint32_t T, uint32_t N, uint32_t K, const
 
 extern "C" size_t ane_hip_linear_i8_workspace_size(uint32_t T, uint32_t N, uint32_t K) {
     if (T == 0 || T > kMaxRows || N == 0 || N > kMaxRows || K == 0 || K > kMaxK) return 0;
-    return linear_space(T, N, K).bytes;
+    const LinearSpace l = linear_space(T, N, K);
+    const uint64_t rows = scaled_split_rows(T, N, K);  // (a call of fewer tokens may split K where this one does not)
+    return std::max(l.bytes, rows ? l.counts + kScaledCounts * 4 + plane_bytes(rows, N) : 0);
 }
 
 extern "C" int ane_hip_linear_i8(uint32_t T, uint32_t N, uint32_t K, int type, const void* x, uint64_t x_stride,

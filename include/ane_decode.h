@@ -415,8 +415,9 @@ int ane_hip_pages_compact(const struct ane_paged_cache* cache, uint32_t* page_ta
  * + bias[n] + residual[t][n], one rounding a step, the sum exact; bias (fp32 [N])
  * and residual (out's type; may be out itself with its stride) may be NULL.
  * linear_i8: both, q and scales in the workspace (256-byte aligned; it belongs to
- * the call until it has run).  The same bits as the two calls.  out may lie in x,
- * otherwise outputs share no memory with what is read. */
+ * the call until it has run).  The size for T tokens is enough for fewer of them as
+ * well.  The same bits as the two calls.  out may lie in x, otherwise outputs share
+ * no memory with what is read. */
 int ane_hip_quantize_tokens(uint32_t T, uint32_t K, int type, const void* x, uint64_t x_stride, const float* norm_w,
                             float eps, int8_t* q, uint64_t q_stride, float* scales, void* stream);
 int ane_hip_dense_i8_scaled(uint32_t T, uint32_t N, uint32_t K, const int8_t* q, uint64_t q_stride,

@@ -464,3 +464,43 @@ def test_plans():
         split = f(T, N, K, True).split
         need = T * (-(-K // 128) * 128) + 4 * T + 1024 + split * T * (-(-N // 4) * 4) * 4
         assert split > 1 and need <= ane_amd.lib().ane_hip_linear_i8_workspace_size(T, N, K) <= need + 1024
+
+
+def test_a_workspace_covers_fewer_tokens():
+    """The size for T tokens is enough for every call of fewer, also where only those split K."""
+    import ctypes
+
+    class Plan(ctypes.Structure):
+        _fields_ = [("kernel", ctypes.c_int), ("split", ctypes.c_uint32)]
+
+    plan = ane_amd.lib()._FuncPtr(("_ZN3ane11scaled_planEjjjb", ane_amd.lib()))
+    plan.restype, plan.argtypes = Plan, [ctypes.c_uint32] * 3 + [ctypes.c_bool]
+    size = ane_amd.lib().ane_hip_linear_i8_workspace_size
+
+    def up(x, m):
+        return -(-x // m) * m
+
+    for N, K in ((6144, 4096), (4096, 4096), (4096, 14336), (28672, 4096), (64, 14336), (39, 7203), (700, 2048), (1, 131071),
+                 (2100, 96)):
+        most = 0
+        for T in [*range(1, 1200), *range(1200, 17000, 61), 100_000]:
+            split = plan(T, N, K, True).split
+            need = up(T * up(K, 128), 256) + up(4 * T, 256) + (1024 + split * T * up(N, 4) * 4 if split > 1 else 0)
+            most = max(most, need)
+            assert size(T, N, K) >= most, (T, N, K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,most", [(6144, 4096, 65), (4096, 4096, 129), (512, 14336, 700)])
+def test_one_workspace_for_batches_of_every_size(ane, N, K, most):
+    """A workspace of the largest batch's size through smaller ones, which split K, and back."""
+    import torch
+
+    work = ane.linear_i8_workspace(most, N, K)
+    x, w, ws, norm, _, res = inputs(most, N, K, seed=14)
+    X, W, S, nw, R = dev(x), rows16(w), dev(ws), dev(norm), dev(res)
+    want = product(*quantized(x, norm), w, ws, None, res)
+    for T in (most, 64, 32, 16, 9, 8, 1, 33, most):
+        out = torch.full((T, N), float("nan"), device="cuda")
+        ane.linear_i8(X[:T], W, S, out, norm_w=nw, residual=R[:T], workspace=work)
+        same(out.cpu().numpy(), want[:T])
