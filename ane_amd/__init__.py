@@ -1258,8 +1258,9 @@ def _attention_rows(cache, q, out):
 class AttentionRule(ctypes.Structure):
     """Mirror of struct ane_attention_rule (include/ane_decode.h), over device tensors that it keeps alive: scores capped
     at softcap by a tanh (0: not), lowered by slopes (float32 [heads]) times the distance, keys window and more positions
-    back not seen (0: all), none before first (int32 [tokens]: where each new token's document begins), all below prefix
-    (int32 [rows of the batch]) seen from both sides.  A call reads the tensors when it runs."""
+    back not seen (0: all), none before first (int32 [tokens]: where each new token's document begins; a token with a
+    negative entry sees nothing), all below prefix (int32 [rows of the batch], none where it is 0 or negative) seen from
+    both sides.  A call reads the tensors when it runs."""
 
     _fields_ = [("softcap", ctypes.c_float), ("window", ctypes.c_uint32), ("slopes_ptr", ctypes.c_void_p),
                 ("first_ptr", ctypes.c_void_p), ("prefix_ptr", ctypes.c_void_p)]

@@ -153,9 +153,9 @@ __device__ __forceinline__ int32_t rule_first(const AttnArgs& a, const Work& w, 
     if (a.first) lo = max(lo, (int32_t)min(a.first[w.tok0 + t], 0x7fffffffu));
     return lo;
 }
-// The end of what they see, whatever the token.
+// The end of what they see, whatever the token (none below 1, a negative entry among them).
 __device__ __forceinline__ int32_t rule_seen(const AttnArgs& a, const Work& w) {
-    return a.seen ? (int32_t)min(a.seen[w.s], (uint32_t)w.len) : 0;
+    return a.seen ? min((int32_t)a.seen[w.s], w.len) : 0;
 }
 
 // The keys of part `part`.

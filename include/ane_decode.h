@@ -316,6 +316,8 @@ int ane_hip_attention_prompt(const struct ane_paged_cache* cache, uint32_t layer
  * A token that sees nothing gets zeros; a token at a negative position sees
  * nothing.  first is indexed by packed row, prefix by batch row; a prefix past
  * the length counts as the length, keys that no token of a tile sees are not read.
+ * An entry from 2^31 on, a negative one of an int32 array, opens nothing: its first
+ * lies behind every key (the token sees none), its prefix is none.
  * softcap: 0, or 2^-20 to 2^20.  Single tokens (q_start NULL) are the decode step.
  * Types, accuracy (of the score before the cap, in fp32) and everything else as
  * above; the workspace is that of the rule (with a window fewer keys are split). */

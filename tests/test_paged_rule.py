@@ -464,3 +464,34 @@ def test_rows_behind_the_last_sequence_stay(ane):
     out = torch.full_like(q, 5.0)
     ane.attention_prompt(c, 0, i32([2, 12, 40]), q, out, rule=AttentionRule(window=30))
     assert bool((out[:2] == 5).all()) and bool((out[40:] == 5).all()) and not bool((out[2:40] == 5).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty,hd", [("f32", 128), ("f16", 128), ("f32", 64), ("f16", 64)])
+def test_negative_prefixes_are_none(ane, ty, hd):
+    """-1 for a sequence without a prefix: no token sees past itself, in 32- and 128-row tiles, alone and in large batches."""
+    import torch
+
+    for new, old, heads, kv in (([40, 3, 9], [0, 300, 20], 8, 2), ([700, 420, 33], [0, 200, 1000], 32, 8)):
+        c = make_cache([a + b for a, b in zip(new, old)], heads, kv, hd, 16, seed=5)
+        q = randq(sum(new), heads, hd, dt(ty), seed=6)
+        for window in (0, 90):
+            outs = []
+            for prefix in ([-1, 200, -(1 << 31)], [0, 200, 0]):
+                out = torch.full_like(q, 5.0)
+                ane.attention_prompt(c, 0, i32([sum(new[:i]) for i in range(len(new) + 1)]), q, out,
+                                     rule=AttentionRule(30.0, window=window, prefix=i32(prefix)))
+                outs.append(out)
+            assert torch.equal(*outs)
+            at = 0
+            for i, (a, b) in enumerate(zip(new, old)):
+                check(c, 0, i, q[at:at + a], outs[0][at:at + a], list(range(b, a + b)), hd ** -0.5, 30.0, window=window,
+                      prefix=min([0, 200, 0][i], a + b))
+                at += a
+    for lens in ([1, 70, 900], [100] * 300):
+        c = make_cache(lens, 8, 4, hd, 16, seed=7)
+        q = randq(len(lens), 8, hd, dt(ty), seed=8)
+        outs = [torch.full_like(q, 5.0) for _ in range(2)]
+        for out, v in zip(outs, (-1, 0)):
+            ane.attention_prompt(c, 0, None, q, out, max_len=max(lens), rule=AttentionRule(30.0, prefix=i32([v] * len(lens))))
+        assert torch.equal(*outs)
