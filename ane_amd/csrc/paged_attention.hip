@@ -415,28 +415,34 @@ struct Rows {
             for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, fabsf(s[t][r])), fabsf(s[t][r + 1]));
-            if (__any(top * down > Tanh<F32>::kSmall) || (!F32 && a.bend[0] == 0.0f)) {
+            auto by_y = [&](float x) { return __builtin_fmaf(Tanh<F32>::small(x * down), x, x); };
+            auto as_is = [&](float x) {  // fp16: the factor is one for all rows
+                const float z = x * x;
+                const float p = __builtin_fmaf(__builtin_fmaf(a.bend[2], z, a.bend[1]), z, a.bend[0]);
+                return x * __builtin_fmaf(p, z, 1.0f);
+            };
+            auto all = [&](auto small) {
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[t][r] = small(s[t][r]);
+            };
+            // small scores as in a tile that has no others: which one it is hangs on keys
+            // that a row does not see, and must not change what the row gets
+            auto mixed = [&](auto small) {
                 const float up = __builtin_amdgcn_rcpf(down);
-#pragma unroll
-                for (int t = 0; t < KT; t++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const float y = s[t][r] * down, l = Tanh<F32>::large(y) * up;
-                        s[t][r] = fabsf(y) > Tanh<F32>::kSmall ? l : __builtin_fmaf(Tanh<F32>::small(y), s[t][r], s[t][r]);
-                    }
+                all([&](float x) {
+                    const float l = Tanh<F32>::large(x * down) * up;
+                    return fabsf(x * down) > Tanh<F32>::kSmall ? l : small(x);
+                });
+            };
+            const bool some = __any(top * down > Tanh<F32>::kSmall);
+            if constexpr (F32) {
+                some ? mixed(by_y) : all(by_y);
+            } else if (a.bend[0] == 0.0f) {
+                mixed(by_y);
             } else {
-#pragma unroll
-                for (int t = 0; t < KT; t++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        if constexpr (F32) {
-                            s[t][r] = __builtin_fmaf(Tanh<F32>::small(s[t][r] * down), s[t][r], s[t][r]);
-                        } else {  // (the factor is one for all rows)
-                            const float z = s[t][r] * s[t][r];
-                            const float p = __builtin_fmaf(__builtin_fmaf(a.bend[2], z, a.bend[1]), z, a.bend[0]);
-                            s[t][r] *= __builtin_fmaf(p, z, 1.0f);
-                        }
-                    }
+                some ? mixed(as_is) : all(as_is);
             }
         }
         if (!a.slopes) return;

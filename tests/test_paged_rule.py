@@ -495,3 +495,28 @@ def test_negative_prefixes_are_none(ane, ty, hd):
         for out, v in zip(outs, (-1, 0)):
             ane.attention_prompt(c, 0, None, q, out, max_len=max(lens), rule=AttentionRule(30.0, prefix=i32([v] * len(lens))))
         assert torch.equal(*outs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("heads,kv,n", [(4, 2, 90), (32, 8, 900)])
+def test_what_a_row_does_not_see_leaves_its_bits(ane, hd, heads, kv, n):
+    """fp16, a cap far above the scores: a key outside the window or document that no score of its tile compares to (finite
+    or not) chooses how the tile's tanh is formed, and changes no bit of a row that does not see it."""
+    import torch
+
+    for cap in (50.0, 20.0):
+        for kw in (dict(window=50), dict(first=[p // 40 * 40 for p in range(n)])):
+            c = make_cache([n], heads, kv, hd, 16, seed=n)
+            q, clean, rule = run(c, [n], "f16", cap=cap, **kw)
+            y = sees(list(range(n)), n, n, kw.get("window", 0), kw.get("first"), 0)
+            for at in (0, 17, n // 2, n // 2 + 21):
+                for bad in (math.inf, math.nan, 900.0):
+                    row = (0, int(c.page_table[0, at // 16]), slice(None), at % 16)
+                    keep = c.k_pages[row].clone()
+                    c.k_pages[row] = bad
+                    out = torch.full_like(q, 5.0)
+                    ane.attention_prompt(c, 0, i32([0, n]), q, out, rule=rule)
+                    c.k_pages[row] = keep
+                    blind = ~y[:, at]
+                    assert bool(blind.any()) and torch.equal(out[blind], clean[blind]), (cap, at, bad)
