@@ -110,6 +110,11 @@ __device__ __forceinline__ float dpp_f32(float v) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), ctrl, 0xf, 0xf, false));
 }
 
+template <int ctrl>
+__device__ __forceinline__ double dpp_f64(double v) {
+    return __hiloint2double((int)dpp_u32<ctrl>((uint32_t)__double2hiint(v)), (int)dpp_u32<ctrl>((uint32_t)__double2loint(v)));
+}
+
 // SVE FADDV over 16 lanes (bytecode_interpreter.s:7059): the pairwise tree
 // ((((a0+a1)+(a2+a3))+((a4+a5)+(a6+a7)))+(((a8+a9)+...))).  Each step adds
 // the partner group's partial; after step k all lanes of a 2^k-group hold

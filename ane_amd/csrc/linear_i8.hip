@@ -54,10 +54,6 @@ __device__ __forceinline__ void apply_norm(float (&y)[8], float inv, const float
     for (int e = 0; e < 8; e++) y[e] = __fmul_rn(__fmul_rn(y[e], inv), w[e]);
 }
 
-template <int ctrl>
-__device__ __forceinline__ double dpp_f64(double v) {
-    return __hiloint2double((int)dpp_u32<ctrl>((uint32_t)__double2hiint(v)), (int)dpp_u32<ctrl>((uint32_t)__double2loint(v)));
-}
 // The sum of squares of the 32-block that lanes 4 i .. 4 i + 3 hold, in the order of
 // common.hpp's canonical sum (in all four lanes).
 __device__ __forceinline__ double block_sumsq(const float (&y)[8]) {

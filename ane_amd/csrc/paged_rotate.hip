@@ -131,16 +131,20 @@ __global__ void __launch_bounds__(256) k_paged_rotate(RotateArgs a) {
         const bool isq = u < qu, isv = u >= qu + ku;
         const float* w = isq ? a.q_norm : a.k_norm;
         if (w && !isv) {  // (whole heads: all lanes of one agree)
-            float ss = 0.0f;
+            // (squares in fp64, and the head brought near 1 by 2^k, 4^k <= mean + eps:
+            // any head of fp32 values has its norm)
+            double ss = 0.0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) ss = __builtin_fmaf(v[e], v[e], ss);
-            ss += dpp_f32<kDppQuadXor1>(ss);
-            ss += dpp_f32<kDppQuadXor2>(ss);
-            ss += dpp_f32<kDppHalfMirror>(ss);
-            if (HD == 128) ss += dpp_f32<kDppRowMirror>(ss);
-            const float inv = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
+            for (int e = 0; e < 8; e++) ss = __builtin_fma((double)v[e], (double)v[e], ss);
+            ss += dpp_f64<kDppQuadXor1>(ss);
+            ss += dpp_f64<kDppQuadXor2>(ss);
+            ss += dpp_f64<kDppHalfMirror>(ss);
+            if (HD == 128) ss += dpp_f64<kDppRowMirror>(ss);
+            const double m = ss * (1.0 / HD) + (double)a.eps;
+            const int k = ((int)((uint32_t)__double2hiint(m) >> 20) - 1023) >> 1;
+            const float inv = 1.0f / sqrtf((float)__builtin_ldexp(m, -2 * k));
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = v[e] * inv * (isq ? qw[e] : kw[e]);
+            for (int e = 0; e < 8; e++) v[e] = __builtin_ldexpf(v[e], -k) * inv * (isq ? qw[e] : kw[e]);
         }
         if (a.rot) {
             float y[8];

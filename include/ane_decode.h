@@ -264,9 +264,10 @@ int ane_hip_paged_rope_append(const struct ane_paged_cache* cache, uint32_t laye
  * a head, or scale the rotation for long contexts: with q_norm and k_norm (fp32
  * [head_dim], each may be NULL) a head becomes x / sqrt(mean(x^2) + eps) * w
  * first; then pair i of its leading rot_dim values (a, b) becomes (a c - b s,
- * a s + b c), c and s = factor * (cos, sin)(position * freqs[i]).  The angle is
- * formed in fp64, its cosine and sine exact to fp32, the rest in fp32; there is no
- * table and no bound on positions but the cache's.  rope NULL or rot_dim 0: no
+ * a s + b c), c and s = factor * (cos, sin)(position * freqs[i]).  A head's mean
+ * square is formed in fp64, so that heads of any fp32 values have their norm.  The
+ * angle is formed in fp64, its cosine and sine exact to fp32, the rest in fp32; there
+ * is no table and no bound on positions but the cache's.  rope NULL or rot_dim 0: no
  * rotation.  A token at a negative position is not appended and its q_out row is
  * zeros.  Everything else as above. */
 struct ane_rope {

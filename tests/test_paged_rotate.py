@@ -353,3 +353,30 @@ def test_special_values(ane):
     f = ane.rope_freqs(128)[0]
     y, tol = want(q.cpu().numpy()[3:], pos[3:], f, 1.0, True, np.ones(128, np.float32), 1e-6, "f32")
     near(o[3:], (y, tol), "q")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,heads,kv", [(128, 3, 3), (64, 4, 2)])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_heads_at_the_ends_of_the_range(ane, hd, heads, kv, eps):
+    """Heads whose squares leave fp32's range, upwards and downwards: normalised like any other.  (A head of denormals
+    beside an eps stays one: six roundings of 2^-150 each on the way, weights and rotation at most double them: below 2^-146.)"""
+    import torch
+
+    powers = [2.0 ** e for e in (66, 80, 100, 120, -66, -76, -100, -126, -140)]
+    n = len(powers)
+    c = make_cache([n], heads, kv, hd, 16, fill_rest=0.0)
+    qkv = randq(n, heads + 2 * kv, hd, dt("f32"), seed=21) * torch.tensor(powers, device="cuda")[:, None, None]
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    qw, kw = (torch.randn(hd, generator=gen, device="cuda") * 0.3 + 1 for _ in range(2))
+    out = torch.full((n, heads, hd), 5.0, device="cuda")
+    f = ane.rope_freqs(hd)[0]
+    ane.paged_norm_rope_append(c, 0, i32([0, n]), q, k, v, Rope(torch.from_numpy(f).cuda(), half=True), out, q_norm=qw, k_norm=kw,
+                               eps=eps)
+    pos = np.arange(n)
+    y, tol = want(q.cpu().numpy(), pos, f, 1.0, True, qw.cpu().numpy(), eps, "f32")
+    near(out.cpu().numpy(), (y, tol + 2.0 ** -146), "q")
+    page = int(c.page_table[0, 0])
+    near(c.k_pages[0, page, :, :n].transpose(0, 1).cpu().numpy(),
+         want(k.cpu().numpy(), pos, f, 1.0, True, kw.cpu().numpy(), eps, "f16"), "k")
