@@ -182,7 +182,9 @@ constexpr uint32_t kMaxRows = 65535u * 128;     // of x and of w: workgroups of 
 // One wave a token from 1024 tokens on (4096 x 4096 fp16 behind a norm 19.9 -> 13.2
 // us, 3.8 TB/s; without one 10.4, 4.8), sixteen up to 256 (32 x 14336 fp32 4.8 -> 3.4),
 // four between.
-constexpr uint32_t kManyTokens = 1024, kFewTokens = 256;
+constexpr uint32_t kManyTokens = 1024, kFewTokens = 256, kMaxFour = 16384;  // (values that four waves hold)
+// Longer tokens take 1024 threads each, and a launch holds fewer than 2^32.
+bool quantize_fits(uint32_t T, uint32_t K) { return K <= kMaxFour || launch_fits(T, 1024); }
 template <class T>
 void launch_quantize(const QuantArgs& a, hipStream_t s) {
     auto go = [&](auto* f, uint32_t nw) {
@@ -191,10 +193,10 @@ void launch_quantize(const QuantArgs& a, hipStream_t s) {
     if (a.K <= 512) return go(k_quantize_tokens<T, 1, 1>, 1);
     if (a.T >= kManyTokens && a.K <= 2048) return go(k_quantize_tokens<T, 1, 4>, 1);
     if (a.T >= kManyTokens && a.K <= 4096) return go(k_quantize_tokens<T, 1, 8>, 1);
-    if (a.T <= kFewTokens || a.K > 16384) {
+    if (a.T <= kFewTokens || a.K > kMaxFour) {
         if (a.K <= 2048) return go(k_quantize_tokens<T, 4, 1>, 4);
         if (a.K <= 8192) return go(k_quantize_tokens<T, 16, 1>, 16);
-        if (a.K <= 16384) return go(k_quantize_tokens<T, 16, 2>, 16);
+        if (a.K <= kMaxFour) return go(k_quantize_tokens<T, 16, 2>, 16);
         return go(k_quantize_tokens<T, 16, 0>, 16);
     }
     switch ((a.K + 2047) / 2048) {
@@ -407,7 +409,8 @@ bool known_type(int type) { return type == ANE_TYPE_F32 || type == ANE_TYPE_F16;
 bool off(const void* p, uint64_t n) { return ((uintptr_t)p) % n != 0; }
 
 int tokens_status(uint32_t T, uint32_t K, int type, const void* x, uint64_t x_stride, const float* norm_w, float eps) {
-    if (T > kMaxRows || K == 0 || K > kMaxK || !known_type(type) || !(eps >= 0.0f) || !(eps < 1e30f)) return ANE_ERR_INVALID_ARG;
+    if (T > kMaxRows || K == 0 || K > kMaxK || !quantize_fits(T, K) || !known_type(type) || !(eps >= 0.0f) || !(eps < 1e30f))
+        return ANE_ERR_INVALID_ARG;
     if (T == 0) return ANE_OK;
     if (!x) return ANE_ERR_BAD_POINTER;
     if (off(x, item_size(type)) || off(norm_w, 4) || (T > 1 && x_stride < K)) return ANE_ERR_INVALID_ARG;

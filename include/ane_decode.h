@@ -400,7 +400,7 @@ int ane_hip_pages_compact(const struct ane_paged_cache* cache, uint32_t* page_ta
  * whose int8 products have one scale a tensor.  Types are ANE_TYPE_F32 or
  * ANE_TYPE_F16; strides are in elements from one token (row of w) to the next,
  * the values of one are contiguous.  1 <= K < 2^17, T and N at most 65535 * 128,
- * T * N below 2^38.  All calls are asynchronous on stream; pointers must belong
+ * T * N below 2^38, quantized tokens below 2^22 where K > 16384.  All calls are asynchronous on stream; pointers must belong
  * to the current device and be aligned to their elements, q and w (and their
  * strides, which are bytes) to 16 bytes.
  *

@@ -504,3 +504,10 @@ def test_one_workspace_for_batches_of_every_size(ane, N, K, most):
         out = torch.full((T, N), float("nan"), device="cuda")
         ane.linear_i8(X[:T], W, S, out, norm_w=nw, residual=R[:T], workspace=work)
         same(out.cpu().numpy(), want[:T])
+
+
+@pytest.mark.parametrize("T", [1 << 22, 65535 * 128])
+def test_launches_past_32_bits_are_refused(T):
+    """Above 16384 values a token takes 1024 threads, and a launch holds fewer than 2^32."""
+    assert c_quant(T=T, K=16385, xs=16385, qs=16400) == INVALID
+    assert c_linear(T=T, K=16385, xs=16385, wst=16400) == INVALID
