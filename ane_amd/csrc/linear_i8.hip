@@ -87,12 +87,14 @@ struct TokenScale {
     float up, per, scale;
     bool plain;
     __device__ __forceinline__ TokenScale(uint32_t top) {
-        // (a maximum below 2^-96 is brought up first: its reciprocal would not be finite)
+        // (a maximum below 2^-96 is brought up first: its reciprocal would not be finite; the
+        // scale is divided as it is, or a denormal one would be rounded twice)
         up = top < 0x0f800000u ? 0x1p96f : 1.0f;
         const float m = __uint_as_float(top) * up;
         per = top == 0 ? 127.0f : __fmul_rn(1.0f / m, 127.0f);
-        scale = top == 0 ? 1.0f : m / 127.0f / up;
-        // (every |y per| is at most 127 (1 + 2^-23)^2 then)
+        scale = top == 0 ? 1.0f : __uint_as_float(top) / 127.0f;
+        // (every |y per| is below 127.5 then: 1 / m is off by 2^-24 of itself, above 2^126, where
+        // it is denormal, by 2^-22, the two products by 2^-24 each)
         plain = up == 1.0f && fast_quant_ok(m, per);
     }
     __device__ __forceinline__ uint2 pack(const float (&y)[8]) const {

@@ -511,3 +511,16 @@ def test_launches_past_32_bits_are_refused(T):
     """Above 16384 values a token takes 1024 threads, and a launch holds fewer than 2^32."""
     assert c_quant(T=T, K=16385, xs=16385, qs=16400) == INVALID
     assert c_linear(T=T, K=16385, xs=16385, wst=16400) == INVALID
+
+
+@pytest.mark.gpu
+def test_denormal_scales_are_rounded_once(ane):
+    """max / 127 just below the middle of two denormals, whose quotient in 24 bits is that middle."""
+    k = np.array([(1 << 17) + 1, (1 << 17) + 77, 200001, 150003, (1 << 18) - 1, 99, 5], np.float64)
+    top = ((127 * k + 63) * 2.0 ** -149).astype(np.float32)
+    assert (top.astype(np.float64) == (127 * k + 63) * 2.0 ** -149).all()
+    x = np.random.default_rng(6).uniform(-1, 1, (len(k), 300)).astype(np.float32) * top[:, None]
+    x[:, 7] = top
+    q, s = run_quant(x)
+    same(s, (k * 2.0 ** -149).astype(np.float32))
+    same(q, quantized(x)[0])
