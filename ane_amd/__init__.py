@@ -1302,7 +1302,8 @@ def attention_prompt_workspace_size(cache, n, n_tokens, max_len=None, rule=None)
 
 
 def attention_prompt_workspace(cache, n, n_tokens, max_len=None, rule=None):
-    """A workspace for attention_prompt calls of these sizes, for callers that keep one."""
+    """A workspace for attention_prompt calls of these very sizes, for callers that keep one (a smaller batch may need a
+    larger one: the largest of theirs does for several)."""
     return _scratch(attention_prompt_workspace_size(cache, n, n_tokens, max_len, rule), cache.k_pages.device)
 
 
@@ -1333,7 +1334,8 @@ def attention_shared_workspace_size(cache, n, n_groups=0, max_prefix=None, max_l
 
 
 def attention_shared_workspace(cache, n, n_groups=0, max_prefix=None, max_len=None):
-    """A workspace for attention_shared calls of these sizes, for callers that keep one."""
+    """A workspace for attention_shared calls of these very sizes, for callers that keep one (a smaller batch may need a
+    larger one: the largest of theirs does for several)."""
     return _scratch(attention_shared_workspace_size(cache, n, n_groups, max_prefix, max_len), cache.k_pages.device)
 
 

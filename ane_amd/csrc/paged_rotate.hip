@@ -7,8 +7,9 @@
 // pairs being neighbours (2i, 2i + 1) or halves (i, i + rot_dim / 2).
 //
 // The angle is formed and reduced in fp64 and its cosine and sine are rounded
-// once, so far positions are as exact as near ones and no table of positions is
-// read.
+// once, and no table of positions is read.  The fp64 product position * freq is off by at
+// most 2^-53 of the angle: nothing beside fp32's rounding up to 2^25 radians, as much
+// as one such rounding (6e-8) at 2^29.
 #include <algorithm>
 
 #include "paged.hpp"

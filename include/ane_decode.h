@@ -298,7 +298,9 @@ int ane_hip_paged_norm_rope_append(const struct ane_paged_cache* cache, uint32_t
  * the split of long rows (longer sequences are still computed whole); 0 stands
  * for max_pages * page_size.  out may be q when the strides agree.  The
  * workspace (256-byte aligned; NULL when its size is 0) belongs to the call
- * until it has run. */
+ * until it has run.  Its size is that of these very arguments: a smaller batch, whose
+ * keys are split over more workgroups, may need more, so one kept for several
+ * batches has the largest of their sizes. */
 size_t ane_hip_attention_prompt_workspace_size(const struct ane_paged_cache* cache, uint32_t n, uint32_t n_tokens,
                                                uint32_t max_len);
 int ane_hip_attention_prompt(const struct ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
@@ -321,7 +323,8 @@ int ane_hip_attention_prompt(const struct ane_paged_cache* cache, uint32_t layer
  * lies behind every key (the token sees none), its prefix is none.
  * softcap: 0, or 2^-20 to 2^20.  Single tokens (q_start NULL) are the decode step.
  * Types, accuracy (of the score before the cap, in fp32) and everything else as
- * above; the workspace is that of the rule (with a window fewer keys are split). */
+ * above; the cap adds 2^-22 of a capped score (F16: 2^-20).  The workspace is that
+ * of the rule (with a window fewer keys are split). */
 struct ane_attention_rule {
     float softcap;
     uint32_t window;
@@ -343,7 +346,8 @@ int ane_hip_attention_rule(const struct ane_paged_cache* cache, uint32_t layer, 
  * [n_groups]): those are read once for the whole group, out of the pages of
  * its first row; rows outside every group share nothing.  A prefix longer than
  * a row's or the first row's length counts as that length.  max_prefix and
- * max_len bound the prefix lengths and the lengths as max_len does above. */
+ * max_len bound the prefix lengths and the lengths as max_len does above.  The
+ * workspace as there. */
 size_t ane_hip_attention_shared_workspace_size(const struct ane_paged_cache* cache, uint32_t n, uint32_t n_groups,
                                                uint32_t max_prefix, uint32_t max_len);
 int ane_hip_attention_shared(const struct ane_paged_cache* cache, uint32_t layer, const uint32_t* seqs, uint32_t n,
@@ -416,7 +420,10 @@ int ane_hip_pages_compact(const struct ane_paged_cache* cache, uint32_t* page_ta
  * of any product is NaN.
  * dense_i8_scaled: out[t][n] = fl(fl((float)sum q w * q_scales[t]) * w_scales[n])
  * + bias[n] + residual[t][n], one rounding a step, the sum exact; bias (fp32 [N])
- * and residual (out's type; may be out itself with its stride) may be NULL.
+ * and residual (out's type; may be out itself with its stride) may be NULL.  It has
+ * no workspace and so never splits K over workgroups, as linear_i8 does.
+ * Weights (and quantized tokens) from 2 GiB on, N * w_stride >= 2^31, go through the
+ * one kernel with 64-bit offsets, which takes 1.6 to 3.6 times as long.
  * linear_i8: both, q and scales in the workspace (256-byte aligned; it belongs to
  * the call until it has run).  The size for T tokens is enough for fewer of them as
  * well.  The same bits as the two calls.  out may lie in x, otherwise outputs share
